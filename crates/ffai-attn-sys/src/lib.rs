@@ -133,6 +133,33 @@ unsafe extern "C" {
                               k_pool: *mut c_void, v_pool: *mut c_void, num_pages: i32,
                               src: *const i32, dst: *const i32, n: i32,
                               stream: *mut c_void) -> c_int;
+    pub fn ffai_attn_shared_prefix(ctx: *mut ffai_attn_ctx, d: *const ffai_attn_desc,
+                                   kv_heads: i32, q: *const c_void, k_pool: *const c_void,
+                                   v_pool: *const c_void, num_pages: i32,
+                                   group_starts: *const i32, n_groups: i32,
+                                   prefix_table: *const i32, prefix_lens: *const i32,
+                                   prefix_pages: i32, block_table: *const i32,
+                                   seq_lens: *const i32, max_pages: i32, o: *mut c_void,
+                                   lse: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ffai_page_plan(ctx: *mut ffai_attn_ctx, batch: i32, max_pages: i32, num_pages: i32,
+                          lens: *const i32, new_tokens: *const i32, free_pages: *const i32,
+                          free_cap: i32, free_count: *const i32, pos_base: *const i32,
+                          block_table: *mut i32, lens_out: *mut i32, cu_new: *mut i32,
+                          slots: *mut i32, positions: *mut i32, slot_cap: i32,
+                          free_count_out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ffai_page_release(ctx: *mut ffai_attn_ctx, batch: i32, max_pages: i32,
+                             lens: *const i32, done: *const i32, block_table: *const i32,
+                             free_pages: *mut i32, free_cap: i32, free_count: *const i32,
+                             lens_out: *mut i32, free_count_out: *mut i32,
+                             stream: *mut c_void) -> c_int;
+    pub fn ffai_kv_write_slots(ctx: *mut ffai_attn_ctx, d: *const ffai_attn_desc,
+                               k_pool: *mut c_void, v_pool: *mut c_void, num_pages: i32,
+                               k_new: *const c_void, v_new: *const c_void, slots: *const i32,
+                               n_tokens: i32, stream: *mut c_void) -> c_int;
+    pub fn ffai_sample(ctx: *mut ffai_attn_ctx, logits: *const c_void, ld: i64, dtype: i32,
+                       batch: i32, vocab: i32, u: *const f32, temperature: *const f32,
+                       top_k: *const i32, top_p: *const f32, min_p: *const f32,
+                       tokens: *mut i32, logprobs: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ffai_int8_gemv_layout(rows: i32, cols: i32, blk: i32, packed_bytes: *mut i64,
                                  corr_count: *mut i64) -> c_int;
     pub fn ffai_int8_gemv_quantize(ctx: *mut ffai_attn_ctx, w: *const c_void, w_dtype: i32,

@@ -92,6 +92,15 @@ SIGNATURES = {
                                ctypes.c_int),
     "ffai_kv_append": ([_vp, _DescP, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp], ctypes.c_int),
     "ffai_kv_copy_pages": ([_vp, _DescP, _vp, _vp, _i32, _vp, _vp, _i32, _vp], ctypes.c_int),
+    "ffai_attn_shared_prefix": ([_vp, _DescP, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _i32,
+                                 _vp, _vp, _i32, _vp, _vp, _vp], ctypes.c_int),
+    "ffai_page_plan": ([_vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                        _vp, _i32, _vp, _vp], ctypes.c_int),
+    "ffai_page_release": ([_vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp],
+                          ctypes.c_int),
+    "ffai_kv_write_slots": ([_vp, _DescP, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp], ctypes.c_int),
+    "ffai_sample": ([_vp, _vp, ctypes.c_int64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                     _vp], ctypes.c_int),
     "ffai_int8_gemv_layout": ([_i32, _i32, _i32, _vp, _vp], ctypes.c_int),
     "ffai_f16_gemv_layout": ([_i32, _i32, _vp], ctypes.c_int),
     "ffai_gemm_bf16": ([_vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_int64,

@@ -1223,6 +1223,218 @@ int ffai_kv_copy_pages(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool
   return FFAI_ATTN_OK;
 }
 
+// ---------------------------------------------------------------------------
+// Batched decode step: attention over a shared prefix, page plans, slot writes,
+// sampling.
+
+int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,
+                            const void* q, const void* k_pool, const void* v_pool,
+                            int32_t num_pages, const int32_t* group_starts, int32_t n_groups,
+                            const int32_t* prefix_table, const int32_t* prefix_lens,
+                            int32_t prefix_pages, const int32_t* block_table,
+                            const int32_t* seq_lens, int32_t max_pages, void* o, float* lse,
+                            void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (!d) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "null descriptor");
+  if (d->head_dim != kHD)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "head_dim %d: only 64 is served", d->head_dim);
+  if (d->batch <= 0 || d->heads <= 0 || d->q_len <= 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "batch %d, heads %d, q_len %d must be >= 1",
+                     d->batch, d->heads, d->q_len);
+  if (kv_heads <= 0 || d->heads % kv_heads != 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "heads %d must be a multiple of kv_heads %d",
+                     d->heads, kv_heads);
+  if (!valid_dtype(d->q_dtype) || !valid_dtype(d->kv_dtype) || !valid_dtype(d->out_dtype))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "unknown dtype (q %d, kv %d, out %d)", d->q_dtype,
+                     d->kv_dtype, d->out_dtype);
+  if (d->kv_dtype == FFAI_DT_F32)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: bf16 or f16 pools only");
+  if (d->q_dtype != FFAI_DT_F32 && d->q_dtype != d->kv_dtype)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: q must be f32 or the cache dtype");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "scale must be finite and > 0");
+  if (d->flags != 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "shared prefix: unknown flags 0x%x", d->flags);
+  for (int l : {d->q_layout, d->out_layout})
+    if (l != FFAI_LAYOUT_HEADS_SPLIT && l != FFAI_LAYOUT_TOKEN_MAJOR)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "q and out are heads-split or token-major");
+  if (d->token_stride != 0 &&
+      (d->q_layout != FFAI_LAYOUT_TOKEN_MAJOR || d->token_stride < d->heads * kHD ||
+       d->token_stride % 8 != 0))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                     "token_stride %d: 0, or for a token-major q a multiple of 8 of at least "
+                     "heads * 64", d->token_stride);
+  constexpr int kMaxPages = (1 << 30) / kPageKeys;
+  if (!q || !o || !k_pool || !v_pool || !block_table || !seq_lens || num_pages <= 0 ||
+      max_pages <= 0 || max_pages > kMaxPages)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "shared prefix: null pointer or empty pool/table");
+  if (n_groups < 0 || (n_groups > 0 && (!group_starts || !prefix_table || !prefix_lens ||
+                                        prefix_pages <= 0 || prefix_pages > kMaxPages)))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "shared prefix: bad prefix tables");
+  for (const void* ptr : {q, k_pool, v_pool, static_cast<const void*>(o)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "shared prefix: operands 16-byte aligned");
+  const long long rows = static_cast<long long>(d->q_len) * (d->heads / kv_heads);
+  if (rows > (1 << 30) ||
+      static_cast<double>(d->batch) * kv_heads * ((rows + 15) / 16) > 2147483647.0)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows");
+  SharedParams p{};
+  p.q = q;
+  const Strides qs = strides_of(d->q_layout, d->heads, d->q_len, d->token_stride);
+  const Strides os = strides_of(d->out_layout, d->heads, d->q_len);
+  p.q_sb = qs.sb, p.q_st = qs.sr, p.q_sh = qs.sh;
+  p.o_sb = os.sb, p.o_st = os.sr, p.o_sh = os.sh;
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.group_starts = group_starts;
+  p.prefix_table = prefix_table;
+  p.prefix_lens = prefix_lens;
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.groups = n_groups;
+  p.prefix_pages = prefix_pages;
+  p.max_pages = max_pages;
+  p.num_pages = num_pages;
+  p.batch = d->batch;
+  p.heads = d->heads;
+  p.kv_heads = kv_heads;
+  p.q_len = d->q_len;
+  p.q_dtype = d->q_dtype;
+  p.kv_dtype = d->kv_dtype;
+  p.out_dtype = d->out_dtype;
+  p.scale_log2 = d->scale * 1.4426950408889634f;
+  p.out = o;
+  p.lse = lse;
+  if (d->out_layout == FFAI_LAYOUT_TOKEN_MAJOR) {
+    p.lse_sh = static_cast<long long>(d->batch) * d->q_len, p.lse_sb = d->q_len, p.lse_st = 1;
+  } else {
+    p.lse_sb = static_cast<long long>(d->heads) * d->q_len, p.lse_sh = d->q_len, p.lse_st = 1;
+  }
+  p.err = ctx->d_err;
+  DeviceGuard g(ctx->device);
+  ProfScope ps(ctx, FFAI_OP_DECODE, static_cast<cudaStream_t>(stream), "ffai_attn_shared_prefix");
+  FFAI_CUDA(ctx, launch_shared_rows(p, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_page_plan(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, int32_t num_pages,
+                   const int32_t* lens, const int32_t* new_tokens, const int32_t* free_pages,
+                   int32_t free_cap, const int32_t* free_count, const int32_t* pos_base,
+                   int32_t* block_table, int32_t* lens_out, int32_t* cu_new, int32_t* slots,
+                   int32_t* positions, int32_t slot_cap, int32_t* free_count_out, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (batch <= 0 || max_pages <= 0 || num_pages <= 0 || free_cap < 0 || slot_cap < 0 ||
+      max_pages > (1 << 30) / kPageKeys || num_pages > INT32_MAX / kPageKeys ||
+      slot_cap > (1 << 30))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                     "page plan: batch %d, max_pages %d, num_pages %d, free_cap %d, slot_cap %d",
+                     batch, max_pages, num_pages, free_cap, slot_cap);
+  if (batch > kPlMaxBatch)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "page plan: batch %d, at most %d", batch, kPlMaxBatch);
+  if (!lens || !new_tokens || (free_cap > 0 && !free_pages) || !free_count || !block_table ||
+      !lens_out || !cu_new || (slot_cap > 0 && !slots) || !free_count_out)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page plan: null pointer");
+  if (lens_out == lens || lens_out == new_tokens || free_count_out == free_count)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page plan: outputs must not alias inputs");
+  PlanParams p{lens,     new_tokens, free_pages, free_count, pos_base,       block_table, lens_out,
+               cu_new,   slots,      positions,  free_count_out, batch, max_pages, num_pages,
+               free_cap, slot_cap,   ctx->d_err};
+  DeviceGuard g(ctx->device);
+  FFAI_CUDA(ctx, launch_page_plan(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_page_release(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, const int32_t* lens,
+                      const int32_t* done, const int32_t* block_table, int32_t* free_pages,
+                      int32_t free_cap, const int32_t* free_count, int32_t* lens_out,
+                      int32_t* free_count_out, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (batch <= 0 || max_pages <= 0 || free_cap <= 0 || max_pages > (1 << 30) / kPageKeys)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page release: batch %d, max_pages %d, free_cap %d",
+                     batch, max_pages, free_cap);
+  if (batch > kPlMaxBatch)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "page release: batch %d, at most %d", batch,
+                     kPlMaxBatch);
+  if (!lens || !done || !block_table || !free_pages || !free_count || !lens_out || !free_count_out)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page release: null pointer");
+  if (lens_out == lens || lens_out == done || free_count_out == free_count)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page release: outputs must not alias inputs");
+  ReleaseParams p{lens,  done,      block_table, free_pages, free_count, lens_out, free_count_out,
+                  batch, max_pages, free_cap,    ctx->d_err};
+  DeviceGuard g(ctx->device);
+  FFAI_CUDA(ctx, launch_page_release(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_kv_write_slots(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool, void* v_pool,
+                        int32_t num_pages, const void* k_new, const void* v_new,
+                        const int32_t* slots, int32_t n_tokens, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (!d) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "null descriptor");
+  if (d->head_dim != kHD)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "head_dim %d: only 64 is served", d->head_dim);
+  if (d->heads <= 0 || n_tokens < 0 || num_pages <= 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "slot write: heads %d, tokens %d, pages %d",
+                     d->heads, n_tokens, num_pages);
+  if (!valid_dtype(d->q_dtype) || !valid_dtype(d->kv_dtype))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "unknown dtype (new %d, kv %d)", d->q_dtype,
+                     d->kv_dtype);
+  if (d->q_dtype != FFAI_DT_F32 && d->q_dtype != d->kv_dtype)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "slot write: new rows f32 or of the cache dtype");
+  if (d->token_stride != 0 && d->token_stride < d->heads * kHD)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "token_stride %d: 0 or at least heads * 64",
+                     d->token_stride);
+  if (n_tokens == 0) return FFAI_ATTN_OK;
+  if (!k_pool || !v_pool || !k_new || !v_new || !slots)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "slot write: null pointer");
+  for (const void* ptr : {static_cast<const void*>(k_pool), static_cast<const void*>(v_pool)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page pools must be 16-byte aligned");
+  const size_t es = dtype_size(d->q_dtype);
+  for (const void* ptr : {k_new, v_new})
+    if (reinterpret_cast<uintptr_t>(ptr) % es != 0)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "slot write: rows not aligned to their type");
+  WriteParams p{};
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.k_new = k_new;
+  p.v_new = v_new;
+  p.slots = slots;
+  p.src_stride = d->token_stride ? d->token_stride : d->heads * kHD;
+  p.tokens = n_tokens;
+  p.heads = d->heads;
+  p.num_pages = num_pages;
+  p.src_dtype = d->q_dtype;
+  p.dst_dtype = d->kv_dtype;
+  p.vec = reinterpret_cast<uintptr_t>(k_new) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(v_new) % 16 == 0 && p.src_stride * es % 16 == 0;
+  p.err = ctx->d_err;
+  DeviceGuard g(ctx->device);
+  FFAI_CUDA(ctx, launch_kv_write(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtype, int32_t batch,
+                int32_t vocab, const float* u, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
+                void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (batch <= 0 || vocab <= 0 || ld < vocab)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: batch %d, vocab %d, ld %lld", batch, vocab,
+                     static_cast<long long>(ld));
+  if (!valid_dtype(dtype)) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "unknown logits dtype");
+  if (vocab > kSmMaxVocab)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "sample: vocab %d, at most %d", vocab, kSmMaxVocab);
+  if (!logits || !u || !tokens)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: null pointer");
+  if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) != 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: logits not aligned to their type");
+  SampleParams p{logits, ld, batch, vocab, dtype, u, temperature, top_k, top_p, min_p, tokens, logprobs};
+  DeviceGuard g(ctx->device);
+  FFAI_CUDA(ctx, launch_sample(p, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
 int ffai_attn_last_error(const ffai_attn_ctx* ctx, char* buf, size_t n) {
   const std::string& msg = ctx ? ctx->last_error : g_tls_error;
   const int st = ctx ? ctx->last_status : g_tls_status;

@@ -322,4 +322,98 @@ struct StageBatch {
 };
 cudaError_t launch_stage_batch(StageBatch sb, int dst_f16, cudaStream_t s);
 
+// ---- attention over a shared prefix (shared_prefix.cu) ---------------------
+
+// Pools (num_pages, kv_heads, kPageKeys, 64) of a 16-bit kv_dtype.  Strides
+// (sb, st, sh: sequence, token, head) in elements; rows of 64 are dense.
+struct SharedParams {
+  const void* q;
+  long long q_sb, q_st, q_sh;
+  const void* k_pool;
+  const void* v_pool;
+  const int* group_starts;  // (groups + 1), rising
+  const int* prefix_table;  // (groups, prefix_pages)
+  const int* prefix_lens;   // (groups)
+  const int* block_table;   // (batch, max_pages)
+  const int* seq_lens;      // (batch)
+  int groups, prefix_pages, max_pages, num_pages;
+  int batch, heads, kv_heads, q_len;
+  int q_dtype, kv_dtype, out_dtype;
+  float scale_log2;
+  void* out;
+  long long o_sb, o_st, o_sh;
+  float* lse;  // or null
+  long long lse_sb, lse_st, lse_sh;
+  unsigned* err;
+};
+cudaError_t launch_shared_rows(const SharedParams& p, cudaStream_t s);
+
+// ---- page plans and slot writes (pages.cu) ----------------------------------
+
+constexpr int kPlMaxBatch = 16384;  // three words of shared memory per request
+
+struct PlanParams {
+  const int* lens;         // (batch) keys held
+  const int* new_tokens;   // (batch) keys asked for
+  const int* free_pages;   // (free_cap) stack of free pages, top at free_count - 1
+  const int* free_count;
+  const int* pos_base;     // (batch) or null
+  int* block_table;        // (batch, max_pages), new entries written
+  int* lens_out;           // (batch)
+  int* cu_new;             // (batch + 1)
+  int* slots;              // (slot_cap)
+  int* positions;          // (slot_cap) or null
+  int* free_count_out;
+  int batch, max_pages, num_pages, free_cap, slot_cap;
+  unsigned* err;
+};
+cudaError_t launch_page_plan(const PlanParams& p, int sms, cudaStream_t s);
+
+struct ReleaseParams {
+  const int* lens;
+  const int* done;
+  const int* block_table;
+  int* free_pages;
+  const int* free_count;
+  int* lens_out;
+  int* free_count_out;
+  int batch, max_pages, free_cap;
+  unsigned* err;
+};
+cudaError_t launch_page_release(const ReleaseParams& p, int sms, cudaStream_t s);
+
+// k_new, v_new: (tokens, heads, 64) rows src_stride elements apart, of
+// src_dtype (f32, or the pools' dst_dtype); slots (tokens), negative: skipped.
+struct WriteParams {
+  void* k_pool;
+  void* v_pool;
+  const void* k_new;
+  const void* v_new;
+  const int* slots;
+  long long src_stride;
+  int tokens, heads, num_pages;
+  int src_dtype, dst_dtype;
+  int vec;  // source rows are 16-byte aligned
+  unsigned* err;
+};
+cudaError_t launch_kv_write(const WriteParams& p, int sms, cudaStream_t s);
+
+// ---- sampling (sample.cu) -----------------------------------------------------
+
+constexpr int kSmMaxVocab = 1 << 18;  // weight sums stay below 2^54
+
+struct SampleParams {
+  const void* logits;  // (batch, vocab), rows ld elements apart
+  long long ld;
+  int batch, vocab, dtype;
+  const float* u;            // (batch)
+  const float* temperature;  // (batch) or null: 1
+  const int* top_k;          // (batch) or null: off
+  const float* top_p;
+  const float* min_p;
+  int* tokens;      // (batch)
+  float* logprobs;  // (batch) or null
+};
+cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
+
 }  // namespace ffai

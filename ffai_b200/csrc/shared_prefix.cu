@@ -1,0 +1,313 @@
+// Attention of a batch whose sequences share long prefixes, over a paged KV
+// cache: group g of consecutive sequences shares prefix_lens[g] keys; sequence
+// b adds seq_lens[b] keys of its own.  Query row (b, i, h), i < q_len, sees
+// the whole prefix of its group and its own keys j < seq_lens[b] - (q_len - 1
+// - i), i.e. up to its own position; query head h reads KV head h / G, G =
+// heads / kv_heads:
+//   s_j = scale q.k_j,  o = sum_j e^(s_j - m) v_j / l,  l = sum_j e^(s_j - m).
+// A row that sees no key gives zeros and an lse of -inf.
+//
+// The R = q_len * G rows of one (sequence, KV head) are served together, in
+// tiles of 16 (the matrix instruction's rows); each warp of a CTA takes every
+// kSpWarps-th step of 32 keys with a softmax state of its own, and the warps
+// merge at the end.  K and V go from global memory straight into the operand
+// registers: the products' inner order is free, so it is chosen such that
+// each lane's operands are whole 16-byte pieces of the key rows.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace ffai {
+
+namespace {
+
+constexpr int kSpWarps = 4;
+constexpr int kSpThreads = kSpWarps * 32;
+constexpr int kSpKeys = 32;  // keys per warp step (divides a page)
+
+template <int F16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Softmax state of a warp's 16 rows: lane (g, t) = (lane / 4, lane % 4) holds
+// rows g and g + 8; o[j][2 v + w] is row g + 8 v, head dim 16 t + 8 w + j.
+struct RowState {
+  float m[2], l[2];
+  float o[8][4];
+};
+
+// The 16 query rows as A operands: k-step s (16 of the 64 head dims) holds
+// dims 32 (s / 2) + 8 t + 4 (s % 2) + {0, 1} and + {2, 3}, so that the lane's
+// part of a key row is the two 16-byte pieces at dims 8 t and 32 + 8 t.
+struct RowQ {
+  uint32_t a[4][4];
+};
+
+__device__ __forceinline__ uint4 zero4() { return make_uint4(0, 0, 0, 0); }
+
+// One step: 32 keys of one page starting at kp / vp; `live` of them hold data
+// (the rest are not read), and row v of this lane sees the first `see[v]`.
+template <int F16>
+__device__ __forceinline__ void step32(RowState& st, const RowQ& q, const uint16_t* kp,
+                                       const uint16_t* vp, int live, const int (&see)[2],
+                                       float scale_log2) {
+  const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+  uint4 k[4][2];  // n-tile i: key 8 i + g
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = 8 * i + g;
+    const uint4* src = reinterpret_cast<const uint4*>(kp + key * 64);
+    k[i][0] = key < live ? __ldg(src + t) : zero4();
+    k[i][1] = key < live ? __ldg(src + 4 + t) : zero4();
+  }
+  uint4 v[2][4];  // 16-key half h: keys 16 h + 2 t + {0, 1, 8, 9}, dims 8 g ..
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int key = 16 * h + 2 * t + (e & 1) + 8 * (e >> 1);
+      v[h][e] = key < live ? __ldg(reinterpret_cast<const uint4*>(vp + key * 64) + g) : zero4();
+    }
+  float s[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+    mma16816<F16>(s[i], q.a[0], k[i][0].x, k[i][0].y);
+    mma16816<F16>(s[i], q.a[1], k[i][0].z, k[i][0].w);
+    mma16816<F16>(s[i], q.a[2], k[i][1].x, k[i][1].y);
+    mma16816<F16>(s[i], q.a[3], k[i][1].z, k[i][1].w);
+  }
+  uint32_t p[2][4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // a key the row does not see weighs nothing, whatever it holds
+        const float x = 8 * i + 2 * t + e < see[r] ? s[i][2 * r + e] * scale_log2 : -INFINITY;
+        s[i][2 * r + e] = x;
+        mx = fmaxf(mx, x);
+      }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float m_new = fmaxf(st.m[r], mx);
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float corr = ex2_approx(st.m[r] - base);
+    st.m[r] = m_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = ex2_approx(s[i][2 * r] - base), p1 = ex2_approx(s[i][2 * r + 1] - base);
+      sum += p0 + p1;
+      // the weights enter the second product in the cache's 16-bit type (at
+      // most 1, relative error 2^-9 or 2^-12); their sum stays unrounded f32
+      p[i >> 1][(i & 1) * 2 + r] = F16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+    }
+    st.l[r] = fmaf(st.l[r], corr, sum);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      st.o[j][2 * r] *= corr;
+      st.o[j][2 * r + 1] *= corr;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t e0[4] = {v[h][0].x, v[h][0].y, v[h][0].z, v[h][0].w};
+    const uint32_t e1[4] = {v[h][1].x, v[h][1].y, v[h][1].z, v[h][1].w};
+    const uint32_t e2[4] = {v[h][2].x, v[h][2].y, v[h][2].z, v[h][2].w};
+    const uint32_t e3[4] = {v[h][3].x, v[h][3].y, v[h][3].z, v[h][3].w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      mma16816<F16>(st.o[2 * c], p[h], __byte_perm(e0[c], e1[c], 0x5410),
+                    __byte_perm(e2[c], e3[c], 0x5410));
+      mma16816<F16>(st.o[2 * c + 1], p[h], __byte_perm(e0[c], e1[c], 0x7632),
+                    __byte_perm(e2[c], e3[c], 0x7632));
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t q_pair(const SharedParams& p, const void* row, int dim) {
+  if (p.q_dtype == 0) {  // f32 queries are rounded to the cache's type
+    const float2 x = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(row) + dim));
+    return p.kv_dtype == 2 ? pack_f16x2(x.x, x.y) : pack_bf16x2(x.x, x.y);
+  }
+  return __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(row) + dim));
+}
+
+__device__ __forceinline__ const void* q_row(const SharedParams& p, int b, int tok, int h) {
+  const size_t off = static_cast<size_t>(b) * p.q_sb + static_cast<size_t>(tok) * p.q_st +
+                     static_cast<size_t>(h) * p.q_sh;
+  return static_cast<const uint8_t*>(p.q) + off * (p.q_dtype == 0 ? 4 : 2);
+}
+
+// The group whose sequences hold b, or -1: starts[] rises, so it is the last
+// group that starts at or before b, if b is before its end.
+__device__ __forceinline__ int group_of(const SharedParams& p, int b) {
+  int lo = 0, hi = p.groups;
+  while (hi - lo > 0) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(p.group_starts + mid) <= b)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  const int g = lo - 1;
+  return g >= 0 && b < __ldg(p.group_starts + g + 1) ? g : -1;
+}
+
+// Walk a list of pages: steps w, w + kSpWarps, ... of 32 keys each.
+template <int F16>
+__device__ __forceinline__ void walk(RowState& st, const RowQ& q, const SharedParams& p, int kvh,
+                                     const int* table, int len, const int (&see)[2], int warp) {
+  const uint16_t* kpool = static_cast<const uint16_t*>(p.k_pool);
+  const uint16_t* vpool = static_cast<const uint16_t*>(p.v_pool);
+  for (int k0 = warp * kSpKeys; k0 < len; k0 += kSpWarps * kSpKeys) {
+    const int page = __ldg(table + k0 / kPageKeys);
+    if (page < 0 || page >= p.num_pages) {  // not read; its keys weigh nothing
+      if (p.err && threadIdx.x % 32 == 0) atomicOr(p.err, kErrBadArgs);
+      continue;
+    }
+    const size_t off =
+        ((static_cast<size_t>(page) * p.kv_heads + kvh) * kPageKeys + k0 % kPageKeys) * 64;
+    const int rel[2] = {see[0] - k0, see[1] - k0};
+    step32<F16>(st, q, kpool + off, vpool + off, len - k0, rel, p.scale_log2);
+  }
+}
+
+__device__ __forceinline__ void store_out(const SharedParams& p, size_t off, float x) {
+  if (p.out_dtype == 0)
+    static_cast<float*>(p.out)[off] = x;
+  else if (p.out_dtype == 1)
+    static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16(x);
+  else
+    static_cast<__half*>(p.out)[off] = __float2half(x);
+}
+
+constexpr int kSpPitch = 68;  // floats per merged row: m, l, then o[64]
+
+template <int F16>
+__global__ void __launch_bounds__(kSpThreads) shared_rows_kernel(SharedParams p) {
+  __shared__ __align__(16) float s_part[kSpWarps][16][kSpPitch];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+  const int G = p.heads / p.kv_heads, R = p.q_len * G;
+  const int tiles = (R + 15) / 16;
+  const long long id = blockIdx.x;
+  const int tile = static_cast<int>(id % tiles);
+  const int kvh = static_cast<int>(id / tiles % p.kv_heads);
+  const int b = static_cast<int>(id / tiles / p.kv_heads);
+
+  RowQ q;
+  RowState st;
+  const int group = group_of(p, b);
+  int plen = 0;
+  if (group >= 0) {
+    plen = __ldg(p.prefix_lens + group);
+    if (plen < 0 || plen > p.prefix_pages * kPageKeys) {
+      if (p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
+      plen = min(max(plen, 0), p.prefix_pages * kPageKeys);
+    }
+  }
+  int len = __ldg(p.seq_lens + b);
+  if (len < 0 || len > p.max_pages * kPageKeys) {
+    if (p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
+    len = min(max(len, 0), p.max_pages * kPageKeys);
+  }
+  int see[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = tile * 16 + g + 8 * r;
+    const int tok = row / G, h = kvh * G + row % G;
+    const bool real = row < R;
+    see[r] = real ? max(0, len - (p.q_len - 1 - tok)) : 0;
+    const void* src = real ? q_row(p, b, tok, h) : nullptr;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int dim = 32 * (s / 2) + 8 * t + 4 * (s % 2);
+      q.a[s][r] = real ? q_pair(p, src, dim) : 0u;
+      q.a[s][2 + r] = real ? q_pair(p, src, dim + 2) : 0u;
+    }
+    st.m[r] = -INFINITY;
+    st.l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.o[j][2 * r] = st.o[j][2 * r + 1] = 0.f;
+  }
+  if (group >= 0) {
+    const int all[2] = {plen, plen};
+    walk<F16>(st, q, p, kvh, p.prefix_table + static_cast<size_t>(group) * p.prefix_pages, plen,
+              all, warp);
+  }
+  walk<F16>(st, q, p, kvh, p.block_table + static_cast<size_t>(b) * p.max_pages, len, see, warp);
+
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float l = st.l[r];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    float* w = s_part[warp][g + 8 * r];
+    if (t == 0) {
+      w[0] = st.m[r];
+      w[1] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[4 + 16 * t + j] = st.o[j][2 * r];
+      w[4 + 16 * t + 8 + j] = st.o[j][2 * r + 1];
+    }
+  }
+  __syncthreads();
+  // merge: 8 threads a row, 8 head dims each
+  const int row = threadIdx.x / 8, part = threadIdx.x % 8, rr = tile * 16 + row;
+  if (rr >= R) return;
+  float M = -INFINITY, L = 0.f, O[8];
+#pragma unroll
+  for (int w = 0; w < kSpWarps; ++w) M = fmaxf(M, s_part[w][row][0]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) O[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSpWarps; ++w) {
+    const float* x = s_part[w][row];
+    const float f = x[0] == -INFINITY ? 0.f : ex2_approx(x[0] - M);
+    L = fmaf(x[1], f, L);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) O[e] = fmaf(x[4 + 8 * part + e], f, O[e]);
+  }
+  const int tok = rr / G, h = kvh * G + rr % G;
+  const size_t o_row = static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(tok) * p.o_st +
+                       static_cast<size_t>(h) * p.o_sh;
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) store_out(p, o_row + 8 * part + e, O[e] * inv);
+  if (p.lse && part == 0)
+    p.lse[static_cast<size_t>(b) * p.lse_sb + static_cast<size_t>(tok) * p.lse_st +
+          static_cast<size_t>(h) * p.lse_sh] =
+        L > 0.f ? (M + log2f(L)) * 0.69314718055994530942f : -INFINITY;
+}
+
+}  // namespace
+
+cudaError_t launch_shared_rows(const SharedParams& p, cudaStream_t s) {
+  const int R = p.q_len * (p.heads / p.kv_heads);
+  const long long ctas = static_cast<long long>(p.batch) * p.kv_heads * ((R + 15) / 16);
+  if (p.kv_dtype == 2)
+    shared_rows_kernel<1><<<static_cast<unsigned>(ctas), kSpThreads, 0, s>>>(p);
+  else
+    shared_rows_kernel<0><<<static_cast<unsigned>(ctas), kSpThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace ffai

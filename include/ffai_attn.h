@@ -253,6 +253,111 @@ int ffai_kv_copy_pages(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool
                        int32_t num_pages, const int32_t* src_pages, const int32_t* dst_pages,
                        int32_t n, void* stream);
 
+/* ---- attention over a shared prefix ---------------------------------------
+ * The requests or beams of a batch that share a long prefix (a prompt) attend
+ * to it together: its pages are read once for all of them.  Group g is the
+ * consecutive sequences [group_starts[g], group_starts[g + 1]) (device int32,
+ * n_groups + 1, rising; sequences outside every group have no prefix) and
+ * shares the first prefix_lens[g] keys of the pages
+ * prefix_table[g * prefix_pages ..]; sequence b adds the seq_lens[b] keys of
+ * its own pages block_table[b * max_pages ..], the newest q_len of which are
+ * the ones its queries were computed with: query i sees the whole prefix and
+ * own keys j < seq_lens[b] - (q_len - 1 - i).  seq_lens counts own keys only.
+ * All five arrays are DEVICE int32, read on the device.
+ *
+ * q: d->q_len tokens per sequence (1: a decode step), (batch, q_len, heads,
+ * 64) with q_layout TOKEN_MAJOR (token_stride as elsewhere) or (batch, heads,
+ * q_len, 64) with HEADS_SPLIT; q_dtype f32 (rounded to the cache's type) or
+ * the cache's type.  Pools (num_pages, kv_heads, FFAI_PAGE_KEYS, 64) of
+ * kv_dtype bf16 or f16 (f32 pools are FFAI_ATTN_DECLINED); heads a multiple
+ * of kv_heads, query head h reads KV head h / (heads / kv_heads).  o in
+ * out_layout, out_dtype f32, bf16 or f16; softmax weights enter the second
+ * product in the cache's type, sums and accumulators are f32.  lse (optional,
+ * f32): the natural log-sum-exp of a row's scaled logits, (heads, batch *
+ * q_len) for TOKEN_MAJOR output, (batch, heads, q_len) for HEADS_SPLIT.  A row
+ * that sees no key gives zeros and -inf.  What lies in a page behind the last
+ * live key is not used, whatever it is.  d->causal, q_offset, kv_len and the
+ * k/v layouts are ignored, flags must be 0.  Page ids outside the pool or
+ * lengths past a table are not read: ffai_attn_sync then reports
+ * FFAI_ATTN_ERR_INVALID.  No reference counterpart (beams there clone whole
+ * caches, text_decoder.rs:1363-1381). */
+int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,
+                            const void* q, const void* k_pool, const void* v_pool,
+                            int32_t num_pages, const int32_t* group_starts, int32_t n_groups,
+                            const int32_t* prefix_table, const int32_t* prefix_lens,
+                            int32_t prefix_pages, const int32_t* block_table,
+                            const int32_t* seq_lens, int32_t max_pages, void* o, float* lse,
+                            void* stream);
+
+/* ---- page plans and slot maps ----------------------------------------------
+ * The bookkeeping of a paged cache's step on the device, from lengths that
+ * may themselves live there.  All arrays are DEVICE int32.  Request b holds
+ * lens[b] keys and asks for new_tokens[b] more.  free_pages (free_cap) is a
+ * stack of page ids, its top at free_count[0] - 1; pages go out in request
+ * order and land in block_table (batch, max_pages) behind those the request
+ * holds.  The new tokens of all requests are packed in request order: cu_new
+ * (batch + 1) receives their running sum, slots (slot_cap) each token's slot
+ * page * FFAI_PAGE_KEYS + key, positions (optional, slot_cap) its key
+ * position plus pos_base[b] (optional); rows past the last token get -1 and
+ * 0.  A request is refused (no pages, slots -1, positions 0, lens_out = lens)
+ * when it would outgrow max_pages, when the stack cannot cover it and all
+ * requests before it that need pages (one that needs no page is served), or
+ * when its rows pass slot_cap; else lens_out[b] = lens[b] + new_tokens[b].
+ * free_count_out[0]: pages left.  lens, free_count and free_pages are not
+ * written, so a plan can be repeated; lens_out and free_count_out must not
+ * alias them.  batch at most 16384 (else FFAI_ATTN_DECLINED).  Negative
+ * lengths, a bad free_count or a bad page id: refused, and reported by
+ * ffai_attn_sync.  No reference counterpart (Tensor::cat per step,
+ * text_decoder.rs:657-664). */
+int ffai_page_plan(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, int32_t num_pages,
+                   const int32_t* lens, const int32_t* new_tokens, const int32_t* free_pages,
+                   int32_t free_cap, const int32_t* free_count, const int32_t* pos_base,
+                   int32_t* block_table, int32_t* lens_out, int32_t* cu_new, int32_t* slots,
+                   int32_t* positions, int32_t slot_cap, int32_t* free_count_out, void* stream);
+
+/* Requests with done[b] != 0 hand their ceil(lens[b] / FFAI_PAGE_KEYS) pages
+ * back: pushed on free_pages in request order, each request's in key order;
+ * lens_out[b] = 0 for them, lens[b] for the others; free_count_out[0] the new
+ * count.  Pages that would pass free_cap are not pushed, and reported by
+ * ffai_attn_sync. */
+int ffai_page_release(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, const int32_t* lens,
+                      const int32_t* done, const int32_t* block_table, int32_t* free_pages,
+                      int32_t free_cap, const int32_t* free_count, int32_t* lens_out,
+                      int32_t* free_count_out, void* stream);
+
+/* Scatter new keys and values into the pools by slot: k_new, v_new
+ * (n_tokens, d->heads KV heads, 64), rows d->token_stride elements apart
+ * (0: dense), of d->q_dtype (f32, rounded to the pools' type, or the pools'
+ * type), to slots[i] (DEVICE int32; negative: skipped) of pools (num_pages,
+ * d->heads, FFAI_PAGE_KEYS, 64) of d->kv_dtype.  Slots are distinct (two
+ * tokens of one slot leave either's row).  The many-token counterpart of
+ * ffai_kv_append. */
+int ffai_kv_write_slots(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool, void* v_pool,
+                        int32_t num_pages, const void* k_new, const void* v_new,
+                        const int32_t* slots, int32_t n_tokens, void* stream);
+
+/* ---- sampling ----------------------------------------------------------------
+ * One token per row of logits (batch, vocab) of dtype, rows ld elements
+ * apart, from the caller's uniform numbers u[b] in [0, 1).  A row's tokens
+ * are ordered by (logit descending, index ascending); with d = (x - max) *
+ * (1 / temperature) in f32 and whole weights w = floor(2^36 e^d) (e^d in
+ * f32), the tokens kept are the first top_k of them, of those the least
+ * number whose weight reaches top_p of theirs (one at least), and of those
+ * the ones with d >= ln(min_p); the token is the first whose running sum
+ * exceeds u times the kept sum.  All sums are exact, so equal inputs give
+ * equal tokens.  temperature, top_k, top_p, min_p: DEVICE arrays (batch), or
+ * null for 1, off, off, off; per row, temperature <= 0 (or one whose
+ * reciprocal overflows) takes the first maximum, top_k <= 0 or >= vocab,
+ * top_p >= 1 and min_p <= 0 are off.  NaN logits are never chosen; a row with
+ * nothing above -inf gives token -1.  tokens (batch) int32; logprobs
+ * (optional, f32): the token's log-softmax of the logits as they are,
+ * untempered and uncut.  vocab at most 262144 (else FFAI_ATTN_DECLINED).
+ * No reference counterpart (its decoder takes the largest logit on the host). */
+int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtype, int32_t batch,
+                int32_t vocab, const float* u, const float* temperature, const int32_t* top_k,
+                const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
+                void* stream);
+
 /* ---- int8 GEMV ---------------------------------------------------------
  * The reference's block-scaled int8 GEMV (Int8Vocab, vocab_int8.rs), which
  * it runs for the vocabulary projection (text_decoder.rs:945-969) and the
