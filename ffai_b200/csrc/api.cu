@@ -86,6 +86,9 @@ struct ffai_attn_ctx {
   // int8 GEMV: quantised activations and their scales, between its two kernels
   uint8_t* d_gemv_x = nullptr;
   size_t gemv_x_cap = 0;
+  // shared prefix: partial results between its two kernels
+  float* d_prefix = nullptr;
+  size_t prefix_cap = 0;
   ffai_attn_ctx* pipe_ctx = nullptr;  // inner context used for the pipeline's kernels
   std::string last_error;
   int last_status = FFAI_ATTN_OK;
@@ -731,6 +734,7 @@ void ffai_attn_destroy(ffai_attn_ctx* ctx) {
   cudaFree(ctx->d_stage);
   cudaFree(ctx->d_pipe);
   cudaFree(ctx->d_gemv_x);
+  cudaFree(ctx->d_prefix);
   for (int i = 0; i < 2; ++i) {
     if (ctx->ev_h2d[i]) cudaEventDestroy(ctx->ev_h2d[i]);
     if (ctx->ev_comp[i]) cudaEventDestroy(ctx->ev_comp[i]);
@@ -1275,8 +1279,9 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
       return set_error(ctx, FFAI_ATTN_ERR_INVALID, "shared prefix: operands 16-byte aligned");
   const long long rows = static_cast<long long>(d->q_len) * (d->heads / kv_heads);
-  if (rows > (1 << 30) ||
-      static_cast<double>(d->batch) * kv_heads * ((rows + 15) / 16) > 2147483647.0)
+  if (static_cast<double>(d->batch) * rows > (1 << 30) ||
+      static_cast<double>(d->batch) * kv_heads * ((rows + 15) / 16) > 2147483647.0 ||
+      static_cast<double>(num_pages) * kv_heads > 2147483647.0)
     return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows");
   SharedParams p{};
   p.q = q;
@@ -1313,6 +1318,28 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
   p.err = ctx->d_err;
   DeviceGuard g(ctx->device);
   ProfScope ps(ctx, FFAI_OP_DECODE, static_cast<cudaStream_t>(stream), "ffai_attn_shared_prefix");
+  if (n_groups > 0) {
+    // Partial slots: one per CTA and one per tile bound them (prefix_tc.cu).
+    const long long tiles =
+        kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + 127) / 128);
+    const long long blocks = tiles * ((prefix_pages + 1) / 2);
+    const int grid = static_cast<int>(std::min<long long>(ctx->num_sms, blocks));
+    p.part_slots = grid + tiles;
+    const size_t floats = static_cast<size_t>(p.part_slots) * 128 * 66;
+    const size_t plan = (1 + 2 * static_cast<size_t>(n_groups)) * 2;  // 64-bit words, in floats
+    int st = ensure(ctx, &ctx->d_prefix, &ctx->prefix_cap, floats + plan + 4);
+    if (st) return st;
+    p.part_plan = reinterpret_cast<long long*>(ctx->d_prefix);
+    p.part_ml = ctx->d_prefix + (plan + 3) / 4 * 4;
+    p.part_o = p.part_ml + static_cast<size_t>(p.part_slots) * 128 * 2;
+    CUtensorMap tmk, tmv;
+    const long long heads = static_cast<long long>(num_pages) * kv_heads;
+    st = make_map(ctx, &tmk, k_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
+    if (st) return st;
+    st = make_map(ctx, &tmv, v_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
+    if (st) return st;
+    FFAI_CUDA(ctx, launch_prefix_tc(tmk, tmv, p, grid, static_cast<cudaStream_t>(stream)));
+  }
   FFAI_CUDA(ctx, launch_shared_rows(p, static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }

@@ -13,8 +13,7 @@
 // merge at the end.  K and V go from global memory straight into the operand
 // registers: the products' inner order is free, so it is chosen such that
 // each lane's operands are whole 16-byte pieces of the key rows.
-#include "common.cuh"
-#include "kernels.h"
+#include "shared_prefix.cuh"
 
 namespace ffai {
 
@@ -189,6 +188,53 @@ __device__ __forceinline__ void walk(RowState& st, const RowQ& q, const SharedPa
   }
 }
 
+// Fold the prefix kernel's partials into the rows' states: warp w takes parts
+// w, w + kSpWarps, ... of each of its rows.
+__device__ __forceinline__ void fold_partials(RowState& st, const SharedParams& p, int group, int b,
+                                              int kvh, int tile, int R, int warp) {
+  const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+  const GroupDims d = group_dims(p, group);
+  if (d.nb == 0) return;
+  // written by the preceding kernel, which may have run beside this one
+  const long long share = __ldcg(p.part_plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
+                  tile0 = __ldcg(p.part_plan + 2 + 2 * group);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = tile * 16 + g + 8 * r;
+    if (row >= R) continue;
+    const int rg = (b - d.b0) * R + row;
+    const long long at = static_cast<long long>(kvh) * d.mt + rg / 128;
+    const long long l0 = lin0 + at * d.nb;
+    const long long c0 = l0 / share, c1 = (l0 + d.nb - 1) / share;
+    for (long long c = c0 + warp; c <= c1; c += kSpWarps) {
+      const long long slot = c + tile0 + at;
+      if (slot >= p.part_slots) break;
+      const size_t pr = static_cast<size_t>(slot) * 128 + rg % 128;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + pr);
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + pr * 64 + 16 * t);
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 f = __ldcg(src + i);
+        x[4 * i] = f.x;
+        x[4 * i + 1] = f.y;
+        x[4 * i + 2] = f.z;
+        x[4 * i + 3] = f.w;
+      }
+      const float M = fmaxf(st.m[r], ml.x);
+      const float f0 = st.m[r] == -INFINITY ? 0.f : ex2_approx(st.m[r] - M);
+      const float f1 = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M);
+      st.m[r] = M;
+      st.l[r] = st.l[r] * f0 + (t == 0 ? ml.y * f1 : 0.f);  // lanes' sums are added later
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        st.o[j][2 * r] = st.o[j][2 * r] * f0 + x[j] * f1;
+        st.o[j][2 * r + 1] = st.o[j][2 * r + 1] * f0 + x[8 + j] * f1;
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ void store_out(const SharedParams& p, size_t off, float x) {
   if (p.out_dtype == 0)
     static_cast<float*>(p.out)[off] = x;
@@ -246,12 +292,15 @@ __global__ void __launch_bounds__(kSpThreads) shared_rows_kernel(SharedParams p)
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.o[j][2 * r] = st.o[j][2 * r + 1] = 0.f;
   }
-  if (group >= 0) {
+  walk<F16>(st, q, p, kvh, p.block_table + static_cast<size_t>(b) * p.max_pages, len, see, warp);
+  if (p.part_o) {
+    griddep_wait();  // the prefix kernel's partials
+    if (group >= 0) fold_partials(st, p, group, b, kvh, tile, R, warp);
+  } else if (group >= 0) {
     const int all[2] = {plen, plen};
     walk<F16>(st, q, p, kvh, p.prefix_table + static_cast<size_t>(group) * p.prefix_pages, plen,
               all, warp);
   }
-  walk<F16>(st, q, p, kvh, p.block_table + static_cast<size_t>(b) * p.max_pages, len, see, warp);
 
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -303,11 +352,18 @@ __global__ void __launch_bounds__(kSpThreads) shared_rows_kernel(SharedParams p)
 cudaError_t launch_shared_rows(const SharedParams& p, cudaStream_t s) {
   const int R = p.q_len * (p.heads / p.kv_heads);
   const long long ctas = static_cast<long long>(p.batch) * p.kv_heads * ((R + 15) / 16);
-  if (p.kv_dtype == 2)
-    shared_rows_kernel<1><<<static_cast<unsigned>(ctas), kSpThreads, 0, s>>>(p);
-  else
-    shared_rows_kernel<0><<<static_cast<unsigned>(ctas), kSpThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  // Behind the prefix kernel it is a programmatic dependent: sequences' own
+  // keys are attended while the last prefix tiles finish.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kSpThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.part_o ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, p.kv_dtype == 2 ? shared_rows_kernel<1> : shared_rows_kernel<0>, p);
 }
 
 }  // namespace ffai
