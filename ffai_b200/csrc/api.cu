@@ -1319,19 +1319,23 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
   DeviceGuard g(ctx->device);
   ProfScope ps(ctx, FFAI_OP_DECODE, static_cast<cudaStream_t>(stream), "ffai_attn_shared_prefix");
   if (n_groups > 0) {
-    // Partial slots: one per CTA and one per tile bound them (prefix_tc.cu).
-    const long long tiles =
-        kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + 127) / 128);
-    const long long blocks = tiles * ((prefix_pages + 1) / 2);
-    const int grid = static_cast<int>(std::min<long long>(ctx->num_sms, blocks));
-    p.part_slots = grid + tiles;
-    const size_t floats = static_cast<size_t>(p.part_slots) * 128 * 66;
-    const size_t plan = (1 + 2 * static_cast<size_t>(n_groups)) * 2;  // 64-bit words, in floats
-    int st = ensure(ctx, &ctx->d_prefix, &ctx->prefix_cap, floats + plan + 4);
+    // Partial slots: slot = CTA + segment.  Chunks are no shorter than a CTA's
+    // share but for each unit's last, or half that where a unit has one tile,
+    // so there are at most 2 * grid + units segments.
+    const long long units =
+        kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + kPxRows - 1) / kPxRows);
+    const long long steps = units * ((prefix_pages + 1) / 2);
+    if (steps > INT32_MAX / 2)
+      return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows and keys");
+    const int grid = static_cast<int>(std::min<long long>(ctx->num_sms, steps));
+    p.part_slots = static_cast<int>(3 * grid + units);
+    const size_t floats = static_cast<size_t>(p.part_slots) * kPxRows * 66;
+    const size_t plan = (1 + 2 * static_cast<size_t>(n_groups) + 3) / 4 * 4;  // words
+    int st = ensure(ctx, &ctx->d_prefix, &ctx->prefix_cap, floats + plan);
     if (st) return st;
-    p.part_plan = reinterpret_cast<long long*>(ctx->d_prefix);
-    p.part_ml = ctx->d_prefix + (plan + 3) / 4 * 4;
-    p.part_o = p.part_ml + static_cast<size_t>(p.part_slots) * 128 * 2;
+    p.part_plan = reinterpret_cast<int*>(ctx->d_prefix);
+    p.part_ml = ctx->d_prefix + plan;
+    p.part_o = p.part_ml + static_cast<size_t>(p.part_slots) * kPxRows * 2;
     CUtensorMap tmk, tmv;
     const long long heads = static_cast<long long>(num_pages) * kv_heads;
     st = make_map(ctx, &tmk, k_pool, false, 0, kPageKeys, heads, 0, kPageKeys);

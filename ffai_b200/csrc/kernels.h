@@ -345,15 +345,17 @@ struct SharedParams {
   float* lse;  // or null
   long long lse_sb, lse_st, lse_sh;
   unsigned* err;
-  // partial results of prefix_tc_kernel, part_slots slots of 128 rows: output
+  // partial results of prefix_tc_kernel, part_slots slots of kPxRows rows: output
   // sums (64 f32), running maximum (log2 domain) and weight sum; null when
   // the rows kernel walks the prefixes itself
   float* part_o;
   float* part_ml;
-  long long part_slots;
-  long long* part_plan;  // pairs per CTA, then each group's first pair and tile
+  int part_slots;
+  int* part_plan;  // steps per CTA, then each group's first step and segment
 };
 cudaError_t launch_shared_rows(const SharedParams& p, cudaStream_t s);
+constexpr int kPxRows = 256;  // query rows per unit of the prefix kernel
+constexpr int kPxKeys = 128;  // keys per block (two pages)
 // tm*: 3-d maps over a pool's (64, 64 keys, num_pages * kv_heads), boxes of one page's head
 cudaError_t launch_prefix_tc(const CUtensorMap& tmK, const CUtensorMap& tmV, const SharedParams& p,
                              int grid, cudaStream_t s);

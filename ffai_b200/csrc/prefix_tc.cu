@@ -1,27 +1,27 @@
 // The shared part of ffai_attn_shared_prefix on the tensor cores: all query
-// rows of a group against the group's prefix, read once per 128 rows.
+// rows of a group against the group's prefix, whose keys are read once for up
+// to 256 rows.
 //
 // A group of s sequences has s * q_len * G query rows per KV head (G = query
-// heads per KV head); they form tiles of 128 rows, the M of tcgen05.mma.  The
-// prefix is cut into blocks of 128 keys (two pages).  All (tile, block) pairs
-// of all groups and heads are laid out on one line, W of them, tile after
-// tile, and CTA c takes the pairs [c S, (c + 1) S), S = ceil(W / CTAs): every
-// CTA gets the same number of key blocks whatever the lengths and group
-// sizes, and a tile that spans CTAs leaves one partial result (running
-// maximum, sum, unnormalised output) per CTA, merged by shared_rows_kernel.
-// The partial of CTA c for tile t lies in slot c + t: along the line either
-// c or t grows from one partial to the next, so slots are distinct.
+// heads per KV head), in units of 256: two tiles of 128, the M of tcgen05.mma.
+// The prefix is cut into blocks of 128 keys (two pages).  The steps of all
+// units of all groups and heads are laid out on one line, W of them
+// (shared_prefix.cuh), and CTA c takes the steps [c S, (c + 1) S), S = ceil(W /
+// CTAs): every CTA gets the same work whatever the lengths and group sizes.
+// What a CTA holds of a segment (same rows, consecutive blocks) leaves one
+// partial result (running maximum, sum, unnormalised output), merged by
+// shared_rows_kernel.  The partial of CTA c for segment t lies in slot c + t:
+// along the line either c or t grows from one partial to the next, so slots
+// are distinct.
 //
-// Per CTA: warp 16 streams the pages through a 4-stage ring of K and V
-// blocks by TMA; blocks alternate between two chains (t = 0, 1), each with an
-// MMA warp (17, 18), scores, weights and an output accumulator of its own in
-// tensor memory and 8 softmax warps, so one chain's softmax runs beside the
-// other's products.  At the end of a tile chain 1 hands its accumulator to
-// chain 0 through shared memory, warp to warp.
-//
-// Bound: a block is 32 KB of HBM traffic for up to 128 rows; at 1/148 of the
-// measured copy rate that is 0.75 us, and a chain pair needs about as long for
-// two 128 x 128 softmax blocks, so up to 128 rows the kernel streams.
+// Per CTA: warp 16 streams the pages through a 4-stage ring of K and V blocks
+// by TMA for two chains (t = 0, 1), each with an MMA warp (17, 18), scores,
+// weights and an output accumulator of its own in tensor memory and 8 softmax
+// warps, so one chain's softmax runs beside the other's products.  With more
+// than 128 rows in the unit chain t takes tile t and both take every block;
+// else both hold the one tile and take the blocks in turn (chain 0 the even
+// ones), and at the end chain 1 hands its accumulator to chain 0 through shared
+// memory, warp to warp.
 //
 // Every wait is bounded (common.cuh); on a timeout the CTA raises an error
 // bit, drains its copies and MMAs, frees tensor memory and exits.
@@ -41,6 +41,29 @@ constexpr uint32_t kPxPage = kPageKeys * 128; // a page's rows of one head
 constexpr uint32_t kPxTmem = 512;
 constexpr uint32_t kPxS = 0, kPxP = 256, kPxO = 384;  // + 128 t, + 64 t, + 64 t
 
+// A walk over a CTA's stretch of the line, segment by segment.
+struct Walk {
+  GroupDims d;
+  int g, h, q, m;  // group, KV head, chunk, unit
+  int cl, len;     // key blocks of a chunk, and of this one
+  int steps, step; // steps of this unit over the chunk, and the current one
+  int left;        // steps left, the current one included
+  int nth;         // segments of this CTA before this one
+  int seg;         // index of the segment on the line
+  int base;        // key blocks of this CTA before this segment
+  int alt;         // one-tile segments of this CTA before this one
+};
+__device__ __forceinline__ bool walk_pair(const Walk& w) { return !(w.d.single && w.m == w.d.mu - 1); }
+// What this CTA has of the current segment: steps, key blocks, the first block.
+__device__ __forceinline__ int walk_steps(const Walk& w) { return min(w.left, w.steps - w.step); }
+__device__ __forceinline__ int walk_blocks(const Walk& w) {
+  const int n = walk_steps(w);
+  return walk_pair(w) ? n : min(2 * n, w.len - 2 * w.step);
+}
+__device__ __forceinline__ int walk_first(const Walk& w) {
+  return w.q * w.cl + (walk_pair(w) ? w.step : 2 * w.step);
+}
+
 struct __align__(8) PxBars {
   uint64_t q_full[2];
   uint64_t k_full[kPxStages], v_full[kPxStages], kv_empty[kPxStages];
@@ -49,54 +72,47 @@ struct __align__(8) PxBars {
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
-  // this CTA's stretch of the line
-  long long total;
-  int start_group, left;
-  long long start_off, start_tile;
+  int share;
+  Walk start;  // this CTA's stretch
 };
 
-constexpr size_t kPxTiles = (2 + 2 * kPxStages) * kPxTile;
-constexpr size_t kPxMerge = 8 * (32 * 32 + 64) * sizeof(float);
-constexpr size_t kPxSmem = kPxTiles + kPxMerge + sizeof(PxBars) + 1024;
+// Shared memory, at fixed offsets from its 1024-byte aligned start (which the
+// kernel checks), so that no pointer into it takes a register.
+constexpr uint32_t kPxOffK = 2 * kPxTile;  // after the chains' query tiles
+constexpr uint32_t kPxOffV = kPxOffK + kPxStages * kPxTile;
+constexpr uint32_t kPxOffMerge = kPxOffV + kPxStages * kPxTile;
+constexpr uint32_t kPxMergeFloats = 32 * 32 + 64;  // per pair of warps
+constexpr uint32_t kPxOffWalks = kPxOffMerge + 8 * kPxMergeFloats * sizeof(float);
+constexpr uint32_t kPxOffBars = kPxOffWalks + 16 * sizeof(Walk);
+constexpr size_t kPxSmem = kPxOffBars + sizeof(PxBars);
+static_assert(sizeof(Walk) % 4 == 0 && kPxOffBars % 8 == 0 && kPxSmem <= 227 * 1024, "shared memory");
+extern __shared__ __align__(1024) uint8_t px_smem[];
+#define PX_BARS (reinterpret_cast<PxBars*>(px_smem + kPxOffBars))
 
-// The pairs of a CTA's stretch, one after another.  Every role walks its own.
-struct Walker {
-  const SharedParams& p;
-  GroupDims d;
-  int g, h, m, blk;  // group, KV head, row tile, key block
-  int left;          // pairs left, the current one included
-  int seg;           // tiles entered before this one (of this CTA)
-  long long tile;    // index of the tile on the line
-  __device__ __forceinline__ Walker(const SharedParams& params, const PxBars* bars) : p(params) {
-    g = bars->start_group;
-    left = bars->left;
-    seg = 0;
-    tile = bars->start_tile;
-    if (left > 0) {
-      d = group_dims(p, g);
-      const long long t = bars->start_off / d.nb;
-      blk = static_cast<int>(bars->start_off - t * d.nb);
-      h = static_cast<int>(t / d.mt);
-      m = static_cast<int>(t - static_cast<long long>(h) * d.mt);
+// To the next segment, if the stretch goes on.
+__device__ __forceinline__ void walk_next(Walk& w, const SharedParams& p) {
+  w.base += walk_blocks(w);
+  w.alt += walk_pair(w) ? 0 : 1;
+  w.left -= walk_steps(w);
+  if (w.left <= 0) return;  // else the segment is done
+  w.step = 0;
+  ++w.nth;
+  ++w.seg;
+  if (++w.m == w.d.mu) {
+    w.m = 0;
+    if (++w.q * w.cl >= w.d.nb) {
+      w.q = 0;
+      if (++w.h == p.kv_heads) {
+        w.h = 0;
+        do w.d = group_dims(p, ++w.g);
+        while (w.d.nb == 0);
+        w.cl = chunk_blocks(w.d, PX_BARS->share);
+      }
     }
+    w.len = min(w.cl, w.d.nb - w.q * w.cl);
   }
-  __device__ __forceinline__ int stretch() const { return min(left, d.nb - blk); }
-  // Step over `n` pairs of the current tile.
-  __device__ __forceinline__ void skip(int n) {
-    left -= n;
-    blk += n;
-    if (left <= 0 || blk < d.nb) return;
-    blk = 0;
-    ++seg;
-    ++tile;
-    if (++m < d.mt) return;
-    m = 0;
-    if (++h < p.kv_heads) return;
-    h = 0;
-    do d = group_dims(p, ++g);
-    while (d.nb == 0);
-  }
-};
+  w.steps = unit_steps(w.d, w.m, w.len);
+}
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                           unsigned* err, unsigned code) {
@@ -104,17 +120,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, ok);
 }
 
-// One warp: lengths of the line and where this CTA starts on it.  CTA 0 also
-// leaves each group's first pair and tile, and S, for the merge.
-__device__ __forceinline__ void find_stretch(const SharedParams& p, PxBars* bars) {
+// One warp: the length of the line and where this CTA starts on it.  CTA 0
+// also leaves each group's first step and segment, and S, for the merge.
+__device__ __forceinline__ void find_stretch(const SharedParams& p) {
+  PxBars* bars = PX_BARS;
   const int lane = threadIdx.x % 32;
-  long long total = 0;
+  int total = 0;
+#pragma unroll 1
   for (int base = 0; base < p.groups; base += 32) {
     const int g = base + lane;
-    long long n = 0;
+    int n = 0;
     if (g < p.groups) {
       const GroupDims d = group_dims(p, g);
-      n = static_cast<long long>(p.kv_heads) * d.mt * d.nb;
+      n = p.kv_heads * head_steps(d, d.nb);
       if (blockIdx.x == 0 && p.err) {
         const int raw = __ldg(p.prefix_lens + g);
         const int s0 = __ldg(p.group_starts + g), s1 = __ldg(p.group_starts + g + 1);
@@ -122,63 +140,84 @@ __device__ __forceinline__ void find_stretch(const SharedParams& p, PxBars* bars
           atomicOr(p.err, kErrBadArgs);
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total += n;
+    total += __reduce_add_sync(0xffffffffu, n);
   }
-  const long long share = (total + gridDim.x - 1) / gridDim.x;
-  const long long first = blockIdx.x * share;
-  const long long end = min(total, first + share);
+  const int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int first = static_cast<int>(blockIdx.x) * share;
+  const int left = min(total, first + share) - first;
   if (lane == 0) {
-    bars->left = first < end ? static_cast<int>(end - first) : 0;
+    bars->share = share;
+    bars->start.left = left;
     if (blockIdx.x == 0) p.part_plan[0] = share;
   }
-  long long lin = 0, tiles = 0;
+  int lin = 0, segs = 0;
+#pragma unroll 1
   for (int base = 0; base < p.groups; base += 32) {
     const int g = base + lane;
-    long long n = 0, t = 0;
+    int n = 0, t = 0, cl = 1;
+    GroupDims d{};
     if (g < p.groups) {
-      const GroupDims d = group_dims(p, g);
-      t = d.nb > 0 ? static_cast<long long>(p.kv_heads) * d.mt : 0;
-      n = t * d.nb;
+      d = group_dims(p, g);
+      if (d.nb > 0) {
+        cl = chunk_blocks(d, share);
+        t = p.kv_heads * d.mu * ((d.nb + cl - 1) / cl);
+        n = p.kv_heads * head_steps(d, d.nb);
+      }
     }
-    long long ni = n, ti = t;
+    int ni = n, ti = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long a = __shfl_up_sync(0xffffffffu, ni, o), b = __shfl_up_sync(0xffffffffu, ti, o);
+      const int a = __shfl_up_sync(0xffffffffu, ni, o), b = __shfl_up_sync(0xffffffffu, ti, o);
       if (lane >= o) {
         ni += a;
         ti += b;
       }
     }
-    const long long l0 = lin + ni - n, t0 = tiles + ti - t;
+    const int l0 = lin + ni - n, t0 = segs + ti - t;
     if (g < p.groups && blockIdx.x == 0) {
       p.part_plan[1 + 2 * g] = l0;
       p.part_plan[2 + 2 * g] = t0;
     }
-    if (first < end && n > 0 && l0 <= first && first < l0 + n) {  // one lane, once
-      bars->start_group = g;
-      bars->start_off = first - l0;
-      bars->start_tile = t0 + (first - l0) / (n / t);
+    if (left > 0 && l0 <= first && first < l0 + n) {  // one lane, once
+      Walk w;
+      w.d = d;
+      w.g = g;
+      w.cl = cl;
+      int rest = first - l0;
+      const int per_head = head_steps(d, d.nb), per_chunk = head_steps(d, cl);
+      w.h = rest / per_head;
+      rest -= w.h * per_head;
+      w.q = rest / per_chunk;
+      rest -= w.q * per_chunk;
+      w.len = min(cl, d.nb - w.q * cl);
+      w.m = min(rest / w.len, d.mu - 1);
+      w.step = rest - w.m * w.len;
+      w.steps = unit_steps(d, w.m, w.len);
+      w.left = left;
+      w.nth = w.base = w.alt = 0;
+      w.seg = t0 + (w.h * ((d.nb + cl - 1) / cl) + w.q) * d.mu + w.m;
+      bars->start = w;
     }
     lin += __shfl_sync(0xffffffffu, ni, 31);
-    tiles += __shfl_sync(0xffffffffu, ti, 31);
+    segs += __shfl_sync(0xffffffffu, ti, 31);
   }
 }
 
 // ---------------------------------------------------------------- producer
 __device__ __forceinline__ void px_producer(const CUtensorMap* tmK, const CUtensorMap* tmV,
-                                            const SharedParams& p, uint8_t* sK, uint8_t* sV,
-                                            PxBars* bars) {
+                                            const SharedParams& p) {
+  PxBars* bars = PX_BARS;
+  uint8_t* sK = px_smem + kPxOffK;
+  uint8_t* sV = px_smem + kPxOffV;
   volatile int* abort_flag = &bars->abort_flag;
   const int lane = threadIdx.x % 32;
-  Walker w(p, bars);
+  Walk w = bars->start;
   uint32_t it = 0;
   bool ok = true;
   while (ok && w.left > 0) {
     const int* table = p.prefix_table + static_cast<size_t>(w.g) * p.prefix_pages;
     const int n_pages = (w.d.plen + kPageKeys - 1) / kPageKeys;
-    const int b0 = w.blk, b1 = w.blk + w.stretch();
+    const int b0 = walk_first(w), b1 = b0 + walk_blocks(w);
     for (int base = b0; ok && base < b1; base += 16) {
       // the page ids of the next 16 blocks, one per lane
       const int pg = 2 * base + lane;
@@ -211,7 +250,7 @@ __device__ __forceinline__ void px_producer(const CUtensorMap* tmK, const CUtens
                         p1 * p.kv_heads + w.h);
       }
     }
-    w.skip(b1 - b0);
+    walk_next(w, p);
   }
   if (!ok || *abort_flag) {  // every copy lands before the CTA exits
     int none = 0;
@@ -224,36 +263,36 @@ __device__ __forceinline__ void px_producer(const CUtensorMap* tmK, const CUtens
 }
 
 // ---------------------------------------------------------------- MMA issuers
-// Chain t takes the blocks it (counted over the CTA's stretch) with it % 2 ==
-// t.  The scores of its next block are issued before the second product of
-// the current one, within a tile and across tiles.
+// The key blocks of chain t, `it` counted over the CTA's stretch: in a pair
+// unit every block, else every second.  The scores of its next block are
+// issued before the second product of the current one within a segment.
 struct ChainBlock {
   uint32_t it;
-  int seg;
-  bool first;  // of this chain's blocks in the tile
+  int nth;     // segment
+  bool first;  // of this chain's blocks in the segment
+  bool alone;  // the other chain does not take this block
 };
 
 struct ChainWalk {
-  Walker w;
-  int t, pos;    // pos: blocks of the current tile's stretch passed by this chain
-  uint32_t base; // it of the current tile's first block
-  __device__ __forceinline__ ChainWalk(const SharedParams& p, const PxBars* bars, int chain)
-      : w(p, bars), t(chain), pos(0), base(0) {}
+  const SharedParams& p;
+  Walk w;
+  int t, pos;  // pos: this chain's blocks of the current segment so far
+  __device__ __forceinline__ ChainWalk(const SharedParams& params, int chain)
+      : p(params), w(PX_BARS->start), t(chain), pos(0) {}
   // The chain's next block, or false at the end of the stretch.
   __device__ __forceinline__ bool next(ChainBlock& b) {
     while (w.left > 0) {
-      const int n = w.stretch();
-      const int off = static_cast<int>((base ^ static_cast<uint32_t>(t)) & 1u);  // first of this chain
-      const int j = off + 2 * pos;
-      if (j < n) {
-        b.it = base + j;
-        b.seg = w.seg;
+      const bool pair = walk_pair(w);
+      const int j = pair ? pos : 2 * pos + t;
+      if (j < walk_blocks(w)) {
+        b.it = static_cast<uint32_t>(w.base + j);
+        b.nth = w.nth;
         b.first = pos == 0;
+        b.alone = !pair;
         ++pos;
         return true;
       }
-      w.skip(n);
-      base += n;
+      walk_next(w, p);
       pos = 0;
     }
     return false;
@@ -261,25 +300,27 @@ struct ChainWalk {
 };
 
 template <int F16>
-__device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint8_t* sQ, uint8_t* sK,
-                                       uint8_t* sV, uint32_t tmem, PxBars* bars) {
+__device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint32_t tmem) {
+  PxBars* bars = PX_BARS;
+  uint8_t* sQ = px_smem;
+  uint8_t* sK = px_smem + kPxOffK;
+  uint8_t* sV = px_smem + kPxOffV;
   volatile int* abort_flag = &bars->abort_flag;
   constexpr uint32_t idesc_s = idesc_f16(F16 ? 0u : 1u, 128, 128, 0, 0);
   constexpr uint32_t idesc_o = idesc_f16(F16 ? 0u : 1u, 128, 64, 0, 1);
-  ChainWalk walk(p, bars, t);
+  ChainWalk walk(p, t);
   uint32_t n_s = 0, n_pv = 0;
   auto issue_s = [&](const ChainBlock& b) -> bool {
     const uint32_t s = b.it % kPxStages;
     if (!warp_wait(&bars->k_full[s], (b.it / kPxStages) & 1, abort_flag, p.err, kErrTimeoutMma))
       return false;
-    if (b.first && !warp_wait(&bars->q_full[b.seg & 1], (b.seg >> 1) & 1, abort_flag, p.err,
-                              kErrTimeoutMma))
+    if (b.first && !warp_wait(&bars->q_full[t], b.nth & 1, abort_flag, p.err, kErrTimeoutMma))
       return false;
     if (n_s > 0 &&
         !warp_wait(&bars->sc_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutMma))
       return false;
     tc_fence_after();
-    const uint64_t dq = smem_desc_sw128(smem_u32(sQ + (b.seg & 1) * kPxTile), 16, 1024);
+    const uint64_t dq = smem_desc_sw128(smem_u32(sQ + t * kPxTile), 16, 1024);
     const uint64_t dk = smem_desc_sw128(smem_u32(sK + s * kPxTile), 16, 1024);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -293,8 +334,8 @@ __device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint8_t* sQ
   if (!issue_s(cur)) return;
   while (true) {
     const bool more = walk.next(nxt);
-    // Within a tile the next scores go first; across tiles the last product
-    // does, since the tile's epilogue waits for it.
+    // Within a segment the next scores go first; across segments the last
+    // product does, since the segment's epilogue waits for it.
     const bool ahead = more && !nxt.first;
     if (ahead && !issue_s(nxt)) return;
     const uint32_t s = cur.it % kPxStages;
@@ -309,6 +350,7 @@ __device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint8_t* sQ
                (!cur.first || k > 0) ? 1u : 0u);
     mma_commit_w(&bars->o_done[t]);
     mma_commit_w(&bars->kv_empty[s]);
+    if (cur.alone) mma_commit_w(&bars->kv_empty[s]);  // it takes two
     ++n_pv;
     if (!more) return;
     if (!ahead && !issue_s(nxt)) return;
@@ -325,87 +367,97 @@ __device__ __forceinline__ int mma_row(int r) {
   return 32 * (c & 3) + 16 * (c >> 2) + (r & 15);
 }
 
-// The tile's query rows into swizzled shared memory: 512 threads, each two
-// 16-byte pieces (8 head dims).  Rows past the tile's end are zero.
-__device__ __forceinline__ void load_q(const SharedParams& p, const Walker& w, uint8_t* dst) {
+// Query rows [row0, row0 + rows) of the unit's group and head into swizzled
+// shared memory, zeros behind them: 256 threads, four 16-byte pieces (8 head
+// dims) each.  Rolled, with copies that hold no register: the code runs once a
+// segment, and what it costs is fetching its instructions.
+__device__ __forceinline__ void load_q(const SharedParams& p, const Walk& w, int row0, int rows,
+                                       uint8_t* dst) {
   const int G = p.heads / p.kv_heads, R = p.q_len * G;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int piece = threadIdx.x + i * 512;
-    const int r = piece >> 3, c = piece & 7;
-    const int row = w.m * 128 + r;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row < w.d.rows) {
-      const int b = w.d.b0 + row / R, rr = row % R;
-      const int tok = rr / G, h = w.h * G + rr % G;
-      const size_t off = static_cast<size_t>(b) * p.q_sb + static_cast<size_t>(tok) * p.q_st +
-                         static_cast<size_t>(h) * p.q_sh + c * 8;
-      if (p.q_dtype == 0) {  // f32 queries are rounded to the cache's type
-        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + off);
-        const float4 a = __ldg(src), e = __ldg(src + 1);
-        x = p.kv_dtype == 2 ? make_uint4(pack_f16x2(a.x, a.y), pack_f16x2(a.z, a.w),
-                                         pack_f16x2(e.x, e.y), pack_f16x2(e.z, e.w))
-                            : make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w),
-                                         pack_bf16x2(e.x, e.y), pack_bf16x2(e.z, e.w));
-      } else {
-        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + off));
-      }
-    }
+  const int c = threadIdx.x & 7;
+#pragma unroll 1
+  for (int r = (threadIdx.x & 255) >> 3; r < 128; r += 32) {
+    const bool have = r < rows;
+    const int row = have ? row0 + r : row0;
+    const int b = row / R, rr = row - b * R, tok = rr / G, h = w.h * G + rr - tok * G;
+    const size_t off = static_cast<size_t>(w.d.b0 + b) * p.q_sb + static_cast<size_t>(tok) * p.q_st +
+                       static_cast<size_t>(h) * p.q_sh + c * 8;
     const int mr = mma_row(r);
-    *reinterpret_cast<uint4*>(dst + mr * 128 + ((c ^ (mr & 7)) << 4)) = x;
+    uint8_t* to = dst + mr * 128 + ((c ^ (mr & 7)) << 4);
+    if (p.q_dtype == 0) {  // f32 queries are rounded to the cache's type
+      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + off);
+      const float4 a = __ldg(src), e = __ldg(src + 1);
+      uint4 x = p.kv_dtype == 2 ? make_uint4(pack_f16x2(a.x, a.y), pack_f16x2(a.z, a.w),
+                                             pack_f16x2(e.x, e.y), pack_f16x2(e.z, e.w))
+                                : make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w),
+                                             pack_bf16x2(e.x, e.y), pack_bf16x2(e.z, e.w));
+      *reinterpret_cast<uint4*>(to) = have ? x : make_uint4(0, 0, 0, 0);
+    } else {
+      cp_async16(to, static_cast<const uint16_t*>(p.q) + off, have);
+    }
   }
+  cp_async_wait_all();
 }
 
 template <int F16>
-__device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem, uint8_t* sQ,
-                                           uint8_t* sV, float* s_merge, PxBars* bars) {
+__device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem) {
+  PxBars* bars = PX_BARS;
+  uint8_t* sQ = px_smem;
+  uint8_t* sV = px_smem + kPxOffV;
+  float* s_merge = reinterpret_cast<float*>(px_smem + kPxOffMerge);
+  Walk& w = *(reinterpret_cast<Walk*>(px_smem + kPxOffWalks) + threadIdx.x / 32);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int t = warp / 8, c = warp % 8;
   const int lb = 32 * (c % 4) + 16 * (c / 4);
   const int t0 = lane & 3, t1 = lane >> 2;
-  const uint32_t lane_addr = static_cast<uint32_t>(lb) << 16;
-  const uint32_t tS = tmem + lane_addr + kPxS + t * 128;
-  const uint32_t tP = tmem + lane_addr + kPxP + t * 64;
-  const uint32_t tO = tmem + lane_addr + kPxO + t * 64;
-  const float sl2 = p.scale_log2;
-  float* mbuf = s_merge + c * (32 * 32 + 64);
-  uint32_t n_s = 0;   // blocks of this chain so far
-  uint32_t base = 0;  // it of the current tile's first block
-  Walker w(p, bars);
+  // this warp's lanes and chain: weights at tP, scores and accumulator from it
+  const uint32_t tP = tmem + (static_cast<uint32_t>(lb) << 16) + kPxP + t * 64;
+  const uint32_t tS = tP + kPxS - kPxP + t * 64;
+  const uint32_t tO = tP + kPxO - kPxP;
+  float* mbuf = s_merge + c * kPxMergeFloats;
+  uint32_t n_s = 0;    // blocks of this chain so far
+  for (uint32_t i = lane; i < sizeof(Walk) / 4; i += 32)
+    reinterpret_cast<int*>(&w)[i] = reinterpret_cast<const int*>(&bars->start)[i];
+  __syncwarp();
 
   while (w.left > 0) {
-    const int n = w.stretch();
-    const int seg = w.seg;
-    // The buffer's last tile, seg - 2, is done with in both chains: a chain 0
-    // warp has met chain 1's hand-over of seg - 1, a chain 1 warp chain 0's
-    // release of seg - 2, and either follows that chain's last product.
-    load_q(p, w, sQ + (seg & 1) * kPxTile);
-    fence_proxy_async_smem();
-    mbar_arrive(&bars->q_full[seg & 1]);
-
-    const int rows = min(128, w.d.rows - w.m * 128);
+    const bool pair = walk_pair(w);
+    int rows;  // of this chain's tile
+    {
+      const int row0 = w.m * kPxRows + (pair ? 128 * t : 0);
+      rows = min(128, w.d.rows - row0);
+      // The chain's last segment is done (its last product was waited for), so
+      // its query buffer is free.
+      load_q(p, w, row0, rows, sQ + t * kPxTile);
+      fence_proxy_async_smem();
+      mbar_arrive(&bars->q_full[t]);
+    }
     const bool active = 16 * c < rows;  // warp-uniform: some row of this warp is real
-    const int off = static_cast<int>((base ^ static_cast<uint32_t>(t)) & 1u);
+    // this chain's blocks: all, or every second one
+    const int cnt = pair ? walk_blocks(w) : (walk_blocks(w) + 1 - t) >> 1;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-    bool any = false;
-    for (int j = off; j < n; j += 2) {
+#pragma unroll 1
+    for (int i = 0; i < cnt; ++i, ++n_s) {
       if (!warp_wait(&bars->s_full[t], n_s & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return;
       tc_fence_after();
-      const int live = w.d.plen - (w.blk + j) * 128;  // keys of this block that exist
-      const uint32_t it = base + j;
-      if (live < 128) {
-        // Value rows behind the last live key may hold anything (a weight of
-        // 0 times a NaN is a NaN): the chain's 256 threads zero them before
-        // the second product.
-        const uint32_t st = it % kPxStages;
-        if (!warp_wait(&bars->v_full[st], (it / kPxStages) & 1, abort_flag, p.err,
-                       kErrTimeoutSoftmax))
-          return;
-        uint4* v = reinterpret_cast<uint4*>(sV + st * kPxTile);
-        for (int i = live * 8 + (threadIdx.x & 255); i < 128 * 8; i += 256)
-          v[i] = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
+      int live = kPxKeys;  // keys of this block that exist; fewer in a prefix's last block only
+      if (i == cnt - 1) {
+        const int j = pair ? i : 2 * i + t;
+        live = w.d.plen - (walk_first(w) + j) * kPxKeys;
+        if (live < kPxKeys) {
+          // Value rows behind the last live key may hold anything (a weight
+          // of 0 times a NaN is a NaN): the chain's 256 threads zero them
+          // before the second product.
+          const uint32_t it = static_cast<uint32_t>(w.base + j), st = it % kPxStages;
+          if (!warp_wait(&bars->v_full[st], (it / kPxStages) & 1, abort_flag, p.err,
+                         kErrTimeoutSoftmax))
+            return;
+          uint4* v = reinterpret_cast<uint4*>(sV + st * kPxTile);
+          for (int k = live * 8 + (threadIdx.x & 255); k < kPxKeys * 8; k += 256)
+            v[k] = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
       }
       if (!active) {
         tc_fence_before();
@@ -415,8 +467,6 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem,
             !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
           return;
         mbar_arrive(&bars->p_full[t]);
-        ++n_s;
-        any = true;
         continue;
       }
       uint32_t sr[64];
@@ -425,7 +475,7 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem,
       tc_fence_before();
       mbar_arrive(&bars->sc_done[t]);
       float* sf = reinterpret_cast<float*>(sr);
-      if (live < 128) {
+      if (live < kPxKeys) {
 #pragma unroll
         for (int k = 0; k < 16; ++k)
 #pragma unroll
@@ -445,74 +495,77 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem,
       }
       // The reference value of a row moves only when the maximum outgrows it
       // by 2^8: weights stay below 2^8 and most blocks never rescale.
-      float corr[2] = {1.f, 1.f};
-      bool grow = false;
-      if (__any_sync(0xffffffffu,
-                     mx[0] * sl2 > m_run[0] + 8.0f || mx[1] * sl2 > m_run[1] + 8.0f)) {
+      if (__any_sync(0xffffffffu, mx[0] * p.scale_log2 > m_run[0] + 8.0f ||
+                                      mx[1] * p.scale_log2 > m_run[1] + 8.0f)) {
+        float corr[2] = {1.f, 1.f};
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           mx[v] = fmaxf(mx[v], __shfl_xor_sync(0xffffffffu, mx[v], 1));
           mx[v] = fmaxf(mx[v], __shfl_xor_sync(0xffffffffu, mx[v], 2));
-          const float m_blk = mx[v] * sl2;
+          const float m_blk = mx[v] * p.scale_log2;
           if (m_blk > m_run[v] + 8.0f) {
             const float m_new = ceilf(m_blk);
             corr[v] = ex2_approx(m_run[v] - m_new);
             m_run[v] = m_new;
-            grow = true;
+            l_run[v] *= corr[v];
           }
+        }
+        if (i > 0) {  // the accumulator so far, once the last product is in it
+          if (!warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
+            return;
+          tc_fence_after();
+#pragma unroll 1
+          for (int h = 0; h < 8; ++h) {
+            uint32_t o4[4];
+            tmem_ld_16x256b_x1(tO + 8 * h, o4);
+            tmem_wait_ld_regs4(o4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o4[e] = __float_as_uint(__uint_as_float(o4[e]) * corr[e >> 1]);
+            tmem_st_16x256b_x1(tO + 8 * h, o4);
+          }
+          tmem_wait_st();
         }
       }
       // weights in pairs; the sum takes them unrounded, the product in 16 bits
       uint32_t pk[32];
-      float bsum[2];
-      const uint64_t c2 = f2_pack(sl2, sl2);
+      {
+        const uint64_t c2 = f2_pack(p.scale_log2, p.scale_log2);
+        uint64_t acc[2];
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const float neg = m_run[v] == -INFINITY ? 0.f : -m_run[v];
-        const uint64_t n2 = f2_pack(neg, neg);
-        uint64_t acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
+        for (int v = 0; v < 2; ++v) acc[v] = f2_pack(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(sf[4 * k + 2 * v], sf[4 * k + 2 * v + 1]), c2, n2), x0, x1);
-          const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-          pk[2 * k + v] = F16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
-          if (k & 1)
-            acc1 = f2_add(acc1, f2_pack(p0, p1));
-          else
-            acc0 = f2_add(acc0, f2_pack(p0, p1));
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(sf[4 * k + 2 * v], sf[4 * k + 2 * v + 1]), c2,
+                             f2_pack(-m_run[v], -m_run[v])), x0, x1);
+            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            pk[2 * k + v] = F16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+            acc[v] = f2_add(acc[v], f2_pack(p0, p1));
+          }
         }
-        float a, b;
-        f2_unpack(f2_add(acc0, acc1), a, b);
-        bsum[v] = a + b;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          float a, b;
+          f2_unpack(acc[v], a, b);
+          l_run[v] += a + b;
+        }
       }
-      l_run[0] = fmaf(l_run[0], corr[0], bsum[0]);
-      l_run[1] = fmaf(l_run[1], corr[1], bsum[1]);
+      // P is free once the previous product has read it
       if (n_s > 0 &&
           !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
         return;
       tc_fence_after();
-      if (__any_sync(0xffffffffu, grow && any)) {
-#pragma unroll 1
-        for (int h = 0; h < 4; ++h) {
-          uint32_t orr[8];
-          tmem_ld_16x256b_x2(tO + 16 * h, orr);
-          tmem_wait_ld_regs8(orr);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            orr[e] = __float_as_uint(__uint_as_float(orr[e]) * corr[(e >> 1) & 1]);
-          tmem_st_16x256b_x2(tO + 16 * h, orr);
-        }
-      }
       tmem_st_16x128b_x16(tP, pk);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&bars->p_full[t]);
-      ++n_s;
-      any = true;
     }
+    const bool any = cnt > 0;
 
-    // ---- end of the tile's stretch: chain 1 hands over to chain 0
+    // ---- end of the segment's stretch
     if (any && !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
       return;
     tc_fence_after();
@@ -523,18 +576,23 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem,
         l_run[v] += __shfl_xor_sync(0xffffffffu, l_run[v], 2);
       }
     }
-    // (an inactive pair has nothing to hand over, but keeps the barriers' count)
-    uint32_t orr[32];
-    if (t == 1) {
-      if (seg >= 1 && !warp_wait(&bars->mrg_empty[c], (seg - 1) & 1, abort_flag, p.err,
-                                 kErrTimeoutSoftmax))
+    // One tile for both chains: chain 1 hands over to chain 0.  (A pair of
+    // warps without rows hands over nothing, but keeps the barriers' count.)
+    // The accumulator is moved eight registers (16 columns) at a time.
+    if (!pair && t == 1) {
+      if (w.alt >= 1 && !warp_wait(&bars->mrg_empty[c], (w.alt - 1) & 1, abort_flag, p.err,
+                                   kErrTimeoutSoftmax))
         return;
       if (active) {
         if (any) {
-          tmem_ld_16x256b_x8(tO, orr);
-          tmem_wait_ld_regs(orr);
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            uint32_t o8[8];
+            tmem_ld_16x256b_x2(tO + 16 * h, o8);
+            tmem_wait_ld_regs8(o8);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mbuf[e * 32 + lane] = __uint_as_float(orr[e]);
+            for (int e = 0; e < 8; ++e) mbuf[(8 * h + e) * 32 + lane] = __uint_as_float(o8[e]);
+          }
         }
         if (t0 == 0) {
 #pragma unroll
@@ -546,49 +604,64 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem,
       }
       mbar_arrive(&bars->mrg_full[c]);
     } else {
-      if (active && any) {
-        tmem_ld_16x256b_x8(tO, orr);
-        tmem_wait_ld_regs(orr);
-      }
-      if (!warp_wait(&bars->mrg_full[c], seg & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return;
-      // (group_starts that do not rise can give more tiles than there is room for)
-      if (active && blockIdx.x + w.tile < p.part_slots) {
-        const size_t slot = static_cast<size_t>(blockIdx.x + w.tile) * 128 + 16 * c;
+      float f0[2] = {1.f, 1.f}, f1[2] = {0.f, 0.f};
+      if (!pair) {
+        if (!warp_wait(&bars->mrg_full[c], w.alt & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return;
+        if (active) {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const int r = t1 + 8 * v;
-          const float m1 = mbuf[32 * 32 + 2 * r], l1 = mbuf[32 * 32 + 2 * r + 1];
-          const float M = fmaxf(m_run[v], m1);
-          // a chain without blocks in this stretch has m = -inf: its
-          // accumulator is stale and not used
-          const float f0 = m_run[v] == -INFINITY ? 0.f : ex2_approx(m_run[v] - M);
-          const float f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - M);
-          if (16 * c + r < rows) {
-            float* dst = p.part_o + (slot + r) * 64 + 2 * t0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              float2 o = make_float2(0.f, 0.f);
-              if (m_run[v] != -INFINITY) {
-                o.x = __uint_as_float(orr[4 * k + 2 * v]) * f0;
-                o.y = __uint_as_float(orr[4 * k + 2 * v + 1]) * f0;
-              }
-              if (m1 != -INFINITY) {
-                o.x = fmaf(mbuf[(4 * k + 2 * v) * 32 + lane], f1, o.x);
-                o.y = fmaf(mbuf[(4 * k + 2 * v + 1) * 32 + lane], f1, o.y);
-              }
-              *reinterpret_cast<float2*>(dst + 8 * k) = o;
-            }
-            if (t0 == 0)
-              *reinterpret_cast<float2*>(p.part_ml + 2 * (slot + r)) =
-                  make_float2(M, l_run[v] * f0 + l1 * f1);
+          for (int v = 0; v < 2; ++v) {
+            const int r = t1 + 8 * v;
+            const float m1 = mbuf[32 * 32 + 2 * r], l1 = mbuf[32 * 32 + 2 * r + 1];
+            const float M = fmaxf(m_run[v], m1);
+            // a chain without blocks here has m = -inf: its accumulator is
+            // stale and its factor, 0, marks it as not used
+            f0[v] = m_run[v] == -INFINITY ? 0.f : ex2_approx(m_run[v] - M);
+            f1[v] = m1 == -INFINITY ? 0.f : ex2_approx(m1 - M);
+            m_run[v] = M;
+            l_run[v] = l_run[v] * f0[v] + l1 * f1[v];
           }
         }
       }
-      mbar_arrive(&bars->mrg_empty[c]);
+      // (group_starts that do not rise can give more segments than there is room for)
+      const int slot = static_cast<int>(blockIdx.x) + w.seg;
+      if (active && slot < p.part_slots) {
+        const size_t at = static_cast<size_t>(slot) * kPxRows + (pair ? 128 * t : 0) + 16 * c + t1;
+        float* dst = p.part_o + at * 64 + 2 * t0;
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          uint32_t o8[8];
+          if (any) {
+            tmem_ld_16x256b_x2(tO + 16 * h, o8);
+            tmem_wait_ld_regs8(o8);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              float o[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int e = 4 * k + 2 * v + x;
+                o[x] = f0[v] > 0.f ? __uint_as_float(o8[e]) * f0[v] : 0.f;
+                if (f1[v] > 0.f) o[x] = fmaf(mbuf[(8 * h + e) * 32 + lane], f1[v], o[x]);
+              }
+              if (16 * c + t1 + 8 * v < rows)
+                *reinterpret_cast<float2*>(dst + 8 * v * 64 + 16 * h + 8 * k) = make_float2(o[0], o[1]);
+            }
+        }
+        if (t0 == 0) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            if (16 * c + t1 + 8 * v < rows)
+              *reinterpret_cast<float2*>(p.part_ml + 2 * (at + 8 * v)) = make_float2(m_run[v], l_run[v]);
+        }
+      }
+      if (!pair) mbar_arrive(&bars->mrg_empty[c]);
     }
     tc_fence_before();
-    base += n;
-    w.skip(n);
+    __syncwarp();
+    if (lane == 0) walk_next(w, p);
+    __syncwarp();
   }
 }
 
@@ -596,21 +669,18 @@ template <int F16>
 __global__ void __launch_bounds__(kPxThreads, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const SharedParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  uint8_t* sQ = smem;
-  uint8_t* sK = sQ + 2 * kPxTile;
-  uint8_t* sV = sK + kPxStages * kPxTile;
-  float* s_merge = reinterpret_cast<float*>(sV + kPxStages * kPxTile);
-  PxBars* bars = reinterpret_cast<PxBars*>(reinterpret_cast<uint8_t*>(s_merge) + kPxMerge);
+  if (smem_u32(px_smem) % 1024 != 0) {  // the whole grid alike
+    if (threadIdx.x == 0 && p.err) atomicOr(p.err, kErrBadArgs);
+    return;
+  }
+  PxBars* bars = PX_BARS;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (warp == kPxMma0) {
-    find_stretch(p, bars);
+    find_stretch(p);
   } else if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&bars->q_full[t], 512);
+      mbar_init(&bars->q_full[t], 256);
       mbar_init(&bars->s_full[t], 1);
       mbar_init(&bars->sc_done[t], 256);
       mbar_init(&bars->p_full[t], 256);
@@ -619,7 +689,7 @@ __global__ void __launch_bounds__(kPxThreads, 1)
     for (int s = 0; s < kPxStages; ++s) {
       mbar_init(&bars->k_full[s], 1);
       mbar_init(&bars->v_full[s], 1);
-      mbar_init(&bars->kv_empty[s], 1);
+      mbar_init(&bars->kv_empty[s], 2);
     }
     for (int c = 0; c < 8; ++c) {
       mbar_init(&bars->mrg_full[c], 32);
@@ -645,14 +715,14 @@ __global__ void __launch_bounds__(kPxThreads, 1)
   griddep_launch_dependents();
 
   if (warp == kPxProducer) {
-    px_producer(&tmK, &tmV, p, sK, sV, bars);
+    px_producer(&tmK, &tmV, p);
   } else if (warp >= kPxMma0) {
-    px_mma<F16>(p, warp - kPxMma0, sQ, sK, sV, tmem, bars);
+    px_mma<F16>(p, warp - kPxMma0, tmem);
     int none = 0;  // every MMA issued has finished before tensor memory is freed
     mma_commit_w(&bars->drain);
     mbar_wait(&bars->drain, 0, &none, p.err, kErrTimeoutDrain);
   } else {
-    px_softmax<F16>(p, tmem, sQ, sV, s_merge, bars);
+    px_softmax<F16>(p, tmem);
   }
   __syncwarp();
   tc_fence_before();

@@ -154,29 +154,42 @@ __device__ __forceinline__ const void* q_row(const SharedParams& p, int b, int t
   return static_cast<const uint8_t*>(p.q) + off * (p.q_dtype == 0 ? 4 : 2);
 }
 
-// The group whose sequences hold b, or -1: starts[] rises, so it is the last
-// group that starts at or before b, if b is before its end.
+// The group whose sequences hold b, or -1 (a whole warp): starts[] rises, so
+// it is the last group that starts at or before b, if b is before its end.
 __device__ __forceinline__ int group_of(const SharedParams& p, int b) {
-  int lo = 0, hi = p.groups;
-  while (hi - lo > 0) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(p.group_starts + mid) <= b)
-      lo = mid + 1;
-    else
-      hi = mid;
+  const int lane = threadIdx.x % 32;
+  int n = 0;  // groups that start at or before b
+  for (int base = 0; base < p.groups; base += 32) {
+    const int g = base + lane;
+    const bool in = g < p.groups && __ldg(p.group_starts + g) <= b;
+    n += __popc(__ballot_sync(0xffffffffu, in));
   }
-  const int g = lo - 1;
-  return g >= 0 && b < __ldg(p.group_starts + g + 1) ? g : -1;
+  if (n == 0) return -1;
+  return b < __ldg(p.group_starts + n) ? n - 1 : -1;
 }
 
-// Walk a list of pages: steps w, w + kSpWarps, ... of 32 keys each.
+// Page ids of a warp's next 32 steps, one per lane: warp w takes the steps w, w
+// + kSpWarps, ... of 32 keys, and `first` counts the warp's own.
+__device__ __forceinline__ int step_page(const int* table, int pages, int warp, int first) {
+  const int page = (warp + kSpWarps * (first + static_cast<int>(threadIdx.x % 32))) / 2;
+  return page < pages ? __ldg(table + page) : -1;
+}
+
+// Walk `len` keys of a list of pages.  `ids` holds the first 32 steps' page
+// ids, loaded ahead (the table does not depend on the lengths).
 template <int F16>
 __device__ __forceinline__ void walk(RowState& st, const RowQ& q, const SharedParams& p, int kvh,
-                                     const int* table, int len, const int (&see)[2], int warp) {
+                                     const int* table, int pages, int ids, int len,
+                                     const int (&see)[2], int warp) {
   const uint16_t* kpool = static_cast<const uint16_t*>(p.k_pool);
   const uint16_t* vpool = static_cast<const uint16_t*>(p.v_pool);
-  for (int k0 = warp * kSpKeys; k0 < len; k0 += kSpWarps * kSpKeys) {
-    const int page = __ldg(table + k0 / kPageKeys);
+  int n = 0;
+  for (int k0 = warp * kSpKeys; k0 < len; k0 += kSpWarps * kSpKeys, ++n) {
+    if (n == 32) {
+      ids = step_page(table, pages, warp, k0 / (kSpWarps * kSpKeys));
+      n = 0;
+    }
+    const int page = __shfl_sync(0xffffffffu, ids, n);
     if (page < 0 || page >= p.num_pages) {  // not read; its keys weigh nothing
       if (p.err && threadIdx.x % 32 == 0) atomicOr(p.err, kErrBadArgs);
       continue;
@@ -188,117 +201,135 @@ __device__ __forceinline__ void walk(RowState& st, const RowQ& q, const SharedPa
   }
 }
 
-// Fold the prefix kernel's partials into the rows' states: warp w takes parts
-// w, w + kSpWarps, ... of each of its rows.
-__device__ __forceinline__ void fold_partials(RowState& st, const SharedParams& p, int group, int b,
-                                              int kvh, int tile, int R, int warp) {
-  const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+constexpr int kSpStage = 96;  // staged (part, row) pairs: 80 floats each
+
+// A merge of partial softmax results of one row, 8 head dims a thread.
+struct Merged {
+  float m, l, o[8];
+  __device__ __forceinline__ void add(const float2 ml, const float4 a, const float4 b) {
+    if (ml.x == -INFINITY) return;  // nothing in it
+    const float M = fmaxf(m, ml.x);
+    const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - M), f1 = ex2_approx(ml.x - M);
+    m = M;
+    l = l * f0 + ml.y * f1;
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = o[e] * f0 + x[e] * f1;
+  }
+};
+
+// The prefix kernel's partials of this CTA's rows (thread = row, 8 head dims),
+// folded into `acc`: copied to shared memory as many at a time as fit, so that
+// their latencies overlap, then added in the order of the line.
+__device__ __forceinline__ void fold_partials(Merged& acc, float* stage, const SharedParams& p,
+                                              int group, int b, int kvh, int row, int R) {
+  const int part = threadIdx.x % 8, lrow = threadIdx.x / 8;
   const GroupDims d = group_dims(p, group);
   if (d.nb == 0) return;
   // written by the preceding kernel, which may have run beside this one
-  const long long share = __ldcg(p.part_plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
-                  tile0 = __ldcg(p.part_plan + 2 + 2 * group);
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = tile * 16 + g + 8 * r;
-    if (row >= R) continue;
-    const int rg = (b - d.b0) * R + row;
-    const long long at = static_cast<long long>(kvh) * d.mt + rg / 128;
-    const long long l0 = lin0 + at * d.nb;
-    const long long c0 = l0 / share, c1 = (l0 + d.nb - 1) / share;
-    for (long long c = c0 + warp; c <= c1; c += kSpWarps) {
-      const long long slot = c + tile0 + at;
-      if (slot >= p.part_slots) break;
-      const size_t pr = static_cast<size_t>(slot) * 128 + rg % 128;
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + pr);
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + pr * 64 + 16 * t);
-      float x[16];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 f = __ldcg(src + i);
-        x[4 * i] = f.x;
-        x[4 * i + 1] = f.y;
-        x[4 * i + 2] = f.z;
-        x[4 * i + 3] = f.w;
+  const int share = __ldcg(p.part_plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
+            seg0 = __ldcg(p.part_plan + 2 + 2 * group);
+  if (row >= R) return;
+  const int cl = chunk_blocks(d, share), chunks = (d.nb + cl - 1) / cl;
+  const int rg = (b - d.b0) * R + row, m = rg / kPxRows;
+  const size_t at = static_cast<size_t>(rg - m * kPxRows);
+  const int head0 = lin0 + kvh * head_steps(d, d.nb);
+  // a thread stages and reads its own pieces: no barrier
+  const int rows = min(R, 16), room = kSpStage / rows;  // parts staged at a time
+  float* mine = stage + (lrow * 8 + part) * 8;
+  float* mine_ml = stage + kSpStage * 64 + (lrow * 8 + part) * 2;
+  const int pitch = rows * 64, pitch_ml = rows * 16;
+  int q = 0, c = -1, c1 = -2, seg = 0;
+  bool more = true;
+  while (more) {
+    int n = 0;
+#pragma unroll 1
+    while (n < room) {
+      if (c > c1 || c1 < 0) {  // next chunk
+        if (q == chunks) {
+          more = false;
+          break;
+        }
+        const int len = min(cl, d.nb - q * cl);
+        const int l0 = head0 + head_steps(d, q * cl) + m * len;
+        seg = seg0 + (kvh * chunks + q) * d.mu + m;
+        c = l0 / share;
+        c1 = (l0 + unit_steps(d, m, len) - 1) / share;
+        ++q;
       }
-      const float M = fmaxf(st.m[r], ml.x);
-      const float f0 = st.m[r] == -INFINITY ? 0.f : ex2_approx(st.m[r] - M);
-      const float f1 = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M);
-      st.m[r] = M;
-      st.l[r] = st.l[r] * f0 + (t == 0 ? ml.y * f1 : 0.f);  // lanes' sums are added later
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        st.o[j][2 * r] = st.o[j][2 * r] * f0 + x[j] * f1;
-        st.o[j][2 * r + 1] = st.o[j][2 * r + 1] * f0 + x[8 + j] * f1;
-      }
+      const int slot = c + seg;
+      const bool have = slot < p.part_slots;
+      const size_t pr = static_cast<size_t>(have ? slot : 0) * kPxRows + at;
+      cp_async16(mine + n * pitch, p.part_o + pr * 64 + 8 * part, have);
+      cp_async16(mine + n * pitch + 4, p.part_o + pr * 64 + 8 * part + 4, have);
+      if (have)
+        cp_async8(mine_ml + n * pitch_ml, p.part_ml + 2 * pr);
+      else
+        *reinterpret_cast<float2*>(mine_ml + n * pitch_ml) = make_float2(-INFINITY, 0.f);
+      ++c;
+      ++n;
     }
+    cp_async_wait_all();
+#pragma unroll 1
+    for (int i = 0; i < n; ++i)
+      acc.add(*reinterpret_cast<const float2*>(mine_ml + i * pitch_ml),
+              *reinterpret_cast<const float4*>(mine + i * pitch),
+              *reinterpret_cast<const float4*>(mine + i * pitch + 4));
   }
-}
-
-__device__ __forceinline__ void store_out(const SharedParams& p, size_t off, float x) {
-  if (p.out_dtype == 0)
-    static_cast<float*>(p.out)[off] = x;
-  else if (p.out_dtype == 1)
-    static_cast<__nv_bfloat16*>(p.out)[off] = __float2bfloat16(x);
-  else
-    static_cast<__half*>(p.out)[off] = __float2half(x);
 }
 
 constexpr int kSpPitch = 68;  // floats per merged row: m, l, then o[64]
 
 template <int F16>
-__global__ void __launch_bounds__(kSpThreads) shared_rows_kernel(SharedParams p) {
+__global__ void __launch_bounds__(kSpThreads, 4) shared_rows_kernel(SharedParams p) {
   __shared__ __align__(16) float s_part[kSpWarps][16][kSpPitch];
+  __shared__ __align__(16) float s_stage[kSpStage * 80];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
   const int G = p.heads / p.kv_heads, R = p.q_len * G;
   const int tiles = (R + 15) / 16;
-  const long long id = blockIdx.x;
-  const int tile = static_cast<int>(id % tiles);
-  const int kvh = static_cast<int>(id / tiles % p.kv_heads);
-  const int b = static_cast<int>(id / tiles / p.kv_heads);
+  const unsigned id = blockIdx.x, job = id / tiles;
+  const int tile = static_cast<int>(id - job * tiles);
+  const int b = static_cast<int>(job / p.kv_heads), kvh = static_cast<int>(job - b * p.kv_heads);
 
+  const int* table = p.block_table + static_cast<size_t>(b) * p.max_pages;
+  const int ids = step_page(table, p.max_pages, warp, 0);
+  int len = __ldg(p.seq_lens + b);
   RowQ q;
   RowState st;
-  const int group = group_of(p, b);
-  int plen = 0;
-  if (group >= 0) {
-    plen = __ldg(p.prefix_lens + group);
-    if (plen < 0 || plen > p.prefix_pages * kPageKeys) {
-      if (p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
-      plen = min(max(plen, 0), p.prefix_pages * kPageKeys);
-    }
-  }
-  int len = __ldg(p.seq_lens + b);
-  if (len < 0 || len > p.max_pages * kPageKeys) {
-    if (p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
-    len = min(max(len, 0), p.max_pages * kPageKeys);
-  }
-  int see[2];
+  int tok[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int row = tile * 16 + g + 8 * r;
-    const int tok = row / G, h = kvh * G + row % G;
-    const bool real = row < R;
-    see[r] = real ? max(0, len - (p.q_len - 1 - tok)) : 0;
-    const void* src = real ? q_row(p, b, tok, h) : nullptr;
+    tok[r] = row < R ? row / G : -1;
+    const void* src = row < R ? q_row(p, b, tok[r], kvh * G + row % G) : nullptr;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int dim = 32 * (s / 2) + 8 * t + 4 * (s % 2);
-      q.a[s][r] = real ? q_pair(p, src, dim) : 0u;
-      q.a[s][2 + r] = real ? q_pair(p, src, dim + 2) : 0u;
+      q.a[s][r] = row < R ? q_pair(p, src, dim) : 0u;
+      q.a[s][2 + r] = row < R ? q_pair(p, src, dim + 2) : 0u;
     }
     st.m[r] = -INFINITY;
     st.l[r] = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.o[j][2 * r] = st.o[j][2 * r + 1] = 0.f;
   }
-  walk<F16>(st, q, p, kvh, p.block_table + static_cast<size_t>(b) * p.max_pages, len, see, warp);
-  if (p.part_o) {
-    griddep_wait();  // the prefix kernel's partials
-    if (group >= 0) fold_partials(st, p, group, b, kvh, tile, R, warp);
-  } else if (group >= 0) {
+  if (len < 0 || len > p.max_pages * kPageKeys) {
+    if (p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
+    len = min(max(len, 0), p.max_pages * kPageKeys);
+  }
+  const int see[2] = {tok[0] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[0])),
+                      tok[1] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[1]))};
+  walk<F16>(st, q, p, kvh, table, p.max_pages, ids, len, see, warp);
+  const int group = group_of(p, b);
+  if (!p.part_o && group >= 0) {  // no prefix kernel: the prefix too
+    int plen = __ldg(p.prefix_lens + group);
+    if (plen < 0 || plen > p.prefix_pages * kPageKeys) {
+      if (p.err && threadIdx.x == 0) atomicOr(p.err, kErrBadArgs);
+      plen = min(max(plen, 0), p.prefix_pages * kPageKeys);
+    }
     const int all[2] = {plen, plen};
-    walk<F16>(st, q, p, kvh, p.prefix_table + static_cast<size_t>(group) * p.prefix_pages, plen,
+    table = p.prefix_table + static_cast<size_t>(group) * p.prefix_pages;
+    walk<F16>(st, q, p, kvh, table, p.prefix_pages, step_page(table, p.prefix_pages, warp, 0), plen,
               all, warp);
   }
 
@@ -308,43 +339,55 @@ __global__ void __launch_bounds__(kSpThreads) shared_rows_kernel(SharedParams p)
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     float* w = s_part[warp][g + 8 * r];
-    if (t == 0) {
-      w[0] = st.m[r];
-      w[1] = l;
-    }
+    if (t == 0) *reinterpret_cast<float2*>(w) = make_float2(st.m[r], l);
+    float4* o = reinterpret_cast<float4*>(w + 4 + 16 * t);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      w[4 + 16 * t + j] = st.o[j][2 * r];
-      w[4 + 16 * t + 8 + j] = st.o[j][2 * r + 1];
+    for (int e = 0; e < 2; ++e) {
+      o[e] = make_float4(st.o[4 * e][2 * r], st.o[4 * e + 1][2 * r], st.o[4 * e + 2][2 * r],
+                         st.o[4 * e + 3][2 * r]);
+      o[2 + e] = make_float4(st.o[4 * e][2 * r + 1], st.o[4 * e + 1][2 * r + 1],
+                             st.o[4 * e + 2][2 * r + 1], st.o[4 * e + 3][2 * r + 1]);
     }
   }
   __syncthreads();
   // merge: 8 threads a row, 8 head dims each
-  const int row = threadIdx.x / 8, part = threadIdx.x % 8, rr = tile * 16 + row;
-  if (rr >= R) return;
-  float M = -INFINITY, L = 0.f, O[8];
-#pragma unroll
-  for (int w = 0; w < kSpWarps; ++w) M = fmaxf(M, s_part[w][row][0]);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) O[e] = 0.f;
-#pragma unroll
+  const int lrow = threadIdx.x / 8, part = threadIdx.x % 8, rr = tile * 16 + lrow;
+  Merged acc{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 1
   for (int w = 0; w < kSpWarps; ++w) {
-    const float* x = s_part[w][row];
-    const float f = x[0] == -INFINITY ? 0.f : ex2_approx(x[0] - M);
-    L = fmaf(x[1], f, L);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) O[e] = fmaf(x[4 + 8 * part + e], f, O[e]);
+    const float* x = s_part[w][lrow];
+    acc.add(*reinterpret_cast<const float2*>(x), *reinterpret_cast<const float4*>(x + 4 + 8 * part),
+            *reinterpret_cast<const float4*>(x + 8 + 8 * part));
   }
-  const int tok = rr / G, h = kvh * G + rr % G;
-  const size_t o_row = static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(tok) * p.o_st +
-                       static_cast<size_t>(h) * p.o_sh;
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  if (p.part_o) {
+    griddep_wait();  // the prefix kernel's partials
+    if (group >= 0) fold_partials(acc, s_stage, p, group, b, kvh, rr, R);
+  }
+  if (rr >= R) return;
+  const int ti = rr / G, h = kvh * G + rr % G;
+  const size_t at = static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(ti) * p.o_st +
+                    static_cast<size_t>(h) * p.o_sh + 8 * part;
+  const float inv = acc.l > 0.f ? 1.f / acc.l : 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) store_out(p, o_row + 8 * part + e, O[e] * inv);
+  for (int e = 0; e < 8; ++e) acc.o[e] *= inv;
+  if (p.out_dtype == 0) {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+    o[0] = make_float4(acc.o[0], acc.o[1], acc.o[2], acc.o[3]);
+    o[1] = make_float4(acc.o[4], acc.o[5], acc.o[6], acc.o[7]);
+  } else {
+    uint4 x;
+    if (p.out_dtype == 1)
+      x = make_uint4(pack_bf16x2(acc.o[0], acc.o[1]), pack_bf16x2(acc.o[2], acc.o[3]),
+                     pack_bf16x2(acc.o[4], acc.o[5]), pack_bf16x2(acc.o[6], acc.o[7]));
+    else
+      x = make_uint4(pack_f16x2(acc.o[0], acc.o[1]), pack_f16x2(acc.o[2], acc.o[3]),
+                     pack_f16x2(acc.o[4], acc.o[5]), pack_f16x2(acc.o[6], acc.o[7]));
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = x;
+  }
   if (p.lse && part == 0)
-    p.lse[static_cast<size_t>(b) * p.lse_sb + static_cast<size_t>(tok) * p.lse_st +
+    p.lse[static_cast<size_t>(b) * p.lse_sb + static_cast<size_t>(ti) * p.lse_st +
           static_cast<size_t>(h) * p.lse_sh] =
-        L > 0.f ? (M + log2f(L)) * 0.69314718055994530942f : -INFINITY;
+        acc.l > 0.f ? (acc.m + log2f(acc.l)) * 0.69314718055994530942f : -INFINITY;
 }
 
 }  // namespace
