@@ -1462,7 +1462,8 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
     return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: logits not aligned to their type");
   SampleParams p{logits, ld, batch, vocab, dtype, u, temperature, top_k, top_p, min_p, tokens, logprobs};
   DeviceGuard g(ctx->device);
-  FFAI_CUDA(ctx, launch_sample(p, static_cast<cudaStream_t>(stream)));
+  FFAI_CUDA(ctx, launch_sample(p, sample_cluster(batch, vocab, ctx->num_sms),
+                               static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }
 

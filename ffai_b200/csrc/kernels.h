@@ -426,6 +426,7 @@ struct SampleParams {
   int* tokens;      // (batch)
   float* logprobs;  // (batch) or null
 };
-cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
+int sample_cluster(int batch, int vocab, int sms);  // CTAs per row
+cudaError_t launch_sample(const SampleParams& p, int cluster, cudaStream_t s);
 
 }  // namespace ffai
