@@ -86,6 +86,9 @@ struct ffai_attn_ctx {
   // int8 GEMV: quantised activations and their scales, between its two kernels
   uint8_t* d_gemv_x = nullptr;
   size_t gemv_x_cap = 0;
+  // sampling: per-row state between its kernels
+  ffai::SampleRow* d_sample = nullptr;
+  size_t sample_cap = 0;
   // shared prefix: partial results between its two kernels
   float* d_prefix = nullptr;
   size_t prefix_cap = 0;
@@ -166,6 +169,8 @@ int ensure(ffai_attn_ctx* ctx, T** ptr, size_t* cap, size_t need_elems, bool zer
   }
   if (zero) {
     e = cudaMemset(*ptr, 0, n * sizeof(T));
+    // done before work on any other stream uses the buffer
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaMemset(workspace)");
   }
   *cap = n;
@@ -735,6 +740,7 @@ void ffai_attn_destroy(ffai_attn_ctx* ctx) {
   cudaFree(ctx->d_pipe);
   cudaFree(ctx->d_gemv_x);
   cudaFree(ctx->d_prefix);
+  cudaFree(ctx->d_sample);
   for (int i = 0; i < 2; ++i) {
     if (ctx->ev_h2d[i]) cudaEventDestroy(ctx->ev_h2d[i]);
     if (ctx->ev_comp[i]) cudaEventDestroy(ctx->ev_comp[i]);
@@ -1460,10 +1466,28 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
     return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: null pointer");
   if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) != 0)
     return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: logits not aligned to their type");
-  SampleParams p{logits, ld, batch, vocab, dtype, u, temperature, top_k, top_p, min_p, tokens, logprobs};
   DeviceGuard g(ctx->device);
-  FFAI_CUDA(ctx, launch_sample(p, sample_cluster(batch, vocab, ctx->num_sms),
-                               static_cast<cudaStream_t>(stream)));
+  const int slab = std::min<int>(batch, kSmMaxRows);
+  int st = ensure(ctx, &ctx->d_sample, &ctx->sample_cap, slab, /*zero=*/true);
+  if (st) return st;
+  SampleParams p{};
+  p.ld = ld;
+  p.vocab = vocab;
+  p.dtype = dtype;
+  p.chunk = sample_chunk(slab, vocab, ctx->num_sms);
+  p.rows = ctx->d_sample;
+  for (int b = 0; b < batch; b += slab) {
+    p.batch = std::min(slab, batch - b);
+    p.logits = static_cast<const char*>(logits) + static_cast<size_t>(b) * ld * dtype_size(dtype);
+    p.u = u + b;
+    p.temperature = temperature ? temperature + b : nullptr;
+    p.top_k = top_k ? top_k + b : nullptr;
+    p.top_p = top_p ? top_p + b : nullptr;
+    p.min_p = min_p ? min_p + b : nullptr;
+    p.tokens = tokens + b;
+    p.logprobs = logprobs ? logprobs + b : nullptr;
+    FFAI_CUDA(ctx, launch_sample(p, static_cast<cudaStream_t>(stream)));
+  }
   return FFAI_ATTN_OK;
 }
 

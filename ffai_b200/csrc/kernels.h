@@ -413,11 +413,37 @@ cudaError_t launch_kv_write(const WriteParams& p, int sms, cudaStream_t s);
 // ---- sampling (sample.cu) -----------------------------------------------------
 
 constexpr int kSmMaxVocab = 1 << 18;  // weight sums stay below 2^54
+constexpr int kSmChunk = 1 << 14;     // tokens per CTA, at most
+constexpr int kSmMinChunk = 1 << 11;  // and at least
+constexpr int kSmBins = 1600;         // of the exponent: (-25, 0] in steps of 1/64
+constexpr int kSmList = 1024;         // listed tokens per set
+constexpr int kSmMaxRows = 1024;      // rows per launch (workspace)
+
+// Which exponent bins can hold a prefix position, and what comes before them.
+struct SampleSet {
+  int b0, b1;
+  unsigned int before_cnt, pad;
+  unsigned long long before;
+};
+// A row's workspace.  best, above, ticket, n, bins and cnt are zero between
+// calls: whoever uses them last clears them.
+struct SampleRow {
+  unsigned long long best;  // (key, ~index) of the first maximum
+  unsigned long long above, total, floor;
+  double log_z;
+  unsigned int ticket, n[3];
+  SampleSet set[3];         // top-k, top-p, the token
+  double z[kSmMaxVocab / kSmMinChunk];
+  alignas(16) unsigned long long bins[kSmBins];
+  alignas(16) unsigned int cnt[kSmBins];
+  unsigned long long list[3][kSmList];
+};
 
 struct SampleParams {
   const void* logits;  // (batch, vocab), rows ld elements apart
   long long ld;
   int batch, vocab, dtype;
+  int chunk;                 // tokens per CTA: sample_chunk
   const float* u;            // (batch)
   const float* temperature;  // (batch) or null: 1
   const int* top_k;          // (batch) or null: off
@@ -425,8 +451,9 @@ struct SampleParams {
   const float* min_p;
   int* tokens;      // (batch)
   float* logprobs;  // (batch) or null
+  SampleRow* rows;  // (batch)
 };
-int sample_cluster(int batch, int vocab, int sms);  // CTAs per row
-cudaError_t launch_sample(const SampleParams& p, int cluster, cudaStream_t s);
+int sample_chunk(int batch, int vocab, int sms);
+cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
 
 }  // namespace ffai

@@ -196,17 +196,6 @@ __global__ void __launch_bounds__(kPlThreads) page_release_kernel(ReleaseParams 
 // ---------------------------------------------------------------- write
 
 template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
-  return __float2bfloat16(x);
-}
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) {
-  return __float2half(x);
-}
-
-template <typename T>
 struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) Vec8 {
   T v[8];
 };

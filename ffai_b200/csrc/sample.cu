@@ -13,21 +13,29 @@
 //   M   = min(M_p, M_m);  token = the first with C > floor(u * M).
 // Prefix masses alone are compared, so no cut needs its token count.
 //
-// A row is spread over a cluster of C CTAs (1 to 16), each keeping its stretch
-// of the logits in shared memory, so they are read from global memory once:
-//  1. load, the row's maximum (exchanged through distributed shared memory);
-//  2. weights, and a histogram of their sums (and counts, for top-k) over bins
-//     1/64 wide in d, which order the tokens coarsely: the CTAs add up a slice
-//     of the bins each, and all of them read all slices and scan them;
-//  3. each prefix position asked for (top-k, top-p, the token) lies in one bin,
-//     whose tokens every CTA lists and sorts by (logit, index).
-// A bin with more tokens than the list holds (flat or coarsely rounded rows)
-// is split by the logits' own bits until one is small or holds equal logits.
+// Three launches, each over (row, stretch of tokens) with thousands of threads
+// per row, the first reading the logits from memory, the others mostly from L2:
+//  1. sample_max_kernel: the row's first maximum, by an atomic maximum of
+//     (order-preserving key, ~index);
+//  2. sample_bins_kernel: weights, and a histogram of their sums (and counts, for
+//     top-k) over bins 1/64 wide in d, which order the tokens coarsely.  The last
+//     CTA of a row to finish scans the bins and works out which of them can hold
+//     the three prefix positions asked for (top-k, top-p, the token): a position
+//     known to lie in one bin bounds the next one's goal to an interval, almost
+//     always within a bin or two;
+//  3. sample_pick_kernel: lists the tokens of those bins; the last CTA of a row
+//     finds each position in its list (finer bins, then one warp ranks the few
+//     tokens left).
+// A set with more tokens than a list holds (flat or coarsely rounded rows) is
+// split by the logits' own bits, by that CTA alone, until a part fits.
 // Weights are summed as two 18-bit halves in 32-bit words, which a stretch of
 // at most 2^14 tokens does not overflow (but for one case, noted below), so plain
 // shared-memory reductions suffice: a 64-bit shared-memory add is a
-// compare-and-swap loop.
-#include <atomic>
+// compare-and-swap loop.  (One cluster of CTAs per row with the logits kept in
+// shared memory was slower everywhere: its exchanges and single-CTA phases take
+// 25 us a row with two rows per SM in flight: 269 us against 105 at 300 rows of
+// 128000 f32 logits, 40 against 20 at 64 rows of 51865 bf16.)
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -40,12 +48,8 @@ constexpr int kSmThreads = 512;
 constexpr int kSmWarps = kSmThreads / 32;
 constexpr int kSmBins = 1600;    // d in (-25, 0]; e^-25 2^36 < 1: nothing beyond
 constexpr int kSmPer = 4;        // bins per scanning thread
-constexpr int kSmLocal = 512;    // listed tokens per CTA
-constexpr int kSmList = 1024;    // per row
-constexpr int kSmMaxCluster = 16;
-constexpr int kSmChunk = 16384;  // tokens per CTA
-static_assert(kSmChunk * kSmMaxCluster >= kSmMaxVocab, "stretches");
-static_assert(kSmBins % kSmPer == 0 && kSmBins / kSmPer <= kSmThreads, "scan");
+constexpr int kSmSub = 512;      // finer bins of a list: 2^-15 wide in d
+static_assert(kSmSub == kSmThreads && kSmBins % kSmPer == 0 && kSmBins / kSmPer <= kSmThreads, "scan");
 // A stretch's low halves sum to at most 2^14 (2^18 - 1), its high ones to 2^14
 // 2^18: 2^32 exactly, when a whole stretch of 2^14 tokens is at the maximum.
 // The add that then wraps to 0 is noted in SampleShared::wrapped.
@@ -94,38 +98,31 @@ __device__ __forceinline__ int bin_of(float d) {
   return min(static_cast<int>(__float_as_uint(__fmaf_rz(d, -64.0f, 8388608.0f)) & 0x7fffffu),
              kSmBins - 1);
 }
-
-// What the CTAs of a cluster tell one another, one entry per CTA.
-struct Slot {
-  float xmax;
-  int first;                  // lowest index of the maximum
-  double z;                   // sum of e^(x - max)
-  unsigned long long above;   // weight above the min-p cut
-  uint32_t count[2];          // listed tokens, by search parity
-  uint32_t kmin, kmax;        // keys of a bin to be split
-  uint32_t ties;              // tokens with one key
-};
+// Its finer bin within a set that starts at `first` of them.
+__device__ __forceinline__ int fine_of(float d) {
+  return static_cast<int>(__float_as_uint(__fmaf_rz(d, -64.0f * kSmSub, 8388608.0f)) & 0x7fffffu);
+}
 
 struct SampleShared {
-  uint32_t lo[kSmBins], hi[kSmBins];  // then: mass before each bin (64 bits)
-  uint32_t cnt[kSmBins];              // then: tokens before each bin
-  uint32_t wrapped;                   // hi[0] passed 2^32
-  unsigned long long local[2][kSmLocal];
+  uint2 half[kSmBins];    // sums of low and high halves; then: mass before each bin
+  uint32_t cnt[kSmBins];  // tokens; then: tokens before each bin
   unsigned long long list[kSmList];
+  uint2 sub[kSmSub];      // a list's finer bins
+  uint32_t sub_cnt[kSmSub];
   unsigned long long red[kSmWarps];
   unsigned long long red2[kSmWarps];
-  Slot mine;                  // read by the other CTAs
-  unsigned long long total;   // mass and tokens of all bins
+  unsigned long long few[32];  // a fine bin's tokens
+  uint32_t n_few, n_list;
+  uint32_t wrapped;       // half[0].y passed 2^32
+  unsigned long long total;  // mass and tokens of all bins
   uint32_t total_cnt;
-  int bin;
-  unsigned long long before;
-  uint32_t before_cnt, bin_cnt;
-  uint32_t n;                 // local list's length
-  int token;
+  int bin, token, last;
   unsigned long long found;
   uint32_t found_key, found_rank;
 };
-constexpr size_t kSmSlice = (kSmBins + 1) / 2 * 12;  // a CTA's slice of the bins (C >= 2)
+
+__shared__ SampleShared sm_shared;
+#define SM_SHARED sm_shared
 
 template <typename V, typename Op>
 __device__ __forceinline__ V block_reduce(V v, V* s_red, Op op) {
@@ -142,207 +139,210 @@ __device__ __forceinline__ V block_reduce(V v, V* s_red, Op op) {
 }
 
 // Exclusive prefix sums over the CTA of a 64-bit and a 32-bit number.
-__device__ __forceinline__ void block_exclusive(unsigned long long& a, uint32_t& c,
-                                                unsigned long long& ta, uint32_t& tc,
-                                                SampleShared& s) {
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  unsigned long long ai = a;
-  uint32_t ci = c;
+struct Sums {
+  unsigned long long a;
+  uint32_t c;
+};
+__device__ __forceinline__ Sums warp_inclusive(Sums v) {
+  const int lane = threadIdx.x % 32;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long x = __shfl_up_sync(0xffffffffu, ai, o);
-    const uint32_t y = __shfl_up_sync(0xffffffffu, ci, o);
+    const unsigned long long x = __shfl_up_sync(0xffffffffu, v.a, o);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, v.c, o);
     if (lane >= o) {
-      ai += x;
-      ci += y;
+      v.a += x;
+      v.c += y;
     }
-  }
-  if (lane == 31) {
-    s.red[warp] = ai;
-    s.red2[warp] = ci;
-  }
-  __syncthreads();
-  unsigned long long ba = 0;
-  uint32_t bc = 0;
-  ta = 0;
-  tc = 0;
-#pragma unroll
-  for (int w = 0; w < kSmWarps; ++w) {
-    if (w == warp) {
-      ba = ta;
-      bc = tc;
-    }
-    ta += s.red[w];
-    tc += static_cast<uint32_t>(s.red2[w]);
-  }
-  __syncthreads();
-  a = ba + ai - a;
-  c = bc + ci - c;
-}
-
-__device__ __forceinline__ void cluster_sync_all() {
-  __syncwarp();
-  cluster_arrive();
-  cluster_wait();
-}
-template <typename V>
-__device__ __forceinline__ V ld_cluster(const V* local, int rank) {
-  V v;
-  const uint32_t a = mapa_shared(smem_u32(local), rank);
-  if constexpr (sizeof(V) == 8) {
-    unsigned long long x;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(a) : "memory");
-    v = *reinterpret_cast<V*>(&x);
-  } else {
-    uint32_t x;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(a) : "memory");
-    v = *reinterpret_cast<V*>(&x);
   }
   return v;
 }
+__device__ __noinline__ Sums block_exclusive(Sums v, Sums* total) {
+  SampleShared& s = SM_SHARED;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const Sums in = warp_inclusive(v);
+  if (lane == 31) {
+    s.red[warp] = in.a;
+    s.red2[warp] = in.c;
+  }
+  __syncthreads();
+  Sums w{0, 0};
+  if (lane < kSmWarps) {
+    w.a = s.red[lane];
+    w.c = static_cast<uint32_t>(s.red2[lane]);
+  }
+  w = warp_inclusive(w);
+  total->a = __shfl_sync(0xffffffffu, w.a, 31);
+  total->c = __shfl_sync(0xffffffffu, w.c, 31);
+  const unsigned long long ba = __shfl_sync(0xffffffffu, w.a, (warp + 31) & 31);
+  const uint32_t bc = __shfl_sync(0xffffffffu, w.c, (warp + 31) & 31);
+  __syncthreads();
+  return {(warp ? ba : 0) + in.a - v.a, (warp ? bc : 0) + in.c - v.c};
+}
 
-template <typename T>
-struct Row {
-  const T* x;   // this CTA's stretch, in shared memory
-  int n, i0;    // its tokens, and the index of the first
-  int C, rank;  // CTAs of the row, and this one
-  RowScale rs;
-};
+// f(x, i) for tokens [0, n) of a stretch in global memory, in no order: 16-byte
+// loads where the stretch allows, kUnroll of them in flight a thread.
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T* src, int n, F f) {
+  constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
+  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T));
+  const int head = min(n, (kVec - skew) % kVec), vecs = (n - head) / kVec;
+  const int t = threadIdx.x, tail = head + vecs * kVec + t;
+  if (t < head) f(to_f32<T>(src[t]), t);
+  if (tail < n) f(to_f32<T>(src[tail]), tail);
+  const uint4* mid = reinterpret_cast<const uint4*>(src + head);
+  for (int v0 = t; v0 < vecs; v0 += kUnroll * kSmThreads) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (v0 + k * kSmThreads < vecs) w[k] = __ldg(mid + v0 + k * kSmThreads);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      if (v0 + k * kSmThreads >= vecs) break;
+      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        float x;
+        if constexpr (sizeof(T) == 4)
+          x = __uint_as_float(u[e]);
+        else
+          x = e & 1 ? hi_half(u[e / 2], std::is_same<T, __half>::value)
+                    : lo_half(u[e / 2], std::is_same<T, __half>::value);
+        f(x, head + (v0 + k * kSmThreads) * kVec + e);
+      }
+    }
+  }
+}
 
-// The local histograms of all CTAs into mass and tokens before each bin.
-__device__ __forceinline__ void finish_bins(SampleShared& s, uint8_t* slice, int C, int rank) {
-  unsigned long long m[kSmPer];
-  uint32_t c[kSmPer];
+// The bins of the CTA's histogram into mass and tokens before each; `global`:
+// the row's bins, which are cleared (null: s.half and s.cnt).
+__device__ __noinline__ void finish_bins(unsigned long long* global, uint32_t* global_cnt,
+                                         bool counts) {
+  SampleShared& s = SM_SHARED;
+  unsigned long long m[kSmPer] = {0, 0, 0, 0};
+  uint32_t c[kSmPer] = {0, 0, 0, 0};
   const int b0 = threadIdx.x * kSmPer;
-  if (C == 1) {
-    __syncthreads();
-    if (b0 < kSmBins) {
+  __syncthreads();
+  if (b0 < kSmBins) {
+    if (global) {  // written by other CTAs' atomics: read and clear at L2
+      ulonglong2* g = reinterpret_cast<ulonglong2*>(global + b0);
+      const ulonglong2 x = __ldcg(g), y = __ldcg(g + 1);
+      m[0] = x.x, m[1] = x.y, m[2] = y.x, m[3] = y.y;
+      __stcg(g, make_ulonglong2(0, 0));
+      __stcg(g + 1, make_ulonglong2(0, 0));
+      if (counts) {
+        const uint4 n = __ldcg(reinterpret_cast<const uint4*>(global_cnt + b0));
+        c[0] = n.x, c[1] = n.y, c[2] = n.z, c[3] = n.w;
+        __stcg(reinterpret_cast<uint4*>(global_cnt + b0), make_uint4(0, 0, 0, 0));
+      }
+    } else {
 #pragma unroll
       for (int e = 0; e < kSmPer; ++e) {
-        m[e] = (static_cast<unsigned long long>(s.hi[b0 + e]) << 18) + s.lo[b0 + e];
+        const uint2 h = s.half[b0 + e];
+        m[e] = (static_cast<unsigned long long>(h.y) << 18) + h.x;
         c[e] = s.cnt[b0 + e];
       }
-      if (b0 == 0) m[0] += static_cast<unsigned long long>(s.wrapped) << 50;
-    }
-    __syncthreads();
-  } else {
-    const int per = (kSmBins + C - 1) / C;
-    unsigned long long* sm = reinterpret_cast<unsigned long long*>(slice);
-    uint32_t* sc = reinterpret_cast<uint32_t*>(slice + (kSmBins + 1) / 2 * 8);
-    cluster_sync_all();
-    for (int i = threadIdx.x; i < per; i += kSmThreads) {
-      const int b = rank * per + i;
-      unsigned long long mass = 0;
-      uint32_t cnt = 0;
-      if (b < kSmBins) {
-#pragma unroll 4
-        for (int r = 0; r < C; ++r) {
-          mass += (static_cast<unsigned long long>(ld_cluster(&s.hi[b], r)) << 18) +
-                  ld_cluster(&s.lo[b], r);
-          cnt += ld_cluster(&s.cnt[b], r);
-          if (b == 0) mass += static_cast<unsigned long long>(ld_cluster(&s.wrapped, r)) << 50;
-        }
-      }
-      sm[i] = mass;
-      sc[i] = cnt;
-    }
-    cluster_sync_all();
-    if (b0 < kSmBins) {
-#pragma unroll
-      for (int e = 0; e < kSmPer; ++e) {
-        const int r = (b0 + e) / per, i = b0 + e - r * per;
-        m[e] = ld_cluster(sm + i, r);
-        c[e] = ld_cluster(sc + i, r);
-      }
     }
   }
-  unsigned long long a = 0, ta;
-  uint32_t k = 0, tk;
-  if (b0 < kSmBins) {
+  __syncthreads();
+  Sums v{0, 0}, total;
 #pragma unroll
-    for (int e = 0; e < kSmPer; ++e) {
-      a += m[e];
-      k += c[e];
-    }
+  for (int e = 0; e < kSmPer; ++e) {
+    v.a += m[e];
+    v.c += c[e];
   }
-  block_exclusive(a, k, ta, tk, s);
+  v = block_exclusive(v, &total);
   if (b0 < kSmBins) {
-    // bin b's mass at word b of the joined lo / hi arrays
-    unsigned long long* mass = reinterpret_cast<unsigned long long*>(s.lo);
+    unsigned long long* mass = reinterpret_cast<unsigned long long*>(s.half);
 #pragma unroll
     for (int e = 0; e < kSmPer; ++e) {
-      mass[b0 + e] = a;
-      s.cnt[b0 + e] = k;
-      a += m[e];
-      k += c[e];
+      mass[b0 + e] = v.a;
+      s.cnt[b0 + e] = v.c;
+      v.a += m[e];
+      v.c += c[e];
     }
   }
   if (threadIdx.x == 0) {
-    s.total = ta;
-    s.total_cnt = tk;
+    s.total = total.a;
+    s.total_cnt = total.c;
   }
   __syncthreads();
 }
 
-// The bin where the running count or mass reaches `goal` (1 .. the total).
-template <bool BY_COUNT>
-__device__ __forceinline__ void find_bin(unsigned long long goal, SampleShared& s) {
-  const unsigned long long* mass = reinterpret_cast<const unsigned long long*>(s.lo);
-  for (int b = threadIdx.x; b < kSmBins; b += kSmThreads) {
-    const bool end = b + 1 == kSmBins;
-    const unsigned long long m1 = end ? s.total : mass[b + 1];
-    const uint32_t c1 = end ? s.total_cnt : s.cnt[b + 1];
-    const unsigned long long v0 = BY_COUNT ? s.cnt[b] : mass[b], v1 = BY_COUNT ? c1 : m1;
-    if (v0 < goal && goal <= v1) {  // one bin only
-      s.bin = b;
-      s.before = mass[b];
-      s.before_cnt = s.cnt[b];
-      s.bin_cnt = c1 - s.cnt[b];
-    }
+// The bin where the running count or mass reaches `goal` (1 .. the total):
+// the last one with less before it.  Every thread searches for itself.
+__device__ __forceinline__ int find_bin(bool by_count, unsigned long long goal) {
+  SampleShared& s = SM_SHARED;
+  const unsigned long long* mass = reinterpret_cast<const unsigned long long*>(s.half);
+  int lo = 0;
+#pragma unroll 1
+  for (int step = 1024; step > 0; step >>= 1) {
+    const int b = lo + step;
+    if (b < kSmBins && (by_count ? s.cnt[b] : mass[b]) < goal) lo = b;
   }
-  __syncthreads();
+  return lo;
+}
+__device__ __forceinline__ unsigned long long mass_before(int b) {
+  return b < kSmBins ? reinterpret_cast<const unsigned long long*>(SM_SHARED.half)[b] : SM_SHARED.total;
 }
 
-__device__ __forceinline__ void clear_bins(SampleShared& s) {
-  for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) s.lo[i] = s.hi[i] = s.cnt[i] = 0;
+__device__ __forceinline__ void clear_bins() {
+  SampleShared& s = SM_SHARED;
+  for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) {
+    s.half[i] = make_uint2(0, 0);
+    s.cnt[i] = 0;
+  }
   if (threadIdx.x == 0) s.wrapped = 0;
   __syncthreads();
 }
 
-// Histogram over the exponents.
-template <typename T>
-__device__ __forceinline__ void exponent_bins(const Row<T>& row, bool counts, SampleShared& s) {
-  clear_bins(s);
-  for (int i = threadIdx.x; i < row.n; i += kSmThreads) {
-    const float d = exponent(to_f32<T>(row.x[i]), row.rs);
-    if (!(d >= -25.0f)) continue;
-    const Halves h = halves(expf(d));
-    const int b = bin_of(d);
-    atomicAdd(&s.lo[b], h.lo);
-    if (h.hi < (1u << 18)) {
-      if (h.hi) atomicAdd(&s.hi[b], h.hi);
-    } else if (atomicAdd(&s.hi[b], 1u << 18) == 0u - (1u << 18)) {
-      s.wrapped = 1;
-    }
-    if (counts) atomicAdd(&s.cnt[b], 1u);
-  }
+// The goals that follow from the mass kept so far: top-p's, and the token's.
+__device__ __forceinline__ unsigned long long goal_p(unsigned long long mass, float top_p) {
+  const double want = ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(mass));
+  return max(1ull, min(mass, static_cast<unsigned long long>(want)));
+}
+__device__ __forceinline__ unsigned long long goal_t(unsigned long long mass, float u) {
+  const double t = floor(static_cast<double>(u) * static_cast<double>(mass));
+  return (t > 0.0 ? min(mass - 1, static_cast<unsigned long long>(t)) : 0ull) + 1;
 }
 
-// A set of tokens: one exponent bin, or a range of keys.
+// A set of tokens: exponent bins b0 .. b1, or a range of keys.
 struct Pick {
-  int bin;  // -1: keys klo .. khi
+  int b0, b1;  // b0 -1: keys klo .. khi
   uint32_t klo, khi;
-  template <typename T>
-  __device__ __forceinline__ bool has(const Row<T>& row, int i, uint32_t& key) const {
-    const float x = to_f32<T>(row.x[i]);
-    if (bin >= 0) {
-      const float d = exponent(x, row.rs);
-      if (!(d >= -25.0f) || bin_of(d) != bin) return false;
-      key = key_of(x + 0.0f);
-      return true;
+  float xlo, xhi;  // every token of the set lies between them
+  // The bins' logits, widened by more than the roundings of the exponent.
+  __device__ __forceinline__ void bin_range(int first, int last, float xmax, float T0) {
+    b0 = first;
+    b1 = last;
+    const float far = (last + 1) / 64.0f * T0;
+    const float slack = 4e-6f * (fabsf(xmax) + far) + 1e-30f;
+    xlo = xmax - far - slack;
+    xhi = xmax - first / 64.0f * T0 + slack;
+    if (!(far < 1e30f && slack < 1e30f)) {
+      xlo = -INFINITY;
+      xhi = INFINITY;
     }
-    key = key_of(clean(x));
-    return key >= klo && key <= khi;
+  }
+  __device__ __forceinline__ void nothing() {
+    b0 = b1 = 0;
+    xlo = INFINITY;
+    xhi = -INFINITY;
+  }
+  __device__ __forceinline__ void key_range(uint32_t lo, uint32_t hi) {
+    b0 = -1;
+    klo = lo;
+    khi = hi;
+    xlo = logit_of(lo);
+    xhi = logit_of(hi);
+  }
+  __device__ __forceinline__ bool has(float x, const RowScale& rs, uint32_t& key) const {
+    if (!(x >= xlo && x <= xhi)) return false;
+    key = key_of(x + 0.0f);
+    if (b0 < 0) return key >= klo && key <= khi;
+    const float d = exponent(x, rs);
+    if (!(d >= -25.0f)) return false;
+    const int b = bin_of(d);
+    return b >= b0 && b <= b1;
   }
 };
 
@@ -352,364 +352,547 @@ struct Found {
   uint32_t key, rank;
 };
 
-// The token where the running count or mass of the whole row first reaches
-// `goal`.  `nth` counts the searches of the row; the exponent bins are valid
-// on entry if `*bins`, which a split clears.
-template <typename T, bool BY_COUNT>
-__device__ Found find_prefix(const Row<T>& row, unsigned long long goal, int& nth, bool& bins,
-                             bool counts, SampleShared& s, uint8_t* slice) {
-  if (!bins) {
-    exponent_bins(row, counts, s);
-    finish_bins(s, slice, row.C, row.rank);
-    bins = true;
+// The token of the list (n tokens, all of a set) where the running count or
+// mass reaches `goal`, counted from the set's start: in s.found (the mass up to
+// and with it), s.token, s.found_key.  The list is binned again, finer (2^-15
+// 2^coarse in the exponent, from fine bin fine0 on), and the few tokens of the
+// fine bin that holds the goal are ranked by one warp; should they be many, the
+// list is sorted.
+__device__ __noinline__ void find_listed(bool by_count, uint32_t n, unsigned long long goal,
+                                         int fine0, int coarse, float xmax, float inv) {
+  SampleShared& s = SM_SHARED;
+  const RowScale rs{xmax, inv};
+  const int lane = threadIdx.x % 32;
+  s.sub[threadIdx.x] = make_uint2(0, 0);
+  s.sub_cnt[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s.n_few = 0;
+  __syncthreads();
+  int fine[2] = {-1, -1};
+#pragma unroll
+  for (int e = 0; e < kSmList / kSmThreads; ++e) {
+    const uint32_t i = threadIdx.x + e * kSmThreads;
+    if (i >= n) continue;
+    const float d = exponent(logit_of(~static_cast<uint32_t>(s.list[i] >> 32)), rs);
+    const Halves h = halves(expf(d));
+    fine[e] = min(max(fine_of(d) - fine0, 0) >> coarse, kSmSub - 1);
+    atomicAdd(&s.sub[fine[e]].x, h.lo);
+    if (h.hi) atomicAdd(&s.sub[fine[e]].y, h.hi);
+    atomicAdd(&s.sub_cnt[fine[e]], 1u);
   }
-  find_bin<BY_COUNT>(goal, s);
-  Pick pick{s.bin, 0, 0};
-  while (true) {
-    const unsigned long long before = s.before;
-    const uint32_t before_cnt = s.before_cnt;
-    // ---- list the set's tokens
-    const int par = nth++ & 1;
+  __syncthreads();
+  const uint2 h = s.sub[threadIdx.x];
+  const Sums v{(static_cast<unsigned long long>(h.y) << 18) + h.x, s.sub_cnt[threadIdx.x]};
+  Sums total;
+  const Sums at = block_exclusive(v, &total);
+  if (by_count ? at.c < goal && goal <= at.c + v.c : at.a < goal && goal <= at.a + v.a) {
+    s.bin = threadIdx.x;  // one bin only
+    s.found = at.a;
+    s.found_rank = at.c;
+  }
+  __syncthreads();
+  const int bin = s.bin;
+  const unsigned long long mass0 = s.found;
+  const uint32_t cnt0 = s.found_rank, few = s.sub_cnt[bin];
+  if (few <= 32) {
+#pragma unroll
+    for (int e = 0; e < kSmList / kSmThreads; ++e)
+      if (fine[e] == bin) s.few[atomicAdd(&s.n_few, 1u)] = s.list[threadIdx.x + e * kSmThreads];
     __syncthreads();
-    if (threadIdx.x == 0) s.n = 0;
+    if (threadIdx.x < 32) {
+      const bool real = lane < static_cast<int>(few);
+      const unsigned long long mine = real ? s.few[lane] : ~0ull;
+      unsigned long long w = 0;
+      if (real) w = weight(exponent(logit_of(~static_cast<uint32_t>(mine >> 32)), rs));
+      unsigned long long mass = mass0;  // up to and with this token
+      uint32_t cnt = cnt0;
+#pragma unroll 1
+      for (uint32_t j = 0; j < few; ++j) {
+        const unsigned long long other = __shfl_sync(0xffffffffu, mine, j);
+        const unsigned long long ow = __shfl_sync(0xffffffffu, w, j);
+        if (other <= mine) {
+          mass += ow;
+          ++cnt;
+        }
+      }
+      if (real && (by_count ? cnt == goal : mass - w < goal && goal <= mass)) {
+        s.found = mass;
+        s.token = static_cast<int>(mine & 0xffffffffu);
+        s.found_key = ~static_cast<uint32_t>(mine >> 32);
+      }
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < row.n; i += kSmThreads) {
+    return;
+  }
+  // ---- sort the list (bitonic, ascending: the largest logit, lowest index first)
+  uint32_t size = 2;
+  while (size < n) size <<= 1;
+  for (uint32_t i = n + threadIdx.x; i < size; i += kSmThreads) s.list[i] = ~0ull;
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t k = 2; k <= size; k <<= 1)
+#pragma unroll 1
+    for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+      for (uint32_t i = threadIdx.x; i < size / 2; i += kSmThreads) {
+        const uint32_t lo = ((i & ~(j - 1)) << 1) | (i & (j - 1)), hi = lo | j;
+        const unsigned long long a = s.list[lo], b = s.list[hi];
+        if ((a > b) == ((lo & k) == 0)) {
+          s.list[lo] = b;
+          s.list[hi] = a;
+        }
+      }
+      __syncthreads();
+    }
+  // ---- running mass over it, two tokens a thread
+  const uint32_t i = 2 * threadIdx.x;
+  unsigned long long w[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    w[e] = i + e < n ? weight(exponent(logit_of(~static_cast<uint32_t>(s.list[i + e] >> 32)), rs)) : 0;
+  unsigned long long a = block_exclusive({w[0] + w[1], 0}, &total).a;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const bool hit = by_count ? i + e + 1 == goal : a < goal && goal <= a + w[e];
+    a += w[e];
+    if (hit && i + e < n) {
+      s.found = a;
+      s.token = static_cast<int>(s.list[i + e] & 0xffffffffu);
+      s.found_key = ~static_cast<uint32_t>(s.list[i + e] >> 32);
+    }
+  }
+  __syncthreads();
+}
+
+// The slow way to the token where the running count or mass of the row first
+// reaches `goal`, for a set that its list did not hold, by this CTA alone: bins
+// first .. last of the exponent hold the goal, and before / before_cnt come
+// before them.
+template <typename T>
+__device__ __noinline__ Found find_by_splitting(const T* row, int vocab, RowScale rs, float T0,
+                                                bool by_count, unsigned long long goal, int first,
+                                                int last, unsigned long long before,
+                                                uint32_t before_cnt) {
+  SampleShared& s = SM_SHARED;
+  Pick pick;
+  pick.bin_range(first, last, rs.xmax, T0);
+  {
+    uint32_t kmin = 0xffffffffu, kmax = 0;
+    each(row, vocab, [&](float x, int) {
       uint32_t key;
-      if (!pick.has(row, i, key)) continue;
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < kSmLocal)
-        s.local[par][at] = (static_cast<unsigned long long>(~key) << 32) |
-                           static_cast<uint32_t>(row.i0 + i);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) s.mine.count[par] = s.n;
-    cluster_sync_all();
-    uint32_t total = 0;
-    bool fits = true;
-    for (int r = 0; r < row.C; ++r) {
-      const uint32_t n = ld_cluster(&s.mine.count[par], r);
-      fits = fits && n <= kSmLocal;
-      if (fits && total + n <= kSmList)
-        for (uint32_t i = threadIdx.x; i < n; i += kSmThreads)
-          s.list[total + i] = ld_cluster(&s.local[par][i], r);
-      total += n;
-    }
-    if (fits && total <= kSmList) {
-      // ---- sort it (bitonic, ascending: the largest logit, lowest index first)
-      uint32_t size = 2;
-      while (size < total) size <<= 1;
-      for (uint32_t i = total + threadIdx.x; i < size; i += kSmThreads) s.list[i] = ~0ull;
-      __syncthreads();
-      for (uint32_t k = 2; k <= size; k <<= 1)
-        for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-          for (uint32_t i = threadIdx.x; i < size / 2; i += kSmThreads) {
-            const uint32_t lo = ((i & ~(j - 1)) << 1) | (i & (j - 1)), hi = lo | j;
-            const unsigned long long a = s.list[lo], b = s.list[hi];
-            if ((a > b) == ((lo & k) == 0)) {
-              s.list[lo] = b;
-              s.list[hi] = a;
-            }
-          }
-          __syncthreads();
-        }
-      // ---- running mass over it, two tokens a thread
-      const uint32_t i = 2 * threadIdx.x;
-      unsigned long long w[2], a, ta;
-      uint32_t c = 0, tc;
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        w[e] = i + e < total
-                   ? weight(exponent(logit_of(~static_cast<uint32_t>(s.list[i + e] >> 32)), row.rs))
-                   : 0;
-      a = w[0] + w[1];
-      block_exclusive(a, c, ta, tc, s);
-      a += before;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool hit = BY_COUNT ? before_cnt + i + e + 1 == goal
-                                  : a < goal && goal <= a + w[e];
-        a += w[e];
-        if (hit && i + e < total) {
-          s.found = a;
-          s.token = static_cast<int>(s.list[i + e] & 0xffffffffu);
-          s.found_key = ~static_cast<uint32_t>(s.list[i + e] >> 32);
-        }
-      }
-      __syncthreads();
-      return {s.found, s.token, s.found_key, 0};
-    }
-    // ---- too many: split the set by its keys
-    if (pick.bin >= 0) {
-      uint32_t kmin = 0xffffffffu, kmax = 0;
-      for (int i = threadIdx.x; i < row.n; i += kSmThreads) {
-        uint32_t key;
-        if (!pick.has(row, i, key)) continue;
-        kmin = min(kmin, key);
-        kmax = max(kmax, key);
-      }
-      uint32_t* red = reinterpret_cast<uint32_t*>(s.red);
-      kmin = block_reduce(kmin, red, [](uint32_t a, uint32_t b) { return min(a, b); });
-      kmax = block_reduce(kmax, red, [](uint32_t a, uint32_t b) { return max(a, b); });
-      if (threadIdx.x == 0) {
-        s.mine.kmin = kmin;
-        s.mine.kmax = kmax;
-      }
-      cluster_sync_all();
-      for (int r = 0; r < row.C; ++r) {
-        kmin = min(kmin, ld_cluster(&s.mine.kmin, r));
-        kmax = max(kmax, ld_cluster(&s.mine.kmax, r));
-      }
-      pick = {-1, kmin, kmax};
-    }
+      if (!pick.has(x, rs, key)) return;
+      kmin = min(kmin, key);
+      kmax = max(kmax, key);
+    });
+    uint32_t* red = reinterpret_cast<uint32_t*>(s.red);
+    kmin = block_reduce(kmin, red, [](uint32_t a, uint32_t b) { return min(a, b); });
+    kmax = block_reduce(kmax, red, [](uint32_t a, uint32_t b) { return max(a, b); });
+    pick.key_range(kmin, kmax);
+  }
+  while (true) {
     if (pick.klo == pick.khi) {  // equal logits: the rank follows from the goal
-      const unsigned long long w = weight(exponent(logit_of(pick.klo), row.rs));
-      const uint32_t rank = BY_COUNT ? static_cast<uint32_t>(goal - before_cnt)
+      const unsigned long long w = weight(exponent(logit_of(pick.klo), rs));
+      const uint32_t rank = by_count ? static_cast<uint32_t>(goal - before_cnt)
                                      : static_cast<uint32_t>((goal - before + w - 1) / w);
       return {before + rank * w, -1, pick.klo, rank};
     }
-    bins = false;
     const uint32_t range = pick.khi - pick.klo;
     const int shift = max(0, 32 - __clz(range) - 10);  // at most 1024 bins
-    clear_bins(s);
-    for (int i = threadIdx.x; i < row.n; i += kSmThreads) {
-      uint32_t key;
-      if (!pick.has(row, i, key)) continue;
-      const uint32_t b = (pick.khi - key) >> shift;
-      const unsigned long long w = weight(exponent(logit_of(key), row.rs));
-      atomicAdd(&s.lo[b], static_cast<uint32_t>(w) & 0x3ffffu);
-      atomicAdd(&s.hi[b], static_cast<uint32_t>(w >> 18));
-      atomicAdd(&s.cnt[b], 1u);
+    // The row is histogrammed by stretches whose halves cannot overflow (not
+    // all of these tokens are at the maximum: there are two keys), into 64-bit
+    // sums kept one bin or two a thread.
+    unsigned long long mass[2] = {0, 0};
+    uint32_t cnt[2] = {0, 0};
+    for (int i0 = 0; i0 < vocab; i0 += kSmChunk) {
+      __syncthreads();
+      clear_bins();
+      each(row + i0, min(vocab - i0, kSmChunk), [&](float x, int) {
+        uint32_t key;
+        if (!pick.has(x, rs, key)) return;
+        const uint32_t b = (pick.khi - key) >> shift;
+        const unsigned long long w = weight(exponent(logit_of(key), rs));
+        atomicAdd(&s.half[b].x, static_cast<uint32_t>(w) & 0x3ffffu);
+        if (atomicAdd(&s.half[b].y, static_cast<uint32_t>(w >> 18)) >= 0u - (1u << 18) &&
+            (w >> 36))
+          s.wrapped = 1;  // a whole stretch at the maximum
+        atomicAdd(&s.cnt[b], 1u);
+      });
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint2 h = s.half[2 * threadIdx.x + e];
+        mass[e] += (static_cast<unsigned long long>(h.y) << 18) + h.x;
+        if (s.wrapped && threadIdx.x + e == 0) mass[e] += 1ull << 50;
+        cnt[e] += s.cnt[2 * threadIdx.x + e];
+      }
     }
-    finish_bins(s, slice, row.C, row.rank);
-    // the goal counts from the row's start, the bins from the set's
-    find_bin<BY_COUNT>(goal - (BY_COUNT ? before_cnt : before), s);
+    Sums total;
+    Sums at = block_exclusive({mass[0] + mass[1], cnt[0] + cnt[1]}, &total);
+    const unsigned long long want = goal - (by_count ? before_cnt : before);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const Sums end{at.a + mass[e], at.c + cnt[e]};
+      if (by_count ? at.c < want && want <= end.c : at.a < want && want <= end.a) {
+        s.bin = 2 * threadIdx.x + e;  // one bin only
+        s.found = at.a;
+        s.found_rank = at.c;
+      }
+      at = end;
+    }
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
     const uint32_t top = pick.khi - (static_cast<uint32_t>(s.bin) << shift);
     const uint32_t low = shift == 0 ? top : top - min(top - pick.klo, (1u << shift) - 1);
+    before += s.found;
+    before_cnt += s.found_rank;
+    pick.key_range(low, top);
+    each(row, vocab, [&](float x, int i) {
+      uint32_t key;
+      if (!pick.has(x, rs, key)) return;
+      const uint32_t n = atomicAdd(&s.n_list, 1u);
+      if (n < kSmList)
+        s.list[n] = (static_cast<unsigned long long>(~key) << 32) | static_cast<uint32_t>(i);
+    });
     __syncthreads();
-    if (threadIdx.x == 0) {
-      s.before += before;
-      s.before_cnt += before_cnt;
+    const uint32_t n = s.n_list;
+    if (n <= kSmList) {
+      find_listed(by_count, n, goal - (by_count ? before_cnt : before),
+                  fine_of(exponent(logit_of(top), rs)), 0, rs.xmax, rs.inv);
+      return {before + s.found, s.token, s.found_key, 0};
     }
     __syncthreads();
-    pick = {-1, low, top};
   }
 }
 
-// Writes the index of the `rank`-th (1-based) token of the row with this key.
+// Index of the `rank`-th (1-based) token of the row with this key.
 template <typename T>
-__device__ void write_ranked(const Row<T>& row, uint32_t key, uint32_t rank, int* out,
-                             SampleShared& s) {
+__device__ __noinline__ int find_ranked(const T* row, int vocab, uint32_t key, uint32_t rank) {
+  SampleShared& s = SM_SHARED;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int per = ((row.n + kSmWarps - 1) / kSmWarps + 31) / 32 * 32;
-  const int i0 = min(row.n, warp * per), i1 = min(row.n, i0 + per);
+  const int per = ((vocab + kSmWarps - 1) / kSmWarps + 31) / 32 * 32;
+  const int i0 = min(vocab, warp * per), i1 = min(vocab, i0 + per);
   uint32_t n = 0;
-  for (int i = i0 + lane; i < i1; i += 32) n += key_of(clean(to_f32<T>(row.x[i]))) == key;
+  for (int i = i0 + lane; i < i1; i += 32) n += key_of(clean(to_f32<T>(row[i]))) == key;
   n = __reduce_add_sync(0xffffffffu, n);
+  __syncthreads();
   if (lane == 0) s.red[warp] = n;
   __syncthreads();
-  uint32_t before = 0, mine = 0;
-  for (int w = 0; w < kSmWarps; ++w) {
-    if (w == warp) before = mine;
-    mine += static_cast<uint32_t>(s.red[w]);
-  }
-  if (threadIdx.x == 0) s.mine.ties = mine;
-  cluster_sync_all();
-  for (int r = 0; r < row.rank; ++r) before += ld_cluster(&s.mine.ties, r);
-  if (before < rank && before + n >= rank) {  // one warp of the row
+  uint32_t before = 0;
+  for (int w = 0; w < warp; ++w) before += static_cast<uint32_t>(s.red[w]);
+  if (before < rank && before + n >= rank) {  // one warp
     for (int i = i0; i < i1; i += 32) {
-      const bool hit = i + lane < i1 && key_of(clean(to_f32<T>(row.x[i + lane]))) == key;
+      const bool hit = i + lane < i1 && key_of(clean(to_f32<T>(row[i + lane]))) == key;
       const uint32_t m = __ballot_sync(0xffffffffu, hit);
       const uint32_t here = __popc(m);
       if (before + here >= rank) {
-        if (hit && before + __popc(m & ((1u << lane) - 1)) + 1 == rank) *out = row.i0 + i + lane;
+        if (hit && before + __popc(m & ((1u << lane) - 1)) + 1 == rank) s.token = i + lane;
         break;
       }
       before += here;
     }
   }
+  __syncthreads();
+  return s.token;
+}
+
+// ---------------------------------------------------------------- the launches
+
+// The row's settings.
+struct Setting {
+  float T0, inv, top_p, min_p, u;
+  int top_k;
+  bool greedy;
+};
+__device__ __forceinline__ Setting setting(const SampleParams& p, int b) {
+  Setting c;
+  c.T0 = p.temperature ? __ldg(p.temperature + b) : 1.0f;
+  c.top_k = p.top_k ? __ldg(p.top_k + b) : 0;
+  c.top_p = p.top_p ? __ldg(p.top_p + b) : 1.0f;
+  c.min_p = p.min_p ? __ldg(p.min_p + b) : 0.0f;
+  c.u = __ldg(p.u + b);
+  c.inv = __fdiv_rn(1.0f, c.T0);
+  c.greedy = !(c.T0 > 0.0f && c.inv < INFINITY);
+  return c;
+}
+// The stretch of a CTA.
+template <typename T>
+struct Stretch {
+  const T* row;
+  int b, i0, n, parts, part;
+  SampleRow* ws;
+  __device__ __forceinline__ Stretch(const SampleParams& p) {
+    parts = (p.vocab + p.chunk - 1) / p.chunk;
+    b = blockIdx.x / parts;
+    part = blockIdx.x - b * parts;
+    i0 = part * p.chunk;
+    n = min(p.vocab - i0, p.chunk);
+    row = static_cast<const T*>(p.logits) + b * p.ld;
+    ws = p.rows + b;
+  }
+};
+__device__ __forceinline__ float best_logit(unsigned long long best) {
+  return logit_of(static_cast<uint32_t>(best >> 32));
+}
+// True for the last CTA of the row to come here; everything the others wrote
+// before is then visible.  The ticket is left at zero.
+__device__ __forceinline__ bool last_of_row(uint32_t* ticket, int parts) {
+  SampleShared& s = SM_SHARED;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    const bool last = atomicAdd(ticket, 1u) == static_cast<uint32_t>(parts) - 1;
+    if (last) *ticket = 0;
+    __threadfence();
+    s.last = last;
+  }
+  __syncthreads();
+  return s.last != 0;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSmThreads) sample_kernel(SampleParams p, int C) {
-  extern __shared__ __align__(16) uint8_t sm_smem[];
-  SampleShared& s = *reinterpret_cast<SampleShared*>(sm_smem);
-  uint8_t* slice = sm_smem + (sizeof(SampleShared) + 15) / 16 * 16;
-  T* data = reinterpret_cast<T*>(slice + (C > 1 ? (kSmSlice + 15) / 16 * 16 : 0));
-  const int b = blockIdx.x / C, rank = blockIdx.x - b * C;
-  const int per = (p.vocab + C - 1) / C;
-  Row<T> row;
-  row.C = C;
-  row.rank = rank;
-  row.i0 = min(p.vocab, rank * per);
-  row.n = min(p.vocab, row.i0 + per) - row.i0;
-  const T* src = static_cast<const T*>(p.logits) + b * p.ld + row.i0;
-
-  // ---- 1. the stretch into shared memory, at the source's offset within 16
-  // bytes so that the middle goes by 16-byte copies
-  constexpr int kVec = 16 / sizeof(T);
-  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T));
-  T* x = data + skew;
-  row.x = x;
-  const int head = min(row.n, (kVec - skew) % kVec), vecs = (row.n - head) / kVec;
-  for (int i = threadIdx.x; i < vecs; i += kSmThreads)
-    cp_async16(x + head + i * kVec, src + head + i * kVec, true);
-  if (threadIdx.x < head) x[threadIdx.x] = src[threadIdx.x];
-  const int tail = head + vecs * kVec + threadIdx.x;
-  if (tail < row.n) x[tail] = src[tail];
-  const float T0 = p.temperature ? p.temperature[b] : 1.0f;
-  const int k = p.top_k ? p.top_k[b] : 0;
-  const float tp = p.top_p ? p.top_p[b] : 1.0f;
-  const float mp = p.min_p ? p.min_p[b] : 0.0f;
-  row.rs.inv = __fdiv_rn(1.0f, T0);
-  const bool greedy = !(T0 > 0.0f && row.rs.inv < INFINITY);
-  cp_async_wait_all();
-  __syncthreads();
+__global__ void __launch_bounds__(kSmThreads) sample_max_kernel(SampleParams p) {
+  griddep_launch_dependents();
+  griddep_wait();  // the logits, and the previous call's use of the workspace
+  const Stretch<T> st(p);
   float mx = -INFINITY;
-  for (int i = threadIdx.x; i < row.n; i += kSmThreads) mx = fmaxf(mx, to_f32<T>(x[i]));
-  mx = block_reduce(mx, reinterpret_cast<float*>(s.red), [](float a, float c) { return fmaxf(a, c); });
-  if (threadIdx.x == 0) s.mine.xmax = mx;
-  cluster_sync_all();
-  for (int r = 0; r < C; ++r) mx = fmaxf(mx, ld_cluster(&s.mine.xmax, r));
-  row.rs.xmax = mx + 0.0f;
-
-  if (mx == -INFINITY) {  // nothing to choose from
-    if (rank == 0 && threadIdx.x == 0) {
-      p.tokens[b] = -1;
-      if (p.logprobs) p.logprobs[b] = -INFINITY;
+  int at = INT32_MAX;
+  each(st.row + st.i0, st.n, [&](float x, int i) {
+    if (x > mx || (x == mx && i < at)) {  // false for NaN; -0 ties with 0
+      mx = x;
+      at = i;
     }
-    cluster_sync_all();  // shared memory is read by the other CTAs until here
-    return;
-  }
+  });
+  if (at == INT32_MAX) at = 0;  // nothing above -inf here
+  const unsigned long long mine =
+      (static_cast<unsigned long long>(key_of(mx + 0.0f)) << 32) | ~static_cast<uint32_t>(st.i0 + at);
+  const unsigned long long best =
+      block_reduce(mine, SM_SHARED.red, [](unsigned long long a, unsigned long long b) { return max(a, b); });
+  if (threadIdx.x == 0) atomicMax(&st.ws->best, best);
+}
 
-  // ---- sums that need no order: e^(x - max) for the log-probability (f64 over
-  // f32 terms: a peaked row adds tens of thousands of tiny terms to 1), the
-  // weight above the min-p cut, and the first maximum of a greedy row
-  const float dmin = mp > 0.0f ? fminf(static_cast<float>(log(static_cast<double>(mp))), 0.0f)
-                               : -INFINITY;
+template <typename T>
+__global__ void __launch_bounds__(kSmThreads) sample_bins_kernel(SampleParams p) {
+  SampleShared& s = SM_SHARED;
+  griddep_launch_dependents();
+  const Stretch<T> st(p);
+  clear_bins();
+  griddep_wait();
+  const Setting c = setting(p, st.b);
+  const RowScale rs{best_logit(__ldcg(&st.ws->best)), c.inv};
+  const bool empty = rs.xmax == -INFINITY;
+  if (empty || (c.greedy && !p.logprobs)) return;  // every CTA of the row alike
+  const bool sampled = !c.greedy, counts = sampled && c.top_k > 0 && c.top_k < p.vocab;
+  const float dmin = c.min_p > 0.0f
+                         ? fminf(static_cast<float>(log(static_cast<double>(c.min_p))), 0.0f)
+                         : -INFINITY;
+  const bool floor_p = sampled && c.min_p > 0.0f;
+  unsigned long long above = 0;  // weight above the min-p cut
+  // sum of e^(x - max) for the log-probability: f64 over f32 terms, because a
+  // peaked row adds tens of thousands of tiny terms to 1
   double z = 0.0;
+  float zpart = 0.0f;
+  int nz = 0;
+  each(st.row + st.i0, st.n, [&](float x, int) {
+    const float d = exponent(x, rs);
+    float e = 0.0f;
+    if (sampled && d >= -25.0f) {
+      e = expf(d);
+      const Halves h = halves(e);
+      const int b = bin_of(d);
+      atomicAdd(&s.half[b].x, h.lo);
+      if (h.hi < (1u << 18)) {
+        if (h.hi) atomicAdd(&s.half[b].y, h.hi);
+      } else if (atomicAdd(&s.half[b].y, 1u << 18) == 0u - (1u << 18)) {
+        s.wrapped = 1;
+      }
+      if (counts) atomicAdd(&s.cnt[b], 1u);
+      if (floor_p && d >= dmin) above += (static_cast<unsigned long long>(h.hi) << 18) + h.lo;
+    }
+    if (p.logprobs) {
+      const float ez = expf(delta(x, rs.xmax));
+      zpart += ez == ez ? ez : 0.0f;
+      if (++nz % 4 == 0) {
+        z += static_cast<double>(zpart);
+        zpart = 0.0f;
+      }
+    }
+  });
   if (p.logprobs) {
-    for (int i = threadIdx.x; i < row.n; i += kSmThreads) {
-      const float e = expf(delta(to_f32<T>(x[i]), mx));
-      z += e == e ? static_cast<double>(e) : 0.0;
-    }
-    z = block_reduce(z, reinterpret_cast<double*>(s.red), [](double a, double c) { return a + c; });
+    z = block_reduce(z + static_cast<double>(zpart), reinterpret_cast<double*>(s.red),
+                     [](double a, double b) { return a + b; });
+    if (threadIdx.x == 0) st.ws->z[st.part] = z;
   }
-  unsigned long long above = 0;
-  if (!greedy && mp > 0.0f) {
-    for (int i = threadIdx.x; i < row.n; i += kSmThreads) {
-      const float d = exponent(to_f32<T>(x[i]), row.rs);
-      if (d >= dmin) above += weight(d);
-    }
-    above = block_reduce(above, s.red, [](unsigned long long a, unsigned long long c) { return a + c; });
+  if (floor_p) {
+    above = block_reduce(above, s.red, [](unsigned long long a, unsigned long long b) { return a + b; });
+    if (threadIdx.x == 0) atomicAdd(&st.ws->above, above);
   }
-  int first = INT32_MAX;
-  if (greedy) {
-    for (int i = threadIdx.x; i < row.n; i += kSmThreads)
-      if (to_f32<T>(x[i]) == mx) first = min(first, row.i0 + i);
-    first = block_reduce(first, reinterpret_cast<int*>(s.red), [](int a, int c) { return min(a, c); });
+  if (sampled) {  // the row's bins: whole numbers, in any order
+    __syncthreads();
+    for (int b = threadIdx.x; b < kSmBins; b += kSmThreads) {
+      const uint2 h = s.half[b];
+      unsigned long long m = (static_cast<unsigned long long>(h.y) << 18) + h.x;
+      if (b == 0) m += static_cast<unsigned long long>(s.wrapped) << 50;
+      if (m) atomicAdd(&st.ws->bins[b], m);
+      if (counts && s.cnt[b]) atomicAdd(&st.ws->cnt[b], s.cnt[b]);
+    }
+  }
+  if (!last_of_row(&st.ws->ticket, st.parts)) return;
+
+  // ---- the whole row is in: where each position can lie
+  if (p.logprobs && threadIdx.x < 32) {  // in one order, whatever CTA does it
+    double sum = 0.0;
+    for (int r = threadIdx.x; r < st.parts; r += 32) sum += __ldcg(&st.ws->z[r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x == 0) st.ws->log_z = log(sum);
+  }
+  if (!sampled) return;
+  finish_bins(st.ws->bins, st.ws->cnt, counts);
+  const bool cut_k = counts && static_cast<uint32_t>(c.top_k) < s.total_cnt, cut_p = c.top_p < 1.0f;
+  if (floor_p) above = __ldcg(&st.ws->above);
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  SampleSet* set = st.ws->set;
+  const auto place = [&](SampleSet& q, int first, int last) {
+    q.b0 = first;
+    q.b1 = last;
+    q.before = mass_before(first);
+    q.before_cnt = s.cnt[first];
+  };
+  unsigned long long lo = s.total, hi = lo;  // the mass kept so far lies between
+  set[0].b0 = set[1].b0 = -1;  // not asked for
+  if (cut_k) {
+    const int bin = find_bin(true, c.top_k);
+    place(set[0], bin, bin);
+    lo = max(1ull, set[0].before);
+    hi = mass_before(bin + 1);
+  }
+  if (cut_p) {
+    place(set[1], find_bin(false, goal_p(lo, c.top_p)), find_bin(false, goal_p(hi, c.top_p)));
+    lo = max(1ull, set[1].before);
+    hi = mass_before(set[1].b1 + 1);
+  }
+  if (floor_p) {
+    lo = min(lo, above);
+    hi = min(hi, above);
+  }
+  place(set[2], find_bin(false, goal_t(lo, c.u)), find_bin(false, goal_t(hi, c.u)));
+  st.ws->total = s.total;
+  st.ws->floor = floor_p ? above : ~0ull;
+  st.ws->above = 0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSmThreads, 2) sample_pick_kernel(SampleParams p) {
+  SampleShared& s = SM_SHARED;
+  griddep_launch_dependents();
+  const Stretch<T> st(p);
+  griddep_wait();
+  const Setting c = setting(p, st.b);
+  const unsigned long long best = __ldcg(&st.ws->best);
+  const RowScale rs{best_logit(best), c.inv};
+  const bool empty = rs.xmax == -INFINITY;
+  uint32_t key = static_cast<uint32_t>(best >> 32);
+  int token = empty ? -1 : static_cast<int>(~static_cast<uint32_t>(best));
+  const bool sampled = !empty && !c.greedy;
+  const SampleSet* set = st.ws->set;
+  if (sampled) {  // ---- this stretch's tokens of the sets
+    Pick pick[3];
+    float xlo = INFINITY, xhi = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const int b0 = __ldcg(&set[k].b0), b1 = __ldcg(&set[k].b1);
+      if (b0 >= 0)
+        pick[k].bin_range(b0, b1, rs.xmax, c.T0);
+      else
+        pick[k].nothing();
+      xlo = fminf(xlo, pick[k].xlo);
+      xhi = fmaxf(xhi, pick[k].xhi);
+    }
+    each(st.row + st.i0, st.n, [&](float x, int i) {
+      if (!(x >= xlo && x <= xhi)) return;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        uint32_t kx;
+        if (!pick[k].has(x, rs, kx)) continue;
+        const uint32_t at = atomicAdd(&st.ws->n[k], 1u);
+        if (at < kSmList)
+          st.ws->list[k][at] =
+              (static_cast<unsigned long long>(~kx) << 32) | static_cast<uint32_t>(st.i0 + i);
+      }
+    });
+  }
+  if (!last_of_row(&st.ws->ticket, st.parts)) return;
+  if (sampled) {  // ---- each position in its list
+    const auto find = [&](int k, bool by_count, unsigned long long goal) -> Found {
+      const uint32_t n = __ldcg(&st.ws->n[k]);
+      const int b0 = __ldcg(&set[k].b0), b1 = __ldcg(&set[k].b1);
+      const unsigned long long before = __ldcg(&set[k].before);
+      const uint32_t before_cnt = __ldcg(&set[k].before_cnt);
+      if (n > kSmList)
+        return find_by_splitting(st.row, p.vocab, rs, c.T0, by_count, goal, b0, b1, before,
+                                 before_cnt);
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < n; i += kSmThreads) s.list[i] = __ldcg(&st.ws->list[k][i]);
+      find_listed(by_count, n, goal - (by_count ? before_cnt : before), b0 * kSmSub,
+                  b1 > b0 ? 32 - __clz(b1 - b0) : 0, rs.xmax, rs.inv);
+      return {before + s.found, s.token, s.found_key, 0};
+    };
+    unsigned long long mass = __ldcg(&st.ws->total);
+    if (__ldcg(&set[0].b0) >= 0) mass = find(0, true, c.top_k).mass;
+    if (__ldcg(&set[1].b0) >= 0) mass = find(1, false, goal_p(mass, c.top_p)).mass;
+    mass = min(mass, __ldcg(&st.ws->floor));
+    const Found f = find(2, false, goal_t(mass, c.u));
+    key = f.key;
+    token = f.token >= 0 ? f.token : find_ranked(st.row, p.vocab, f.key, f.rank);
+    __syncthreads();
+    if (threadIdx.x < 3) st.ws->n[threadIdx.x] = 0;
   }
   if (threadIdx.x == 0) {
-    s.mine.z = z;
-    s.mine.above = above;
-    s.mine.first = first;
-  }
-  uint32_t key = key_of(row.rs.xmax), tie_rank = 0;
-  int token = -1;
-  if (!greedy) {
-    // ---- 2. and 3.
-    const bool counts = k > 0 && k < p.vocab;
-    int nth = 0;
-    bool bins = false;
-    exponent_bins(row, counts, s);
-    finish_bins(s, slice, C, rank);
-    bins = true;
-    if (C == 1) __syncthreads();
-    unsigned long long mass = s.total;
-    if (counts && static_cast<unsigned long long>(k) < s.total_cnt)
-      mass = find_prefix<T, true>(row, static_cast<unsigned long long>(k), nth, bins, counts, s, slice).mass;
-    if (tp < 1.0f) {
-      const double want = ceil(static_cast<double>(fmaxf(tp, 0.0f)) * static_cast<double>(mass));
-      const unsigned long long goal = max(1ull, min(mass, static_cast<unsigned long long>(want)));
-      mass = find_prefix<T, false>(row, goal, nth, bins, counts, s, slice).mass;
-    }
-    if (mp > 0.0f) {  // (the slots were written before the bins' barriers)
-      above = 0;
-      for (int r = 0; r < C; ++r) above += ld_cluster(&s.mine.above, r);
-      mass = min(mass, above);
-    }
-    const double t = floor(static_cast<double>(p.u[b]) * static_cast<double>(mass));
-    const unsigned long long target =
-        t > 0.0 ? min(mass - 1, static_cast<unsigned long long>(t)) : 0ull;
-    const Found f = find_prefix<T, false>(row, target + 1, nth, bins, counts, s, slice);
-    key = f.key;
-    token = f.token;
-    tie_rank = f.rank;
-    if (token < 0) write_ranked(row, key, tie_rank, p.tokens + b, s);
-  } else {
-    cluster_sync_all();
-    for (int r = 0; r < C; ++r) first = min(first, ld_cluster(&s.mine.first, r));
-    token = first;
-  }
-  if (rank == 0 && threadIdx.x == 0) {
-    if (token >= 0) p.tokens[b] = token;
+    st.ws->best = 0;  // for the next call; every CTA of the row has read it
+    p.tokens[st.b] = token;
     if (p.logprobs) {
-      z = 0.0;
-      for (int r = 0; r < C; ++r) z += ld_cluster(&s.mine.z, r);
       const float v = logit_of(key);
-      p.logprobs[b] = static_cast<float>((v == mx ? 0.0 : static_cast<double>(v) - mx) - log(z));
+      const double dx = v == rs.xmax ? 0.0 : static_cast<double>(v) - rs.xmax;
+      p.logprobs[st.b] = empty ? -INFINITY : static_cast<float>(dx - __ldcg(&st.ws->log_z));
     }
   }
-  cluster_sync_all();  // shared memory is read by the other CTAs until here
+}
+
+template <typename K>
+cudaError_t launch_k(K kernel, const SampleParams& p, int grid, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kSmThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 template <typename T>
-cudaError_t launch_t(const SampleParams& p, int C, cudaStream_t s) {
-  const size_t smem = (sizeof(SampleShared) + 15) / 16 * 16 +
-                      (C > 1 ? (kSmSlice + 15) / 16 * 16 : 0) +
-                      static_cast<size_t>((p.vocab + C - 1) / C) * sizeof(T) + 32;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  static std::atomic<bool> configured[64];
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    configured[dev].store(true, std::memory_order_release);
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * C);
-  cfg.blockDim = dim3(kSmThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p, C);
+cudaError_t launch_t(const SampleParams& p, cudaStream_t s) {
+  const int grid = p.batch * ((p.vocab + p.chunk - 1) / p.chunk);
+  cudaError_t e = launch_k(sample_max_kernel<T>, p, grid, s);
+  if (e == cudaSuccess) e = launch_k(sample_bins_kernel<T>, p, grid, s);
+  if (e == cudaSuccess) e = launch_k(sample_pick_kernel<T>, p, grid, s);
+  return e;
 }
 
 }  // namespace
 
-// CTAs per row: enough that a stretch fits (kSmChunk tokens), and up to 8 while
-// the batch leaves SMs idle.
-int sample_cluster(int batch, int vocab, int sms) {
-  int C = 1;
-  while ((vocab + C - 1) / C > kSmChunk) C *= 2;
-  while (C < 8 && batch * 2ll * C <= sms && vocab > 1024 * C) C *= 2;
-  return C;
+// Tokens per CTA: as many as give every SM two CTAs, within 2^11 .. 2^14.
+int sample_chunk(int batch, int vocab, int sms) {
+  const long long want = (static_cast<long long>(batch) * vocab + 2 * sms - 1) / (2 * sms);
+  return static_cast<int>(want < kSmMinChunk ? kSmMinChunk : want > kSmChunk ? kSmChunk : (want + 7) / 8 * 8);
 }
 
-cudaError_t launch_sample(const SampleParams& p, int C, cudaStream_t s) {
+cudaError_t launch_sample(const SampleParams& p, cudaStream_t s) {
   switch (p.dtype) {
-    case 0: return launch_t<float>(p, C, s);
-    case 1: return launch_t<__nv_bfloat16>(p, C, s);
-    case 2: return launch_t<__half>(p, C, s);
+    case 0: return launch_t<float>(p, s);
+    case 1: return launch_t<__nv_bfloat16>(p, s);
+    case 2: return launch_t<__half>(p, s);
   }
   return cudaErrorInvalidValue;
 }
