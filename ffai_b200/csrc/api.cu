@@ -1474,7 +1474,8 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
   p.ld = ld;
   p.vocab = vocab;
   p.dtype = dtype;
-  p.chunk = sample_chunk(slab, vocab, ctx->num_sms);
+  p.chunk = sample_chunk(slab, vocab, ctx->num_sms, kSmChunk);
+  p.long_chunk = sample_chunk(slab, vocab, ctx->num_sms, kSmLongChunk);
   p.rows = ctx->d_sample;
   for (int b = 0; b < batch; b += slab) {
     p.batch = std::min(slab, batch - b);

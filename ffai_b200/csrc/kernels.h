@@ -413,8 +413,9 @@ cudaError_t launch_kv_write(const WriteParams& p, int sms, cudaStream_t s);
 // ---- sampling (sample.cu) -----------------------------------------------------
 
 constexpr int kSmMaxVocab = 1 << 18;  // weight sums stay below 2^54
-constexpr int kSmChunk = 1 << 14;     // tokens per CTA, at most
-constexpr int kSmMinChunk = 1 << 11;  // and at least
+constexpr int kSmChunk = (1 << 14) - 8;  // tokens per CTA, at most
+constexpr int kSmLongChunk = 1 << 15;  // of the passes without a histogram
+constexpr int kSmMinChunk = 1 << 12;  // and at least
 constexpr int kSmBins = 1600;         // of the exponent: (-25, 0] in steps of 1/64
 constexpr int kSmList = 1024;         // listed tokens per set
 constexpr int kSmMaxRows = 1024;      // rows per launch (workspace)
@@ -424,6 +425,7 @@ struct SampleSet {
   int b0, b1;
   unsigned int before_cnt, pad;
   unsigned long long before;
+  float xlo, xhi;  // every token of the bins lies between them
 };
 // A row's workspace.  best, above, ticket, n, bins and cnt are zero between
 // calls: whoever uses them last clears them.
@@ -443,7 +445,7 @@ struct SampleParams {
   const void* logits;  // (batch, vocab), rows ld elements apart
   long long ld;
   int batch, vocab, dtype;
-  int chunk;                 // tokens per CTA: sample_chunk
+  int chunk, long_chunk;     // tokens per CTA: sample_chunk
   const float* u;            // (batch)
   const float* temperature;  // (batch) or null: 1
   const int* top_k;          // (batch) or null: off
@@ -453,7 +455,7 @@ struct SampleParams {
   float* logprobs;  // (batch) or null
   SampleRow* rows;  // (batch)
 };
-int sample_chunk(int batch, int vocab, int sms);
+int sample_chunk(int batch, int vocab, int sms, int most);
 cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
 
 }  // namespace ffai

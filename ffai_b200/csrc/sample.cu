@@ -29,12 +29,18 @@
 // A set with more tokens than a list holds (flat or coarsely rounded rows) is
 // split by the logits' own bits, by that CTA alone, until a part fits.
 // Weights are summed as two 18-bit halves in 32-bit words, which a stretch of
-// at most 2^14 tokens does not overflow (but for one case, noted below), so plain
-// shared-memory reductions suffice: a 64-bit shared-memory add is a
-// compare-and-swap loop.  (One cluster of CTAs per row with the logits kept in
-// shared memory was slower everywhere: its exchanges and single-CTA phases take
-// 25 us a row with two rows per SM in flight: 269 us against 105 at 300 rows of
-// 128000 f32 logits, 40 against 20 at 64 rows of 51865 bf16.)
+// less than 2^14 tokens cannot overflow, so plain shared-memory reductions
+// suffice: a 64-bit shared-memory add is a compare-and-swap loop.
+//
+// Measured (device, us): 24 at 5 rows of 51865 f32 logits, 44 at 64 rows bf16 with
+// every setting, 158 at 300 rows of 128000 f32 (28 + 74 + 56; one read of the
+// logits takes 24).  A few rows are bound by the chain of dependent passes, many
+// by the instructions of the second pass (about 35 a token).  The alternative,
+// a cluster of CTAs per row that keeps the logits in shared memory, took 25, 40
+// and 269: it reads them once, but its exchanges and single-CTA phases leave
+// only two stretches per SM in flight.
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "common.cuh"
@@ -48,12 +54,12 @@ constexpr int kSmThreads = 512;
 constexpr int kSmWarps = kSmThreads / 32;
 constexpr int kSmBins = 1600;    // d in (-25, 0]; e^-25 2^36 < 1: nothing beyond
 constexpr int kSmPer = 4;        // bins per scanning thread
+constexpr int kSmQueue = 1024;   // tokens of a stretch that may be in a set
+constexpr int kSmPair = 256;     // tokens of a short list
 constexpr int kSmSub = 512;      // finer bins of a list: 2^-15 wide in d
-static_assert(kSmSub == kSmThreads && kSmBins % kSmPer == 0 && kSmBins / kSmPer <= kSmThreads, "scan");
-// A stretch's low halves sum to at most 2^14 (2^18 - 1), its high ones to 2^14
-// 2^18: 2^32 exactly, when a whole stretch of 2^14 tokens is at the maximum.
-// The add that then wraps to 0 is noted in SampleShared::wrapped.
-static_assert((static_cast<unsigned long long>(kSmChunk) << 18) <= (1ull << 32), "halves");
+static_assert(kSmSub == kSmThreads && 2 * kSmPair == kSmThreads && kSmBins % kSmPer == 0 && kSmBins / kSmPer <= kSmThreads, "scan");
+// The high half of the weight 2^36 is 2^18.
+static_assert((static_cast<unsigned long long>(kSmChunk) << 18) < (1ull << 32), "halves");
 
 // NaN counts as -inf (never chosen), -0 as 0 (they tie).
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
@@ -104,16 +110,24 @@ __device__ __forceinline__ int fine_of(float d) {
 }
 
 struct SampleShared {
-  uint2 half[kSmBins];    // sums of low and high halves; then: mass before each bin
-  uint32_t cnt[kSmBins];  // tokens; then: tokens before each bin
-  unsigned long long list[kSmList];
+  union {
+    struct {
+      uint32_t lo[kSmBins], hi[kSmBins];  // sums of the weights' halves
+    };
+    unsigned long long mass[kSmBins];     // then: mass before each bin
+  };
+  uint32_t cnt[kSmBins];  // tokens of weight; then: those before each bin
+  union {
+    unsigned long long list[kSmList];
+    float2 queue[kSmQueue];  // (logit, index) of tokens that may be in a set
+  };
+  unsigned long long pair[3][kSmPair], pair_w[3][kSmPair];  // short lists and weights
   uint2 sub[kSmSub];      // a list's finer bins
   uint32_t sub_cnt[kSmSub];
   unsigned long long red[kSmWarps];
   unsigned long long red2[kSmWarps];
   unsigned long long few[32];  // a fine bin's tokens
   uint32_t n_few, n_list;
-  uint32_t wrapped;       // half[0].y passed 2^32
   unsigned long long total;  // mass and tokens of all bins
   uint32_t total_cnt;
   int bin, token, last;
@@ -121,6 +135,7 @@ struct SampleShared {
   uint32_t found_key, found_rank;
 };
 
+static_assert(offsetof(SampleShared, cnt) == kSmBins * 8, "add_weight");
 __shared__ SampleShared sm_shared;
 #define SM_SHARED sm_shared
 
@@ -179,6 +194,19 @@ __device__ __noinline__ Sums block_exclusive(Sums v, Sums* total) {
   return {(warp ? ba : 0) + in.a - v.a, (warp ? bc : 0) + in.c - v.c};
 }
 
+// The logits of a 16-byte piece.
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& w, float (&x)[16 / sizeof(T)]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
+    if constexpr (sizeof(T) == 4)
+      x[e] = __uint_as_float(u[e]);
+    else
+      x[e] = e & 1 ? hi_half(u[e / 2], std::is_same<T, __half>::value)
+                   : lo_half(u[e / 2], std::is_same<T, __half>::value);
+  }
+}
 // f(x, i) for tokens [0, n) of a stretch in global memory, in no order: 16-byte
 // loads where the stretch allows, kUnroll of them in flight a thread.
 template <typename T, typename F>
@@ -186,10 +214,9 @@ __device__ __forceinline__ void each(const T* src, int n, F f) {
   constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
   const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T));
   const int head = min(n, (kVec - skew) % kVec), vecs = (n - head) / kVec;
-  const int t = threadIdx.x, tail = head + vecs * kVec + t;
-  if (t < head) f(to_f32<T>(src[t]), t);
-  if (tail < n) f(to_f32<T>(src[tail]), tail);
+  const int t = threadIdx.x;
   const uint4* mid = reinterpret_cast<const uint4*>(src + head);
+#pragma unroll 1
   for (int v0 = t; v0 < vecs; v0 += kUnroll * kSmThreads) {
     uint4 w[kUnroll];
 #pragma unroll
@@ -198,18 +225,58 @@ __device__ __forceinline__ void each(const T* src, int n, F f) {
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
       if (v0 + k * kSmThreads >= vecs) break;
-      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      float x[kVec];
+      unpack<T>(w[k], x);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        float x;
-        if constexpr (sizeof(T) == 4)
-          x = __uint_as_float(u[e]);
-        else
-          x = e & 1 ? hi_half(u[e / 2], std::is_same<T, __half>::value)
-                    : lo_half(u[e / 2], std::is_same<T, __half>::value);
-        f(x, head + (v0 + k * kSmThreads) * kVec + e);
-      }
+      for (int e = 0; e < kVec; ++e) f(x[e], head + (v0 + k * kSmThreads) * kVec + e);
     }
+  }
+  // the tokens before and behind the pieces: fewer than 2 kVec, one a thread
+  const int rest = n - vecs * kVec;
+  if (t < rest) {
+    const int i = t < head ? t : vecs * kVec + t;
+    f(to_f32<T>(src[i]), i);
+  }
+}
+// take(x, i) for the few tokens near(x) holds for: the test sets a bit a token,
+// without a branch, and the bits of four pieces are gone through afterwards.
+template <typename T, typename N, typename F>
+__device__ __forceinline__ void each_near(const T* src, int n, N near, F take) {
+  constexpr int kVec = 16 / sizeof(T), kUnroll = 4;  // at most 32 tokens
+  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T));
+  const int head = min(n, (kVec - skew) % kVec), vecs = (n - head) / kVec;
+  const int t = threadIdx.x;
+  const uint4* mid = reinterpret_cast<const uint4*>(src + head);
+#pragma unroll 1
+  for (int v0 = t; v0 < vecs; v0 += kUnroll * kSmThreads) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      w[k] = make_uint4(0, 0, 0, 0);
+      if (v0 + k * kSmThreads < vecs) w[k] = __ldg(mid + v0 + k * kSmThreads);
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      float x[kVec];
+      unpack<T>(w[k], x);
+      uint32_t part = 0;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) part |= near(x[e]) ? 1u << (k * kVec + e) : 0u;
+      if (v0 + k * kSmThreads < vecs) bits |= part;
+    }
+    while (bits) {
+      const int j = __ffs(bits) - 1;
+      bits &= bits - 1;
+      const int i = head + (v0 + j / kVec * kSmThreads) * kVec + j % kVec;
+      take(to_f32<T>(src[i]), i);  // read again: a register cannot be indexed
+    }
+  }
+  const int rest = n - vecs * kVec;
+  if (t < rest) {
+    const int i = t < head ? t : vecs * kVec + t;
+    const float x = to_f32<T>(src[i]);
+    if (near(x)) take(x, i);
   }
 }
 
@@ -237,8 +304,7 @@ __device__ __noinline__ void finish_bins(unsigned long long* global, uint32_t* g
     } else {
 #pragma unroll
       for (int e = 0; e < kSmPer; ++e) {
-        const uint2 h = s.half[b0 + e];
-        m[e] = (static_cast<unsigned long long>(h.y) << 18) + h.x;
+        m[e] = (static_cast<unsigned long long>(s.hi[b0 + e]) << 18) + s.lo[b0 + e];
         c[e] = s.cnt[b0 + e];
       }
     }
@@ -252,10 +318,9 @@ __device__ __noinline__ void finish_bins(unsigned long long* global, uint32_t* g
   }
   v = block_exclusive(v, &total);
   if (b0 < kSmBins) {
-    unsigned long long* mass = reinterpret_cast<unsigned long long*>(s.half);
 #pragma unroll
     for (int e = 0; e < kSmPer; ++e) {
-      mass[b0 + e] = v.a;
+      s.mass[b0 + e] = v.a;
       s.cnt[b0 + e] = v.c;
       v.a += m[e];
       v.c += c[e];
@@ -268,30 +333,30 @@ __device__ __noinline__ void finish_bins(unsigned long long* global, uint32_t* g
   __syncthreads();
 }
 
-// The bin where the running count or mass reaches `goal` (1 .. the total):
-// the last one with less before it.  Every thread searches for itself.
+// The bin where the running count or mass reaches `goal` (1 .. the total): the
+// last one with less before it.  One warp: every lane probes the last bin of
+// each 32nd of what is left.
 __device__ __forceinline__ int find_bin(bool by_count, unsigned long long goal) {
   SampleShared& s = SM_SHARED;
-  const unsigned long long* mass = reinterpret_cast<const unsigned long long*>(s.half);
+  const int lane = threadIdx.x % 32;
   int lo = 0;
 #pragma unroll 1
-  for (int step = 1024; step > 0; step >>= 1) {
-    const int b = lo + step;
-    if (b < kSmBins && (by_count ? s.cnt[b] : mass[b]) < goal) lo = b;
+  for (int step = 1024; step > 0; step /= 32) {
+    const int b = lo + lane * step;  // rising: the lanes below the goal come first
+    const bool below = b < kSmBins && (by_count ? s.cnt[b] : s.mass[b]) < goal;
+    lo += max(__popc(__ballot_sync(0xffffffffu, below)) - 1, 0) * step;
   }
   return lo;
 }
 __device__ __forceinline__ unsigned long long mass_before(int b) {
-  return b < kSmBins ? reinterpret_cast<const unsigned long long*>(SM_SHARED.half)[b] : SM_SHARED.total;
+  return b < kSmBins ? SM_SHARED.mass[b] : SM_SHARED.total;
 }
 
 __device__ __forceinline__ void clear_bins() {
   SampleShared& s = SM_SHARED;
   for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) {
-    s.half[i] = make_uint2(0, 0);
-    s.cnt[i] = 0;
+    s.lo[i] = s.hi[i] = s.cnt[i] = 0;
   }
-  if (threadIdx.x == 0) s.wrapped = 0;
   __syncthreads();
 }
 
@@ -303,6 +368,40 @@ __device__ __forceinline__ unsigned long long goal_p(unsigned long long mass, fl
 __device__ __forceinline__ unsigned long long goal_t(unsigned long long mass, float u) {
   const double t = floor(static_cast<double>(u) * static_cast<double>(mass));
   return (t > 0.0 ? min(mass - 1, static_cast<unsigned long long>(t)) : 0ull) + 1;
+}
+
+// Adds the weight of an exponent to its bin (and 1 to the bin's count), without
+// a branch: the bin's address comes straight from the bits of floor(-64 d) +
+// 2^23, and tokens that weigh nothing (d below -25, NaN, masked) add nothing
+// and, wherever they would fall, touch no bin.  (A weight above zero means d >
+// -24.96: a bin below 1598.)
+template <bool COUNT>
+__device__ __forceinline__ Halves add_weight(float d, uint32_t lo_bins) {
+  d = fmaxf(d, -26.0f);
+  const Halves h = halves(expf(d));
+  const uint32_t at = (__float_as_uint(__fmaf_rz(d, -64.0f, 8388608.0f)) << 2) + lo_bins -
+                      (0x4b000000u << 2);
+  if constexpr (COUNT)
+    asm volatile(
+        "{\n\t.reg .pred p, q, r;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "setp.ne.u32 q, %2, 0;\n\t"
+        "or.pred r, p, q;\n\t"
+        "@p red.shared.add.u32 [%0], %1;\n\t"
+        "@q red.shared.add.u32 [%0 + %3], %2;\n\t"
+        "@r red.shared.add.u32 [%0 + %4], 1;\n\t}" ::"r"(at),
+        "r"(h.lo), "r"(h.hi), "n"(kSmBins * 4), "n"(kSmBins * 8)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "setp.ne.u32 q, %2, 0;\n\t"
+        "@p red.shared.add.u32 [%0], %1;\n\t"
+        "@q red.shared.add.u32 [%0 + %3], %2;\n\t}" ::"r"(at),
+        "r"(h.lo), "r"(h.hi), "n"(kSmBins * 4)
+        : "memory");
+  return h;
 }
 
 // A set of tokens: exponent bins b0 .. b1, or a range of keys.
@@ -323,7 +422,7 @@ struct Pick {
       xhi = INFINITY;
     }
   }
-  __device__ __forceinline__ void nothing() {
+  __device__ __forceinline__ void nothing() {  // no logit lies in its range
     b0 = b1 = 0;
     xlo = INFINITY;
     xhi = -INFINITY;
@@ -365,7 +464,15 @@ __device__ __noinline__ void find_listed(bool by_count, uint32_t n, unsigned lon
   const int lane = threadIdx.x % 32;
   s.sub[threadIdx.x] = make_uint2(0, 0);
   s.sub_cnt[threadIdx.x] = 0;
-  if (threadIdx.x == 0) s.n_few = 0;
+  if (threadIdx.x == 0) {
+    // (The goal lies within the list.  Should a racing write to the logits make
+    // that untrue, every index below stays in range.)
+    s.n_few = 0;
+    s.bin = 0;
+    s.token = 0;
+    s.found = 0;
+    s.found_key = s.found_rank = 0;
+  }
   __syncthreads();
   int fine[2] = {-1, -1};
 #pragma unroll
@@ -396,7 +503,7 @@ __device__ __noinline__ void find_listed(bool by_count, uint32_t n, unsigned lon
   if (few <= 32) {
 #pragma unroll
     for (int e = 0; e < kSmList / kSmThreads; ++e)
-      if (fine[e] == bin) s.few[atomicAdd(&s.n_few, 1u)] = s.list[threadIdx.x + e * kSmThreads];
+      if (fine[e] == bin) s.few[atomicAdd(&s.n_few, 1u) % 32] = s.list[threadIdx.x + e * kSmThreads];
     __syncthreads();
     if (threadIdx.x < 32) {
       const bool real = lane < static_cast<int>(few);
@@ -462,6 +569,37 @@ __device__ __noinline__ void find_listed(bool by_count, uint32_t n, unsigned lon
   __syncthreads();
 }
 
+// The same in a list of at most kSmPair tokens (in s.pair, with weights in
+// s.pair_w): eight threads a token add up what comes before it.
+__device__ __noinline__ void find_paired(bool by_count, int set, uint32_t n, unsigned long long goal) {
+  SampleShared& s = SM_SHARED;
+  __syncthreads();  // the last result is read
+  const uint32_t part = threadIdx.x % 8;
+  for (uint32_t base = 0; base < n; base += kSmThreads / 8) {
+    const uint32_t i = base + threadIdx.x / 8;
+    const unsigned long long mine = i < n ? s.pair[set][i] : 0;
+    unsigned long long mass = 0;  // up to and with this token
+    uint32_t cnt = 0;
+    for (uint32_t j = part; j < n; j += 8)
+      if (s.pair[set][j] <= mine) {
+        mass += s.pair_w[set][j];
+        ++cnt;
+      }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      mass += __shfl_xor_sync(0xffffffffu, mass, o);
+      cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+    }
+    if (part == 0 && i < n &&
+        (by_count ? cnt == goal : mass - s.pair_w[set][i] < goal && goal <= mass)) {  // one token
+      s.found = mass;
+      s.token = static_cast<int>(mine & 0xffffffffu);
+      s.found_key = ~static_cast<uint32_t>(mine >> 32);
+    }
+  }
+  __syncthreads();
+}
+
 // The slow way to the token where the running count or mass of the row first
 // reaches `goal`, for a set that its list did not hold, by this CTA alone: bins
 // first .. last of the exponent hold the goal, and before / before_cnt come
@@ -487,18 +625,24 @@ __device__ __noinline__ Found find_by_splitting(const T* row, int vocab, RowScal
     kmax = block_reduce(kmax, red, [](uint32_t a, uint32_t b) { return max(a, b); });
     pick.key_range(kmin, kmax);
   }
-  while (true) {
-    if (pick.klo == pick.khi) {  // equal logits: the rank follows from the goal
-      const unsigned long long w = weight(exponent(logit_of(pick.klo), rs));
+  for (int level = 0;; ++level) {
+    // equal logits: the rank follows from the goal.  (32 key bits, 10 a level:
+    // the fourth split leaves one key.)
+    if (pick.klo >= pick.khi || level == 5) {
+      const unsigned long long w = max(1ull, weight(exponent(logit_of(pick.klo), rs)));
       const uint32_t rank = by_count ? static_cast<uint32_t>(goal - before_cnt)
                                      : static_cast<uint32_t>((goal - before + w - 1) / w);
       return {before + rank * w, -1, pick.klo, rank};
     }
     const uint32_t range = pick.khi - pick.klo;
     const int shift = max(0, 32 - __clz(range) - 10);  // at most 1024 bins
-    // The row is histogrammed by stretches whose halves cannot overflow (not
-    // all of these tokens are at the maximum: there are two keys), into 64-bit
-    // sums kept one bin or two a thread.
+    // The row is histogrammed by stretches whose halves cannot overflow, into
+    // 64-bit sums, two bins a thread.
+    if (threadIdx.x == 0) {
+      s.bin = 0;
+      s.found = 0;
+      s.found_rank = 0;
+    }
     unsigned long long mass[2] = {0, 0};
     uint32_t cnt[2] = {0, 0};
     for (int i0 = 0; i0 < vocab; i0 += kSmChunk) {
@@ -509,18 +653,15 @@ __device__ __noinline__ Found find_by_splitting(const T* row, int vocab, RowScal
         if (!pick.has(x, rs, key)) return;
         const uint32_t b = (pick.khi - key) >> shift;
         const unsigned long long w = weight(exponent(logit_of(key), rs));
-        atomicAdd(&s.half[b].x, static_cast<uint32_t>(w) & 0x3ffffu);
-        if (atomicAdd(&s.half[b].y, static_cast<uint32_t>(w >> 18)) >= 0u - (1u << 18) &&
-            (w >> 36))
-          s.wrapped = 1;  // a whole stretch at the maximum
+        atomicAdd(&s.lo[b], static_cast<uint32_t>(w) & 0x3ffffu);
+        atomicAdd(&s.hi[b], static_cast<uint32_t>(w >> 18));
         atomicAdd(&s.cnt[b], 1u);
       });
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint2 h = s.half[2 * threadIdx.x + e];
-        mass[e] += (static_cast<unsigned long long>(h.y) << 18) + h.x;
-        if (s.wrapped && threadIdx.x + e == 0) mass[e] += 1ull << 50;
+        mass[e] += (static_cast<unsigned long long>(s.hi[2 * threadIdx.x + e]) << 18) +
+                   s.lo[2 * threadIdx.x + e];
         cnt[e] += s.cnt[2 * threadIdx.x + e];
       }
     }
@@ -577,6 +718,8 @@ __device__ __noinline__ int find_ranked(const T* row, int vocab, uint32_t key, u
   __syncthreads();
   uint32_t before = 0;
   for (int w = 0; w < warp; ++w) before += static_cast<uint32_t>(s.red[w]);
+  if (threadIdx.x == 0) s.token = 0;
+  __syncthreads();
   if (before < rank && before + n >= rank) {  // one warp
     for (int i = i0; i < i1; i += 32) {
       const bool hit = i + lane < i1 && key_of(clean(to_f32<T>(row[i + lane]))) == key;
@@ -618,12 +761,12 @@ struct Stretch {
   const T* row;
   int b, i0, n, parts, part;
   SampleRow* ws;
-  __device__ __forceinline__ Stretch(const SampleParams& p) {
-    parts = (p.vocab + p.chunk - 1) / p.chunk;
+  __device__ __forceinline__ Stretch(const SampleParams& p, int chunk) {
+    parts = (p.vocab + chunk - 1) / chunk;
     b = blockIdx.x / parts;
     part = blockIdx.x - b * parts;
-    i0 = part * p.chunk;
-    n = min(p.vocab - i0, p.chunk);
+    i0 = part * chunk;
+    n = min(p.vocab - i0, chunk);
     row = static_cast<const T*>(p.logits) + b * p.ld;
     ws = p.rows + b;
   }
@@ -651,28 +794,64 @@ template <typename T>
 __global__ void __launch_bounds__(kSmThreads) sample_max_kernel(SampleParams p) {
   griddep_launch_dependents();
   griddep_wait();  // the logits, and the previous call's use of the workspace
-  const Stretch<T> st(p);
+  const Stretch<T> st(p, p.long_chunk);
+  // The largest logit and where a thread met it first: of the 16-byte pieces
+  // only the piece is noted (a comparison a piece, not a token), the token in
+  // it looked up at the end.  fmaxf passes over NaN; -0 ties with 0.
+  constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
+  const T* src = st.row + st.i0;
+  const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T));
+  const int head = min(st.n, (kVec - skew) % kVec), vecs = (st.n - head) / kVec;
+  const uint4* mid = reinterpret_cast<const uint4*>(src + head);
+  const int t = threadIdx.x, tail = head + vecs * kVec + t;
   float mx = -INFINITY;
-  int at = INT32_MAX;
-  each(st.row + st.i0, st.n, [&](float x, int i) {
-    if (x > mx || (x == mx && i < at)) {  // false for NaN; -0 ties with 0
-      mx = x;
-      at = i;
+  int piece = -1;
+  for (int v0 = t; v0 < vecs; v0 += kUnroll * kSmThreads) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      if (v0 + k * kSmThreads < vecs) w[k] = __ldg(mid + v0 + k * kSmThreads);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      if (v0 + k * kSmThreads >= vecs) break;
+      float x[kVec];
+      unpack<T>(w[k], x);
+      float m = x[0];
+#pragma unroll
+      for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[e]);
+      if (m > mx) {
+        mx = m;
+        piece = v0 + k * kSmThreads;
+      }
     }
-  });
+  }
+  float ends = -INFINITY;  // the tokens before and behind the pieces
+  if (t < head) ends = fmaxf(ends, to_f32<T>(src[t]));
+  if (tail < st.n) ends = fmaxf(ends, to_f32<T>(src[tail]));
+  const float top = block_reduce(fmaxf(mx, ends), reinterpret_cast<float*>(SM_SHARED.red),
+                                 [](float a, float b) { return fmaxf(a, b); });
+  int at = INT32_MAX;
+  if (t < head && to_f32<T>(src[t]) == top) at = t;
+  if (at == INT32_MAX && piece >= 0 && mx == top) {
+    float x[kVec];
+    unpack<T>(__ldg(mid + piece), x);
+#pragma unroll
+    for (int e = kVec - 1; e >= 0; --e)
+      if (x[e] == top) at = head + piece * kVec + e;
+  }
+  if (at == INT32_MAX && tail < st.n && to_f32<T>(src[tail]) == top) at = tail;
+  at = block_reduce(at, reinterpret_cast<int*>(SM_SHARED.red), [](int a, int b) { return min(a, b); });
   if (at == INT32_MAX) at = 0;  // nothing above -inf here
-  const unsigned long long mine =
-      (static_cast<unsigned long long>(key_of(mx + 0.0f)) << 32) | ~static_cast<uint32_t>(st.i0 + at);
   const unsigned long long best =
-      block_reduce(mine, SM_SHARED.red, [](unsigned long long a, unsigned long long b) { return max(a, b); });
+      (static_cast<unsigned long long>(key_of(top + 0.0f)) << 32) | ~static_cast<uint32_t>(st.i0 + at);
   if (threadIdx.x == 0) atomicMax(&st.ws->best, best);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSmThreads) sample_bins_kernel(SampleParams p) {
+__global__ void __launch_bounds__(kSmThreads, 3) sample_bins_kernel(SampleParams p) {
   SampleShared& s = SM_SHARED;
   griddep_launch_dependents();
-  const Stretch<T> st(p);
+  const Stretch<T> st(p, p.chunk);
   clear_bins();
   griddep_wait();
   const Setting c = setting(p, st.b);
@@ -685,38 +864,35 @@ __global__ void __launch_bounds__(kSmThreads) sample_bins_kernel(SampleParams p)
                          : -INFINITY;
   const bool floor_p = sampled && c.min_p > 0.0f;
   unsigned long long above = 0;  // weight above the min-p cut
-  // sum of e^(x - max) for the log-probability: f64 over f32 terms, because a
-  // peaked row adds tens of thousands of tiny terms to 1
-  double z = 0.0;
-  float zpart = 0.0f;
-  int nz = 0;
-  each(st.row + st.i0, st.n, [&](float x, int) {
-    const float d = exponent(x, rs);
-    float e = 0.0f;
-    if (sampled && d >= -25.0f) {
-      e = expf(d);
-      const Halves h = halves(e);
-      const int b = bin_of(d);
-      atomicAdd(&s.half[b].x, h.lo);
-      if (h.hi < (1u << 18)) {
-        if (h.hi) atomicAdd(&s.half[b].y, h.hi);
-      } else if (atomicAdd(&s.half[b].y, 1u << 18) == 0u - (1u << 18)) {
-        s.wrapped = 1;
-      }
-      if (counts) atomicAdd(&s.cnt[b], 1u);
-      if (floor_p && d >= dmin) above += (static_cast<unsigned long long>(h.hi) << 18) + h.lo;
-    }
-    if (p.logprobs) {
-      const float ez = expf(delta(x, rs.xmax));
-      zpart += ez == ez ? ez : 0.0f;
-      if (++nz % 4 == 0) {
-        z += static_cast<double>(zpart);
-        zpart = 0.0f;
-      }
-    }
-  });
+  const uint32_t lo_bins = smem_u32(s.lo);
+  if (sampled && !counts && !floor_p && rs.xmax < INFINITY) {
+    // the plain case, with nothing decided per token but the weight itself
+    each(st.row + st.i0, st.n, [&](float x, int) {
+      add_weight<false>(__fmul_rn(__fadd_rn(x, -rs.xmax), rs.inv), lo_bins);
+    });
+  } else if (sampled) {
+    const float from = floor_p ? dmin : INFINITY;
+    each(st.row + st.i0, st.n, [&](float x, int) {
+      const float d = exponent(x, rs);
+      const Halves h = add_weight<true>(d, lo_bins);
+      if (d >= from) above += (static_cast<unsigned long long>(h.hi) << 18) + h.lo;
+    });
+  }
   if (p.logprobs) {
-    z = block_reduce(z + static_cast<double>(zpart), reinterpret_cast<double*>(s.red),
+    // sum of e^(x - max): f64 over f32 sums of a piece, because a peaked row
+    // adds tens of thousands of tiny terms to 1 (a logit 200 below weighs 0, as
+    // do NaN; an infinite maximum is 0 from itself)
+    double z = 0.0;
+    float part = 0.0f;
+    int n = 0;
+    each(st.row + st.i0, st.n, [&](float x, int) {
+      part += expf(fmaxf(delta(x, rs.xmax), -200.0f));
+      if (++n % 4 == 0) {
+        z += static_cast<double>(part);
+        part = 0.0f;
+      }
+    });
+    z = block_reduce(z + static_cast<double>(part), reinterpret_cast<double*>(s.red),
                      [](double a, double b) { return a + b; });
     if (threadIdx.x == 0) st.ws->z[st.part] = z;
   }
@@ -727,9 +903,7 @@ __global__ void __launch_bounds__(kSmThreads) sample_bins_kernel(SampleParams p)
   if (sampled) {  // the row's bins: whole numbers, in any order
     __syncthreads();
     for (int b = threadIdx.x; b < kSmBins; b += kSmThreads) {
-      const uint2 h = s.half[b];
-      unsigned long long m = (static_cast<unsigned long long>(h.y) << 18) + h.x;
-      if (b == 0) m += static_cast<unsigned long long>(s.wrapped) << 50;
+      unsigned long long m = (static_cast<unsigned long long>(s.hi[b]) << 18) + s.lo[b];
       if (m) atomicAdd(&st.ws->bins[b], m);
       if (counts && s.cnt[b]) atomicAdd(&st.ws->cnt[b], s.cnt[b]);
     }
@@ -737,54 +911,68 @@ __global__ void __launch_bounds__(kSmThreads) sample_bins_kernel(SampleParams p)
   if (!last_of_row(&st.ws->ticket, st.parts)) return;
 
   // ---- the whole row is in: where each position can lie
-  if (p.logprobs && threadIdx.x < 32) {  // in one order, whatever CTA does it
+  if (p.logprobs && threadIdx.x >= kSmThreads - 32) {  // in one order, whatever CTA does it
     double sum = 0.0;
-    for (int r = threadIdx.x; r < st.parts; r += 32) sum += __ldcg(&st.ws->z[r]);
+    for (int r = threadIdx.x % 32; r < st.parts; r += 32) sum += __ldcg(&st.ws->z[r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (threadIdx.x == 0) st.ws->log_z = log(sum);
+    if (threadIdx.x % 32 == 0) st.ws->log_z = log(sum);
   }
   if (!sampled) return;
-  finish_bins(st.ws->bins, st.ws->cnt, counts);
-  const bool cut_k = counts && static_cast<uint32_t>(c.top_k) < s.total_cnt, cut_p = c.top_p < 1.0f;
   if (floor_p) above = __ldcg(&st.ws->above);
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  SampleSet* set = st.ws->set;
-  const auto place = [&](SampleSet& q, int first, int last) {
-    q.b0 = first;
-    q.b1 = last;
-    q.before = mass_before(first);
-    q.before_cnt = s.cnt[first];
-  };
+  finish_bins(st.ws->bins, st.ws->cnt, counts);
+  if (threadIdx.x >= 32) return;
+  // One warp, all lanes alike (they search together); lane k writes set k.
+  const int lane = threadIdx.x;
+  const bool cut_k = counts && static_cast<uint32_t>(c.top_k) < s.total_cnt, cut_p = c.top_p < 1.0f;
+  int b0 = -1, b1 = -1;  // this lane's set; -1: not asked for
   unsigned long long lo = s.total, hi = lo;  // the mass kept so far lies between
-  set[0].b0 = set[1].b0 = -1;  // not asked for
   if (cut_k) {
-    const int bin = find_bin(true, c.top_k);
-    place(set[0], bin, bin);
-    lo = max(1ull, set[0].before);
-    hi = mass_before(bin + 1);
+    const int b = find_bin(true, c.top_k);
+    if (lane == 0) b0 = b1 = b;
+    lo = max(1ull, mass_before(b));
+    hi = mass_before(b + 1);
   }
   if (cut_p) {
-    place(set[1], find_bin(false, goal_p(lo, c.top_p)), find_bin(false, goal_p(hi, c.top_p)));
-    lo = max(1ull, set[1].before);
-    hi = mass_before(set[1].b1 + 1);
+    const int first = find_bin(false, goal_p(lo, c.top_p));
+    const int last = hi == lo ? first : find_bin(false, goal_p(hi, c.top_p));
+    if (lane == 1) b0 = first, b1 = last;
+    lo = max(1ull, mass_before(first));
+    hi = mass_before(last + 1);
   }
   if (floor_p) {
     lo = min(lo, above);
     hi = min(hi, above);
   }
-  place(set[2], find_bin(false, goal_t(lo, c.u)), find_bin(false, goal_t(hi, c.u)));
-  st.ws->total = s.total;
-  st.ws->floor = floor_p ? above : ~0ull;
-  st.ws->above = 0;
+  {
+    const int first = find_bin(false, goal_t(lo, c.u));
+    const int last = hi == lo ? first : find_bin(false, goal_t(hi, c.u));
+    if (lane == 2) b0 = first, b1 = last;
+  }
+  if (lane < 3) {
+    Pick pick;
+    pick.nothing();
+    if (b0 >= 0) pick.bin_range(b0, b1, rs.xmax, c.T0);
+    SampleSet& q = st.ws->set[lane];
+    q.b0 = b0;
+    q.b1 = b1;
+    q.xlo = pick.xlo;
+    q.xhi = pick.xhi;
+    q.before = b0 >= 0 ? mass_before(b0) : 0;
+    q.before_cnt = b0 >= 0 && counts ? s.cnt[b0] : 0;
+  }
+  if (lane == 0) {
+    st.ws->total = s.total;
+    st.ws->floor = floor_p ? above : ~0ull;
+    st.ws->above = 0;
+  }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSmThreads, 2) sample_pick_kernel(SampleParams p) {
   SampleShared& s = SM_SHARED;
   griddep_launch_dependents();
-  const Stretch<T> st(p);
+  const Stretch<T> st(p, p.long_chunk);
   griddep_wait();
   const Setting c = setting(p, st.b);
   const unsigned long long best = __ldcg(&st.ws->best);
@@ -796,19 +984,15 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_pick_kernel(SampleParams
   const SampleSet* set = st.ws->set;
   if (sampled) {  // ---- this stretch's tokens of the sets
     Pick pick[3];
-    float xlo = INFINITY, xhi = -INFINITY;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       const int b0 = __ldcg(&set[k].b0), b1 = __ldcg(&set[k].b1);
-      if (b0 >= 0)
-        pick[k].bin_range(b0, b1, rs.xmax, c.T0);
-      else
-        pick[k].nothing();
-      xlo = fminf(xlo, pick[k].xlo);
-      xhi = fmaxf(xhi, pick[k].xhi);
+      pick[k].b0 = b0;
+      pick[k].b1 = b1;
+      pick[k].xlo = __ldcg(&set[k].xlo);
+      pick[k].xhi = __ldcg(&set[k].xhi);
     }
-    each(st.row + st.i0, st.n, [&](float x, int i) {
-      if (!(x >= xlo && x <= xhi)) return;
+    const auto take = [&](float x, int i) {
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
         uint32_t kx;
@@ -818,22 +1002,74 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_pick_kernel(SampleParams
           st.ws->list[k][at] =
               (static_cast<unsigned long long>(~kx) << 32) | static_cast<uint32_t>(st.i0 + i);
       }
-    });
+    };
+    // In the pass only the ranges of x are tested; what passes is queued (one
+    // token in a hundred, but one warp instruction in four would branch).
+    if (threadIdx.x == 0) s.n_list = 0;
+    __syncthreads();
+    const auto queue = [&](float x, int i) {
+      const uint32_t at = atomicAdd(&s.n_list, 1u);
+      if (at < kSmQueue)
+        s.queue[at] = make_float2(x, __int_as_float(i));
+      else
+        take(x, i);
+    };
+    const float a0 = pick[0].xlo, a1 = pick[0].xhi, b0 = pick[1].xlo, b1 = pick[1].xhi,
+                c0 = pick[2].xlo, c1 = pick[2].xhi;
+    if (a0 > a1)  // without top-k, two ranges to test
+      each_near(st.row + st.i0, st.n,
+                [&](float x) { return (x >= b0 && x <= b1) || (x >= c0 && x <= c1); }, queue);
+    else
+      each_near(st.row + st.i0, st.n,
+                [&](float x) {
+                  return (x >= a0 && x <= a1) || (x >= b0 && x <= b1) || (x >= c0 && x <= c1);
+                },
+                queue);
+    __syncthreads();
+    for (uint32_t q = threadIdx.x; q < min(s.n_list, static_cast<uint32_t>(kSmQueue)); q += kSmThreads)
+      take(s.queue[q].x, __float_as_int(s.queue[q].y));
   }
   if (!last_of_row(&st.ws->ticket, st.parts)) return;
   if (sampled) {  // ---- each position in its list
+    // Short lists are loaded together, with their tokens' weights.
+    uint32_t len[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) len[k] = __ldcg(&st.ws->n[k]);
+    {
+      const int k = threadIdx.x / kSmPair, i = threadIdx.x % kSmPair;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // sets 0 and 1, then 2
+        const int set_of = k + 2 * h;
+        if (set_of >= 3 || len[set_of] > kSmPair) continue;
+        if (i < static_cast<int>(len[set_of])) {
+          const unsigned long long e = __ldcg(&st.ws->list[set_of][i]);
+          s.pair[set_of][i] = e;
+          s.pair_w[set_of][i] = weight(exponent(logit_of(~static_cast<uint32_t>(e >> 32)), rs));
+        }
+      }
+    }
+    if (threadIdx.x == 0) {
+      s.token = 0;
+      s.found = 0;
+      s.found_key = key;
+    }
+    __syncthreads();
     const auto find = [&](int k, bool by_count, unsigned long long goal) -> Found {
-      const uint32_t n = __ldcg(&st.ws->n[k]);
       const int b0 = __ldcg(&set[k].b0), b1 = __ldcg(&set[k].b1);
       const unsigned long long before = __ldcg(&set[k].before);
       const uint32_t before_cnt = __ldcg(&set[k].before_cnt);
+      const uint32_t n = len[k];
+      const unsigned long long want = goal - (by_count ? before_cnt : before);
+      if (n <= kSmPair) {
+        find_paired(by_count, k, n, want);
+        return {before + s.found, s.token, s.found_key, 0};
+      }
       if (n > kSmList)
         return find_by_splitting(st.row, p.vocab, rs, c.T0, by_count, goal, b0, b1, before,
                                  before_cnt);
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < n; i += kSmThreads) s.list[i] = __ldcg(&st.ws->list[k][i]);
-      find_listed(by_count, n, goal - (by_count ? before_cnt : before), b0 * kSmSub,
-                  b1 > b0 ? 32 - __clz(b1 - b0) : 0, rs.xmax, rs.inv);
+      find_listed(by_count, n, want, b0 * kSmSub, b1 > b0 ? 32 - __clz(b1 - b0) : 0, rs.xmax, rs.inv);
       return {before + s.found, s.token, s.found_key, 0};
     };
     unsigned long long mass = __ldcg(&st.ws->total);
@@ -874,18 +1110,22 @@ cudaError_t launch_k(K kernel, const SampleParams& p, int grid, cudaStream_t s) 
 template <typename T>
 cudaError_t launch_t(const SampleParams& p, cudaStream_t s) {
   const int grid = p.batch * ((p.vocab + p.chunk - 1) / p.chunk);
-  cudaError_t e = launch_k(sample_max_kernel<T>, p, grid, s);
+  const int long_grid = p.batch * ((p.vocab + p.long_chunk - 1) / p.long_chunk);
+  cudaError_t e = launch_k(sample_max_kernel<T>, p, long_grid, s);
   if (e == cudaSuccess) e = launch_k(sample_bins_kernel<T>, p, grid, s);
-  if (e == cudaSuccess) e = launch_k(sample_pick_kernel<T>, p, grid, s);
+  if (e == cudaSuccess) e = launch_k(sample_pick_kernel<T>, p, long_grid, s);
   return e;
 }
 
 }  // namespace
 
-// Tokens per CTA: as many as give every SM two CTAs, within 2^11 .. 2^14.
-int sample_chunk(int batch, int vocab, int sms) {
-  const long long want = (static_cast<long long>(batch) * vocab + 2 * sms - 1) / (2 * sms);
-  return static_cast<int>(want < kSmMinChunk ? kSmMinChunk : want > kSmChunk ? kSmChunk : (want + 7) / 8 * 8);
+// Tokens per CTA: one wave of two CTAs per SM where the batch allows, within
+// kSmMinChunk and `most` (a CTA's fixed work, some hundreds of instructions a
+// warp, is worth about 2000 tokens of a plain pass).
+int sample_chunk(int batch, int vocab, int sms, int most) {
+  const int parts = 2 * sms / batch > 1 ? 2 * sms / batch : 1;
+  const int want = ((vocab + parts - 1) / parts + 7) / 8 * 8;
+  return want < kSmMinChunk ? kSmMinChunk : want > most ? most : want;
 }
 
 cudaError_t launch_sample(const SampleParams& p, cudaStream_t s) {
