@@ -36,6 +36,9 @@ _contexts: dict[int, int] = {}
 
 def context(device: int) -> int:
     """The library context of CUDA device `device` (created once, kept)."""
+    ctx = _contexts.get(device)
+    if ctx is not None:
+        return ctx
     with _ctx_lock:
         ctx = _contexts.get(device)
         if ctx is None:
@@ -62,6 +65,16 @@ def _ptr(t: torch.Tensor | None):
 
 def _stream(dev: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+# The entries of a decode step are called every few microseconds: they pass
+# addresses as plain integers and take the stream's handle without a Stream
+# object (several microseconds a call between them).
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+else:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 def _need_cuda(*ts: torch.Tensor, strided: bool = False) -> torch.device:

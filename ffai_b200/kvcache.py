@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _abi
-from .attention import _DT, _check, _ptr, _stream, _token_stride, context
+from .attention import _DT, _check, _ptr, _raw_stream, _stream, _token_stride, context
 
 PAGE_KEYS = 64
 
@@ -182,14 +182,20 @@ class PagePlan(NamedTuple):
     free_count: torch.Tensor  # (1,) pages left on the stack
 
 
-def _vec(t: torch.Tensor, name: str, n: int, dev: torch.device) -> None:
-    if t.dtype != torch.int32 or t.shape != (n,) or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"page plan: {name} must be contiguous int32 ({n},) on {dev}")
+def _vec(t: torch.Tensor, name: str, n: int, index: int) -> int:
+    """Address of a contiguous int32 device vector of n."""
+    if (t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 1 or t.numel() != n
+            or not t.is_contiguous()):
+        raise ValueError(f"page plan: {name} must be contiguous int32 ({n},) on cuda:{index}")
+    return t.data_ptr()
 
 
-def _table(t: torch.Tensor) -> None:
-    if t.dim() != 2 or t.dtype != torch.int32 or not t.is_contiguous() or t.device.type != "cuda":
+def _table(t: torch.Tensor):
+    """(rows, pages, device index) of a block table."""
+    if t.dim() != 2 or t.dtype is not torch.int32 or not t.is_contiguous() or not t.is_cuda:
         raise ValueError("page plan: block_table must be contiguous int32 (B, pages) on a CUDA device")
+    B, pages = t.shape
+    return B, pages, t.get_device()
 
 
 def plan_pages(lens, new_tokens, free_pages, free_count, block_table, *, slot_cap: int,
@@ -202,73 +208,74 @@ def plan_pages(lens, new_tokens, free_pages, free_count, block_table, *, slot_ca
     order into slot_cap rows.  A request that cannot be served whole keeps
     lens and gets slots -1.  lens, free_pages and free_count are not written.
     `num_pages`: the pool's size, to check page ids (default: free_pages')."""
-    _table(block_table)
-    B, max_pages = block_table.shape
-    dev = block_table.device
-    _vec(lens, "lens", B, dev)
-    _vec(new_tokens, "new_tokens", B, dev)
-    _vec(free_pages, "free_pages", free_pages.numel(), dev)
-    _vec(free_count, "free_count", 1, dev)
-    if pos_base is not None:
-        _vec(pos_base, "pos_base", B, dev)
-    buf = torch.empty(2 * B + 2 + 2 * slot_cap, dtype=torch.int32, device=dev)
-    lens_out, cu, slots, pos, count = buf.split((B, B + 1, slot_cap, slot_cap, 1))
-    ctx = context(dev.index)
+    B, max_pages, index = _table(block_table)
+    cap = free_pages.numel()
+    ins = (_vec(lens, "lens", B, index), _vec(new_tokens, "new_tokens", B, index),
+           _vec(free_pages, "free_pages", cap, index))
+    count = _vec(free_count, "free_count", 1, index)
+    base = None if pos_base is None else _vec(pos_base, "pos_base", B, index)
+    buf = torch.empty(2 * B + 2 + 2 * slot_cap, dtype=torch.int32, device=block_table.device)
+    at = buf.data_ptr()
+    cu, slots = at + 4 * B, at + 4 * (2 * B + 1)
+    pos = slots + 4 * slot_cap
+    ctx = context(index)
     st = _abi.load().ffai_page_plan(
-        ctx, B, max_pages, free_pages.numel() if num_pages is None else num_pages, _ptr(lens),
-        _ptr(new_tokens), _ptr(free_pages), free_pages.numel(), _ptr(free_count), _ptr(pos_base),
-        _ptr(block_table), _ptr(lens_out), _ptr(cu), _ptr(slots), _ptr(pos), slot_cap, _ptr(count),
-        _stream(dev))
-    _check(st, ctx)
-    return PagePlan(lens_out, cu, slots, pos, count)
+        ctx, B, max_pages, cap if num_pages is None else num_pages, *ins, cap, count, base,
+        block_table.data_ptr(), at, cu, slots, pos, slot_cap, pos + 4 * slot_cap,
+        _raw_stream(index))
+    if st:
+        _check(st, ctx)
+    return PagePlan(*buf.split_with_sizes((B, B + 1, slot_cap, slot_cap, 1)))
 
 
 def release_pages(lens, done, block_table, free_pages, free_count):
     """Requests with done[b] != 0 hand their pages back (ffai_page_release):
     pushed on the stack free_pages in place.  Returns (lens, free_count) after
     it, as new tensors."""
-    _table(block_table)
-    B, max_pages = block_table.shape
-    dev = block_table.device
-    _vec(lens, "lens", B, dev)
-    _vec(done, "done", B, dev)
-    _vec(free_pages, "free_pages", free_pages.numel(), dev)
-    _vec(free_count, "free_count", 1, dev)
-    lens_out, count = torch.empty(B + 1, dtype=torch.int32, device=dev).split((B, 1))
-    ctx = context(dev.index)
-    st = _abi.load().ffai_page_release(ctx, B, max_pages, _ptr(lens), _ptr(done),
-                                       _ptr(block_table), _ptr(free_pages), free_pages.numel(),
-                                       _ptr(free_count), _ptr(lens_out), _ptr(count), _stream(dev))
-    _check(st, ctx)
-    return lens_out, count
+    B, max_pages, index = _table(block_table)
+    cap = free_pages.numel()
+    buf = torch.empty(B + 1, dtype=torch.int32, device=block_table.device)
+    at = buf.data_ptr()
+    ctx = context(index)
+    st = _abi.load().ffai_page_release(
+        ctx, B, max_pages, _vec(lens, "lens", B, index), _vec(done, "done", B, index),
+        block_table.data_ptr(), _vec(free_pages, "free_pages", cap, index), cap,
+        _vec(free_count, "free_count", 1, index), at, at + 4 * B, _raw_stream(index))
+    if st:
+        _check(st, ctx)
+    return buf[:B], buf[B:]
 
 
 def write_slots(k_pool, v_pool, k_new, v_new, slots) -> None:
     """New keys and values into the pools by slot (ffai_kv_write_slots):
     k_new, v_new (T, kv_heads, 64), possibly views of one fused projection,
     f32 or of the pools' type; slots (T,) int32, negative ones skipped."""
-    dev = k_pool.device
-    if (k_pool.dim() != 4 or k_pool.shape[2:] != (PAGE_KEYS, 64) or v_pool.shape != k_pool.shape
-            or v_pool.dtype != k_pool.dtype or v_pool.device != dev or dev.type != "cuda"
+    index = k_pool.get_device()
+    pool = k_pool.shape
+    if (len(pool) != 4 or pool[2] != PAGE_KEYS or pool[3] != 64 or v_pool.shape != pool
+            or v_pool.dtype is not k_pool.dtype or v_pool.get_device() != index or index < 0
             or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
         raise ValueError("write_slots: k and v pools contiguous (num_pages, kv_heads, 64, 64) of "
                          "one type on one CUDA device")
-    H = k_pool.shape[1]
+    H = pool[1]
     T = slots.numel()
-    _vec(slots, "slots", T, dev)
-    for t in (k_new, v_new):
-        if t.shape != (T, H, 64) or t.device != dev or t.dtype != k_new.dtype:
-            raise ValueError(f"write_slots: new rows ({T}, {H}, 64) of one type on {dev}")
+    at = _vec(slots, "slots", T, index)
+    want = (T, H, 64)
+    if (k_new.shape != want or v_new.shape != want or k_new.get_device() != index
+            or v_new.get_device() != index or v_new.dtype is not k_new.dtype):
+        raise ValueError(f"write_slots: new rows ({T}, {H}, 64) of one type on cuda:{index}")
     if k_new.dtype not in _DT or k_pool.dtype not in _DT:
         raise TypeError("write_slots: f32, bf16 or f16")
-    ts = {_token_stride(t) for t in (k_new, v_new)}
-    if len(ts) != 1 or None in ts or (T > 1 and min(t.stride(0) for t in (k_new, v_new)) < H * 64):
+    ts = _token_stride(k_new)
+    if ts is None or _token_stride(v_new) != ts or (
+            T > 1 and min(k_new.stride(0), v_new.stride(0)) < H * 64):
         raise ValueError("write_slots: new rows contiguous, or views with dense heads and one "
                          "shared token stride")
-    d = _abi.new_desc(heads=H, q_dtype=_DT[k_new.dtype], kv_dtype=_DT[k_pool.dtype],
-                      token_stride=ts.pop())
-    ctx = context(dev.index)
-    st = _abi.load().ffai_kv_write_slots(ctx, ctypes.byref(d), _ptr(k_pool), _ptr(v_pool),
-                                         k_pool.shape[0], _ptr(k_new), _ptr(v_new), _ptr(slots), T,
-                                         _stream(dev))
-    _check(st, ctx)
+    d = _abi.Desc(heads=H, head_dim=64, q_dtype=_DT[k_new.dtype], kv_dtype=_DT[k_pool.dtype],
+                  token_stride=ts)
+    ctx = context(index)
+    st = _abi.load().ffai_kv_write_slots(
+        ctx, ctypes.byref(d), k_pool.data_ptr(), v_pool.data_ptr(), pool[0], k_new.data_ptr(),
+        v_new.data_ptr(), at, T, _raw_stream(index))
+    if st:
+        _check(st, ctx)
