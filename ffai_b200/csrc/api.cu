@@ -1324,7 +1324,36 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
   p.err = ctx->d_err;
   DeviceGuard g(ctx->device);
   ProfScope ps(ctx, FFAI_OP_DECODE, static_cast<cudaStream_t>(stream), "ffai_attn_shared_prefix");
-  if (n_groups > 0) {
+  // Where the prefixes' share comes from (bounds the host knows: the tables'
+  // width and the average group).
+  const char* force = std::getenv("FFAI_SP_FORCE");
+  const long long group_rows = n_groups > 0 ? (d->batch * rows + n_groups - 1) / n_groups : 0;
+  int way = n_groups == 0 ? 0 : prefix_pages <= 8 ? 0 : group_rows <= 16 ? 1 : 2;
+  if (force && n_groups > 0) way = std::atoi(force);
+  const auto workspace = [&](long long slots, int slot_rows, size_t plan_words) {
+    const size_t plan = (plan_words + 3) / 4 * 4;
+    const size_t n = static_cast<size_t>(slots) * slot_rows;
+    int st = ensure(ctx, &ctx->d_prefix, &ctx->prefix_cap, n * 66 + plan);
+    if (st) return st;
+    p.part_slots = static_cast<int>(slots);
+    p.part_plan = reinterpret_cast<int*>(ctx->d_prefix);
+    p.part_ml = ctx->d_prefix + plan;
+    p.part_o = p.part_ml + n * 2;
+    return FFAI_ATTN_OK;
+  };
+  if (way == 1) {
+    // CTAs for three per SM, each over 256 keys at least
+    const long long units =
+        kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + 15) / 16);
+    const long long likely = kv_heads * std::max<long long>(n_groups, (d->batch * rows + 15) / 16);
+    p.splits = static_cast<int>(
+        std::max<long long>(1, std::min<long long>(3LL * ctx->num_sms / likely, prefix_pages / 4)));
+    if (units * p.splits > INT32_MAX / 2)
+      return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows");
+    int st = workspace(units * p.splits, 16, n_groups);
+    if (st) return st;
+    FFAI_CUDA(ctx, launch_prefix_rows(p, static_cast<int>(units), static_cast<cudaStream_t>(stream)));
+  } else if (way == 2) {
     // Partial slots: slot = CTA + segment.  Chunks are no shorter than a CTA's
     // share but for each unit's last, or half that where a unit has one tile,
     // so there are at most 2 * grid + units segments.
@@ -1334,14 +1363,8 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
     if (steps > INT32_MAX / 2)
       return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows and keys");
     const int grid = static_cast<int>(std::min<long long>(ctx->num_sms, steps));
-    p.part_slots = static_cast<int>(3 * grid + units);
-    const size_t floats = static_cast<size_t>(p.part_slots) * kPxRows * 66;
-    const size_t plan = (1 + 2 * static_cast<size_t>(n_groups) + 3) / 4 * 4;  // words
-    int st = ensure(ctx, &ctx->d_prefix, &ctx->prefix_cap, floats + plan);
+    int st = workspace(3LL * grid + units, kPxRows, 1 + 2 * static_cast<size_t>(n_groups));
     if (st) return st;
-    p.part_plan = reinterpret_cast<int*>(ctx->d_prefix);
-    p.part_ml = ctx->d_prefix + plan;
-    p.part_o = p.part_ml + static_cast<size_t>(p.part_slots) * kPxRows * 2;
     CUtensorMap tmk, tmv;
     const long long heads = static_cast<long long>(num_pages) * kv_heads;
     st = make_map(ctx, &tmk, k_pool, false, 0, kPageKeys, heads, 0, kPageKeys);

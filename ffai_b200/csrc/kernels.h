@@ -345,15 +345,19 @@ struct SharedParams {
   float* lse;  // or null
   long long lse_sb, lse_st, lse_sh;
   unsigned* err;
-  // partial results of prefix_tc_kernel, part_slots slots of kPxRows rows: output
+  // partial results of the prefix kernel, part_slots slots of kPxRows rows
+  // (prefix_tc_kernel) or 16 (prefix_rows_kernel, when splits > 0): output
   // sums (64 f32), running maximum (log2 domain) and weight sum; null when
   // the rows kernel walks the prefixes itself
   float* part_o;
   float* part_ml;
   int part_slots;
-  int* part_plan;  // steps per CTA, then each group's first step and segment
+  int splits;      // of a unit's pages, prefix_rows_kernel; 0 otherwise
+  int* part_plan;  // steps per CTA, then each group's first step and segment;
+                   // with splits, each group's first unit
 };
 cudaError_t launch_shared_rows(const SharedParams& p, cudaStream_t s);
+cudaError_t launch_prefix_rows(const SharedParams& p, int units, cudaStream_t s);
 constexpr int kPxRows = 256;  // query rows per unit of the prefix kernel
 constexpr int kPxKeys = 128;  // keys per block (two pages)
 // tm*: 3-d maps over a pool's (64, 64 keys, num_pages * kv_heads), boxes of one page's head
