@@ -48,7 +48,6 @@ struct Walk {
   int cl, len;     // key blocks of a chunk, and of this one
   int steps, step; // steps of this unit over the chunk, and the current one
   int left;        // steps left, the current one included
-  int nth;         // segments of this CTA before this one
   int seg;         // index of the segment on the line
   int base;        // key blocks of this CTA before this segment
   int alt;         // one-tile segments of this CTA before this one
@@ -96,7 +95,6 @@ __device__ __forceinline__ void walk_next(Walk& w, const SharedParams& p) {
   w.left -= walk_steps(w);
   if (w.left <= 0) return;  // else the segment is done
   w.step = 0;
-  ++w.nth;
   ++w.seg;
   if (++w.m == w.d.mu) {
     w.m = 0;
@@ -148,6 +146,7 @@ __device__ __forceinline__ void find_stretch(const SharedParams& p) {
   if (lane == 0) {
     bars->share = share;
     bars->start.left = left;
+    bars->start.base = 0;  // all that is read of a stretch without steps
     if (blockIdx.x == 0) p.part_plan[0] = share;
   }
   int lin = 0, segs = 0;
@@ -194,7 +193,7 @@ __device__ __forceinline__ void find_stretch(const SharedParams& p) {
       w.step = rest - w.m * w.len;
       w.steps = unit_steps(d, w.m, w.len);
       w.left = left;
-      w.nth = w.base = w.alt = 0;
+      w.base = w.alt = 0;
       w.seg = t0 + (w.h * ((d.nb + cl - 1) / cl) + w.q) * d.mu + w.m;
       bars->start = w;
     }
@@ -268,9 +267,7 @@ __device__ __forceinline__ void px_producer(const CUtensorMap* tmK, const CUtens
 // issued before the second product of the current one within a segment.
 struct ChainBlock {
   uint32_t it;
-  int nth;     // segment
   bool first;  // of this chain's blocks in the segment
-  bool alone;  // the other chain does not take this block
 };
 
 struct ChainWalk {
@@ -286,9 +283,7 @@ struct ChainWalk {
       const int j = pair ? pos : 2 * pos + t;
       if (j < walk_blocks(w)) {
         b.it = static_cast<uint32_t>(w.base + j);
-        b.nth = w.nth;
         b.first = pos == 0;
-        b.alone = !pair;
         ++pos;
         return true;
       }
@@ -310,11 +305,28 @@ __device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint32_t tm
   constexpr uint32_t idesc_o = idesc_f16(F16 ? 0u : 1u, 128, 64, 0, 1);
   ChainWalk walk(p, t);
   uint32_t n_s = 0, n_pv = 0;
+  uint32_t n_q = 0;   // segments of this chain
+  uint32_t seen = 0;  // blocks taken or passed
+  // Blocks of the other chain alone are passed, not skipped: a wait by parity
+  // holds only for who has seen the barrier's every phase, and a stage is
+  // loaded again once both chains have seen it.
+  auto pass = [&](uint32_t to) -> bool {
+    for (; seen < to; ++seen) {
+      const uint32_t s = seen % kPxStages, parity = (seen / kPxStages) & 1;
+      if (!warp_wait(&bars->k_full[s], parity, abort_flag, p.err, kErrTimeoutMma) ||
+          !warp_wait(&bars->v_full[s], parity, abort_flag, p.err, kErrTimeoutMma))
+        return false;
+      mbar_arrive_w(&bars->kv_empty[s]);
+    }
+    return true;
+  };
   auto issue_s = [&](const ChainBlock& b) -> bool {
     const uint32_t s = b.it % kPxStages;
+    if (!pass(b.it)) return false;
+    ++seen;
     if (!warp_wait(&bars->k_full[s], (b.it / kPxStages) & 1, abort_flag, p.err, kErrTimeoutMma))
       return false;
-    if (b.first && !warp_wait(&bars->q_full[t], b.nth & 1, abort_flag, p.err, kErrTimeoutMma))
+    if (b.first && !warp_wait(&bars->q_full[t], n_q++ & 1, abort_flag, p.err, kErrTimeoutMma))
       return false;
     if (n_s > 0 &&
         !warp_wait(&bars->sc_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutMma))
@@ -330,10 +342,10 @@ __device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint32_t tm
     return true;
   };
   ChainBlock cur, nxt;
-  if (!walk.next(cur)) return;
-  if (!issue_s(cur)) return;
-  while (true) {
-    const bool more = walk.next(nxt);
+  bool more = walk.next(cur);
+  if (more && !issue_s(cur)) return;
+  while (more) {
+    more = walk.next(nxt);
     // Within a segment the next scores go first; across segments the last
     // product does, since the segment's epilogue waits for it.
     const bool ahead = more && !nxt.first;
@@ -350,12 +362,11 @@ __device__ __forceinline__ void px_mma(const SharedParams& p, int t, uint32_t tm
                (!cur.first || k > 0) ? 1u : 0u);
     mma_commit_w(&bars->o_done[t]);
     mma_commit_w(&bars->kv_empty[s]);
-    if (cur.alone) mma_commit_w(&bars->kv_empty[s]);  // it takes two
     ++n_pv;
-    if (!more) return;
-    if (!ahead && !issue_s(nxt)) return;
+    if (more && !ahead && !issue_s(nxt)) return;
     cur = nxt;
   }
+  pass(static_cast<uint32_t>(walk.w.base));
 }
 
 // ---------------------------------------------------------------- softmax
@@ -423,10 +434,12 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
 
   while (w.left > 0) {
     const bool pair = walk_pair(w);
-    int rows;  // of this chain's tile
-    {
-      const int row0 = w.m * kPxRows + (pair ? 128 * t : 0);
-      rows = min(128, w.d.rows - row0);
+    // this chain's blocks: all, or every second one (none of a single one for chain 1)
+    const int cnt = pair ? walk_blocks(w) : (walk_blocks(w) + 1 - t) >> 1;
+    const bool any = cnt > 0;
+    const int row0 = w.m * kPxRows + (pair ? 128 * t : 0);
+    const int rows = min(128, w.d.rows - row0);  // of this chain's tile
+    if (any) {
       // The chain's last segment is done (its last product was waited for), so
       // its query buffer is free.
       load_q(p, w, row0, rows, sQ + t * kPxTile);
@@ -434,8 +447,6 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
       mbar_arrive(&bars->q_full[t]);
     }
     const bool active = 16 * c < rows;  // warp-uniform: some row of this warp is real
-    // this chain's blocks: all, or every second one
-    const int cnt = pair ? walk_blocks(w) : (walk_blocks(w) + 1 - t) >> 1;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 #pragma unroll 1
     for (int i = 0; i < cnt; ++i, ++n_s) {
@@ -563,7 +574,6 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
       tc_fence_before();
       mbar_arrive(&bars->p_full[t]);
     }
-    const bool any = cnt > 0;
 
     // ---- end of the segment's stretch
     if (any && !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
