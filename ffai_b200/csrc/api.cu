@@ -15,6 +15,7 @@
 #include <deque>
 #include <functional>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -58,6 +59,25 @@ size_t dtype_size(int dt) { return dt == FFAI_DT_F32 ? 4 : 2; }
 
 }  // namespace
 
+namespace ffai {
+// What a kernel leaves for the next of the same call.  Growing keeps the old
+// buffer, for a captured graph may name it: sizes double at least, so all of
+// them together are at most twice the last.
+struct Grown {
+  void* ptr = nullptr;
+  size_t cap = 0;  // bytes
+  Grown* old = nullptr;
+};
+struct StreamSpace {
+  uint64_t key = 0;
+  Grown prefix;  // partial results of a prefix kernel
+  Grown own;     // and of the kernel on the sequences' own keys beside it,
+  Grown queue;   // with its job queue
+  Grown sample;  // per-row state between the sampling kernels
+  StreamSpace* next = nullptr;
+};
+}  // namespace ffai
+
 struct ffai_attn_ctx {
   int device = 0;
   int num_sms = 148;
@@ -86,12 +106,11 @@ struct ffai_attn_ctx {
   // int8 GEMV: quantised activations and their scales, between its two kernels
   uint8_t* d_gemv_x = nullptr;
   size_t gemv_x_cap = 0;
-  // sampling: per-row state between its kernels
-  ffai::SampleRow* d_sample = nullptr;
-  size_t sample_cap = 0;
-  // shared prefix: partial results between its two kernels
-  float* d_prefix = nullptr;
-  size_t prefix_cap = 0;
+  // sampling and shared prefixes: workspaces per stream, so that calls on
+  // different streams may overlap (below); the mutex covers the list and a
+  // call's launches
+  StreamSpace* spaces = nullptr;
+  std::mutex space_mutex;
   ffai_attn_ctx* pipe_ctx = nullptr;  // inner context used for the pipeline's kernels
   std::string last_error;
   int last_status = FFAI_ATTN_OK;
@@ -169,12 +188,68 @@ int ensure(ffai_attn_ctx* ctx, T** ptr, size_t* cap, size_t need_elems, bool zer
   }
   if (zero) {
     e = cudaMemset(*ptr, 0, n * sizeof(T));
-    // done before work on any other stream uses the buffer
-    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaMemset(workspace)");
   }
   *cap = n;
   return FFAI_ATTN_OK;
+}
+
+// The workspaces of a stream (null: out of memory).  The caller holds the mutex.
+StreamSpace* stream_space(ffai_attn_ctx* ctx, void* stream) {
+  const auto s = static_cast<cudaStream_t>(stream);
+  uint64_t key = s == cudaStreamLegacy ? 0 : reinterpret_cast<uint64_t>(stream);
+  unsigned long long id = 0;  // one handle for a stream of each thread
+  if (s == cudaStreamPerThread && cudaStreamGetId(s, &id) == cudaSuccess) key = ~uint64_t{id};
+  for (StreamSpace* w = ctx->spaces; w; w = w->next)
+    if (w->key == key) return w;
+  auto* w = new (std::nothrow) StreamSpace;
+  if (!w) return nullptr;
+  w->key = key;
+  w->next = ctx->spaces;
+  return ctx->spaces = w;
+}
+
+// At least `bytes` in w, zeroed when new if asked.  Also while the stream is being
+// captured: nothing here is queued on it.
+int grow(ffai_attn_ctx* ctx, Grown* w, size_t bytes, bool zero = false) {
+  if (w->cap >= bytes && w->ptr) return FFAI_ATTN_OK;
+  const size_t n = std::max(std::max<size_t>(bytes, 256), 2 * w->cap);
+  auto* old = w->ptr ? new (std::nothrow) Grown(*w) : nullptr;
+  if (w->ptr && !old) return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  void* ptr = nullptr;
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaMalloc(&ptr, n);
+  const bool nomem = e != cudaSuccess;
+  if (e == cudaSuccess && zero) {
+    e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(ptr, 0, n, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (s) cudaStreamDestroy(s);
+  }
+  if (e != cudaSuccess) cudaFree(ptr);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    delete old;
+    if (!nomem) return cuda_fail(ctx, e, "zeroing a workspace");
+    cudaGetLastError();
+    return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "workspace allocation of %zu bytes failed: %s", n,
+                     cudaGetErrorString(e));
+  }
+  w->old = old;
+  w->ptr = ptr;
+  w->cap = n;
+  return FFAI_ATTN_OK;
+}
+
+void free_grown(Grown* w) {
+  cudaFree(w->ptr);
+  while (Grown* o = w->old) {
+    cudaFree(o->ptr);
+    w->old = o->old;
+    delete o;
+  }
 }
 
 bool valid_dtype(int dt) { return dt == FFAI_DT_F32 || dt == FFAI_DT_BF16 || dt == FFAI_DT_F16; }
@@ -739,8 +814,11 @@ void ffai_attn_destroy(ffai_attn_ctx* ctx) {
   cudaFree(ctx->d_stage);
   cudaFree(ctx->d_pipe);
   cudaFree(ctx->d_gemv_x);
-  cudaFree(ctx->d_prefix);
-  cudaFree(ctx->d_sample);
+  while (StreamSpace* w = ctx->spaces) {
+    ctx->spaces = w->next;
+    for (Grown* b : {&w->prefix, &w->own, &w->queue, &w->sample}) free_grown(b);
+    delete w;
+  }
   for (int i = 0; i < 2; ++i) {
     if (ctx->ev_h2d[i]) cudaEventDestroy(ctx->ev_h2d[i]);
     if (ctx->ev_comp[i]) cudaEventDestroy(ctx->ev_comp[i]);
@@ -1324,46 +1402,87 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
   p.err = ctx->d_err;
   DeviceGuard g(ctx->device);
   ProfScope ps(ctx, FFAI_OP_DECODE, static_cast<cudaStream_t>(stream), "ffai_attn_shared_prefix");
-  // Where the prefixes' share comes from (bounds the host knows: the tables'
-  // width and the average group).
-  const char* force = std::getenv("FFAI_SP_FORCE");
-  const long long group_rows = n_groups > 0 ? (d->batch * rows + n_groups - 1) / n_groups : 0;
-  int way = n_groups == 0 ? 0 : prefix_pages <= 8 ? 0 : group_rows <= 16 ? 1 : 2;
-  if (force && n_groups > 0) way = std::atoi(force);
+  // Who reads the prefixes, from bounds that the host knows: the tables'
+  // width, the average group, own tables half full.
+  enum { kEach, kRowTiles, kTensor };
+  const long long tiles = kv_heads * std::max<long long>(n_groups, (d->batch * rows + 15) / 16);
+  const long long units =
+      kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + kPxRows - 1) / kPxRows);
+  const long long likely_units =
+      kv_heads * std::max<long long>(n_groups, (d->batch * rows + kPxRows - 1) / kPxRows);
+  const long long unit_steps = (prefix_pages + 1) / 2;
+  // Microseconds times SMs.  A page against 16 rows costs 0.27, two pages
+  // against 256 rows (on the tensor cores' accumulators) 1.46, and that
+  // kernel's start and its larger partial results 6 us.  Measured, tiles of 16
+  // against units of 256: 64 rows and 6000 keys of 8 heads 16.4 and 19.1 us,
+  // 30000 keys 39.6 and 29.4; 4 rows and 60000 keys 27.6 and 37.6; 256 rows
+  // and 1500 keys 16.1 and 20.7, 6000 keys 29.1 and 27.7.
+  const double t_tiles = 0.27 * static_cast<double>(tiles) * prefix_pages;
+  const double t_units = 1.46 * static_cast<double>(likely_units) * unit_steps;
+  // Up to four pages each sequence reads its group's prefix itself, one launch:
+  // 300 keys 7.7 and 7.7 us for one sequence, 18.0 and 16.1 for 128 in 8 groups.
+  const int way = n_groups == 0 || prefix_pages <= 4          ? kEach
+                  : t_tiles <= 6.0 * ctx->num_sms + t_units ? kRowTiles
+                                                            : kTensor;
+  int st = FFAI_ATTN_OK;
+  std::lock_guard<std::mutex> lock(ctx->space_mutex);
+  StreamSpace* space = stream_space(ctx, stream);
+  if (!space) return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
   const auto workspace = [&](long long slots, int slot_rows, size_t plan_words) {
     const size_t plan = (plan_words + 3) / 4 * 4;
     const size_t n = static_cast<size_t>(slots) * slot_rows;
-    int st = ensure(ctx, &ctx->d_prefix, &ctx->prefix_cap, n * 66 + plan);
+    int st = grow(ctx, &space->prefix, (n * 66 + plan) * 4);
     if (st) return st;
     p.part_slots = static_cast<int>(slots);
-    p.part_plan = reinterpret_cast<int*>(ctx->d_prefix);
-    p.part_ml = ctx->d_prefix + plan;
+    p.part_plan = static_cast<int*>(space->prefix.ptr);
+    p.part_ml = static_cast<float*>(space->prefix.ptr) + plan;
     p.part_o = p.part_ml + n * 2;
     return FFAI_ATTN_OK;
   };
-  if (way == 1) {
-    // CTAs for three per SM, each over 256 keys at least
-    const long long units =
+  if (way == kRowTiles) {
+    // Two CTAs an SM, each over 256 keys at least (one to six an SM differ by a
+    // tenth at most, from two on upwards).
+    const long long bound =
         kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + 15) / 16);
-    const long long likely = kv_heads * std::max<long long>(n_groups, (d->batch * rows + 15) / 16);
-    p.splits = static_cast<int>(
-        std::max<long long>(1, std::min<long long>(3LL * ctx->num_sms / likely, prefix_pages / 4)));
-    if (units * p.splits > INT32_MAX / 2)
+    p.splits = static_cast<int>(std::max<long long>(
+        1, std::min<long long>(2 * ctx->num_sms / tiles, prefix_pages / 4)));
+    if (bound * p.splits > INT32_MAX / 2)
       return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows");
-    int st = workspace(units * p.splits, 16, n_groups);
+    st = workspace(bound * p.splits, 16, n_groups);
     if (st) return st;
-    FFAI_CUDA(ctx, launch_prefix_rows(p, static_cast<int>(units), static_cast<cudaStream_t>(stream)));
-  } else if (way == 2) {
+    FFAI_CUDA(ctx, launch_prefix_rows(p, static_cast<int>(bound), static_cast<cudaStream_t>(stream)));
+  } else if (way == kTensor) {
     // Partial slots: slot = CTA + segment.  Chunks are no shorter than a CTA's
     // share but for each unit's last, or half that where a unit has one tile,
     // so there are at most 2 * grid + units segments.
-    const long long units =
-        kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + kPxRows - 1) / kPxRows);
-    const long long steps = units * ((prefix_pages + 1) / 2);
+    const long long steps = units * unit_steps;
     if (steps > INT32_MAX / 2)
       return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows and keys");
-    const int grid = static_cast<int>(std::min<long long>(ctx->num_sms, steps));
-    int st = workspace(3LL * grid + units, kPxRows, 1 + 2 * static_cast<size_t>(n_groups));
+    // The sequences' own keys are read beside the prefixes, on SMs left to them,
+    // where that is worth the launch that joins both and leaves the tensor cores
+    // enough SMs: from 8 us of the whole device on (a page is 0.37 us of an SM,
+    // its part of HBM's rate), and a fifth of the prefixes' time; after them
+    // otherwise.  Measured, beside and after: one prompt of 8200 keys, 64
+    // sequences of up to 1000 36.5 and 42.0 us; 60000 keys, 64 of 1500 74.1 and
+    // 84.8; 6000 keys, 64 of 200 31.0 and 27.7; three of 32768, 96 of 700 with
+    // four queries each 169.8 and 158.4.
+    const double t_own = 0.37 * 0.5 * d->batch * kv_heads * max_pages * ((rows + 15) / 16);
+    const bool beside = t_own > 8.0 * ctx->num_sms && t_own > 0.2 * t_units;
+    const int spare =
+        beside ? static_cast<int>(ctx->num_sms * std::min(0.5, t_own / (t_units + t_own))) : 0;
+    const int grid = static_cast<int>(std::min<long long>(ctx->num_sms - spare, steps));
+    if (beside) {
+      // (rounded up: the outputs behind the pairs start on 16 bytes)
+      const size_t own_rows = (static_cast<size_t>(d->batch) * kv_heads * rows + 1) / 2 * 2;
+      st = grow(ctx, &space->own, own_rows * 66 * 4);
+      if (st) return st;
+      p.own_ml = static_cast<float*>(space->own.ptr);
+      p.own_o = p.own_ml + own_rows * 2;
+      st = grow(ctx, &space->queue, 4, /*zero=*/true);
+      if (st) return st;
+      p.queue = static_cast<unsigned*>(space->queue.ptr);
+    }
+    st = workspace(3LL * grid + units, kPxRows, 1 + 2 * static_cast<size_t>(n_groups));
     if (st) return st;
     CUtensorMap tmk, tmv;
     const long long heads = static_cast<long long>(num_pages) * kv_heads;
@@ -1372,8 +1491,12 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
     st = make_map(ctx, &tmv, v_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
     if (st) return st;
     FFAI_CUDA(ctx, launch_prefix_tc(tmk, tmv, p, grid, static_cast<cudaStream_t>(stream)));
+    if (beside) {
+      FFAI_CUDA(ctx, launch_own_and_merge(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
+      return FFAI_ATTN_OK;
+    }
   }
-  FFAI_CUDA(ctx, launch_shared_rows(p, static_cast<cudaStream_t>(stream)));
+  FFAI_CUDA(ctx, launch_shared_rows(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }
 
@@ -1491,7 +1614,10 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
     return set_error(ctx, FFAI_ATTN_ERR_INVALID, "sample: logits not aligned to their type");
   DeviceGuard g(ctx->device);
   const int slab = std::min<int>(batch, kSmMaxRows);
-  int st = ensure(ctx, &ctx->d_sample, &ctx->sample_cap, slab, /*zero=*/true);
+  std::lock_guard<std::mutex> lock(ctx->space_mutex);
+  StreamSpace* space = stream_space(ctx, stream);
+  if (!space) return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
+  int st = grow(ctx, &space->sample, slab * sizeof(SampleRow), /*zero=*/true);
   if (st) return st;
   SampleParams p{};
   p.ld = ld;
@@ -1499,7 +1625,7 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
   p.dtype = dtype;
   p.chunk = sample_chunk(slab, vocab, ctx->num_sms, kSmChunk);
   p.long_chunk = sample_chunk(slab, vocab, ctx->num_sms, kSmLongChunk);
-  p.rows = ctx->d_sample;
+  p.rows = static_cast<SampleRow*>(space->sample.ptr);
   for (int b = 0; b < batch; b += slab) {
     p.batch = std::min(slab, batch - b);
     p.logits = static_cast<const char*>(logits) + static_cast<size_t>(b) * ld * dtype_size(dtype);

@@ -355,8 +355,12 @@ struct SharedParams {
   int splits;      // of a unit's pages, prefix_rows_kernel; 0 otherwise
   int* part_plan;  // steps per CTA, then each group's first step and segment;
                    // with splits, each group's first unit
+  float* own_o;    // own_rows_kernel's partials: (sequence, KV head, row)
+  float* own_ml;
+  unsigned* queue; // its next job; zero between calls
 };
-cudaError_t launch_shared_rows(const SharedParams& p, cudaStream_t s);
+cudaError_t launch_shared_rows(const SharedParams& p, int sms, cudaStream_t s);
+cudaError_t launch_own_and_merge(const SharedParams& p, int sms, cudaStream_t s);
 cudaError_t launch_prefix_rows(const SharedParams& p, int units, cudaStream_t s);
 constexpr int kPxRows = 256;  // query rows per unit of the prefix kernel
 constexpr int kPxKeys = 128;  // keys per block (two pages)

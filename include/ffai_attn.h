@@ -279,8 +279,12 @@ int ffai_kv_copy_pages(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool
  * live key is not used, whatever it is.  d->causal, q_offset, kv_len and the
  * k/v layouts are ignored, flags must be 0.  Page ids outside the pool or
  * lengths past a table are not read: ffai_attn_sync then reports
- * FFAI_ATTN_ERR_INVALID.  No reference counterpart (beams there clone whole
- * caches, text_decoder.rs:1363-1381). */
+ * FFAI_ATTN_ERR_INVALID.  Partial results lie in a workspace of the context
+ * per stream: calls on different streams may overlap.  They may be captured;
+ * captures of one stream share its workspace, so their replays and its own
+ * calls must not overlap.  A stream is destroyed after its calls have
+ * finished.  No reference counterpart (beams there clone whole caches,
+ * text_decoder.rs:1363-1381). */
 int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,
                             const void* q, const void* k_pool, const void* v_pool,
                             int32_t num_pages, const int32_t* group_starts, int32_t n_groups,
@@ -352,6 +356,7 @@ int ffai_kv_write_slots(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_poo
  * nothing above -inf gives token -1.  tokens (batch) int32; logprobs
  * (optional, f32): the token's log-softmax of the logits as they are,
  * untempered and uncut.  vocab at most 262144 (else FFAI_ATTN_DECLINED).
+ * Streams and captures: as ffai_attn_shared_prefix.
  * No reference counterpart (its decoder takes the largest logit on the host). */
 int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtype, int32_t batch,
                 int32_t vocab, const float* u, const float* temperature, const int32_t* top_k,

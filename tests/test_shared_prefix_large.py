@@ -1,0 +1,171 @@
+"""Attention over a shared prefix at the sizes where the prefix has a kernel of
+its own, against the formula in 64 bits (computed on the device) on the same
+16-bit operands; streams and captured calls.
+
+Tolerances are those of the small sizes: with A = sum_j w_j |v_j| an output
+errs by at most (u + 1e-4) A + u |o|, u = 2^-8 (bf16) or 2^-11 (f16, where a
+weight below 2^-14 adds 2^-25 |v| a key, |v| < 5.5); the log-sum-exp by 2e-5,
+plus 2^-23 of each of up to 8300 weights' sum, which is random: 2e-5 in all.
+"""
+
+import pytest
+import torch
+
+DEV = "cuda:0"
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def build(prefix, sizes, own, heads, kv, q_len, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    B = sum(sizes)
+    pp, sp = max((n + 63) // 64 for n in prefix), max(1, (own + 63) // 64)
+    n_pages = len(prefix) * pp + B * sp + 1
+    shape = (n_pages, kv, 64, 64)
+    kp = (torch.randn(shape, generator=g, device=DEV) * 1.5).to(dtype)
+    vp = torch.randn(shape, generator=g, device=DEV).clamp(-5.5, 5.5).to(dtype)
+    ids = torch.randperm(n_pages, generator=g, device=DEV).to(torch.int32)
+    ptab = ids[:len(prefix) * pp].view(len(prefix), pp).contiguous()
+    stab = ids[len(prefix) * pp:len(prefix) * pp + B * sp].view(B, sp).contiguous()
+    lens = [(i * 37) % (own + 1) for i in range(B)]
+    starts = [0]
+    for s in sizes:
+        starts.append(starts[-1] + s)
+    # behind the live keys of a last page: not numbers
+    for table, ns in ((ptab, prefix), (stab, lens)):
+        for i, n in enumerate(ns):
+            if n % 64:
+                kp[table[i, n // 64].long(), :, n % 64:] = float("nan")
+                vp[table[i, n // 64].long(), :, n % 64:] = float("inf")
+    q = torch.randn((B, q_len, heads, 64), generator=g, device=DEV).to(dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    return dict(q=q, k_pool=kp, v_pool=vp, prefix_table=ptab, prefix_lens=i32(prefix),
+                group_starts=i32(starts), block_table=stab, seq_lens=i32(lens),
+                lists=(prefix, lens, starts))
+
+
+def gather(pool, pages, n):
+    """(kv, n, 64) f64: the first n keys of a list of pages."""
+    return pool[pages[:(n + 63) // 64].long()].transpose(0, 1).flatten(1, 2)[:, :n].double()
+
+
+def reference(c, scale):
+    prefix, lens, starts = c["lists"]
+    B, n, H, _ = c["q"].shape
+    kv = c["k_pool"].shape[1]
+    o = torch.zeros((B, n, H, 64), dtype=torch.float64, device=DEV)
+    a = torch.zeros_like(o)
+    lse = torch.full((B, n, H), float("-inf"), dtype=torch.float64, device=DEV)
+    for g in range(len(prefix)):
+        pk, pv = (gather(c[x], c["prefix_table"][g], prefix[g]) for x in ("k_pool", "v_pool"))
+        for b in range(starts[g], starts[g + 1]):
+            k = torch.cat([pk, gather(c["k_pool"], c["block_table"][b], lens[b])], 1)
+            v = torch.cat([pv, gather(c["v_pool"], c["block_table"][b], lens[b])], 1)
+            qb = c["q"][b].double().transpose(0, 1).reshape(kv, H // kv, n, 64)
+            s = torch.einsum("hgnd,hkd->hgnk", qb, k) * scale
+            for i in range(n):
+                s[:, :, i, prefix[g] + max(0, lens[b] - (n - 1 - i)):] = float("-inf")
+            l = torch.logsumexp(s, 3)
+            w = torch.exp(s - l.unsqueeze(3)).nan_to_num(0.0)
+            o[b] = torch.einsum("hgnk,hkd->hgnd", w, v).flatten(0, 1).transpose(0, 1)
+            a[b] = torch.einsum("hgnk,hkd->hgnd", w, v.abs()).flatten(0, 1).transpose(0, 1)
+            lse[b] = l.flatten(0, 1).transpose(0, 1)
+    return o, a, lse
+
+
+def attend(c, **kw):
+    from ffai_b200 import shared_prefix
+    return shared_prefix.attend(c["q"], c["k_pool"], c["v_pool"], c["prefix_table"],
+                                c["prefix_lens"], c["group_starts"], c["block_table"],
+                                c["seq_lens"], scale=0.125, **kw)
+
+
+CASES = {
+    # prefix keys, sequences per group, own keys, heads, kv heads, q_len
+    # few rows a KV head: tiles of 16
+    "tiles": ([4097, 1, 0, 650], [3, 2, 2, 1], 130, 12, 4, 1),
+    "tiles_one_sequence": ([8300], [1], 0, 7, 1, 3),
+    "tiles_odd_rows": ([2000, 321], [5, 40], 65, 9, 3, 1),
+    # many rows and long prefixes: tcgen05, own keys after it
+    "units": ([8300], [50], 70, 6, 2, 2),
+    "units_groups": ([8300, 1, 0, 129, 6000], [20, 0, 5, 25, 60], 200, 10, 2, 3),
+    "units_one_tile": ([7000, 6999, 127], [43, 40, 1], 33, 6, 2, 1),
+    # segments of one key block, that one of the kernel's two chains has no part in
+    "units_of_one_block": ([1, 100, 129, 8300], [1, 2, 1, 60], 20, 24, 8, 2),
+    "units_many": ([900, 2500], [100, 31], 40, 32, 4, 2),
+    # and with long own keys: beside it
+    "beside_odd_rows": ([6400], [91], 1600, 9, 3, 1),
+    "beside_groups": ([5000, 0, 6400, 70], [60, 9, 70, 2], 1300, 8, 4, 4),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", CASES)
+def test_matches_the_formula(name, dtype):
+    from ffai_b200 import attention
+    attention.sync(0)
+    c = build(*CASES[name], dtype, seed=len(name))
+    out, lse = attend(c, with_lse=True)
+    o, a, want = reference(c, 0.125)
+    B, n, H, _ = c["q"].shape
+    tol = (U[dtype] + 1e-4) * a + U[dtype] * o.abs() + 1e-7
+    if dtype == torch.float16:
+        keys = c["lists"][0][0] + max(c["lists"][1])
+        tol = tol + keys * 2.0 ** -25 * 5.5 + 2.0 ** -24
+    assert torch.isfinite(out).all()
+    over = (out.double() - o).abs() - tol
+    assert over.max().item() <= 0, f"{over.max():.3e} over"
+    got = lse.double().view(H, B, n).permute(1, 2, 0)
+    empty = want == float("-inf")
+    assert torch.equal(got == float("-inf"), empty)
+    assert (got[~empty] - want[~empty]).abs().max().item() <= 2e-5
+    assert (out[empty] == 0).all()
+    for _ in range(2):
+        assert torch.equal(attend(c), out)
+    attention.sync(0)  # no wait ran out, no table was out of range
+
+
+@pytest.mark.gpu
+def test_streams_do_not_share_partial_results():
+    """Calls queued on two streams without any order between them."""
+    cs = [build(*CASES[n], torch.bfloat16, seed=i)
+          for i, n in enumerate(("beside_odd_rows", "units_groups"))]
+    want = [attend(c) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(attend(cs[i]))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        for x in outs:
+            assert torch.equal(x, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["tiles", "units", "beside_odd_rows"])
+def test_captured_and_replayed(name):
+    """A capture makes its stream's workspace; replays follow the lengths and
+    outlive a larger call on the same stream."""
+    c = build(*CASES[name], torch.bfloat16, seed=3)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        g.capture_begin()
+        out = attend(c)
+        g.capture_end()
+    s.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, attend(c))
+    big = build(*CASES["beside_groups"], torch.bfloat16, seed=4)
+    with torch.cuda.stream(s):
+        attend(big)
+    s.synchronize()
+    c["seq_lens"] //= 2
+    c["prefix_lens"] -= c["prefix_lens"] // 3
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, attend(c))
