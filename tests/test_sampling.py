@@ -192,3 +192,31 @@ def test_refusals():
         sampling.sample(x, u[:1])
     with pytest.raises(attention.AttnError):
         sampling.sample(torch.zeros(0, 10, device=DEV), u[:0])
+
+
+@pytest.mark.gpu
+def test_streams_and_captures_do_not_share_state():
+    """Calls queued on two streams without order between them, and a capture on
+    a stream of its own."""
+    from ffai_b200 import sampling
+    g = torch.Generator(device="cuda").manual_seed(8)
+    sets = [(torch.randn(n, 60001, generator=g, device="cuda") * 3,
+             torch.rand(n, generator=g, device="cuda")) for n in (7, 90)]
+    want = [sampling.sample(x, u, top_p=0.9) for x, u in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(sampling.sample(*sets[i], top_p=0.9))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w) for o in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sampling.sample(*sets[1], top_p=0.9)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want[1])
