@@ -1408,21 +1408,21 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
   const long long tiles = kv_heads * std::max<long long>(n_groups, (d->batch * rows + 15) / 16);
   const long long units =
       kv_heads * (static_cast<long long>(n_groups) + (d->batch * rows + kPxRows - 1) / kPxRows);
-  const long long likely_units =
-      kv_heads * std::max<long long>(n_groups, (d->batch * rows + kPxRows - 1) / kPxRows);
+  const long long halves =  // units of 128 rows, two of which make a step's 256
+      kv_heads * std::max<long long>(n_groups, (d->batch * rows + kPxRows / 2 - 1) / (kPxRows / 2));
   const long long unit_steps = (prefix_pages + 1) / 2;
   // Microseconds times SMs.  A page against 16 rows costs 0.27, two pages
   // against 256 rows (on the tensor cores' accumulators) 1.46, and that
-  // kernel's start and its larger partial results 6 us.  Measured, tiles of 16
-  // against units of 256: 64 rows and 6000 keys of 8 heads 16.4 and 19.1 us,
-  // 30000 keys 39.6 and 29.4; 4 rows and 60000 keys 27.6 and 37.6; 256 rows
-  // and 1500 keys 16.1 and 20.7, 6000 keys 29.1 and 27.7.
+  // kernel's start and its larger partial results 14 us.  Measured, tiles of 16
+  // against units of 256, 8 KV heads: 64 rows and 6000 keys 16.5 and 19.8 us,
+  // 30000 keys 39.6 and 29.9; 256 rows and 3000 keys 20.2 and 23.1, 6000 keys
+  // 29.1 and 25.3; 2048 rows and 700 keys 33.9 and 38.6, 1500 keys 49.5 and 36.3.
   const double t_tiles = 0.27 * static_cast<double>(tiles) * prefix_pages;
-  const double t_units = 1.46 * static_cast<double>(likely_units) * unit_steps;
+  const double t_units = 0.73 * static_cast<double>(halves) * unit_steps;
   // Up to four pages each sequence reads its group's prefix itself, one launch:
   // 300 keys 7.7 and 7.7 us for one sequence, 18.0 and 16.1 for 128 in 8 groups.
   const int way = n_groups == 0 || prefix_pages <= 4          ? kEach
-                  : t_tiles <= 6.0 * ctx->num_sms + t_units ? kRowTiles
+                  : t_tiles <= 14.0 * ctx->num_sms + t_units ? kRowTiles
                                                             : kTensor;
   int st = FFAI_ATTN_OK;
   std::lock_guard<std::mutex> lock(ctx->space_mutex);
@@ -1460,14 +1460,14 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
       return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows and keys");
     // The sequences' own keys are read beside the prefixes, on SMs left to them,
     // where that is worth the launch that joins both and leaves the tensor cores
-    // enough SMs: from 8 us of the whole device on (a page is 0.37 us of an SM,
-    // its part of HBM's rate), and a fifth of the prefixes' time; after them
+    // enough SMs: from 7 us of the whole device on (a page is 0.32 us of an SM,
+    // its part of HBM's rate), and a sixth of the prefixes' time; after them
     // otherwise.  Measured, beside and after: one prompt of 8200 keys, 64
-    // sequences of up to 1000 36.5 and 42.0 us; 60000 keys, 64 of 1500 74.1 and
-    // 84.8; 6000 keys, 64 of 200 31.0 and 27.7; three of 32768, 96 of 700 with
-    // four queries each 169.8 and 158.4.
-    const double t_own = 0.37 * 0.5 * d->batch * kv_heads * max_pages * ((rows + 15) / 16);
-    const bool beside = t_own > 8.0 * ctx->num_sms && t_own > 0.2 * t_units;
+    // sequences of up to 1000 32.3 and 42.3 us; 60000 keys, 64 of 1500 76 and 86;
+    // three of 20000, 96 of 1500 67 and 72; three of 32768, 96 of 700 with four
+    // queries each 173 and 160.
+    const double t_own = 0.32 * 0.5 * d->batch * kv_heads * max_pages * ((rows + 15) / 16);
+    const bool beside = t_own > 7.0 * ctx->num_sms && t_own > 0.17 * t_units;
     const int spare =
         beside ? static_cast<int>(ctx->num_sms * std::min(0.5, t_own / (t_units + t_own))) : 0;
     const int grid = static_cast<int>(std::min<long long>(ctx->num_sms - spare, steps));

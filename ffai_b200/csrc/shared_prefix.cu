@@ -35,8 +35,8 @@
 // tensor memory and registers.  Device time, bf16 or f16 caches, on one B200:
 //   5 sequences, 12 heads, 224 + up to 224 keys            6.9 us (2.4 MB)
 //   12 groups of 5, 20 heads, up to 1500 + up to 448 keys 34.5 us (145 MB, 4.2 TB/s)
-//   64 sequences, 32 / 8 heads, 8200 + up to 1000 keys    36.5 us (82 MB)
-//   96 in 3 groups, 4 queries, 32768 + up to 700 keys      159 us (89 GFLOP, 0.56 PFLOP/s)
+//   64 sequences, 32 / 8 heads, 8200 + up to 1000 keys    32.4 us (82 MB)
+//   96 in 3 groups, 4 queries, 32768 + up to 700 keys      160 us (89 GFLOP, 0.56 PFLOP/s)
 #include <algorithm>
 
 #include "shared_prefix.cuh"
@@ -416,11 +416,11 @@ __device__ __forceinline__ void fold_partials(Merged& acc, Staging<THREADS>& sm,
     return;
   }
   // prefix_tc_kernel's: segments of the line, each one per CTA that has a share of it
-  const int share = __ldcg(p.part_plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
+  const int plan = __ldcg(p.part_plan), share = abs(plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
             seg0 = __ldcg(p.part_plan + 2 + 2 * group);
   if (d.nb == 0) return;
   const int cl = chunk_blocks(d, share), chunks = (d.nb + cl - 1) / cl;
-  const int head0 = lin0 + kvh * head_steps(d, d.nb), m = rg / kPxRows;
+  const int head0 = lin0 + kvh * line_steps(d, share, plan < 0), m = rg / kPxRows;
   int skip = copy;  // partials to pass over before this copy's next
 #pragma unroll 1
   for (int q = 0; q < chunks; ++q) {

@@ -44,6 +44,12 @@ __device__ __forceinline__ int chunk_blocks(const GroupDims& d, int share) {
 __device__ __forceinline__ int head_steps(const GroupDims& d, int blocks) {
   return (d.mu - d.single) * blocks + d.single * ((blocks + 1) >> 1);
 }
+// What a head takes of the line: its steps, in whole shares if each head begins
+// on a CTA of its own.
+__device__ __forceinline__ int line_steps(const GroupDims& d, int share, int even) {
+  const int n = head_steps(d, d.nb);
+  return even && share > 0 ? (n + share - 1) / share * share : n;
+}
 // Steps of unit m over `len` blocks.
 __device__ __forceinline__ int unit_steps(const GroupDims& d, int m, int len) {
   return d.single && m == d.mu - 1 ? (len + 1) >> 1 : len;
