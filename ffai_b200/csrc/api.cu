@@ -1448,7 +1448,7 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
         1, std::min<long long>(2 * ctx->num_sms / tiles, prefix_pages / 4)));
     if (bound * p.splits > INT32_MAX / 2)
       return set_error(ctx, FFAI_ATTN_DECLINED, "shared prefix: too many rows");
-    st = workspace(bound * p.splits, 16, n_groups);
+    st = workspace(bound * p.splits, 16, 1 + static_cast<size_t>(n_groups));
     if (st) return st;
     FFAI_CUDA(ctx, launch_prefix_rows(p, static_cast<int>(bound), static_cast<cudaStream_t>(stream)));
   } else if (way == kTensor) {

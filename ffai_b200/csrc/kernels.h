@@ -353,7 +353,8 @@ struct SharedParams {
   float* part_ml;
   int part_slots;
   int splits;      // of a unit's pages, prefix_rows_kernel; 0 otherwise
-  int* part_plan;  // steps per CTA (negative: heads padded to them), then each group's first step and segment;
+  int* part_plan;  // kBadPlan, or steps per CTA (negative: heads padded to them; with splits
+                   // 0), then each group's first step and segment;
                    // with splits, each group's first unit
   float* own_o;    // own_rows_kernel's partials: (sequence, KV head, row)
   float* own_ml;

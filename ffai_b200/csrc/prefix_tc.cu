@@ -124,6 +124,7 @@ __device__ __forceinline__ void find_stretch(const SharedParams& p) {
   PxBars* bars = PX_BARS;
   const int lane = threadIdx.x % 32;
   int total = 0;
+  bool bad = false;
 #pragma unroll 1
   for (int base = 0; base < p.groups; base += 32) {
     const int g = base + lane;
@@ -131,14 +132,16 @@ __device__ __forceinline__ void find_stretch(const SharedParams& p) {
     if (g < p.groups) {
       const GroupDims d = group_dims(p, g);
       n = p.kv_heads * head_steps(d, d.nb);
-      if (blockIdx.x == 0 && p.err) {
-        const int raw = __ldg(p.prefix_lens + g);
-        const int s0 = __ldg(p.group_starts + g), s1 = __ldg(p.group_starts + g + 1);
-        if (raw < 0 || raw > p.prefix_pages * kPageKeys || s0 < 0 || s1 < s0 || s1 > p.batch)
-          atomicOr(p.err, kErrBadArgs);
-      }
+      bad = bad || !group_ok(p, g, blockIdx.x == 0);
     }
     total += __reduce_add_sync(0xffffffffu, n);
+  }
+  if (__any_sync(0xffffffffu, bad)) {
+    if (lane == 0) {
+      bars->share = bars->start.left = bars->start.base = 0;
+      if (blockIdx.x == 0) p.part_plan[0] = kBadPlan;
+    }
+    return;
   }
   int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   // A CTA that goes from one head to the next drains and fills its pipelines
@@ -658,7 +661,6 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
           }
         }
       }
-      // (group_starts that do not rise can give more segments than there is room for)
       const int slot = static_cast<int>(blockIdx.x) + w.seg;
       if (active && slot < p.part_slots) {
         const size_t at = static_cast<size_t>(slot) * kPxRows + (pair ? 128 * t : 0) + 16 * c + t1;

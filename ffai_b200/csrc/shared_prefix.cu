@@ -212,8 +212,8 @@ __device__ __forceinline__ int group_of(const SharedParams& p, int b) {
     const bool in = g < p.groups && __ldg(p.group_starts + g) <= b;
     n += __popc(__ballot_sync(0xffffffffu, in));
   }
-  if (n == 0) return -1;
-  return b < __ldg(p.group_starts + n) ? n - 1 : -1;
+  // (the first test holds unless the starts do not rise)
+  return n > 0 && __ldg(p.group_starts + n - 1) <= b && b < __ldg(p.group_starts + n) ? n - 1 : -1;
 }
 
 // The same for a lane by itself.
@@ -226,7 +226,7 @@ __device__ __forceinline__ int group_of_lane(const SharedParams& p, int b) {
     else
       hi = mid;
   }
-  return lo > 0 && b < __ldg(p.group_starts + lo) ? lo - 1 : -1;
+  return lo > 0 && __ldg(p.group_starts + lo - 1) <= b && b < __ldg(p.group_starts + lo) ? lo - 1 : -1;
 }
 
 // Page ids of a warp's next 32 steps, one per lane: warp w of the job's W takes
@@ -405,18 +405,20 @@ __device__ __forceinline__ void fold_partials(Merged& acc, Staging<THREADS>& sm,
   const GroupDims d = group_dims(p, group);
   const int rg = (b - d.b0) * R + row;
   // the plan was written by the preceding kernel, which may have run beside this one
+  const int plan = __ldcg(p.part_plan);
+  if (plan == kBadPlan) return;
   if (p.splits > 0) {  // prefix_rows_kernel's: one per split that has pages
     const int pages = (d.plen + kPageKeys - 1) / kPageKeys;
     if (pages == 0) return;
     const int tiles = (d.rows + 15) / 16, per = (pages + p.splits - 1) / p.splits;
-    const int slot = (__ldcg(p.part_plan + group) + kvh * tiles + rg / 16) * p.splits;
+    const int slot = (__ldcg(p.part_plan + 1 + group) + kvh * tiles + rg / 16) * p.splits;
     const int n = min((pages + per - 1) / per, p.part_slots - slot);
     fold_run(acc, sm, p, static_cast<size_t>(slot + copy) * 16 + rg % 16,
              static_cast<size_t>(copies) * 16, (n - copy + copies - 1) / copies, part, jt);
     return;
   }
   // prefix_tc_kernel's: segments of the line, each one per CTA that has a share of it
-  const int plan = __ldcg(p.part_plan), share = abs(plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
+  const int share = abs(plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
             seg0 = __ldcg(p.part_plan + 2 + 2 * group);
   if (d.nb == 0) return;
   const int cl = chunk_blocks(d, share), chunks = (d.nb + cl - 1) / cl;
@@ -501,12 +503,10 @@ __global__ void __launch_bounds__(kSpThreads, 3) shared_rows_kernel(SharedParams
                       tok[1] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[1]))};
   walk<F16, W>(st, q, p, kvh, table, p.max_pages, ids, len, see, warp, ring);
   const int group = group_of(p, b);
+  if (!p.part_o && blockIdx.x == 0 && threadIdx.x < 32)  // a prefix kernel's business otherwise
+    for (int gi = lane; gi < p.groups; gi += 32) group_ok(p, gi, true);
   if (!p.part_o && group >= 0) {  // the prefix too
-    int plen = __ldg(p.prefix_lens + group);
-    if (plen < 0 || plen > p.prefix_pages * kPageKeys) {
-      if (p.err && jt == 0) atomicOr(p.err, kErrBadArgs);
-      plen = min(max(plen, 0), p.prefix_pages * kPageKeys);
-    }
+    const int plen = min(max(__ldg(p.prefix_lens + group), 0), p.prefix_pages * kPageKeys);
     const int all[2] = {plen, plen};
     table = p.prefix_table + static_cast<size_t>(group) * p.prefix_pages;
     walk<F16, W>(st, q, p, kvh, table, p.prefix_pages,
@@ -674,18 +674,14 @@ __global__ void __launch_bounds__(kSpThreads, 3) prefix_rows_kernel(SharedParams
   const int unit = blockIdx.x / p.splits, split = blockIdx.x - unit * p.splits;
   // ---- the unit's group: every warp scans the groups' unit counts
   int group = -1, unit0 = 0, before = 0;
+  bool bad = false;
 #pragma unroll 1
   for (int base = 0; base < p.groups; base += 32) {
     const int gi = base + lane;
     int n = 0;
     if (gi < p.groups) {
       n = p.kv_heads * ((group_dims(p, gi).rows + 15) / 16);
-      if (blockIdx.x == 0 && warp == 0 && p.err) {
-        const int raw = __ldg(p.prefix_lens + gi);
-        const int s0 = __ldg(p.group_starts + gi), s1 = __ldg(p.group_starts + gi + 1);
-        if (raw < 0 || raw > p.prefix_pages * kPageKeys || s0 < 0 || s1 < s0 || s1 > p.batch)
-          atomicOr(p.err, kErrBadArgs);
-      }
+      bad = bad || !group_ok(p, gi, blockIdx.x == 0 && warp == 0);
     }
     int upto = n;
 #pragma unroll
@@ -694,7 +690,7 @@ __global__ void __launch_bounds__(kSpThreads, 3) prefix_rows_kernel(SharedParams
       if (lane >= o) upto += v;
     }
     const int from = before + upto - n;
-    if (blockIdx.x == 0 && warp == 0 && gi < p.groups) p.part_plan[gi] = from;
+    if (blockIdx.x == 0 && warp == 0 && gi < p.groups) p.part_plan[1 + gi] = from;
     const unsigned hit = __ballot_sync(0xffffffffu, from <= unit && unit < from + n);
     if (hit) {
       group = base + __ffs(hit) - 1;
@@ -702,7 +698,9 @@ __global__ void __launch_bounds__(kSpThreads, 3) prefix_rows_kernel(SharedParams
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  if (group < 0 || static_cast<int>(blockIdx.x) >= p.part_slots) return;
+  bad = __any_sync(0xffffffffu, bad);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.part_plan[0] = bad ? kBadPlan : 0;
+  if (bad || group < 0 || static_cast<int>(blockIdx.x) >= p.part_slots) return;
   const GroupDims d = group_dims(p, group);
   const int tiles = (d.rows + 15) / 16, kvh = (unit - unit0) / tiles;
   const int row0 = (unit - unit0 - kvh * tiles) * 16;

@@ -1,6 +1,8 @@
 // What the two kernels of ffai_attn_shared_prefix agree on.
 #pragma once
 
+#include <limits.h>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -28,6 +30,20 @@ __device__ __forceinline__ GroupDims group_dims(const SharedParams& p, int g) {
   d.nb = d.rows > 0 ? (d.plen + kPxKeys - 1) / kPxKeys : 0;
   return d;
 }
+
+// Group g of all: does it start and end in order within the batch?  The lengths
+// must lie within the table too, but are clamped; starts that do not rise would
+// give sequences to several groups, so then no group's prefix is attended.
+__device__ __forceinline__ bool group_ok(const SharedParams& p, int g, bool report) {
+  const int s0 = __ldg(p.group_starts + g), s1 = __ldg(p.group_starts + g + 1);
+  const bool ok = s0 >= 0 && s1 >= s0 && s1 <= p.batch;
+  if (report && p.err) {
+    const int len = __ldg(p.prefix_lens + g);
+    if (!ok || len < 0 || len > p.prefix_pages * kPageKeys) atomicOr(p.err, kErrBadArgs);
+  }
+  return ok;
+}
+constexpr int kBadPlan = INT_MIN;  // in part_plan[0]: as above
 
 // Work is counted in steps of the prefix kernel's two chains: a unit of two
 // tiles passes over one key block a step (one tile a chain), a unit of one

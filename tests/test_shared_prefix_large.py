@@ -169,3 +169,24 @@ def test_captured_and_replayed(name):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, attend(c))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["tiles_odd_rows", "units_one_tile", "beside_odd_rows"])
+def test_starts_that_do_not_rise_are_reported(name):
+    """No group's prefix is attended then: the result is that of no prefixes."""
+    from ffai_b200 import attention
+    prefix, sizes, own, heads, kv, n = CASES[name]
+    c = build([max(16000, prefix[0])] * 4, [1, 2, 3, sum(sizes) - 6], own, heads, kv, n, torch.bfloat16, seed=5)
+    B = c["q"].shape[0]
+    c["group_starts"].copy_(torch.tensor([3, 2, B, 1, B], dtype=torch.int32))
+    out = attend(c)
+    with pytest.raises(attention.AttnError) as e:
+        attention.sync(0)
+    assert e.value.status == -1
+    none = dict(c, prefix_lens=torch.zeros_like(c["prefix_lens"]),
+                group_starts=torch.tensor([0, 1, 3, 6, B], dtype=torch.int32, device=DEV))
+    want = attend(none)
+    attention.sync(0)
+    U8 = 2.0 ** -7  # two ways to the same sums: each rounds weights and result once
+    assert ((out.float() - want.float()).abs() <= U8 * 5.5).all()
