@@ -23,6 +23,12 @@
 // ones), and at the end chain 1 hands its accumulator to chain 0 through shared
 // memory, warp to warp.
 //
+// Bound by the exponentials (16 a clock and SM) and the moves between tensor
+// memory and registers around them: a step, 256 rows by 128 keys, takes 1.46 us
+// where its exponentials take 1.07 and its products 0.63.  Filling costs 4 us to
+// the first scores, a segment's end 2.  89 GFLOP over three prefixes of up to
+// 32768 keys: 150 us, tensor pipe 29 % active.
+//
 // Every wait is bounded (common.cuh); on a timeout the CTA raises an error
 // bit, drains its copies and MMAs, frees tensor memory and exits.
 #include <atomic>

@@ -32,8 +32,8 @@
 // less than 2^14 tokens cannot overflow, so plain shared-memory reductions
 // suffice: a 64-bit shared-memory add is a compare-and-swap loop.
 //
-// Measured (device, us): 24 at 5 rows of 51865 f32 logits, 44 at 64 rows bf16 with
-// every setting, 158 at 300 rows of 128000 f32 (28 + 74 + 56; one read of the
+// Measured (device, us): 25 at 5 rows of 51865 f32 logits, 44 at 64 rows bf16 with
+// every setting, 160 at 300 rows of 128000 f32 (28 + 75 + 60; one read of the
 // logits takes 24).  A few rows are bound by the chain of dependent passes, many
 // by the instructions of the second pass (about 35 a token).  The alternative,
 // a cluster of CTAs per row that keeps the logits in shared memory, took 25, 40

@@ -34,8 +34,8 @@
 // keys, values, merge.  Of the third: the exponentials and the moves between
 // tensor memory and registers.  Device time, bf16 or f16 caches, on one B200:
 //   5 sequences, 12 heads, 224 + up to 224 keys            6.9 us (2.4 MB)
-//   12 groups of 5, 20 heads, up to 1500 + up to 448 keys 34.5 us (145 MB, 4.2 TB/s)
-//   64 sequences, 32 / 8 heads, 8200 + up to 1000 keys    32.4 us (82 MB)
+//   12 groups of 5, 20 heads, up to 1500 + up to 448 keys 35 us   (145 MB, 4.1 TB/s)
+//   64 sequences, 32 / 8 heads, 8200 + up to 1000 keys    33 us   (82 MB)
 //   96 in 3 groups, 4 queries, 32768 + up to 700 keys      160 us (89 GFLOP, 0.56 PFLOP/s)
 #include <algorithm>
 

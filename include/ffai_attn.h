@@ -257,7 +257,8 @@ int ffai_kv_copy_pages(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool
  * The requests or beams of a batch that share a long prefix (a prompt) attend
  * to it together: its pages are read once for all of them.  Group g is the
  * consecutive sequences [group_starts[g], group_starts[g + 1]) (device int32,
- * n_groups + 1, rising; sequences outside every group have no prefix) and
+ * n_groups + 1, rising: else reported by ffai_attn_sync, and prefixes are left
+ * out; sequences outside every group have no prefix) and
  * shares the first prefix_lens[g] keys of the pages
  * prefix_table[g * prefix_pages ..]; sequence b adds the seq_lens[b] keys of
  * its own pages block_table[b * max_pages ..], the newest q_len of which are
