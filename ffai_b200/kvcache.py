@@ -214,7 +214,7 @@ def plan_pages(lens, new_tokens, free_pages, free_count, block_table, *, slot_ca
            _vec(free_pages, "free_pages", cap, index))
     count = _vec(free_count, "free_count", 1, index)
     base = None if pos_base is None else _vec(pos_base, "pos_base", B, index)
-    buf = torch.empty(2 * B + 2 + 2 * slot_cap, dtype=torch.int32, device=block_table.device)
+    buf = block_table.new_empty(2 * B + 2 + 2 * slot_cap)
     at = buf.data_ptr()
     cu, slots = at + 4 * B, at + 4 * (2 * B + 1)
     pos = slots + 4 * slot_cap
@@ -225,7 +225,8 @@ def plan_pages(lens, new_tokens, free_pages, free_count, block_table, *, slot_ca
         _raw_stream(index))
     if st:
         _check(st, ctx)
-    return PagePlan(*buf.split_with_sizes((B, B + 1, slot_cap, slot_cap, 1)))
+    # (integers need none of what autograd keeps for views: 0.7 us of a call's 14.5)
+    return PagePlan(*buf.unsafe_split_with_sizes((B, B + 1, slot_cap, slot_cap, 1)))
 
 
 def release_pages(lens, done, block_table, free_pages, free_count):
@@ -234,7 +235,7 @@ def release_pages(lens, done, block_table, free_pages, free_count):
     it, as new tensors."""
     B, max_pages, index = _table(block_table)
     cap = free_pages.numel()
-    buf = torch.empty(B + 1, dtype=torch.int32, device=block_table.device)
+    buf = block_table.new_empty(B + 1)
     at = buf.data_ptr()
     ctx = context(index)
     st = _abi.load().ffai_page_release(
@@ -243,7 +244,7 @@ def release_pages(lens, done, block_table, free_pages, free_count):
         _vec(free_count, "free_count", 1, index), at, at + 4 * B, _raw_stream(index))
     if st:
         _check(st, ctx)
-    return buf[:B], buf[B:]
+    return buf.unsafe_split_with_sizes((B, 1))
 
 
 def write_slots(k_pool, v_pool, k_new, v_new, slots) -> None:

@@ -48,10 +48,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=None, top_k=Non
     p = None if top_p is None else _setting(top_p, "top_p", f32, B, dev)
     m = None if min_p is None else _setting(min_p, "min_p", f32, B, dev)
     if out is None:
-        out = torch.empty(B, dtype=torch.int32, device=dev)
+        out = u.new_empty(B, dtype=torch.int32)
     elif out.shape != (B,) or out.dtype != torch.int32 or out.device != dev or not out.is_contiguous():
         raise ValueError(f"sample: out must be contiguous int32 ({B},) on {dev}")
-    logprob = torch.empty(B, dtype=f32, device=dev) if with_logprob else None
+    logprob = u.new_empty(B) if with_logprob else None
     index = dev.index
     ctx = context(index)
     st = _abi.load().ffai_sample(

@@ -76,13 +76,12 @@ def attend(q, k_pool, v_pool, prefix_table, prefix_lens, group_starts, block_tab
               _int32(seq_lens, "seq_lens", (B,), index), max_pages)
     shape = (B, n, H, 64) if out_layout == "token" else (B, H, n, 64)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype if out_dtype is None else out_dtype, device=q.device)
+        out = q.new_empty(shape) if out_dtype is None else q.new_empty(shape, dtype=out_dtype)
     elif out.shape != shape or out.get_device() != index or not out.is_contiguous():
         raise ValueError(f"shared prefix: out must be contiguous {shape} on cuda:{index}")
     lse = None
     if with_lse:
-        lse = torch.empty((H, B * n) if out_layout == "token" else (B, H, n),
-                          dtype=torch.float32, device=q.device)
+        lse = q.new_empty((H, B * n) if out_layout == "token" else (B, H, n), dtype=torch.float32)
     dt = _DT.get(q.dtype), _DT.get(k_pool.dtype), _DT.get(out.dtype)
     if None in dt:
         raise TypeError("shared prefix: f32, bf16 or f16 operands")
