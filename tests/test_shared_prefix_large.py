@@ -94,6 +94,7 @@ CASES = {
     "units_many": ([900, 2500], [100, 31], 40, 32, 4, 2),
     # and with long own keys: beside it
     "beside_odd_rows": ([12000], [91], 1600, 9, 3, 1),
+    "beside_short": ([7000], [260], 300, 16, 8, 2),
     "beside_groups": ([5000, 0, 6400, 70], [60, 9, 70, 2], 1300, 8, 4, 4),
 }
 
