@@ -577,6 +577,12 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
       uint32_t pk[32];
       {
         const uint64_t c2 = f2_pack(p.scale_log2, p.scale_log2);
+        uint64_t neg_m[2];  // (0 while every score was -inf)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const float n = m_run[v] == -INFINITY ? 0.f : -m_run[v];
+          neg_m[v] = f2_pack(n, n);
+        }
         uint64_t acc[2];
 #pragma unroll
         for (int v = 0; v < 2; ++v) acc[v] = f2_pack(0.f, 0.f);
@@ -585,8 +591,8 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
             float x0, x1;
-            f2_unpack(f2_fma(f2_pack(sf[4 * k + 2 * v], sf[4 * k + 2 * v + 1]), c2,
-                             f2_pack(-m_run[v], -m_run[v])), x0, x1);
+            f2_unpack(f2_fma(f2_pack(sf[4 * k + 2 * v], sf[4 * k + 2 * v + 1]), c2, neg_m[v]), x0,
+                      x1);
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             pk[2 * k + v] = F16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
             acc[v] = f2_add(acc[v], f2_pack(p0, p1));

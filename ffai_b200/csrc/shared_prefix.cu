@@ -36,7 +36,7 @@
 //   5 sequences, 12 heads, 224 + up to 224 keys            6.9 us (2.4 MB)
 //   12 groups of 5, 20 heads, up to 1500 + up to 448 keys 35 us   (145 MB, 4.1 TB/s)
 //   64 sequences, 32 / 8 heads, 8200 + up to 1000 keys    32 us   (82 MB)
-//   96 in 3 groups, 4 queries, 32768 + up to 700 keys      160 us (89 GFLOP, 0.56 PFLOP/s)
+//   96 in 3 groups, 4 queries, 32768 + up to 700 keys      161 us (89 GFLOP, 0.55 PFLOP/s)
 #include <algorithm>
 
 #include "shared_prefix.cuh"
@@ -109,10 +109,60 @@ __device__ __forceinline__ void fetch32(uint8_t* buf, const uint16_t* kp, const 
   }
 }
 
-// One step from buf; row v of this lane sees the first `see[v]` of its keys.
+// Value rows lo .. hi of a step are seen by some rows and not by others, whose
+// weight 0 a value that is not finite would turn into a NaN.  If there is one,
+// it is added to the rows that see it, and is 0 for the product of all.
 template <int F16>
-__device__ __forceinline__ void step32(RowState& st, const RowQ& q, const uint8_t* buf,
-                                       const int (&see)[2], float scale_log2) {
+__device__ __forceinline__ void guard_values(RowState& st, const uint32_t (&p)[2][4], uint8_t* buf,
+                                             const int (&see)[2], int lo, int hi) {
+  constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
+  const int lane = threadIdx.x % 32, t = lane & 3;
+  const auto bad = [](uint32_t x) {  // which halves are infinite or NaN
+    return ((x & kExp) == kExp ? 0xffffu : 0u) | ((x >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
+  };
+  bool any = false;
+  for (int i = lo * 8 + lane; i < hi * 8; i += 32) {
+    const uint4 v = *reinterpret_cast<const uint4*>(buf + v_piece(i >> 3, i & 7));
+    any = any || (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w));
+  }
+  if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll 1
+  for (int key = lo; key < hi; ++key) {
+    const int n = key >> 3;  // the weights' n-tile, and the lane that holds them
+    uint32_t w[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      w[r] = n == 0 ? p[0][r] : n == 1 ? p[0][2 + r] : n == 2 ? p[1][r] : p[1][2 + r];
+      w[r] = __shfl_sync(0xffffffffu, w[r], (lane & ~3) | ((key & 7) >> 1)) >> 16 * (key & 1);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint4 v = *reinterpret_cast<const uint4*>(buf + v_piece(key, 2 * t + x));
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (!(bad(u[j / 2]) >> 16 * (j & 1) & 1u)) continue;
+        const float f = j & 1 ? hi_half(u[j / 2], F16) : lo_half(u[j / 2], F16);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (key < see[r]) st.o[j][2 * r + x] = fmaf(lo_half(w[r], F16), f, st.o[j][2 * r + x]);
+      }
+    }
+  }
+  __syncwarp();
+  for (int i = lo * 8 + lane; i < hi * 8; i += 32) {
+    uint4* at = reinterpret_cast<uint4*>(buf + v_piece(i >> 3, i & 7));
+    const uint4 v = *at;
+    *at = make_uint4(v.x & ~bad(v.x), v.y & ~bad(v.y), v.z & ~bad(v.z), v.w & ~bad(v.w));
+  }
+  __syncwarp();
+}
+
+// One step from buf; row v of this lane sees the first `see[v]` of its keys.  TAIL:
+// not all rows alike, but all the first lo, and none those from hi on.
+template <int F16, bool TAIL>
+__device__ __forceinline__ void step32(RowState& st, const RowQ& q, uint8_t* buf,
+                                       const int (&see)[2], int lo, int hi, float scale_log2) {
   const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
   uint4 k[4][2];  // n-tile i: key 8 i + g
 #pragma unroll
@@ -165,6 +215,8 @@ __device__ __forceinline__ void step32(RowState& st, const RowQ& q, const uint8_
       st.o[j][2 * r + 1] *= corr;
     }
   }
+  if constexpr (TAIL)
+    if (lo < hi) guard_values<F16>(st, p, buf, see, lo, hi);
   uint4 v[2][4];  // 16-key half h: keys 16 h + 2 t + {0, 1, 8, 9}, dims 8 g ..
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -237,12 +289,12 @@ __device__ __forceinline__ int step_page(const int* table, int pages, int warp, 
   return page < pages ? __ldg(table + page) : -1;
 }
 
-// Walk `len` keys of a list of pages.  `ids` holds the first 32 steps' page
-// ids, loaded ahead (the table does not depend on the lengths).  `ring`: this
+// Walk `len` keys of a list of pages (TAIL: the first `common` of which all rows
+// see; else all rows see all).  `ids` holds the first 32 steps' page ids, loaded ahead (the table does not depend on the lengths).  `ring`: this
 // warp's kSpRing bytes, not in use.
-template <int F16, int W>
+template <int F16, int W, bool TAIL>
 __device__ __forceinline__ void walk(RowState& st, const RowQ& q, const SharedParams& p, int kvh,
-                                     const int* table, int pages, int ids, int len,
+                                     const int* table, int pages, int ids, int len, int common,
                                      const int (&see)[2], int warp, uint8_t* ring) {
   const uint16_t* kpool = static_cast<const uint16_t*>(p.k_pool);
   const uint16_t* vpool = static_cast<const uint16_t*>(p.v_pool);
@@ -273,7 +325,8 @@ __device__ __forceinline__ void walk(RowState& st, const RowQ& q, const SharedPa
     __syncwarp();
     const int k0 = i * kStride + warp * kSpKeys;
     const int rel[2] = {see[0] - k0, see[1] - k0};
-    step32<F16>(st, q, ring + i % kSpDepth * kSpStep, rel, p.scale_log2);
+    step32<F16, TAIL>(st, q, ring + i % kSpDepth * kSpStep, rel, max(common - k0, 0),
+                min(len - k0, kSpKeys), p.scale_log2);
     __syncwarp();
     fetch(i + kSpDepth);
   }
@@ -306,7 +359,7 @@ constexpr int kSpStage = 8;  // partials a thread stages at a time
 struct Merged {
   float m, l, o[8];
   __device__ __forceinline__ void add(const float2 ml, const float4 a, const float4 b) {
-    if (ml.x == -INFINITY) return;  // nothing in it
+    if (ml.y == 0.f) return;  // nothing in it (NaN: scores that were none)
     const float M = fmaxf(m, ml.x);
     const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - M), f1 = ex2_approx(ml.x - M);
     m = M;
@@ -444,7 +497,7 @@ __device__ __forceinline__ void store_row(const SharedParams& p, Merged& acc, in
   const int ti = rr / G, h = kvh * G + rr % G;
   const size_t at = static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(ti) * p.o_st +
                     static_cast<size_t>(h) * p.o_sh + 8 * part;
-  const float inv = acc.l > 0.f ? 1.f / acc.l : 0.f;
+  const float inv = acc.l == 0.f ? 0.f : 1.f / acc.l;  // 0: the row saw no key
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc.o[e] *= inv;
   if (p.out_dtype == 0) {
@@ -464,10 +517,10 @@ __device__ __forceinline__ void store_row(const SharedParams& p, Merged& acc, in
   if (p.lse && part == 0)
     p.lse[static_cast<size_t>(b) * p.lse_sb + static_cast<size_t>(ti) * p.lse_st +
           static_cast<size_t>(h) * p.lse_sh] =
-        acc.l > 0.f ? (acc.m + log2f(acc.l)) * 0.69314718055994530942f : -INFINITY;
+        acc.l == 0.f ? -INFINITY : (acc.m + log2f(acc.l)) * 0.69314718055994530942f;
 }
 
-template <int F16, int W>
+template <int F16, int W, bool TAIL>
 __global__ void __launch_bounds__(kSpThreads, 3) shared_rows_kernel(SharedParams p, int jobs) {
   extern __shared__ __align__(128) uint8_t sp_smem[];
   const int warp = threadIdx.x / 32 % W, slot = threadIdx.x / 32 / W, jt = threadIdx.x % (W * 32);
@@ -501,7 +554,9 @@ __global__ void __launch_bounds__(kSpThreads, 3) shared_rows_kernel(SharedParams
   }
   const int see[2] = {tok[0] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[0])),
                       tok[1] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[1]))};
-  walk<F16, W>(st, q, p, kvh, table, p.max_pages, ids, len, see, warp, ring);
+  // the tile's first token sees the fewest
+  const int common = max(0, len - (p.q_len - 1 - tile * 16 / G));
+  walk<F16, W, TAIL>(st, q, p, kvh, table, p.max_pages, ids, len, common, see, warp, ring);
   const int group = group_of(p, b);
   if (!p.part_o && blockIdx.x == 0 && threadIdx.x < 32)  // a prefix kernel's business otherwise
     for (int gi = lane; gi < p.groups; gi += 32) group_ok(p, gi, true);
@@ -509,8 +564,8 @@ __global__ void __launch_bounds__(kSpThreads, 3) shared_rows_kernel(SharedParams
     const int plen = min(max(__ldg(p.prefix_lens + group), 0), p.prefix_pages * kPageKeys);
     const int all[2] = {plen, plen};
     table = p.prefix_table + static_cast<size_t>(group) * p.prefix_pages;
-    walk<F16, W>(st, q, p, kvh, table, p.prefix_pages,
-                 step_page<W>(table, p.prefix_pages, warp, 0), plen, all, warp, ring);
+    walk<F16, W, false>(st, q, p, kvh, table, p.prefix_pages,
+                 step_page<W>(table, p.prefix_pages, warp, 0), plen, plen, all, warp, ring);
   }
 
   cp_async_wait_all();
@@ -565,7 +620,7 @@ __global__ void __launch_bounds__(kSpThreads, 3) shared_rows_kernel(SharedParams
 // The sequences' own keys beside the prefix kernel: teams of W warps take jobs
 // (a tile of 16 rows of a sequence and KV head) from the queue and leave one
 // partial per row in own_o / own_ml.
-template <int F16, int W>
+template <int F16, int W, bool TAIL>
 __global__ void __launch_bounds__(kSpThreads, 3) own_rows_kernel(SharedParams p, int jobs) {
   extern __shared__ __align__(128) uint8_t sp_smem[];
   __shared__ int s_job[kSpWarps];
@@ -603,7 +658,8 @@ __global__ void __launch_bounds__(kSpThreads, 3) own_rows_kernel(SharedParams p,
     }
     const int see[2] = {tok[0] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[0])),
                         tok[1] < 0 ? 0 : max(0, len - (p.q_len - 1 - tok[1]))};
-    walk<F16, W>(st, q, p, kvh, table, p.max_pages, ids, len, see, warp, ring);
+    const int common = max(0, len - (p.q_len - 1 - tile * 16 / G));
+    walk<F16, W, TAIL>(st, q, p, kvh, table, p.max_pages, ids, len, common, see, warp, ring);
     cp_async_wait_all();
     job_sync<W>(slot);
     put_state(st, sm, warp);
@@ -722,7 +778,7 @@ __global__ void __launch_bounds__(kSpThreads, 3) prefix_rows_kernel(SharedParams
     see[r] = row < d.rows ? len : 0;
   }
   load_rows(q, st, p, seq, tok, head);
-  walk<F16, kSpWarps>(st, q, p, kvh, table, mine, ids, len, see, warp, sp_smem + warp * kSpRing);
+  walk<F16, kSpWarps, false>(st, q, p, kvh, table, mine, ids, len, len, see, warp, sp_smem + warp * kSpRing);
   cp_async_wait_all();
   __syncthreads();
   put_state(st, sm, warp);
@@ -758,7 +814,9 @@ cudaError_t launch_rows(K kernel, long long ctas, size_t smem, bool dependent, c
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int F16>
+// TAIL: several queries a sequence, which see different numbers of its keys (without
+// it a walk is 2 to 4 % shorter).
+template <int F16, bool TAIL>
 cudaError_t launch_rows_f(const SharedParams& p, int sms, cudaStream_t s) {
   const int R = p.q_len * (p.heads / p.kv_heads);
   const int jobs = p.batch * p.kv_heads * ((R + 15) / 16);
@@ -766,13 +824,13 @@ cudaError_t launch_rows_f(const SharedParams& p, int sms, cudaStream_t s) {
   const bool dep = p.part_o != nullptr;
   const auto ctas = [&](int w) { return (static_cast<long long>(jobs) * w + kSpWarps - 1) / kSpWarps; };
   if (jobs <= room / 4)
-    return launch_rows(shared_rows_kernel<F16, 4>, ctas(4), kSpSmem, dep, s, p, jobs);
+    return launch_rows(shared_rows_kernel<F16, 4, TAIL>, ctas(4), kSpSmem, dep, s, p, jobs);
   if (jobs <= room / 2)
-    return launch_rows(shared_rows_kernel<F16, 2>, ctas(2), kSpSmem, dep, s, p, jobs);
-  return launch_rows(shared_rows_kernel<F16, 1>, ctas(1), kSpSmem, dep, s, p, jobs);
+    return launch_rows(shared_rows_kernel<F16, 2, TAIL>, ctas(2), kSpSmem, dep, s, p, jobs);
+  return launch_rows(shared_rows_kernel<F16, 1, TAIL>, ctas(1), kSpSmem, dep, s, p, jobs);
 }
 
-template <int F16>
+template <int F16, bool TAIL>
 cudaError_t launch_own_f(const SharedParams& p, int sms, cudaStream_t s) {
   const int R = p.q_len * (p.heads / p.kv_heads);
   const int jobs = p.batch * p.kv_heads * ((R + 15) / 16);
@@ -782,8 +840,8 @@ cudaError_t launch_own_f(const SharedParams& p, int sms, cudaStream_t s) {
   const int w = p.max_pages >= 8 ? 4 : 2;
   const long long ctas = std::min<long long>(
       3LL * sms, (static_cast<long long>(jobs) * w + kSpWarps - 1) / kSpWarps);
-  cudaError_t e = w == 4 ? launch_rows(own_rows_kernel<F16, 4>, ctas, kSpSmem, true, s, p, jobs)
-                         : launch_rows(own_rows_kernel<F16, 2>, ctas, kSpSmem, true, s, p, jobs);
+  cudaError_t e = w == 4 ? launch_rows(own_rows_kernel<F16, 4, TAIL>, ctas, kSpSmem, true, s, p, jobs)
+                         : launch_rows(own_rows_kernel<F16, 2, TAIL>, ctas, kSpSmem, true, s, p, jobs);
   if (e != cudaSuccess) return e;
   const int rows = p.batch * p.kv_heads * R;
   // as many octets a row as leave the merge in one wave
@@ -793,16 +851,21 @@ cudaError_t launch_own_f(const SharedParams& p, int sms, cudaStream_t s) {
   return launch_rows(merge_rows_kernel<1>, (rows + 15LL) / 16, 0, true, s, p, rows);
 }
 
+// f<element is f16, several queries a sequence>
+#define FFAI_ROWS(f, ...)                                                               \
+  (p.kv_dtype == 2 ? (p.q_len > 1 ? f<1, true>(__VA_ARGS__) : f<1, false>(__VA_ARGS__)) \
+                   : (p.q_len > 1 ? f<0, true>(__VA_ARGS__) : f<0, false>(__VA_ARGS__)))
+
 }  // namespace
 
 // Behind a prefix kernel the rows kernel is a programmatic dependent: sequences'
 // own keys are attended while the last of the prefix finishes.
 cudaError_t launch_shared_rows(const SharedParams& p, int sms, cudaStream_t s) {
-  return p.kv_dtype == 2 ? launch_rows_f<1>(p, sms, s) : launch_rows_f<0>(p, sms, s);
+  return FFAI_ROWS(launch_rows_f, p, sms, s);
 }
 
 cudaError_t launch_own_and_merge(const SharedParams& p, int sms, cudaStream_t s) {
-  return p.kv_dtype == 2 ? launch_own_f<1>(p, sms, s) : launch_own_f<0>(p, sms, s);
+  return FFAI_ROWS(launch_own_f, p, sms, s);
 }
 
 cudaError_t launch_prefix_rows(const SharedParams& p, int units, cudaStream_t s) {

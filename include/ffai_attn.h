@@ -277,7 +277,8 @@ int ffai_kv_copy_pages(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool
  * f32): the natural log-sum-exp of a row's scaled logits, (heads, batch *
  * q_len) for TOKEN_MAJOR output, (batch, heads, q_len) for HEADS_SPLIT.  A row
  * that sees no key gives zeros and -inf.  What lies in a page behind the last
- * live key is not used, whatever it is.  d->causal, q_offset, kv_len and the
+ * live key, or behind the last key a query sees, does not reach its row,
+ * whatever it is; NaN among the keys it sees does.  d->causal, q_offset, kv_len and the
  * k/v layouts are ignored, flags must be 0.  Page ids outside the pool or
  * lengths past a table are not read: ffai_attn_sync then reports
  * FFAI_ATTN_ERR_INVALID.  Partial results lie in a workspace of the context

@@ -191,3 +191,85 @@ def test_starts_that_do_not_rise_are_reported(name):
     attention.sync(0)
     U8 = 2.0 ** -7  # two ways to the same sums: each rounds weights and result once
     assert ((out.float() - want.float()).abs() <= U8 * 5.5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", [
+    ([100], [3], 90, 6, 2, 5), ([200, 0], [2, 4], 130, 4, 4, 17), ([300], [9], 40, 10, 1, 3),
+    CASES["tiles_one_sequence"], CASES["units"], CASES["beside_groups"],
+], ids=["own_prefix", "two_tiles", "ten_heads", "tiles", "units", "beside"])
+def test_a_bad_newest_key_reaches_its_own_query_alone(case, dtype):
+    """An infinite or NaN key or value of a sequence's newest token: earlier
+    queries of the same sequence do not see it, and come out to the bit as
+    with a finite one; the newest query's row shows it."""
+    prefix, sizes, own, heads, kv, n = case
+    c = build(prefix, sizes, max(own, n + 3), heads, kv, n, dtype, seed=11)
+    lens = [max(x, n) for x in c["lists"][1]]
+    c["seq_lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+    # (build leaves NaN behind the lengths it chose: new finite rows for those)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for b, ln in enumerate(lens):
+        for j in range(c["lists"][1][b], ln):
+            page = c["block_table"][b, j // 64].long()
+            for pool in ("k_pool", "v_pool"):
+                c[pool][page, :, j % 64] = torch.randn((kv, 64), generator=g, device=DEV).to(dtype)
+    clean = attend(c)
+    assert torch.isfinite(clean).all()
+    for pool, value, dims in (("v_pool", float("nan"), slice(5, 6)),
+                              ("v_pool", float("inf"), slice(0, 64)),
+                              ("k_pool", float("nan"), slice(9, 30))):
+        d = dict(c, **{pool: c[pool].clone()})
+        for b, ln in enumerate(lens):
+            d[pool][c["block_table"][b, (ln - 1) // 64].long(), :, (ln - 1) % 64, dims] = value
+        out = attend(d)
+        assert torch.equal(out[:, :-1], clean[:, :-1])
+        last = out[:, -1, :, dims if pool == "v_pool" else slice(0, 64)]
+        assert not torch.isfinite(last).any()
+        if pool == "v_pool" and dims == slice(5, 6):
+            rest = [x for x in range(64) if x != 5]
+            assert torch.equal(out[:, -1][..., rest], clean[:, -1][..., rest])
+
+
+PREFIXES = {"each": ([250, 140], [3, 4], 40, 6, 2, 2), "tiles": ([4097, 650], [3, 2], 130, 12, 4, 1),
+            "units": ([8300, 6000], [30, 40], 70, 12, 4, 2),
+            "beside": ([12000, 9000], [50, 41], 1600, 9, 3, 1)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", PREFIXES)
+def test_bad_prefix_keys_stay_in_their_group(name, dtype):
+    """128 NaN keys in one group's prefix: its rows are NaN, the other group's
+    the same to the bit."""
+    c = build(*PREFIXES[name], dtype, seed=2)
+    clean, lse = attend(c, with_lse=True)
+    pages = c["prefix_table"][0, :2].long()
+    bad = dict(c, k_pool=c["k_pool"].clone())
+    bad["k_pool"][pages] = float("nan")
+    out, bad_lse = attend(bad, with_lse=True)
+    n, first = c["q"].shape[1], c["lists"][2][1]
+    assert torch.isnan(out[:first]).all() and torch.isnan(bad_lse[:, :first * n]).all()
+    assert torch.equal(out[first:], clean[first:])
+    assert torch.equal(bad_lse[:, first * n:], lse[:, first * n:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", PREFIXES)
+def test_scores_of_minus_infinity_weigh_nothing(name, dtype):
+    """The first 128 keys' scores are all -inf: the formula's result, without
+    them."""
+    c = build(*PREFIXES[name], dtype, seed=4)
+    c["q"][..., 0] = 1.0
+    for g in range(2):
+        c["k_pool"][c["prefix_table"][g, :2].long(), :, :, 0] = float("-inf")
+    out, lse = attend(c, with_lse=True)
+    o, a, want = reference(c, 0.125)
+    keys = max(c["lists"][0]) + max(c["lists"][1])
+    tol = (U[dtype] + 1e-4) * a + U[dtype] * o.abs() + 1e-7
+    if dtype == torch.float16:
+        tol = tol + keys * 2.0 ** -25 * 5.5 + 2.0 ** -24
+    assert ((out.double() - o).abs() <= tol).all()
+    B, n, H, _ = c["q"].shape
+    assert (lse.double().view(H, B, n).permute(1, 2, 0) - want).abs().max().item() <= 2e-5
