@@ -76,15 +76,13 @@ __global__ void __launch_bounds__(kPlThreads) page_plan_kernel(PlanParams p) {
   bool bad = count < 0 || count > p.free_cap;
   count = min(max(count, 0), p.free_cap);
 
-  // Tokens are counted up to slot_cap + 1 a request (one that long does not
-  // fit anyway), so 64-bit sums cannot overflow.
   Sum2 sum{0, 0};
   for (int b = b0; b < b1; ++b) {
     const int len = __ldg(p.lens + b), want = __ldg(p.new_tokens + b);
     const bool ok = len >= 0 && want >= 0 && static_cast<long long>(len) + want <= reach;
     bad |= len < 0 || want < 0;
     s_len[b] = len;
-    sum.a += min(max(want, 0), p.slot_cap + 1);
+    sum.a += max(want, 0);
     sum.b += ok ? pages_of(len + want) - pages_of(len) : 0;
   }
   Sum2 at = block_exclusive(sum, s_warp);
@@ -95,7 +93,7 @@ __global__ void __launch_bounds__(kPlThreads) page_plan_kernel(PlanParams p) {
     const int need = ok ? pages_of(len + want) - pages_of(len) : 0;
     s_cu[b] = static_cast<int>(min(at.a, static_cast<long long>(INT32_MAX)));
     const long long first = at.b;
-    at.a += min(max(want, 0), p.slot_cap + 1);
+    at.a += max(want, 0);
     at.b += need;
     const bool served = ok && (need == 0 || at.b <= count) && at.a <= p.slot_cap;
     s_first[b] = served ? static_cast<int>(need == 0 ? 0 : first) : -1;

@@ -302,7 +302,8 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
  * stack of page ids, its top at free_count[0] - 1; pages go out in request
  * order and land in block_table (batch, max_pages) behind those the request
  * holds.  The new tokens of all requests are packed in request order: cu_new
- * (batch + 1) receives their running sum, slots (slot_cap) each token's slot
+ * (batch + 1) receives their running sum (negative counts as none, INT32_MAX
+ * at most), refused requests included, slots (slot_cap) each token's slot
  * page * FFAI_PAGE_KEYS + key, positions (optional, slot_cap) its key
  * position plus pos_base[b] (optional); rows past the last token get -1 and
  * 0.  A request is refused (no pages, slots -1, positions 0, lens_out = lens)

@@ -216,3 +216,29 @@ def test_write_slots_keeps_bits_and_refuses():
         kvcache.write_slots(kp, vp, new.expand(1, 2, 64), new, i32([1]))
     with pytest.raises(ValueError):
         kvcache.write_slots(kp, vp[:1], new, new, i32([1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,cap", [([5, 1], 2), ([1000], 0), ([3, 700, 2], 9), ([2, 0, 9, 1], 5),
+                                     ([-4, 6, 1], 3), ([2 ** 31 - 1, 2 ** 31 - 1, 5], 4)])
+def test_plan_sums_requests_that_ask_for_more_than_the_rows(new, cap):
+    """cu_new is the running sum whatever fits (of nothing for a negative
+    request, and at most the largest int32)."""
+    from ffai_b200 import attention, kvcache
+    B = len(new)
+    p = kvcache.plan_pages(i32([7] * B), i32(new), i32(list(range(8))), i32([8]),
+                           i32([[8 + b, -1, -1] for b in range(B)]), slot_cap=cap, num_pages=20)
+    want = [0]
+    for n in new:
+        want.append(want[-1] + max(n, 0))
+    assert p.cu_new.tolist() == [min(c, 2 ** 31 - 1) for c in want]
+    fits = [n >= 0 and 7 + n <= 192 and want[b + 1] <= cap for b, n in enumerate(new)]
+    assert p.lens.tolist() == [7 + n if f else 7 for n, f in zip(new, fits)]
+    rows = [(8 + b) * 64 + 7 + i if f else -1 for b, (n, f) in enumerate(zip(new, fits))
+            for i in range(min(max(n, 0), cap))]
+    assert p.slots.tolist() == (rows + [-1] * cap)[:cap]
+    assert p.free_count.tolist() == [8]
+    if min(new) < 0:
+        with pytest.raises(attention.AttnError):
+            attention.sync(0)
+    attention.sync(0)
