@@ -152,8 +152,8 @@ __global__ void __launch_bounds__(kPlThreads) page_plan_kernel(PlanParams p) {
 }
 
 // The pages of requests with done != 0 are pushed on the stack in request
-// order, each request's in key order.  Every CTA scans all requests, then its
-// warps copy the pages of every gridDim-th request.
+// order, each request's in key order, as far as the stack reaches.  Every CTA
+// scans all requests, then its warps copy the pages of every gridDim-th request.
 __global__ void __launch_bounds__(kPlThreads) page_release_kernel(ReleaseParams p) {
   extern __shared__ int s_at[];  // batch: stack position of a request's first page, or -1
   __shared__ Sum2 s_warp[kPlWarps];
@@ -177,9 +177,9 @@ __global__ void __launch_bounds__(kPlThreads) page_release_kernel(ReleaseParams 
   Sum2 at = block_exclusive(sum, s_warp);
   for (int b = b0; b < b1; ++b) {
     const int n = gives(b);
-    const bool fits = count + at.a + n <= p.free_cap;
-    s_at[b] = n > 0 && fits ? static_cast<int>(count + at.a) : -1;
-    bad |= !fits;
+    const long long dst = count + at.a;
+    s_at[b] = n > 0 && dst < p.free_cap ? static_cast<int>(dst) : -1;
+    bad |= dst + n > p.free_cap;
     at.a += n;
     if (blockIdx.x == 0) p.lens_out[b] = __ldg(p.done + b) != 0 ? 0 : __ldg(p.lens + b);
   }
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kPlThreads) page_release_kernel(ReleaseParams 
   for (int b = blockIdx.x * kPlWarps + warp; b < p.batch; b += gridDim.x * kPlWarps) {
     const int dst = s_at[b];
     if (dst < 0) continue;
-    const int n = pages_of(__ldg(p.lens + b));
+    const int n = min(pages_of(__ldg(p.lens + b)), p.free_cap - dst);
     for (int i = lane; i < n; i += 32)
       p.free_pages[dst + i] = __ldg(p.block_table + static_cast<size_t>(b) * p.max_pages + i);
   }

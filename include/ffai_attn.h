@@ -325,8 +325,9 @@ int ffai_page_plan(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, int32_t
 /* Requests with done[b] != 0 hand their ceil(lens[b] / FFAI_PAGE_KEYS) pages
  * back: pushed on free_pages in request order, each request's in key order;
  * lens_out[b] = 0 for them, lens[b] for the others; free_count_out[0] the new
- * count.  Pages that would pass free_cap are not pushed, and reported by
- * ffai_attn_sync. */
+ * count, of what lies on the stack.  Pages that would pass free_cap are not
+ * pushed and not counted, and a free_count outside 0 .. free_cap is taken for
+ * the nearer end: both are reported by ffai_attn_sync. */
 int ffai_page_release(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, const int32_t* lens,
                       const int32_t* done, const int32_t* block_table, int32_t* free_pages,
                       int32_t free_cap, const int32_t* free_count, int32_t* lens_out,

@@ -242,3 +242,33 @@ def test_plan_sums_requests_that_ask_for_more_than_the_rows(new, cap):
         with pytest.raises(attention.AttnError):
             attention.sync(0)
     attention.sync(0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,done,count,cap", [
+    ([64, 128], [1, 1], 0, 2), ([64, 128, 5], [1, 1, 1], 0, 2), ([10, 300, 64, 1], [1, 0, 1, 1], 5, 6),
+    ([300, 64], [1, 1], 3, 3), ([192, 64], [0, 1], 4, 5), ([640] * 700, [1] * 700, 11, 1003)])
+def test_release_counts_the_pages_it_pushed(lens, done, count, cap):
+    """Pages past the stack's end are not pushed; the count is of those that
+    were, and a plan hands out nothing else."""
+    from ffai_b200 import attention, kvcache
+    mp = max(1, max((n + 63) // 64 for n in lens))
+    table = (torch.arange(len(lens) * mp) + cap).view(len(lens), mp)
+    stack = [i if i < count else -9 for i in range(cap)]
+    free = i32(stack)
+    given = [int(table[b, j]) for b, n in enumerate(lens) if done[b] for j in range((n + 63) // 64)]
+    want = (stack[:count] + given)[:cap]
+    out, left = kvcache.release_pages(i32(lens), i32(done), i32(table), free, i32([count]))
+    assert left.tolist() == [len(want)]
+    assert free.tolist() == (want + stack[len(want):])[:cap]
+    assert out.tolist() == [0 if d else n for n, d in zip(lens, done)]
+    if count + len(given) > cap:
+        with pytest.raises(attention.AttnError):
+            attention.sync(0)
+    attention.sync(0)
+    tables = i32(torch.full((cap + 1, 1), -1))
+    p = kvcache.plan_pages(i32([0] * (cap + 1)), i32([1] * (cap + 1)), free, left, tables,
+                           slot_cap=cap + 1, num_pages=cap + len(lens) * mp)
+    got = [t for (t,) in tables.tolist() if t >= 0]
+    assert got == want[::-1] and p.lens.tolist() == [1] * len(want) + [0] * (cap + 1 - len(want))
+    attention.sync(0)
