@@ -60,42 +60,84 @@ __device__ __forceinline__ int pages_of(long long keys) {
 // than a second launch or a grid-wide exchange) and then maps its own stretch
 // of the packed tokens.  Shared memory per request: the packed row of its
 // first token, its length, and the stack offset of its first new page, or
-// -1 when it is refused.
+// -1 when it is refused.  Page ids are looked at before anything is promised:
+// the stack ends at its first bad id, and a request whose last page is bad
+// and still has room takes part as if it outgrew the table.
 __global__ void __launch_bounds__(kPlThreads) page_plan_kernel(PlanParams p) {
   extern __shared__ int s_plan[];
   int* s_cu = s_plan;                 // batch + 1
   int* s_len = s_plan + p.batch + 1;  // batch
-  int* s_first = s_len + p.batch;     // batch
+  int* s_first = s_len + p.batch;     // batch; before that the pages needed, or -1
   __shared__ Sum2 s_warp[kPlWarps];
-  __shared__ int s_taken;
+  __shared__ int s_taken, s_usable;
   const int per = (p.batch + kPlThreads - 1) / kPlThreads;
   const int b0 = min(p.batch, static_cast<int>(threadIdx.x) * per), b1 = min(p.batch, b0 + per);
   const int reach = p.max_pages * kPageKeys;  // host: fits 30 bits
-  if (threadIdx.x == 0) s_taken = 0;
-  int count = __ldg(p.free_count);
-  bool bad = count < 0 || count > p.free_cap;
-  count = min(max(count, 0), p.free_cap);
+  const int held_count = __ldg(p.free_count);
+  bool bad = held_count < 0 || held_count > p.free_cap;
+  const int count = bad ? 0 : held_count;
+  if (threadIdx.x == 0) {
+    s_taken = 0;
+    s_usable = count;
+  }
+  __syncthreads();
+  // The pages that requests within the rows can ask for: one a request and one
+  // for every 64 rows.  Behind the first bad id the stack is not used.
+  const int asked = min(count, p.slot_cap / kPageKeys + min(p.batch, p.slot_cap));
+  int first_bad = INT32_MAX;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < asked; i += kPlThreads) {
+    const int id = __ldg(p.free_pages + (count - 1 - i));
+    if (id < 0 || id >= p.num_pages) first_bad = min(first_bad, i);
+  }
+  if (first_bad != INT32_MAX) atomicMin(&s_usable, first_bad);
 
   Sum2 sum{0, 0};
-  for (int b = b0; b < b1; ++b) {
-    const int len = __ldg(p.lens + b), want = __ldg(p.new_tokens + b);
-    const bool ok = len >= 0 && want >= 0 && static_cast<long long>(len) + want <= reach;
-    bad |= len < 0 || want < 0;
-    s_len[b] = len;
-    sum.a += max(want, 0);
-    sum.b += ok ? pages_of(len + want) - pages_of(len) : 0;
+  constexpr int kTogether = 4;  // requests whose loads are in flight together
+  for (int bb = b0; bb < b1; bb += kTogether) {
+    int len[kTogether], want[kTogether], id[kTogether];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      const int b = min(bb + k, b1 - 1);
+      len[k] = __ldg(p.lens + b);
+      want[k] = __ldg(p.new_tokens + b);
+    }
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      const int b = min(bb + k, b1 - 1);
+      id[k] = 0;
+      if (len[k] > 0 && len[k] < reach && len[k] % kPageKeys != 0 && want[k] > 0)
+        // (an entry that no thread writes: new ones lie behind it)
+        id[k] = p.block_table[static_cast<size_t>(b) * p.max_pages + len[k] / kPageKeys];
+    }
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      if (bb + k >= b1) break;
+      bool ok = len[k] >= 0 && want[k] >= 0 && static_cast<long long>(len[k]) + want[k] <= reach;
+      bad |= len[k] < 0 || want[k] < 0;
+      if (ok && (id[k] < 0 || id[k] >= p.num_pages)) {
+        ok = false;
+        bad = true;
+      }
+      const int need = ok ? pages_of(len[k] + want[k]) - pages_of(len[k]) : -1;
+      s_len[bb + k] = len[k];
+      s_first[bb + k] = need;
+      sum.a += max(want[k], 0);
+      sum.b += max(need, 0);
+    }
   }
   Sum2 at = block_exclusive(sum, s_warp);
+  const int usable = s_usable;
   int taken = 0;
   for (int b = b0; b < b1; ++b) {
-    const int len = s_len[b], want = __ldg(p.new_tokens + b);
-    const bool ok = len >= 0 && want >= 0 && static_cast<long long>(len) + want <= reach;
-    const int need = ok ? pages_of(len + want) - pages_of(len) : 0;
+    const int len = s_len[b], want = __ldg(p.new_tokens + b), need = s_first[b];
     s_cu[b] = static_cast<int>(min(at.a, static_cast<long long>(INT32_MAX)));
     const long long first = at.b;
     at.a += max(want, 0);
-    at.b += need;
-    const bool served = ok && (need == 0 || at.b <= count) && at.a <= p.slot_cap;
+    at.b += max(need, 0);
+    const bool fits = need >= 0 && at.a <= p.slot_cap;
+    const bool served = fits && (need == 0 || at.b <= usable);
+    bad |= fits && !served && at.b <= count;  // for a bad id on the stack alone
     s_first[b] = served ? static_cast<int>(need == 0 ? 0 : first) : -1;
     if (served && need > 0) taken = static_cast<int>(at.b);
     if (blockIdx.x == 0) {
@@ -109,7 +151,7 @@ __global__ void __launch_bounds__(kPlThreads) page_plan_kernel(PlanParams p) {
   }
   if (taken > 0) atomicMax(&s_taken, taken);
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.free_count_out = count - s_taken;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.free_count_out = held_count - s_taken;
   if (bad && blockIdx.x == 0 && p.err) atomicOr(p.err, kErrBadArgs);
 
   const int total = s_cu[p.batch];
@@ -138,12 +180,8 @@ __global__ void __launch_bounds__(kPlThreads) page_plan_kernel(PlanParams p) {
           // the page's first key of this request writes its table entry
           if (at_key % kPageKeys == 0) row[pg] = id;
         }
-        if (id >= 0 && id < p.num_pages) {
-          slot = id * kPageKeys + at_key % kPageKeys;
-          pos = at_key + (p.pos_base ? __ldg(p.pos_base + b) : 0);
-        } else if (p.err) {
-          atomicOr(p.err, kErrBadArgs);
-        }
+        slot = id * kPageKeys + at_key % kPageKeys;
+        pos = at_key + (p.pos_base ? __ldg(p.pos_base + b) : 0);
       }
     }
     p.slots[t] = slot;

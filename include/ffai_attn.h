@@ -312,9 +312,12 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
  * when its rows pass slot_cap; else lens_out[b] = lens[b] + new_tokens[b].
  * free_count_out[0]: pages left.  lens, free_count and free_pages are not
  * written, so a plan can be repeated; lens_out and free_count_out must not
- * alias them.  batch at most 16384 (else FFAI_ATTN_DECLINED).  Negative
- * lengths, a bad free_count or a bad page id: refused, and reported by
- * ffai_attn_sync.  No reference counterpart (Tensor::cat per step,
+ * alias them.  batch at most 16384 (else FFAI_ATTN_DECLINED).  Refused too,
+ * and reported by ffai_attn_sync: a negative length; a request whose last
+ * page has room for its keys but an id outside the pool (0 .. num_pages - 1);
+ * and what needs a page from behind such an id on the stack, which ends
+ * there, or under a free_count outside 0 .. free_cap, which is left as it is.
+ * No reference counterpart (Tensor::cat per step,
  * text_decoder.rs:657-664). */
 int ffai_page_plan(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, int32_t num_pages,
                    const int32_t* lens, const int32_t* new_tokens, const int32_t* free_pages,

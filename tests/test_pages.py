@@ -272,3 +272,70 @@ def test_release_counts_the_pages_it_pushed(lens, done, count, cap):
     got = [t for (t,) in tables.tolist() if t >= 0]
     assert got == want[::-1] and p.lens.tolist() == [1] * len(want) + [0] * (cap + 1 - len(want))
     attention.sync(0)
+
+
+def refused_plan(lens, new, free, count, table, num_pages, cap):
+    """The rule for inputs that hold a bad count or page id: the stack has no
+    pages under a bad count and ends at a bad id, and a request whose last page
+    is bad and not full takes part as if it outgrew the table."""
+    bad = lambda i: not 0 <= i < num_pages  # noqa: E731
+    held_bad = [n % 64 != 0 and w > 0 and bad(table[b][n // 64])
+                for b, (n, w) in enumerate(zip(lens, new))]
+    usable = 0 if not 0 <= count <= len(free) else next(
+        (i for i in range(count) if bad(free[count - 1 - i])), count)
+    out, want, used = [], 0, 0
+    t = [list(r) for r in table]
+    slots, cu = [], 0
+    for b, (n, w) in enumerate(zip(lens, new)):
+        need = 0 if held_bad[b] else (n + w + 63) // 64 - (n + 63) // 64
+        first, want, cu = want, want + need, cu + w
+        if held_bad[b] or (need and want > usable) or cu > cap:
+            out.append(n)
+            slots += [-1] * w
+            continue
+        for j in range(need):
+            t[b][(n + 63) // 64 + j] = free[count - 1 - first - j]
+        used = max(used, want if need else 0)
+        slots += [t[b][(n + i) // 64] * 64 + (n + i) % 64 for i in range(w)]
+        out.append(n + w)
+    return t, out, (slots + [-1] * cap)[:cap], count - used
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,new,free,count,table,cap", [
+    # a count that is not one: what needs a page is refused, and the count stays
+    ([63, 64], [1, 1], [5, 4], 99, [[0, -1], [1, -1]], 4),
+    ([63, 64], [1, 1], [5, 4], -1, [[0, -1], [1, -1]], 4),
+    ([0], [200], [5, 4, 3], 4, [[-1] * 4], 200),
+    # a bad id on the stack, within, at the end of and behind what is asked for
+    ([0, 0, 0], [1, 1, 1], [6, 7, 99, 5], 4, [[-1], [-1], [-1]], 3),
+    ([0, 64, 10], [130, 1, 4], [8, 9, -2, 4, 5], 5, [[-1] * 3, [1, -1, -1], [2, -1, -1]], 140),
+    ([0, 0], [1, 1], [99, 6, 5], 3, [[-1], [-1]], 2),
+    ([0, 0], [64, 64], [5, 20], 2, [[-1], [-1]], 128),
+    # a bad id in the table, where new keys go and where none do
+    ([10, 10, 64], [1, 1, 1], [5, 4], 2, [[0, -1], [77, -1], [1, -1]], 3),
+    ([100, 10], [60, 1], [5, 4], 2, [[0, -1, -1], [2, -1, -1]], 61),
+    ([128, 10, 70], [1, 0, 1], [5, 4], 2, [[0, 50, -1], [-3, -1, -1], [60, 3, -1]], 3),
+    # and many requests
+    ([0] * 1200, [65] * 1200, list(range(700)) + [-1] + list(range(701, 3000)), 3000,
+     [[-1, -1]] * 1200, 1200 * 65),
+    ([1 + b % 64 for b in range(1200)], [1] * 1200, list(range(1200, 1240)), 40,
+     [[b if b % 7 else -1, -1] for b in range(1200)], 1200),
+])
+def test_plan_refuses_bad_counts_and_pages(lens, new, free, count, table, cap):
+    from ffai_b200 import attention, kvcache
+    num_pages = 10 if len(lens) < 100 else 3000
+    t, out, slots, left = refused_plan(lens, new, free, count, table, num_pages, cap)
+    dev = i32(table)
+    p = kvcache.plan_pages(i32(lens), i32(new), i32(free), i32([count]), dev, slot_cap=cap,
+                           num_pages=num_pages)
+    assert p.lens.tolist() == out
+    assert p.slots.tolist() == slots
+    assert dev.tolist() == t
+    assert p.free_count.tolist() == [left]
+    met = (out != [n + w for n, w in zip(lens, new)])  # nothing else refuses these
+    if met:
+        with pytest.raises(attention.AttnError) as e:
+            attention.sync(0)
+        assert e.value.status == -1
+    attention.sync(0)
