@@ -255,17 +255,20 @@ __device__ __forceinline__ const void* q_row(const SharedParams& p, int b, int t
 }
 
 // The group whose sequences hold b, or -1 (a whole warp): starts[] rises, so
-// it is the last group that starts at or before b, if b is before its end.
+// it is the last group that starts at or before b, if b is before its end.  If
+// it does not rise within the batch, no sequence has a group.
 __device__ __forceinline__ int group_of(const SharedParams& p, int b) {
   const int lane = threadIdx.x % 32;
   int n = 0;  // groups that start at or before b
+  bool bad = false;
   for (int base = 0; base < p.groups; base += 32) {
     const int g = base + lane;
+    if (g < p.groups) bad = bad || !group_ok(p, g, false);
     const bool in = g < p.groups && __ldg(p.group_starts + g) <= b;
     n += __popc(__ballot_sync(0xffffffffu, in));
   }
-  // (the first test holds unless the starts do not rise)
-  return n > 0 && __ldg(p.group_starts + n - 1) <= b && b < __ldg(p.group_starts + n) ? n - 1 : -1;
+  if (__any_sync(0xffffffffu, bad)) return -1;
+  return n > 0 && b < __ldg(p.group_starts + n) ? n - 1 : -1;
 }
 
 // The same for a lane by itself.

@@ -263,3 +263,25 @@ def test_bad_tables_are_reported_not_read(what):
         attention.sync(0)
     assert e.value.status == -1
     attention.sync(0)  # the word is cleared
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[0, 3, 2, 4], [0, 1, 2, 7], [-1, 1, 2, 4], [2, 1, 3, 4], [0, 4, 4, 2]])
+@pytest.mark.parametrize("n", [1, 3])
+def test_starts_that_do_not_rise_leave_short_prefixes_out_too(starts, n):
+    """To the bit the result without prefixes, and an error at the next sync;
+    with 40 groups as well, more than a warp has lanes."""
+    from ffai_b200 import attention
+    for more in (0, 37):
+        c = build([70, 0, 9] + [5] * more, [3, 40, 0, 66], [2, 1, 1] + [0] * more, 4, 2, n,
+                  torch.bfloat16, seed=len(starts) + n)
+        plain = dict(c, prefix_lens=torch.zeros_like(c["prefix_lens"]))
+        want = run(plain, 0.125)
+        attention.sync(0)
+        assert not torch.equal(run(c, 0.125), want)
+        bad = dict(c, group_starts=torch.tensor([0] * more + starts, dtype=torch.int32))
+        got = run(bad, 0.125)
+        with pytest.raises(attention.AttnError) as e:
+            attention.sync(0)
+        assert e.value.status == -1
+        assert torch.equal(got, want)
