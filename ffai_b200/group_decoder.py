@@ -14,8 +14,9 @@ A step is seven calls without a host round trip:
   6. the vocabulary projection;
   7. `sampling.sample`.
 
-The state lives in fixed tensors that the calls update, so a step can be
-captured in a CUDA graph and replayed.  Requests that end hand their pages
+The state lives in tensors that are made once and that every call, `open` and
+`close_groups` too, updates in place: a step captured in a CUDA graph can be
+replayed for the decoder's whole life.  Requests that end hand their pages
 back (`kvcache.release_pages`).  Layer norms, the MLP and embeddings stay with
 the caller, as in `encoder_attention`; a model with more layers keeps pools per
 layer and shares the plan.  No reference counterpart (its decoder serves one
@@ -37,10 +38,13 @@ HD = 64
 class GroupDecoder:
     """One attention layer and the vocabulary projection for up to `batch`
     requests: w_qkv ((heads + 2 kv_heads) * 64, D), w_out (D, heads * 64),
-    w_vocab (V, D), bf16 on the device."""
+    w_vocab (V, D), bf16 on the device.  At most max_groups prompts at a time
+    (default: `batch`) of max_prompt tokens (default: what num_pages hold);
+    attention is laid out for these bounds, so close ones make it faster."""
 
     def __init__(self, w_qkv, w_out, w_vocab, *, heads: int, kv_heads: int, batch: int,
-                 max_len: int, num_pages: int, scale: float = HD ** -0.5):
+                 max_len: int, num_pages: int, scale: float = HD ** -0.5,
+                 max_groups: int | None = None, max_prompt: int | None = None):
         if w_qkv.shape != ((heads + 2 * kv_heads) * HD, w_out.shape[0]) or \
                 w_out.shape[1] != heads * HD or w_vocab.shape[1] != w_out.shape[0]:
             raise ValueError("group decoder: w_qkv ((heads + 2 kv_heads) * 64, D), "
@@ -60,9 +64,12 @@ class GroupDecoder:
         pages = (max_len + kvcache.PAGE_KEYS - 1) // kvcache.PAGE_KEYS
         self.block_table = torch.full((batch, pages), -1, **i32)
         self.lens = torch.zeros(batch, **i32)
-        self.prefix_table = torch.zeros((0, 1), **i32)
-        self.prefix_lens = torch.zeros(0, **i32)
-        self.group_starts = torch.zeros(1, **i32)
+        self.max_groups = batch if max_groups is None else max_groups
+        self.max_prompt = num_pages * kvcache.PAGE_KEYS if max_prompt is None else max_prompt
+        pages = max(1, (self.max_prompt + kvcache.PAGE_KEYS - 1) // kvcache.PAGE_KEYS)
+        self.prefix_table = torch.full((self.max_groups, pages), -1, **i32)
+        self.prefix_lens = torch.zeros(self.max_groups, **i32)
+        self.group_starts = torch.zeros(self.max_groups + 1, **i32)
 
     def _project(self, x):
         """(T, D) -> q (T, heads, 64), k, v (T, kv_heads, 64): views of one buffer."""
@@ -74,22 +81,23 @@ class GroupDecoder:
         """Start groups: prompts[g] (n_g, D) bf16 hidden states (after the
         caller's norm) of group g's prompt, shared by sizes[g] consecutive
         requests.  The requests and groups before must have been closed."""
-        if len(prompts) != len(sizes) or sum(sizes) > self.batch:
-            raise ValueError("group decoder: a size for each prompt, at most `batch` requests")
-        dev = self.lens.device
-        i32 = dict(dtype=torch.int32, device=dev)
         ns = [p.shape[0] for p in prompts]
-        pages = max(1, max(-(-n // kvcache.PAGE_KEYS) for n in ns))
+        if len(ns) != len(sizes) or sum(sizes) > self.batch:
+            raise ValueError("group decoder: a size for each prompt, at most `batch` requests")
+        if len(ns) > self.max_groups or max(ns) > self.max_prompt:
+            raise ValueError(f"group decoder: at most {self.max_groups} prompts of "
+                             f"{self.max_prompt} tokens")
+        i32 = dict(dtype=torch.int32, device=self.lens.device)
+        none = self.max_groups - len(ns)  # groups without requests, behind the others
         starts = [0]
-        for s in sizes:
+        for s in list(sizes) + [0] * none:
             starts.append(starts[-1] + s)
-        self.prefix_table = torch.full((len(ns), pages), -1, **i32)
-        self.group_starts = torch.tensor(starts, **i32)
-        want = torch.tensor(ns, **i32)
+        self.group_starts.copy_(torch.tensor(starts, **i32))
+        want = torch.tensor(ns + [0] * none, **i32)
         plan = kvcache.plan_pages(torch.zeros_like(want), want, self.free_pages, self.free_count,
                                   self.prefix_table, slot_cap=sum(ns))
         self.free_count.copy_(plan.free_count)
-        self.prefix_lens = plan.lens
+        self.prefix_lens.copy_(plan.lens)
         if not torch.equal(plan.lens, want):
             self.close_groups()
             raise MemoryError("group decoder: no free pages for the prompts")
@@ -139,7 +147,7 @@ class GroupDecoder:
         """All prompts' pages go back."""
         lens, count = kvcache.release_pages(self.prefix_lens, torch.ones_like(self.prefix_lens),
                                             self.prefix_table, self.free_pages, self.free_count)
-        self.prefix_lens = lens
+        self.prefix_lens.copy_(lens)
         self.free_count.copy_(count)
 
 
@@ -150,7 +158,8 @@ def main(groups: int = 12, beams: int = 5, prompt: int = 1500, steps: int = 64) 
     g = torch.Generator(device="cuda:0").manual_seed(0)
     w = lambda *s: (torch.randn(s, generator=g, device="cuda:0") * s[-1] ** -0.5).to(torch.bfloat16)  # noqa: E731
     dec = GroupDecoder(w(3 * D, D), w(D, D), w(vocab, D), heads=heads, kv_heads=heads, batch=B,
-                       max_len=448, num_pages=groups * 24 + B * 7)
+                       max_len=448, num_pages=groups * 24 + B * 7, max_groups=groups,
+                       max_prompt=prompt)
     dec.open([w(prompt, D) * D ** 0.5 for _ in range(groups)], [beams] * groups)
     table = w(vocab, D) * D ** 0.5  # embeddings
     active = torch.ones(B, dtype=torch.int32, device="cuda:0")

@@ -139,3 +139,75 @@ def test_a_captured_step_continues():
                 out.append(dec.step(x, active, u, temperature=0.9, min_p=0.01))
         runs.append((torch.stack(out), dec.lens.clone()))
     assert torch.equal(runs[0][0], runs[1][0]) and runs[0][1].tolist() == runs[1][1].tolist() == [8] * 6
+
+
+@pytest.mark.gpu
+def test_a_captured_step_outlives_its_groups():
+    """A step captured over one set of prompts, replayed over others, more and
+    fewer, shorter and longer: the tokens of steps that were never captured, to
+    the bit, with other work taking the memory that a call sets free."""
+    from ffai_b200 import attention
+    rounds = [([300, 1], [4, 2]), ([700, 30, 65, 129], [1, 2, 2, 1]), ([64], [5]), ([10, 900], [0, 6])]
+    runs = []
+    for captured in (False, True):
+        dec, rand, g = make(num_pages=60, seed=5)
+        held = [(t, t.data_ptr()) for t in (dec.prefix_table, dec.prefix_lens, dec.group_starts,
+                                            dec.block_table, dec.lens, dec.free_pages, dec.free_count)]
+        active = torch.ones(6, dtype=torch.int32, device=DEV)
+        x, u = rand(6, 1, D), torch.rand(6, generator=g, device=DEV)
+        tokens, graph = [], None
+        for ns, sizes in rounds:
+            dec.open([rand(n, D) for n in ns], sizes)
+            for _ in range(3):
+                x.copy_(rand(6, 1, D))
+                u.copy_(torch.rand(6, generator=g, device=DEV))
+                noise = [torch.full((2 ** k,), -1, dtype=torch.int32, device=DEV) for k in range(12)]
+                if not captured:
+                    got = dec.step(x, active, u, temperature=0.9, min_p=0.01)
+                else:
+                    if graph is None:
+                        lens, count = dec.lens.clone(), dec.free_count.clone()
+                        table = dec.block_table.clone()
+                        dec.step(x, active, u, temperature=0.9, min_p=0.01)
+                        for t, v in ((dec.lens, lens), (dec.free_count, count), (dec.block_table, table)):
+                            t.copy_(v)
+                        graph = torch.cuda.CUDAGraph()
+                        with torch.cuda.graph(graph):
+                            out = dec.step(x, active, u, temperature=0.9, min_p=0.01)
+                    graph.replay()
+                    got = out
+                tokens.append(got.clone())
+                del noise
+            dec.close(active)
+            dec.close_groups()
+            assert dec.free_count.item() == 60
+        assert all(t.data_ptr() == at for t, at in held)
+        assert all(a is b for a, (b, _) in zip((dec.prefix_table, dec.prefix_lens, dec.group_starts),
+                                               held))
+        runs.append(torch.stack(tokens))
+    assert (runs[0] >= 0).all() and torch.equal(runs[0], runs[1])
+    attention.sync(0)
+
+
+@pytest.mark.gpu
+def test_bounds_on_prompts():
+    """Prompts past the bounds are refused before anything changes."""
+    from ffai_b200.group_decoder import GroupDecoder
+    dec, rand, g = make(num_pages=20)
+    w = lambda *s: rand(*s)  # noqa: E731
+    tight = GroupDecoder(dec.w_qkv, dec.w_out, w(V, D), heads=H, kv_heads=HK, batch=6, max_len=200,
+                         num_pages=20, max_groups=2, max_prompt=100)
+    for prompts, sizes in (([rand(101, D)], [1]), ([rand(1, D)] * 3, [1, 1, 1])):
+        with pytest.raises(ValueError):
+            tight.open(prompts, sizes)
+        assert tight.free_count.item() == 20 and tight.group_starts.tolist() == [0, 0, 0]
+    prompts = [rand(100, D), rand(65, D)]
+    x, active = rand(6, 1, D), torch.ones(6, dtype=torch.int32, device=DEV)
+    out = []
+    for d in (tight, dec):  # bounds change the layout, not the result
+        d.open(prompts, [2, 3])
+        out.append(d.hidden(x, active)[0].double())
+    prefix = [tuple(t.clone() for t in dec._project(p)[1:]) for p in prompts]
+    k, v = dec._project(x.view(6, D))[1:]
+    want, tol = expected(dec, x, [(k[b:b + 1], v[b:b + 1]) for b in range(6)], prefix, [0, 2, 5])
+    assert all(((y - want).abs() <= tol).all() for y in out)
