@@ -84,7 +84,7 @@ class GroupDecoder:
         ns = [p.shape[0] for p in prompts]
         if len(ns) != len(sizes) or sum(sizes) > self.batch:
             raise ValueError("group decoder: a size for each prompt, at most `batch` requests")
-        if len(ns) > self.max_groups or max(ns) > self.max_prompt:
+        if len(ns) > self.max_groups or max(ns, default=0) > self.max_prompt:
             raise ValueError(f"group decoder: at most {self.max_groups} prompts of "
                              f"{self.max_prompt} tokens")
         i32 = dict(dtype=torch.int32, device=self.lens.device)
@@ -101,8 +101,9 @@ class GroupDecoder:
         if not torch.equal(plan.lens, want):
             self.close_groups()
             raise MemoryError("group decoder: no free pages for the prompts")
-        _, k, v = self._project(torch.cat(list(prompts)))
-        kvcache.write_slots(self.k_pool, self.v_pool, k, v, plan.slots)
+        if sum(ns) > 0:
+            _, k, v = self._project(torch.cat(list(prompts)))
+            kvcache.write_slots(self.k_pool, self.v_pool, k, v, plan.slots)
 
     def hidden(self, x, active):
         """The layer on x (B, n, D) bf16, n new tokens of every request with

@@ -211,3 +211,25 @@ def test_bounds_on_prompts():
     k, v = dec._project(x.view(6, D))[1:]
     want, tol = expected(dec, x, [(k[b:b + 1], v[b:b + 1]) for b in range(6)], prefix, [0, 2, 5])
     assert all(((y - want).abs() <= tol).all() for y in out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,sizes", [([], []), ([0], [3]), ([0, 0], [1, 5]), ([0, 70], [2, 2])])
+def test_empty_prompts(lens, sizes):
+    from ffai_b200 import attention
+    dec, rand, _ = make(seed=8)
+    prompts = [rand(n, D) for n in lens]
+    dec.open(prompts, sizes)
+    x, active = rand(6, 1, D), torch.ones(6, dtype=torch.int32, device=DEV)
+    y, served = dec.hidden(x, active)
+    assert served.all()
+    prefix = [tuple(t.clone() for t in dec._project(p)[1:]) if len(p) else
+              (torch.zeros((0, HK, 64), dtype=torch.bfloat16, device=DEV),) * 2 for p in prompts]
+    starts = [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+    k, v = dec._project(x.view(6, D))[1:]
+    want, tol = expected(dec, x, [(k[b:b + 1], v[b:b + 1]) for b in range(6)], prefix, starts)
+    assert ((y.double() - want).abs() <= tol).all()
+    dec.close(active)
+    dec.close_groups()
+    assert dec.free_count.item() == 40
+    attention.sync(0)
