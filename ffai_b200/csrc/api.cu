@@ -6,6 +6,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <condition_variable>
 #include <cstdarg>
@@ -61,19 +62,27 @@ size_t dtype_size(int dt) { return dt == FFAI_DT_F32 ? 4 : 2; }
 
 namespace ffai {
 // What a kernel leaves for the next of the same call.  Growing keeps the old
-// buffer, for a captured graph may name it: sizes double at least, so all of
-// them together are at most twice the last.
+// buffer, for work queued or captured before may name it: sizes double at
+// least, so all of them together are at most twice the last.
 struct Grown {
   void* ptr = nullptr;
   size_t cap = 0;  // bytes
   Grown* old = nullptr;
 };
+// Whether a captured graph, or an instance of it, is left.  The graph and the
+// context both know it; whoever lets go of it last deletes it.
+struct CaptureMark {
+  std::atomic<bool> live{true};
+  std::atomic<int> owners{2};
+};
 struct StreamSpace {
-  uint64_t key = 0;
-  Grown prefix;  // partial results of a prefix kernel
-  Grown own;     // and of the kernel on the sequences' own keys beside it,
-  Grown queue;   // with its job queue
-  Grown sample;  // per-row state between the sampling kernels
+  uint64_t key = 0;                // the stream
+  unsigned long long capture = 0;  // the capture on it that this serves, or 0
+  CaptureMark* mark = nullptr;     // of that
+  Grown prefix;                    // partial results of a prefix kernel
+  Grown own;                       // and of the kernel on the sequences' own keys beside it,
+  Grown queue;                     // with its job queue
+  Grown sample;                    // per-row state between the sampling kernels
   StreamSpace* next = nullptr;
 };
 }  // namespace ffai
@@ -106,9 +115,9 @@ struct ffai_attn_ctx {
   // int8 GEMV: quantised activations and their scales, between its two kernels
   uint8_t* d_gemv_x = nullptr;
   size_t gemv_x_cap = 0;
-  // sampling and shared prefixes: workspaces per stream, so that calls on
-  // different streams may overlap (below); the mutex covers the list and a
-  // call's launches
+  // sampling and shared prefixes: workspaces per stream and per captured graph,
+  // so that calls on different streams and replays may overlap (below); the
+  // mutex covers the list and a call's launches
   StreamSpace* spaces = nullptr;
   std::mutex space_mutex;
   ffai_attn_ctx* pipe_ctx = nullptr;  // inner context used for the pipeline's kernels
@@ -194,19 +203,75 @@ int ensure(ffai_attn_ctx* ctx, T** ptr, size_t* cap, size_t need_elems, bool zer
   return FFAI_ATTN_OK;
 }
 
-// The workspaces of a stream (null: out of memory).  The caller holds the mutex.
-StreamSpace* stream_space(ffai_attn_ctx* ctx, void* stream) {
+void let_go(CaptureMark* m) {
+  if (m->owners.fetch_sub(1, std::memory_order_acq_rel) == 1) delete m;
+}
+// Runs when the last of a captured graph is gone and its work is done.
+void CUDART_CB capture_gone(void* mark) {
+  auto* m = static_cast<CaptureMark*>(mark);
+  m->live.store(false, std::memory_order_release);
+  let_go(m);
+}
+
+// The workspaces of a stream's own calls or, while it is captured, of the
+// graph: a graph may be replayed on any stream, beside calls on the one it was
+// captured on and beside other graphs captured there.  A graph's workspaces
+// serve another capture once it is gone.  The caller holds the mutex.
+int stream_space(ffai_attn_ctx* ctx, void* stream, StreamSpace** space) {
   const auto s = static_cast<cudaStream_t>(stream);
   uint64_t key = s == cudaStreamLegacy ? 0 : reinterpret_cast<uint64_t>(stream);
   unsigned long long id = 0;  // one handle for a stream of each thread
   if (s == cudaStreamPerThread && cudaStreamGetId(s, &id) == cudaSuccess) key = ~uint64_t{id};
-  for (StreamSpace* w = ctx->spaces; w; w = w->next)
-    if (w->key == key) return w;
-  auto* w = new (std::nothrow) StreamSpace;
-  if (!w) return nullptr;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(s, &status, &capture, &graph) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream beside a capture: the launch reports it
+    status = cudaStreamCaptureStatusNone;
+  }
+  if (status != cudaStreamCaptureStatusActive) capture = 0;
+  StreamSpace* w = ctx->spaces;
+  while (w && !(w->key == key && w->capture == capture)) w = w->next;
+  if (!w && capture)
+    for (w = ctx->spaces; w; w = w->next)
+      if (w->capture && !w->mark->live.load(std::memory_order_acquire)) break;
+  if (w && w->capture == capture && w->key == key) {
+    *space = w;
+    return FFAI_ATTN_OK;
+  }
+  CaptureMark* mark = nullptr;
+  if (capture) {
+    mark = new (std::nothrow) CaptureMark;
+    if (!mark) return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
+    cudaUserObject_t object;
+    cudaError_t e = cudaUserObjectCreate(&object, mark, capture_gone, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+      delete mark;
+      return cuda_fail(ctx, e, "cudaUserObjectCreate");
+    }
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+      cudaUserObjectRelease(object, 1);
+      let_go(mark);
+      return cuda_fail(ctx, e, "cudaGraphRetainUserObject");
+    }
+  }
+  if (w) {
+    let_go(w->mark);
+  } else {
+    w = new (std::nothrow) StreamSpace;
+    if (!w) {
+      if (mark) let_go(mark);
+      return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
+    }
+    w->next = ctx->spaces;
+    ctx->spaces = w;
+  }
   w->key = key;
-  w->next = ctx->spaces;
-  return ctx->spaces = w;
+  w->capture = capture;
+  w->mark = mark;
+  *space = w;
+  return FFAI_ATTN_OK;
 }
 
 // At least `bytes` in w, zeroed when new if asked.  Also while the stream is being
@@ -817,6 +882,7 @@ void ffai_attn_destroy(ffai_attn_ctx* ctx) {
   while (StreamSpace* w = ctx->spaces) {
     ctx->spaces = w->next;
     for (Grown* b : {&w->prefix, &w->own, &w->queue, &w->sample}) free_grown(b);
+    if (w->mark) let_go(w->mark);
     delete w;
   }
   for (int i = 0; i < 2; ++i) {
@@ -1424,10 +1490,10 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
   const int way = n_groups == 0 || prefix_pages <= 4          ? kEach
                   : t_tiles <= 14.0 * ctx->num_sms + t_units ? kRowTiles
                                                             : kTensor;
-  int st = FFAI_ATTN_OK;
   std::lock_guard<std::mutex> lock(ctx->space_mutex);
-  StreamSpace* space = stream_space(ctx, stream);
-  if (!space) return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
+  StreamSpace* space = nullptr;
+  int st = way == kEach ? FFAI_ATTN_OK : stream_space(ctx, stream, &space);
+  if (st) return st;
   const auto workspace = [&](long long slots, int slot_rows, size_t plan_words) {
     const size_t plan = (plan_words + 3) / 4 * 4;
     const size_t n = static_cast<size_t>(slots) * slot_rows;
@@ -1615,9 +1681,10 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
   DeviceGuard g(ctx->device);
   const int slab = std::min<int>(batch, kSmMaxRows);
   std::lock_guard<std::mutex> lock(ctx->space_mutex);
-  StreamSpace* space = stream_space(ctx, stream);
-  if (!space) return set_error(ctx, FFAI_ATTN_ERR_NOMEM, "out of host memory");
-  int st = grow(ctx, &space->sample, slab * sizeof(SampleRow), /*zero=*/true);
+  StreamSpace* space = nullptr;
+  int st = stream_space(ctx, stream, &space);
+  if (st) return st;
+  st = grow(ctx, &space->sample, slab * sizeof(SampleRow), /*zero=*/true);
   if (st) return st;
   SampleParams p{};
   p.ld = ld;

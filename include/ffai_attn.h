@@ -281,11 +281,13 @@ int ffai_kv_copy_pages(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool
  * whatever it is; NaN among the keys it sees does.  d->causal, q_offset, kv_len and the
  * k/v layouts are ignored, flags must be 0.  Page ids outside the pool or
  * lengths past a table are not read: ffai_attn_sync then reports
- * FFAI_ATTN_ERR_INVALID.  Partial results lie in a workspace of the context
- * per stream: calls on different streams may overlap.  They may be captured;
- * captures of one stream share its workspace, so their replays and its own
- * calls must not overlap.  A stream is destroyed after its calls have
- * finished.  No reference counterpart (beams there clone whole caches,
+ * FFAI_ATTN_ERR_INVALID.  Partial results lie in workspaces of the context,
+ * one per stream for its own calls and one per captured graph while that or
+ * an instance of it is left: calls on different streams, replays of different
+ * graphs and calls on the stream they were captured on may overlap; two
+ * instances of one graph may not.  A stream is destroyed after its calls have
+ * finished, the context after the graphs.
+ * No reference counterpart (beams there clone whole caches,
  * text_decoder.rs:1363-1381). */
 int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,
                             const void* q, const void* k_pool, const void* v_pool,

@@ -273,3 +273,88 @@ def test_scores_of_minus_infinity_weigh_nothing(name, dtype):
     assert ((out.double() - o).abs() <= tol).all()
     B, n, H, _ = c["q"].shape
     assert (lse.double().view(H, B, n).permute(1, 2, 0) - want).abs().max().item() <= 2e-5
+
+
+def captured(call):
+    """A graph of `call` (captured on the stream that torch.cuda.graph shares) and its output."""
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    return graph, out
+
+
+@pytest.mark.gpu
+def test_graphs_captured_on_one_stream_do_not_share_state():
+    """Attention and sampling captured in the ordinary way, replayed on streams
+    without order between them, beside calls on the stream of the captures."""
+    from ffai_b200 import attention, sampling
+    cs = [build(*CASES[n], torch.bfloat16, seed=i)
+          for i, n in enumerate(("beside_odd_rows", "units_groups", "tiles_odd_rows"))]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    logits = [torch.randn((n, 60001), generator=g, device=DEV) * 3 for n in (90, 33)]
+    u = torch.rand(90, generator=g, device=DEV)
+    calls = [lambda c=c: attend(c) for c in cs]
+    calls += [lambda x=x: sampling.sample(x, u[:x.shape[0]].clone(), top_p=0.9) for x in logits]
+    want = [call() for call in calls]
+    graphs = [captured(call) for call in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    shared = torch.cuda.graph.default_capture_stream
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for _, out in graphs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(shared):
+            again = [call() for call in calls]
+        torch.cuda.synchronize()
+        for w, (_, out), a in zip(want, graphs, again):
+            assert torch.equal(out, w) and torch.equal(a, w)
+    attention.sync(0)
+
+
+@pytest.mark.gpu
+def test_branches_of_one_capture_do_not_share_state():
+    cs = [build(*CASES[n], torch.bfloat16, seed=i) for i, n in enumerate(("units", "beside_short"))]
+    want = [attend(c) for c in cs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        out = [attend(cs[0])]
+        with torch.cuda.stream(side):
+            out.append(attend(cs[1]))
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(10):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_workspaces_of_graphs_that_are_gone_serve_others():
+    import gc
+    import time
+    c = build(*CASES["units"], torch.bfloat16, seed=3)
+    want = attend(c)
+
+    def once():
+        graph, out = captured(lambda: attend(c))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del graph, out
+        gc.collect()
+        torch.cuda.synchronize()
+        time.sleep(0.05)
+        torch.cuda.empty_cache()
+        return torch.cuda.mem_get_info()[0]
+    once()
+    first = once()
+    for _ in range(12):
+        last = once()
+    # a workspace of this case holds over 30 MB; twelve more would take 360
+    assert first - last < 100 * 2 ** 20
