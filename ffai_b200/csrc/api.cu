@@ -1275,8 +1275,12 @@ int ffai_attn_sync(ffai_attn_ctx* ctx, void* stream) {
     FFAI_CUDA(ctx, cudaMemset(ctx->d_err, 0, sizeof(unsigned)));
     if (err & kErrBadArgs)
       return set_error(ctx, FFAI_ATTN_ERR_INVALID,
-                       "a paged-cache call met a page id outside the pool or a length past its "
-                       "block table (error bits 0x%x)", err);
+                       "a paged-cache call met a page id outside the pool, a length or count "
+                       "outside its table, or group starts that do not rise (error bits 0x%x)", err);
+    if (err & kErrNoSlot)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                       "a shared prefix's lengths or starts changed while a call read them (error "
+                       "bits 0x%x)", err);
     return set_error(ctx, FFAI_ATTN_ERR_TIMEOUT, "in-kernel wait timed out (error bits 0x%x)", err);
   }
   return FFAI_ATTN_OK;

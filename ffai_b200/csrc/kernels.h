@@ -16,6 +16,7 @@ enum : unsigned {
   kErrTimeoutDrain = 1u << 3,
   kErrTimeoutConsumer = 1u << 4,
   kErrBadArgs = 1u << 8,
+  kErrNoSlot = 1u << 9,  // a shared prefix's partial result has no place in the workspace
 };
 
 // ---- decode (decode.cu) ----------------------------------------------------

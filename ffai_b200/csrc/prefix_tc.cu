@@ -674,7 +674,9 @@ __device__ __forceinline__ void px_softmax(const SharedParams& p, uint32_t tmem)
         }
       }
       const int slot = static_cast<int>(blockIdx.x) + w.seg;
-      if (active && slot < p.part_slots) {
+      if (active && slot >= p.part_slots) {  // the workspace's size rules it out
+        if (p.err && lane == 0) atomicOr(p.err, kErrNoSlot);
+      } else if (active) {
         const size_t at = static_cast<size_t>(slot) * kPxRows + (pair ? 128 * t : 0) + 16 * c + t1;
         float* dst = p.part_o + at * 64 + 2 * t0;
 #pragma unroll 1

@@ -451,6 +451,15 @@ __device__ __forceinline__ void fold_run(Merged& acc, Staging<THREADS>& sm, cons
   }
 }
 
+// The n partials from `slot` on, if the workspace holds them.  It always does
+// (its size is a bound on the plan's slots), unless the lengths or starts were
+// written between the prefix kernel's look at them and this one.
+__device__ __forceinline__ int in_slots(const SharedParams& p, int slot, int n) {
+  if (slot >= 0 && n <= p.part_slots - slot) return n;
+  if (p.err) atomicOr(p.err, kErrNoSlot);
+  return 0;
+}
+
 // The prefix kernel's partials of row `row` of sequence b's R rows of a KV head,
 // folded into `acc` in the order of the line: copy k of `copies` takes every
 // copies-th.
@@ -468,7 +477,7 @@ __device__ __forceinline__ void fold_partials(Merged& acc, Staging<THREADS>& sm,
     if (pages == 0) return;
     const int tiles = (d.rows + 15) / 16, per = (pages + p.splits - 1) / p.splits;
     const int slot = (__ldcg(p.part_plan + 1 + group) + kvh * tiles + rg / 16) * p.splits;
-    const int n = min((pages + per - 1) / per, p.part_slots - slot);
+    const int n = in_slots(p, slot, (pages + per - 1) / per);
     fold_run(acc, sm, p, static_cast<size_t>(slot + copy) * 16 + rg % 16,
              static_cast<size_t>(copies) * 16, (n - copy + copies - 1) / copies, part, jt);
     return;
@@ -476,7 +485,7 @@ __device__ __forceinline__ void fold_partials(Merged& acc, Staging<THREADS>& sm,
   // prefix_tc_kernel's: segments of the line, each one per CTA that has a share of it
   const int share = abs(plan), lin0 = __ldcg(p.part_plan + 1 + 2 * group),
             seg0 = __ldcg(p.part_plan + 2 + 2 * group);
-  if (d.nb == 0) return;
+  if (d.nb == 0 || in_slots(p, 0, share > 0 ? 1 : INT_MAX) == 0) return;
   const int cl = chunk_blocks(d, share), chunks = (d.nb + cl - 1) / cl;
   const int head0 = lin0 + kvh * line_steps(d, share, plan < 0), m = rg / kPxRows;
   int skip = copy;  // partials to pass over before this copy's next
@@ -486,7 +495,7 @@ __device__ __forceinline__ void fold_partials(Merged& acc, Staging<THREADS>& sm,
     const int l0 = head0 + head_steps(d, q * cl) + m * len;
     const int seg = seg0 + (kvh * chunks + q) * d.mu + m;
     const int c0 = l0 / share, c1 = (l0 + unit_steps(d, m, len) - 1) / share;
-    const int n = min(c1 - c0 + 1, p.part_slots - (c0 + seg));
+    const int n = in_slots(p, c0 + seg, c1 - c0 + 1);
     fold_run(acc, sm, p, static_cast<size_t>(c0 + seg + skip) * kPxRows + rg % kPxRows,
              static_cast<size_t>(copies) * kPxRows, (n - skip + copies - 1) / copies, part, jt);
     // the next chunk's go on being dealt where this one's stopped (copies: a power of two)
