@@ -426,7 +426,7 @@ constexpr int kSmMaxVocab = 1 << 18;  // weight sums stay below 2^54
 constexpr int kSmChunk = (1 << 14) - 8;  // tokens per CTA, at most
 constexpr int kSmLongChunk = 1 << 15;  // of the passes without a histogram
 constexpr int kSmMinChunk = 1 << 12;  // and at least
-constexpr int kSmBins = 1600;         // of the exponent: (-25, 0] in steps of 1/64
+constexpr int kSmBins = 1600;  // of the exponent, (-25, 0] in steps of 1/64; e^-25 2^36 < 1
 constexpr int kSmList = 1024;         // listed tokens per set
 constexpr int kSmMaxRows = 1024;      // rows per launch (workspace)
 

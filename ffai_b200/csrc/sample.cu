@@ -52,7 +52,6 @@ namespace {
 
 constexpr int kSmThreads = 512;
 constexpr int kSmWarps = kSmThreads / 32;
-constexpr int kSmBins = 1600;    // d in (-25, 0]; e^-25 2^36 < 1: nothing beyond
 constexpr int kSmPer = 4;        // bins per scanning thread
 constexpr int kSmQueue = 1024;   // tokens of a stretch that may be in a set
 constexpr int kSmPair = 256;     // tokens of a short list
@@ -280,33 +279,24 @@ __device__ __forceinline__ void each_near(const T* src, int n, N near, F take) {
   }
 }
 
-// The bins of the CTA's histogram into mass and tokens before each; `global`:
-// the row's bins, which are cleared (null: s.half and s.cnt).
-__device__ __noinline__ void finish_bins(unsigned long long* global, uint32_t* global_cnt,
-                                         bool counts) {
+// The row's bins into mass and tokens before each; the bins are cleared.
+__device__ __noinline__ void finish_bins(unsigned long long* bins, uint32_t* bins_cnt, bool counts) {
   SampleShared& s = SM_SHARED;
   unsigned long long m[kSmPer] = {0, 0, 0, 0};
   uint32_t c[kSmPer] = {0, 0, 0, 0};
   const int b0 = threadIdx.x * kSmPer;
   __syncthreads();
   if (b0 < kSmBins) {
-    if (global) {  // written by other CTAs' atomics: read and clear at L2
-      ulonglong2* g = reinterpret_cast<ulonglong2*>(global + b0);
-      const ulonglong2 x = __ldcg(g), y = __ldcg(g + 1);
-      m[0] = x.x, m[1] = x.y, m[2] = y.x, m[3] = y.y;
-      __stcg(g, make_ulonglong2(0, 0));
-      __stcg(g + 1, make_ulonglong2(0, 0));
-      if (counts) {
-        const uint4 n = __ldcg(reinterpret_cast<const uint4*>(global_cnt + b0));
-        c[0] = n.x, c[1] = n.y, c[2] = n.z, c[3] = n.w;
-        __stcg(reinterpret_cast<uint4*>(global_cnt + b0), make_uint4(0, 0, 0, 0));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kSmPer; ++e) {
-        m[e] = (static_cast<unsigned long long>(s.hi[b0 + e]) << 18) + s.lo[b0 + e];
-        c[e] = s.cnt[b0 + e];
-      }
+    // written by other CTAs' atomics: read and clear at L2
+    ulonglong2* g = reinterpret_cast<ulonglong2*>(bins + b0);
+    const ulonglong2 x = __ldcg(g), y = __ldcg(g + 1);
+    m[0] = x.x, m[1] = x.y, m[2] = y.x, m[3] = y.y;
+    __stcg(g, make_ulonglong2(0, 0));
+    __stcg(g + 1, make_ulonglong2(0, 0));
+    if (counts) {
+      const uint4 n = __ldcg(reinterpret_cast<const uint4*>(bins_cnt + b0));
+      c[0] = n.x, c[1] = n.y, c[2] = n.z, c[3] = n.w;
+      __stcg(reinterpret_cast<uint4*>(bins_cnt + b0), make_uint4(0, 0, 0, 0));
     }
   }
   __syncthreads();
