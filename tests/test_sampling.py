@@ -220,3 +220,41 @@ def test_streams_and_captures_do_not_share_state():
         out.zero_()
         graph.replay()
         assert torch.equal(out, want[1])
+
+
+def logprob_bounds(x, tokens):
+    """(log-probabilities of tokens in 64 bits, bounds of the f32 ones).
+
+    A term e^(x - max) is off by the rounding of x - max, 2^-24 |x - max|, an
+    f32 exponential, 2^-23, and three additions within a group of four, 3 2^-24;
+    what follows is 64 bits, up to the result's own rounding, 2^-24 of it:
+    2^-24 (mean of |x - max| under the softmax + 6 + |result|)."""
+    x = x.double().cpu()
+    d = x - x.amax(1, keepdim=True)
+    z = torch.logsumexp(d, 1)
+    lp = d.gather(1, tokens.long().cpu().view(-1, 1))[:, 0] - z
+    w = torch.softmax(d, 1)
+    mean = torch.where(w > 0, w * d.abs(), torch.zeros_like(w)).sum(1)
+    return lp, 2.0 ** -24 * (mean + 6 + lp.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [37, 5003, 51865, 131072, 262144])
+def test_logprobs_hold_to_f32_rounding(V, dtype):
+    from ffai_b200 import sampling
+    g = torch.Generator().manual_seed(V + 1)
+    kinds = ["normal", "peak", "flat", "ties", "tiny", "low"]
+    x = torch.cat([rows(k, 2, V, g) for k in kinds]).to(dtype)
+    x[0, ::3] = -math.inf
+    x[2] -= 30.0  # a peak that outweighs the rest by far, away from zero
+    B = x.shape[0]
+    u = torch.rand(B, generator=g).to(DEV)
+    temperature = torch.tensor([0.0, 1.0] * (B // 2), device=DEV)
+    for settings in (dict(), dict(temperature=0.0), dict(temperature=temperature, top_p=0.9),
+                     dict(temperature=2.0, top_k=40, min_p=0.01)):
+        tok, lp = sampling.sample(x.to(DEV), u, with_logprob=True, **settings)
+        assert (tok >= 0).all()
+        want, tol = logprob_bounds(x.float(), tok)
+        err = (lp.cpu().double() - want).abs()
+        assert (err <= tol).all(), f"{(err / tol).max():.2f} of the bound"

@@ -285,3 +285,23 @@ def test_starts_that_do_not_rise_leave_short_prefixes_out_too(starts, n):
             attention.sync(0)
         assert e.value.status == -1
         assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", [([130], [2], [64, 70], 2, 1, 64, 0), ([0], [1], [129], 3, 1, 129, 0),
+                                  ([65, 300], [1, 2], [100, 5, 33], 4, 2, 33, 0),
+                                  ([700], [1], [200], 2, 2, 200, 0)],
+                         ids=["whole", "no_prefix", "ragged", "tiles"])
+def test_prompts_behind_a_prefix(case, dtype):
+    """More new tokens a sequence than a tile has rows, more than it holds keys among them."""
+    prefix, sizes, suffix, heads, kv, n, extra = case
+    c = build(prefix, suffix, sizes, heads, kv, n, dtype, seed=n, extra=extra)
+    out, lse = run(c, 0.125, with_lse=True)
+    ref = reference(c, 0.125)
+    check(out, ref, c, dtype, dtype)
+    got = lse.cpu().double().view(heads, len(suffix), n).permute(1, 2, 0)
+    empty = ref[2] == float("-inf")
+    assert torch.equal(got == float("-inf"), empty)
+    assert (got[~empty] - ref[2][~empty]).abs().max().item() <= 2e-5
+    assert (out.cpu()[empty] == 0).all()

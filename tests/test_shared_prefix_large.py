@@ -358,3 +358,33 @@ def test_workspaces_of_graphs_that_are_gone_serve_others():
         last = once()
     # a workspace of this case holds over 30 MB; twelve more would take 360
     assert first - last < 100 * 2 ** 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["tiles", "tiles_odd_rows", "units_groups", "beside_odd_rows"])
+@pytest.mark.parametrize("prefix_by,own_by", [(1, 40), (3, 1), (2, 17)])
+def test_tables_with_spare_columns(name, prefix_by, own_by):
+    """Tables as wide as the longest request may become, what lies behind the
+    live pages being anything: the formula's result whichever way is taken."""
+    from ffai_b200 import attention
+    c = build(*CASES[name], torch.bfloat16, seed=7)
+    o, a, want = reference(c, 0.125)
+
+    def wide(table, by):
+        t = torch.full((table.shape[0], table.shape[1] * by + 1), 10 ** 9, dtype=torch.int32, device=DEV)
+        t[:, :table.shape[1]] = table
+        return t
+    prefix, lens, _ = c["lists"]
+    for table, ns in ((c["prefix_table"], prefix), (c["block_table"], lens)):
+        for i, n in enumerate(ns):  # nothing valid behind a row's own pages either
+            table[i, (n + 63) // 64:] = -5
+    c["prefix_table"], c["block_table"] = wide(c["prefix_table"], prefix_by), wide(c["block_table"], own_by)
+    out, lse = attend(c, with_lse=True)
+    attention.sync(0)
+    B, n, H, _ = c["q"].shape
+    u = U[torch.bfloat16]
+    assert ((out.double() - o).abs() <= (u + 1e-4) * a + u * o.abs() + 1e-7).all()
+    got = lse.double().view(H, B, n).permute(1, 2, 0)
+    empty = want == float("-inf")
+    assert torch.equal(got == float("-inf"), empty)
+    assert (got[~empty] - want[~empty]).abs().max().item() <= 2e-5
