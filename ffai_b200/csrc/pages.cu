@@ -11,10 +11,11 @@
 // order matters: the result depends on the inputs alone.
 //
 // Bounds and device time on one B200: plans and releases are a chain of
-// dependent loads and two scans, 4.2 us for 32 requests, 7.0 for 2000 with 130000
-// tokens, 3.5 for the release of 500 (a launch alone is about 2).  The scatter
-// is bound by its bytes: 20001 tokens of 8 heads, f32 to bf16, move 123 MB in
-// 24 us (5.1 TB/s, measured copies reach 6.46); 60 tokens of 20 heads take 2.8.
+// dependent loads and two scans, 3.8 us for 32 requests, 7.7 for 2000 with 130000
+// tokens (1.2 of it for the looks at page ids), 3.1 for the release of 500 (a
+// launch alone is about 2).  The scatter is bound by its bytes: 20001 tokens of
+// 8 heads, f32 to bf16, move 123 MB in 23 us (5.3 TB/s, measured copies reach
+// 6.46); 60 tokens of 20 heads take 2.1.
 #include "common.cuh"
 #include "kernels.h"
 

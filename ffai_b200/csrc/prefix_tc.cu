@@ -10,9 +10,9 @@
 // CTAs): every CTA gets the same work whatever the lengths and group sizes.
 // What a CTA holds of a segment (same rows, consecutive blocks) leaves one
 // partial result (running maximum, sum, unnormalised output), merged by
-// shared_rows_kernel.  The partial of CTA c for segment t lies in slot c + t:
-// along the line either c or t grows from one partial to the next, so slots
-// are distinct.
+// shared_rows_kernel, or with own keys beside by merge_rows_kernel.  The
+// partial of CTA c for segment t lies in slot c + t: along the line either c or
+// t grows from one partial to the next, so slots are distinct.
 //
 // Per CTA: warp 16 streams the pages through a 4-stage ring of K and V blocks
 // by TMA for two chains (t = 0, 1), each with an MMA warp (17, 18), scores,
@@ -27,7 +27,9 @@
 // memory and registers around them: a step, 256 rows by 128 keys, takes 1.46 us
 // where its exponentials take 1.07 and its products 0.63.  Filling costs 4 us to
 // the first scores, a segment's end 2.  89 GFLOP over three prefixes of up to
-// 32768 keys: 150 us, tensor pipe 29 % active.
+// 32768 keys: 150 us, tensor pipe 29 % active.  Of these the 74 to 77 steps of a
+// CTA make 108 to 112; the rest goes into fills and ends, for a CTA has up to
+// five segments (2.2 on average) there.
 //
 // Every wait is bounded (common.cuh); on a timeout the CTA raises an error
 // bit, drains its copies and MMAs, frees tensor memory and exits.

@@ -36,7 +36,7 @@
 //   5 sequences, 12 heads, 224 + up to 224 keys            6.9 us (2.4 MB)
 //   12 groups of 5, 20 heads, up to 1500 + up to 448 keys 35 us   (145 MB, 4.1 TB/s)
 //   64 sequences, 32 / 8 heads, 8200 + up to 1000 keys    32 us   (82 MB)
-//   96 in 3 groups, 4 queries, 32768 + up to 700 keys      161 us (89 GFLOP, 0.55 PFLOP/s)
+//   96 in 3 groups, 4 queries, 32768 + up to 700 keys      163 us (89 GFLOP, 0.55 PFLOP/s)
 #include <algorithm>
 
 #include "shared_prefix.cuh"
