@@ -160,6 +160,32 @@ unsafe extern "C" {
                        batch: i32, vocab: i32, u: *const f32, temperature: *const f32,
                        top_k: *const i32, top_p: *const f32, min_p: *const f32,
                        tokens: *mut i32, logprobs: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ffai_attn_chunk_paged(ctx: *mut ffai_attn_ctx, d: *const ffai_attn_desc, kv_heads: i32,
+                                 q: *const c_void, n_tokens: i32, cu_q: *const i32,
+                                 k_pool: *const c_void, v_pool: *const c_void, num_pages: i32,
+                                 block_table: *const i32, seq_lens: *const i32, max_pages: i32,
+                                 o: *mut c_void, lse: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn ffai_page_fork(ctx: *mut ffai_attn_ctx, batch: i32, new_batch: i32, max_pages: i32,
+                          num_pages: i32, src: *const i32, keep: *const i32, lens: *const i32,
+                          block_table: *const i32, free_pages: *mut i32, free_cap: i32,
+                          free_count: *const i32, table_out: *mut i32, lens_out: *mut i32,
+                          copy_src: *mut i32, copy_dst: *mut i32, copy_keys: *mut i32,
+                          free_count_out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ffai_page_compact(ctx: *mut ffai_attn_ctx, batch: i32, max_pages: i32, num_pages: i32,
+                             lens: *const i32, block_table: *const i32, free_pages: *const i32,
+                             free_cap: i32, free_count: *const i32, table_out: *mut i32,
+                             free_out: *mut i32, copy_src: *mut i32, copy_dst: *mut i32,
+                             copy_cap: i32, stream: *mut c_void) -> c_int;
+    pub fn ffai_kv_copy_keys(ctx: *mut ffai_attn_ctx, d: *const ffai_attn_desc,
+                             k_pool: *mut c_void, v_pool: *mut c_void, num_pages: i32,
+                             src: *const i32, dst: *const i32, keys: *const i32, n: i32,
+                             stream: *mut c_void) -> c_int;
+    pub fn ffai_verify(ctx: *mut ffai_attn_ctx, logits: *const c_void, ld: i64,
+                       draft_logits: *const c_void, draft_ld: i64, dtype: i32, batch: i32,
+                       rows: i32, vocab: i32, cu_rows: *const i32, tokens: *const i32,
+                       u: *const f32, u_last: *const f32, temperature: *const f32,
+                       draft_temperature: *const f32, accepted: *mut i32, next: *mut i32,
+                       tokens_out: *mut i32, logprobs: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ffai_int8_gemv_layout(rows: i32, cols: i32, blk: i32, packed_bytes: *mut i64,
                                  corr_count: *mut i64) -> c_int;
     pub fn ffai_int8_gemv_quantize(ctx: *mut ffai_attn_ctx, w: *const c_void, w_dtype: i32,

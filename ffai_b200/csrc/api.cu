@@ -83,6 +83,10 @@ struct StreamSpace {
   Grown own;                       // and of the kernel on the sequences' own keys beside it,
   Grown queue;                     // with its job queue
   Grown sample;                    // per-row state between the sampling kernels
+  Grown pages;                     // words per page of forks and compactions
+  Grown chunk;                     // partial results of a chunk's attention,
+  Grown tickets;                   // and whose turn it is to merge them
+  Grown verify;                    // per-row state between the verifying kernels
   StreamSpace* next = nullptr;
 };
 }  // namespace ffai
@@ -305,6 +309,19 @@ int grow(ffai_attn_ctx* ctx, Grown* w, size_t bytes, bool zero = false) {
   w->old = old;
   w->ptr = ptr;
   w->cap = n;
+  return FFAI_ATTN_OK;
+}
+
+// The words per page of a fork or a compaction, zero between calls, and what its
+// CTAs tell one another.  The caller holds the mutex.
+int page_words(ffai_attn_ctx* ctx, void* stream, int num_pages, int4** words, int2** totals) {
+  StreamSpace* space = nullptr;
+  int st = stream_space(ctx, stream, &space);
+  if (st) return st;
+  st = grow(ctx, &space->pages, 128 + static_cast<size_t>(num_pages) * sizeof(int4), /*zero=*/true);
+  if (st) return st;
+  *totals = static_cast<int2*>(space->pages.ptr);
+  *words = reinterpret_cast<int4*>(static_cast<char*>(space->pages.ptr) + 128);
   return FFAI_ATTN_OK;
 }
 
@@ -881,7 +898,8 @@ void ffai_attn_destroy(ffai_attn_ctx* ctx) {
   cudaFree(ctx->d_gemv_x);
   while (StreamSpace* w = ctx->spaces) {
     ctx->spaces = w->next;
-    for (Grown* b : {&w->prefix, &w->own, &w->queue, &w->sample}) free_grown(b);
+    for (Grown* b : {&w->prefix, &w->own, &w->queue, &w->sample, &w->pages, &w->chunk, &w->tickets, &w->verify})
+      free_grown(b);
     if (w->mark) let_go(w->mark);
     delete w;
   }
@@ -1671,6 +1689,194 @@ int ffai_kv_write_slots(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_poo
   return FFAI_ATTN_OK;
 }
 
+int ffai_page_fork(ffai_attn_ctx* ctx, int32_t batch, int32_t new_batch, int32_t max_pages,
+                   int32_t num_pages, const int32_t* src, const int32_t* keep, const int32_t* lens,
+                   const int32_t* block_table, int32_t* free_pages, int32_t free_cap,
+                   const int32_t* free_count, int32_t* table_out, int32_t* lens_out,
+                   int32_t* copy_src, int32_t* copy_dst, int32_t* copy_keys,
+                   int32_t* free_count_out, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (batch <= 0 || new_batch <= 0 || max_pages <= 0 || num_pages <= 0 || free_cap <= 0 ||
+      max_pages > (1 << 30) / kPageKeys || num_pages > INT32_MAX / kPageKeys)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                     "page fork: batch %d, new_batch %d, max_pages %d, num_pages %d, free_cap %d",
+                     batch, new_batch, max_pages, num_pages, free_cap);
+  if (static_cast<long long>(std::max(batch, new_batch)) * max_pages > (1 << 30))
+    return set_error(ctx, FFAI_ATTN_DECLINED, "page fork: more than 2^30 table entries");
+  if (!src || !lens || !block_table || !free_pages || !free_count || !table_out || !lens_out ||
+      !copy_src || !copy_dst || !copy_keys || !free_count_out)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page fork: null pointer");
+  if (table_out == block_table || lens_out == lens || lens_out == src || lens_out == keep ||
+      free_count_out == free_count)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page fork: outputs must not alias inputs");
+  DeviceGuard g(ctx->device);
+  std::lock_guard<std::mutex> lock(ctx->space_mutex);
+  ForkParams p{src,      keep,      lens,      block_table,    free_pages, free_count, table_out,
+               lens_out, copy_src,  copy_dst,  copy_keys,      free_count_out, batch,  new_batch,
+               max_pages, num_pages, free_cap, nullptr,        nullptr,    ctx->d_err};
+  int st = page_words(ctx, stream, num_pages, &p.words, &p.totals);
+  if (st) return st;
+  FFAI_CUDA(ctx, launch_page_fork(p, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_page_compact(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, int32_t num_pages,
+                      const int32_t* lens, const int32_t* block_table, const int32_t* free_pages,
+                      int32_t free_cap, const int32_t* free_count, int32_t* table_out,
+                      int32_t* free_out, int32_t* copy_src, int32_t* copy_dst, int32_t copy_cap,
+                      void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (batch <= 0 || max_pages <= 0 || num_pages <= 0 || free_cap <= 0 ||
+      max_pages > (1 << 30) / kPageKeys || num_pages > INT32_MAX / kPageKeys)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                     "page compaction: batch %d, max_pages %d, num_pages %d, free_cap %d", batch,
+                     max_pages, num_pages, free_cap);
+  const long long entries = static_cast<long long>(batch) * max_pages;
+  if (entries > (1 << 30))
+    return set_error(ctx, FFAI_ATTN_DECLINED, "page compaction: more than 2^30 table entries");
+  if (copy_cap < std::min<long long>(entries, free_cap))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                     "page compaction: copy_cap %d, at least the table's entries or free_cap",
+                     copy_cap);
+  if (!lens || !block_table || !free_pages || !free_count || !table_out || !free_out ||
+      !copy_src || !copy_dst)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page compaction: null pointer");
+  if (table_out == block_table || free_out == free_pages)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page compaction: outputs must not alias inputs");
+  DeviceGuard g(ctx->device);
+  std::lock_guard<std::mutex> lock(ctx->space_mutex);
+  CompactParams p{lens,     block_table, free_pages, free_count, table_out, free_out, copy_src,
+                  copy_dst, batch,       max_pages,  num_pages,  free_cap,  copy_cap, nullptr,
+                  nullptr,  nullptr,     ctx->d_err};
+  int st = page_words(ctx, stream, num_pages, &p.words, &p.totals);
+  if (st) return st;
+  p.below = reinterpret_cast<int*>(p.totals + 8);
+  FFAI_CUDA(ctx, launch_page_compact(p, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_kv_copy_keys(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool, void* v_pool,
+                      int32_t num_pages, const int32_t* src, const int32_t* dst,
+                      const int32_t* keys, int32_t n, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (!d) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "null descriptor");
+  if (d->head_dim != kHD)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "head_dim %d: only 64 is served", d->head_dim);
+  if (d->heads <= 0 || num_pages <= 0 || n < 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "key copy: heads %d, pages %d, n %d", d->heads,
+                     num_pages, n);
+  if (!valid_dtype(d->kv_dtype)) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "unknown kv dtype");
+  if (n == 0) return FFAI_ATTN_OK;
+  if (!k_pool || !v_pool || !src || !dst)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "key copy: null pointer");
+  for (const void* ptr : {static_cast<const void*>(k_pool), static_cast<const void*>(v_pool)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "page pools must be 16-byte aligned");
+  DeviceGuard g(ctx->device);
+  CopyParams p{k_pool,    v_pool, src, dst, keys, n, d->heads, num_pages,
+               static_cast<int>(kHD * dtype_size(d->kv_dtype) / 16), ctx->d_err};
+  FFAI_CUDA(ctx, launch_kv_copy_keys(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
+int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,
+                          const void* q, int32_t n_tokens, const int32_t* cu_q,
+                          const void* k_pool, const void* v_pool, int32_t num_pages,
+                          const int32_t* block_table, const int32_t* seq_lens, int32_t max_pages,
+                          void* o, float* lse, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (!d) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "null descriptor");
+  if (d->head_dim != kHD)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "head_dim %d: only 64 is served", d->head_dim);
+  if (d->batch <= 0 || d->heads <= 0 || d->q_len < 0 || n_tokens < 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "batch %d, heads %d, q_len %d, tokens %d",
+                     d->batch, d->heads, d->q_len, n_tokens);
+  if (kv_heads <= 0 || d->heads % kv_heads != 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "heads %d must be a multiple of kv_heads %d",
+                     d->heads, kv_heads);
+  if (!valid_dtype(d->q_dtype) || !valid_dtype(d->kv_dtype) || !valid_dtype(d->out_dtype))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "unknown dtype (q %d, kv %d, out %d)", d->q_dtype,
+                     d->kv_dtype, d->out_dtype);
+  if (d->kv_dtype == FFAI_DT_F32)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: bf16 or f16 pools only");
+  if (d->q_dtype != FFAI_DT_F32 && d->q_dtype != d->kv_dtype)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: q must be f32 or the cache dtype");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "scale must be finite and > 0");
+  if (d->flags != 0)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "chunk: unknown flags 0x%x", d->flags);
+  if (d->q_layout != FFAI_LAYOUT_TOKEN_MAJOR || d->out_layout != FFAI_LAYOUT_TOKEN_MAJOR)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "chunk: q and out are token-major");
+  if (d->token_stride != 0 && (d->token_stride < d->heads * kHD || d->token_stride % 8 != 0))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID,
+                     "token_stride %d: 0, or a multiple of 8 of at least heads * 64",
+                     d->token_stride);
+  constexpr int kMaxPages = (1 << 30) / kPageKeys;
+  if (num_pages <= 0 || max_pages <= 0 || max_pages > kMaxPages)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "chunk: empty pool or table");
+  if (n_tokens == 0) return FFAI_ATTN_OK;
+  if (!q || !o || !k_pool || !v_pool || !cu_q || !block_table || !seq_lens)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "chunk: null pointer");
+  for (const void* ptr : {q, k_pool, v_pool, static_cast<const void*>(o)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "chunk: operands 16-byte aligned");
+  const long long G = d->heads / kv_heads;
+  const long long blocks = (max_pages + 1) / 2;
+  if (static_cast<double>(n_tokens) * d->heads > (1 << 30) ||
+      static_cast<double>(num_pages) * kv_heads > 2147483647.0)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: too many rows");
+  // units of `rows` rows: one started per sequence, and as many as are full
+  const auto units = [&](int rows) {
+    return static_cast<double>(kv_heads) *
+           (std::min<double>(d->batch, n_tokens) + static_cast<double>(n_tokens) * G / rows);
+  };
+  ChunkParams p{};
+  p.q = q;
+  p.q_st = d->token_stride ? d->token_stride : static_cast<long long>(d->heads) * kHD;
+  p.q_sh = kHD;
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.cu_q = cu_q;
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.batch = d->batch;
+  p.tokens = n_tokens;
+  p.max_pages = max_pages;
+  p.num_pages = num_pages;
+  p.heads = d->heads;
+  p.kv_heads = kv_heads;
+  p.q_dtype = d->q_dtype;
+  p.kv_dtype = d->kv_dtype;
+  p.out_dtype = d->out_dtype;
+  p.causal = d->causal != 0;
+  p.scale_log2 = d->scale * 1.4426950408889634f;
+  p.out = o;
+  p.lse = lse;
+  p.err = ctx->d_err;
+  DeviceGuard g(ctx->device);
+  ProfScope ps(ctx, FFAI_OP_VARLEN, static_cast<cudaStream_t>(stream), "ffai_attn_chunk_paged");
+  if (units(16) * blocks > INT32_MAX / 2)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: too many rows and keys");
+  std::lock_guard<std::mutex> lock(ctx->space_mutex);
+  StreamSpace* space = nullptr;
+  int st = stream_space(ctx, stream, &space);
+  if (st) return st;
+  const int resident = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32 ? 2 : 3;
+  const int grid = static_cast<int>(std::min<double>(1.0 * resident * ctx->num_sms, units(16) * blocks));
+  p.min_share = 4;
+  p.precise = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32;
+  st = grow(ctx, &space->tickets, static_cast<size_t>(grid) * 4, /*zero=*/true);
+  if (st) return st;
+  p.tickets = static_cast<unsigned*>(space->tickets.ptr);
+  const size_t rows = static_cast<size_t>(grid) * kChunkRowsPerCta;
+  st = grow(ctx, &space->chunk, rows * 66 * 4);
+  if (st) return st;
+  p.part_ml = static_cast<float*>(space->chunk.ptr);
+  p.part_o = p.part_ml + rows * 2;
+  FFAI_CUDA(ctx, launch_chunk_rows(p, grid, static_cast<cudaStream_t>(stream)));
+  return FFAI_ATTN_OK;
+}
+
 int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtype, int32_t batch,
                 int32_t vocab, const float* u, const float* temperature, const int32_t* top_k,
                 const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
@@ -1713,6 +1919,42 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
     p.logprobs = logprobs ? logprobs + b : nullptr;
     FFAI_CUDA(ctx, launch_sample(p, static_cast<cudaStream_t>(stream)));
   }
+  return FFAI_ATTN_OK;
+}
+
+int ffai_verify(ffai_attn_ctx* ctx, const void* logits, int64_t ld, const void* draft_logits,
+                int64_t draft_ld, int32_t dtype, int32_t batch, int32_t rows, int32_t vocab,
+                const int32_t* cu_rows, const int32_t* tokens, const float* u, const float* u_last,
+                const float* temperature, const float* draft_temperature, int32_t* accepted,
+                int32_t* next, int32_t* tokens_out, float* logprobs, void* stream) {
+  if (!ctx) return set_error(nullptr, FFAI_ATTN_ERR_INVALID, "null context");
+  if (batch <= 0 || rows < 0 || vocab <= 0 || ld < vocab || (draft_logits && draft_ld < vocab))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "verify: batch %d, rows %d, vocab %d, ld %lld, %lld",
+                     batch, rows, vocab, static_cast<long long>(ld), static_cast<long long>(draft_ld));
+  if (!valid_dtype(dtype)) return set_error(ctx, FFAI_ATTN_ERR_INVALID, "unknown logits dtype");
+  if (vocab > kSmMaxVocab)
+    return set_error(ctx, FFAI_ATTN_DECLINED, "verify: vocab %d, at most %d", vocab, kSmMaxVocab);
+  if (batch > (1 << 24) || rows > (1 << 24))
+    return set_error(ctx, FFAI_ATTN_DECLINED, "verify: batch %d, rows %d, at most 2^24", batch, rows);
+  if (!cu_rows || !u_last || !accepted || !next ||
+      (rows > 0 && (!logits || !tokens || !u || !tokens_out)))
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "verify: null pointer");
+  for (const void* ptr : {logits, draft_logits})
+    if (reinterpret_cast<uintptr_t>(ptr) % dtype_size(dtype) != 0)
+      return set_error(ctx, FFAI_ATTN_ERR_INVALID, "verify: logits not aligned to their type");
+  if (tokens_out && tokens_out == tokens)
+    return set_error(ctx, FFAI_ATTN_ERR_INVALID, "verify: outputs must not alias inputs");
+  DeviceGuard g(ctx->device);
+  std::lock_guard<std::mutex> lock(ctx->space_mutex);
+  StreamSpace* space = nullptr;
+  int st = stream_space(ctx, stream, &space);
+  if (st) return st;
+  st = grow(ctx, &space->verify, 2 * static_cast<size_t>(rows) * sizeof(VerifyRow));
+  if (st) return st;
+  VerifyParams p{logits, draft_logits, ld, draft_ld, batch, rows, vocab, dtype, cu_rows, tokens, u,
+                 u_last, temperature, draft_temperature, accepted, next, tokens_out, logprobs,
+                 static_cast<VerifyRow*>(space->verify.ptr), ctx->d_err, 1, 1};
+  FFAI_CUDA(ctx, launch_verify(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }
 

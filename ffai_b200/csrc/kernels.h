@@ -370,6 +370,37 @@ constexpr int kPxKeys = 128;  // keys per block (two pages)
 cudaError_t launch_prefix_tc(const CUtensorMap& tmK, const CUtensorMap& tmV, const SharedParams& p,
                              int grid, cudaStream_t s);
 
+// ---- attention of a chunk over a paged cache (chunk_rows.cu, chunk_tc.cu) ----
+
+// Pools as above; q (tokens, heads, 64) rows q_st elements apart, out dense.
+struct ChunkParams {
+  const void* q;
+  long long q_sb, q_st, q_sh;  // q_sb: not used (one packed sequence of tokens)
+  const void* k_pool;
+  const void* v_pool;
+  const int* cu_q;         // (batch + 1)
+  const int* block_table;  // (batch, max_pages)
+  const int* seq_lens;     // (batch), new tokens included
+  int batch, tokens, max_pages, num_pages;
+  int heads, kv_heads;
+  int q_dtype, kv_dtype, out_dtype;
+  int causal;
+  float scale_log2;
+  void* out;
+  float* lse;  // (heads, tokens) or null
+  unsigned* err;
+  // two partial results per CTA, of units that lie in several CTAs' stretches:
+  // output sums (64 f32 a row), running maximum (log2 domain) and weight sum;
+  // and a ticket per CTA, zero between calls
+  float* part_o;
+  float* part_ml;
+  unsigned* tickets;
+  int min_share;  // steps per CTA, at least
+  int precise;    // f32 queries and weights are not rounded to 16 bits
+};
+constexpr int kChunkRowsPerCta = 2 * 16;  // rows of partial results
+cudaError_t launch_chunk_rows(const ChunkParams& p, int grid, cudaStream_t s);
+
 // ---- page plans and slot writes (pages.cu) ----------------------------------
 
 constexpr int kPlMaxBatch = 16384;  // three words of shared memory per request
@@ -420,6 +451,58 @@ struct WriteParams {
 };
 cudaError_t launch_kv_write(const WriteParams& p, int sms, cudaStream_t s);
 
+// ---- page forks, compaction and copies (page_moves.cu) ------------------------
+
+struct ForkParams {
+  const int* src;          // (new_batch) old rows, negative: none
+  const int* keep;         // (new_batch) or null
+  const int* lens;         // (batch)
+  const int* block_table;  // (batch, max_pages)
+  int* free_pages;         // (free_cap) stack
+  const int* free_count;
+  int* table_out;          // (new_batch, max_pages)
+  int* lens_out;           // (new_batch)
+  int* copy_src;
+  int* copy_dst;
+  int* copy_keys;
+  int* free_count_out;
+  int batch, new_batch, max_pages, num_pages, free_cap;
+  int4* words;             // (num_pages), zero between calls
+  int2* totals;            // (8), one per CTA of the cluster
+  unsigned* err;
+};
+cudaError_t launch_page_fork(const ForkParams& p, cudaStream_t s);
+
+struct CompactParams {
+  const int* lens;
+  const int* block_table;
+  const int* free_pages;
+  const int* free_count;
+  int* table_out;  // (batch, max_pages)
+  int* free_out;   // (free_cap)
+  int* copy_src;   // (cap)
+  int* copy_dst;
+  int batch, max_pages, num_pages, free_cap, cap;
+  int4* words;
+  int2* totals;
+  int* below;      // (1) live pages below the rank of the last
+  unsigned* err;
+};
+cudaError_t launch_page_compact(const CompactParams& p, cudaStream_t s);
+
+// keys[i] (null: all) rows of page src[i] to page dst[i] in both pools, n times.
+struct CopyParams {
+  void* k_pool;
+  void* v_pool;
+  const int* src;
+  const int* dst;
+  const int* keys;
+  int n, heads, num_pages;
+  int row_vecs;  // 16-byte pieces of a key's row
+  unsigned* err;
+};
+cudaError_t launch_kv_copy_keys(const CopyParams& p, int sms, cudaStream_t s);
+
 // ---- sampling (sample.cu) -----------------------------------------------------
 
 constexpr int kSmMaxVocab = 1 << 18;  // weight sums stay below 2^54
@@ -467,5 +550,34 @@ struct SampleParams {
 };
 int sample_chunk(int batch, int vocab, int sms, int most);
 cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
+
+// ---- verification of drafted tokens (verify.cu) ---------------------------------
+
+// What the first kernel leaves of a row for the second.
+struct VerifyRow {
+  unsigned long long mass, at;  // sum of the weights, and that of the token drafted there
+  float xmax, log_z;
+  int first;  // index of the first maximum
+};
+struct VerifyParams {
+  const void* logits;  // (rows, vocab), rows ld elements apart
+  const void* draft;   // the same of the draft model, or null
+  long long ld, draft_ld;
+  int batch, rows, vocab, dtype;
+  const int* cu_rows;  // (batch + 1)
+  const int* tokens;   // (rows) fed at each row
+  const float* u;      // (rows)
+  const float* u_last; // (batch)
+  const float* temperature;        // (batch) or null: 1
+  const float* draft_temperature;  // (batch) or null: 1
+  int* accepted;       // (batch)
+  int* next;           // (batch)
+  int* tokens_out;     // (rows)
+  float* logprobs;     // (rows) or null
+  VerifyRow* stats;    // (rows) of the target, then (rows) of the draft
+  unsigned* err;
+  int row_ctas, pick_ctas;  // set by the launcher: CTAs per row, per request
+};
+cudaError_t launch_verify(const VerifyParams& p, int sms, cudaStream_t s);
 
 }  // namespace ffai

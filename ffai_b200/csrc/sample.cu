@@ -49,6 +49,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "weights.cuh"
 
 namespace ffai {
 
@@ -64,8 +65,6 @@ static_assert(kSmSub == kSmThreads && 2 * kSmPair == kSmThreads && kSmBins % kSm
 // The high half of the weight 2^36 is 2^18.
 static_assert((static_cast<unsigned long long>(kSmChunk) << 18) < (1ull << 32), "halves");
 
-// NaN counts as -inf (never chosen), -0 as 0 (they tie).
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
 // Larger logit, larger key.
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x);
@@ -78,29 +77,9 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 struct RowScale {
   float xmax, inv;
 };
-// x - xmax, with 0 for the maximum itself (also when it is infinite).
-__device__ __forceinline__ float delta(float x, float xmax) {
-  return x == xmax ? 0.0f : __fadd_rn(x, -xmax);
-}
 // NaN for a NaN or masked logit; NaN and -inf both weigh nothing.
 __device__ __forceinline__ float exponent(float x, const RowScale& r) {
   return __fmul_rn(delta(x, r.xmax), r.inv);
-}
-// floor(2^36 e) for e in [0, 1], as two 18-bit halves: adding 2^23 and
-// rounding towards zero leaves the whole part in the low mantissa bits.
-struct Halves {
-  uint32_t hi, lo;
-};
-__device__ __forceinline__ Halves halves(float e) {
-  const float x = __fmul_rn(e, 262144.0f);
-  const float t = __fadd_rz(x, 8388608.0f);
-  const float r = __fmul_rn(__fadd_rn(x, -__fadd_rn(t, -8388608.0f)), 262144.0f);
-  return {__float_as_uint(t) & 0x7fffffu, __float_as_uint(__fadd_rz(r, 8388608.0f)) & 0x7fffffu};
-}
-__device__ __forceinline__ unsigned long long weight(float d) {
-  if (!(d >= -25.0f)) return 0;
-  const Halves h = halves(expf(d));
-  return (static_cast<unsigned long long>(h.hi) << 18) + h.lo;
 }
 // The bin of an exponent in [-25, 0]: floor(-64 d), at most 1600.
 __device__ __forceinline__ int bin_of(float d) {
@@ -197,19 +176,6 @@ __device__ __noinline__ Sums block_exclusive(Sums v, Sums* total) {
   return {(warp ? ba : 0) + in.a - v.a, (warp ? bc : 0) + in.c - v.c};
 }
 
-// The logits of a 16-byte piece.
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& w, float (&x)[16 / sizeof(T)]) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
-    if constexpr (sizeof(T) == 4)
-      x[e] = __uint_as_float(u[e]);
-    else
-      x[e] = e & 1 ? hi_half(u[e / 2], std::is_same<T, __half>::value)
-                   : lo_half(u[e / 2], std::is_same<T, __half>::value);
-  }
-}
 // f(x, i) for tokens [0, n) of a stretch in global memory, in no order: 16-byte
 // loads where the stretch allows, kUnroll of them in flight a thread.
 template <typename T, typename F>

@@ -280,3 +280,99 @@ def write_slots(k_pool, v_pool, k_new, v_new, slots) -> None:
         v_new.data_ptr(), at, T, _raw_stream(index))
     if st:
         _check(st, ctx)
+
+
+# ------------------------------------------- pages that rows share, and their copies
+
+class Fork(NamedTuple):
+    """Rows after a fork (fork_pages): device int32 tensors of the new batch."""
+    block_table: torch.Tensor  # (B', pages), -1 behind a row's pages
+    lens: torch.Tensor         # (B',) keys of each row
+    copy_src: torch.Tensor     # (B',) pages to copy keys from, -1: none
+    copy_dst: torch.Tensor     # (B',) and to
+    copy_keys: torch.Tensor    # (B',) how many
+    free_count: torch.Tensor   # (1,) pages left on the stack
+
+
+class Compaction(NamedTuple):
+    """A pool made dense (compact_pages): device int32 tensors."""
+    block_table: torch.Tensor  # (B, pages) with the new numbers
+    free_pages: torch.Tensor   # the stack, its lowest number on top
+    copy_src: torch.Tensor     # pages to copy, -1 behind the last
+    copy_dst: torch.Tensor     # and where to
+
+
+def fork_pages(src, lens, block_table, free_pages, free_count, *, keep=None,
+               num_pages: int | None = None) -> Fork:
+    """Row b of the new batch continues row src[b] of the old one (-1: none) with
+    its first keep[b] keys (default: all), sharing its pages (ffai_page_fork):
+    beams that are reordered, requests that split, are cut back or end.  A row
+    that would append to a page others name too gets a page of its own, to be
+    filled by `copy_pages(k_pool, v_pool, f.copy_src, f.copy_dst, keys=f.copy_keys)`
+    before anything is appended.  Pages that no row names any more are pushed on
+    the stack free_pages in place; lens, block_table and free_count are not
+    written.  `num_pages`: the pool's size (default: free_pages')."""
+    B, max_pages, index = _table(block_table)
+    n, cap = src.numel(), free_pages.numel()
+    ins = (_vec(src, "src", n, index), None if keep is None else _vec(keep, "keep", n, index),
+           _vec(lens, "lens", B, index), block_table.data_ptr(),
+           _vec(free_pages, "free_pages", cap, index), cap,
+           _vec(free_count, "free_count", 1, index))
+    buf = block_table.new_empty(n * max_pages + 4 * n + 1)
+    at = buf.data_ptr()
+    rows = at + 4 * n * max_pages
+    ctx = context(index)
+    st = _abi.load().ffai_page_fork(
+        ctx, B, n, max_pages, cap if num_pages is None else num_pages, *ins, at, rows,
+        rows + 4 * n, rows + 8 * n, rows + 12 * n, rows + 16 * n, _raw_stream(index))
+    if st:
+        _check(st, ctx)
+    table, *rest = buf.unsafe_split_with_sizes((n * max_pages, n, n, n, n, 1))
+    return Fork(table.view(n, max_pages), *rest)
+
+
+def compact_pages(lens, block_table, free_pages, free_count, *,
+                  num_pages: int | None = None) -> Compaction:
+    """The pages that block_table names take the lowest numbers of its and the
+    stack's (ffai_page_compact); `copy_pages(k_pool, v_pool, c.copy_src,
+    c.copy_dst)` moves their contents.  Nothing is written in place; the count
+    of free pages stays.  `num_pages`: the pool's size (default: free_pages')."""
+    B, max_pages, index = _table(block_table)
+    cap = free_pages.numel()
+    n = min(B * max_pages, cap)
+    buf = block_table.new_empty(B * max_pages + cap + 2 * n)
+    at = buf.data_ptr()
+    stack = at + 4 * B * max_pages
+    copies = stack + 4 * cap
+    ctx = context(index)
+    st = _abi.load().ffai_page_compact(
+        ctx, B, max_pages, cap if num_pages is None else num_pages, _vec(lens, "lens", B, index),
+        block_table.data_ptr(), _vec(free_pages, "free_pages", cap, index), cap,
+        _vec(free_count, "free_count", 1, index), at, stack, copies, copies + 4 * n, n,
+        _raw_stream(index))
+    if st:
+        _check(st, ctx)
+    table, *rest = buf.unsafe_split_with_sizes((B * max_pages, cap, n, n))
+    return Compaction(table.view(B, max_pages), *rest)
+
+
+def copy_pages(k_pool, v_pool, src, dst, *, keys=None) -> None:
+    """The first keys[i] keys (default: all 64) of page src[i] to page dst[i] in
+    both pools (ffai_kv_copy_keys); negative ids are skipped.  int32 device
+    vectors of one length; no dst is another copy's src or dst."""
+    index = k_pool.get_device()
+    pool = k_pool.shape
+    if (len(pool) != 4 or pool[2] != PAGE_KEYS or pool[3] != 64 or v_pool.shape != pool
+            or v_pool.dtype is not k_pool.dtype or v_pool.get_device() != index or index < 0
+            or k_pool.dtype not in _DT or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
+        raise ValueError("copy_pages: k and v pools contiguous (num_pages, kv_heads, 64, 64) of "
+                         "one type (f32, bf16 or f16) on one CUDA device")
+    n = src.numel()
+    lists = (_vec(src, "src", n, index), _vec(dst, "dst", n, index),
+             None if keys is None else _vec(keys, "keys", n, index))
+    d = _abi.Desc(heads=pool[1], head_dim=64, kv_dtype=_DT[k_pool.dtype])
+    ctx = context(index)
+    st = _abi.load().ffai_kv_copy_keys(ctx, ctypes.byref(d), k_pool.data_ptr(), v_pool.data_ptr(),
+                                       pool[0], *lists, n, _raw_stream(index))
+    if st:
+        _check(st, ctx)

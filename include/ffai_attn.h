@@ -297,6 +297,37 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
                             const int32_t* seq_lens, int32_t max_pages, void* o, float* lse,
                             void* stream);
 
+/* ---- attention of a chunk of new tokens over a paged cache -------------------
+ * Sequence b brings the packed tokens [cu_q[b], cu_q[b + 1]) of q, the newest
+ * of the seq_lens[b] keys in its pages block_table[b * max_pages ..]: a prompt's
+ * next chunk, a last token with its drafts, or one token; any mix of them is
+ * one call.  With d->causal, token i of n sees the keys j < seq_lens[b] - (n - 1
+ * - i), i.e. up to its own; without it, all of them.  cu_q (batch + 1, rising
+ * within 0 .. n_tokens), block_table and seq_lens are DEVICE int32, read on
+ * the device.
+ *
+ * q (n_tokens, heads, 64), token_stride as elsewhere, f32 or the cache's type;
+ * o (n_tokens, heads, 64) dense, f32, bf16 or f16; layouts TOKEN_MAJOR.  With
+ * both f32, queries and softmax weights enter the products as sums of two or
+ * three numbers of the cache's type (22 bits of them at least), which costs two
+ * to three times the products; else f32 queries are rounded to it.  Pools,
+ * kv_heads, types, and otherwise the rounding of softmax weights, and values
+ * that are not numbers: as ffai_attn_shared_prefix.  lse
+ * (optional, f32): (heads, n_tokens).  A row that sees no key gives zeros and
+ * -inf; rows of q outside every sequence's leave o and lse as they are.
+ * d->q_len: the most tokens of a sequence, if the host knows it (0: n_tokens);
+ * it chooses between kernels and binds nothing.  d->q_offset, kv_len and the
+ * k/v layouts are ignored, flags must be 0.  A sequence whose cu_q does not
+ * rise or leaves 0 .. n_tokens is skipped, a length outside the table cut, and
+ * page ids outside the pool are not read: ffai_attn_sync then reports
+ * FFAI_ATTN_ERR_INVALID.  Streams and captures: as ffai_attn_shared_prefix.
+ * No reference counterpart (prompts there run whole, text_decoder.rs:904-923). */
+int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,
+                          const void* q, int32_t n_tokens, const int32_t* cu_q,
+                          const void* k_pool, const void* v_pool, int32_t num_pages,
+                          const int32_t* block_table, const int32_t* seq_lens, int32_t max_pages,
+                          void* o, float* lse, void* stream);
+
 /* ---- page plans and slot maps ----------------------------------------------
  * The bookkeeping of a paged cache's step on the device, from lengths that
  * may themselves live there.  All arrays are DEVICE int32.  Request b holds
@@ -349,6 +380,65 @@ int ffai_kv_write_slots(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_poo
                         int32_t num_pages, const void* k_new, const void* v_new,
                         const int32_t* slots, int32_t n_tokens, void* stream);
 
+/* ---- forks, compaction and copies of pages -----------------------------------
+ * Fork: row b of the new table continues row src[b] (negative: none) of the old
+ * one with its first min(lens[src[b]], keep[b]) keys (keep null: all; negative:
+ * none), sharing its pages.  That is a beam search's reordering, a request that
+ * splits, one that is cut back to what was accepted (src[b] = b) and one that
+ * ends (src[b] = -1) in one call.  Rows that end in the middle of a page append
+ * to it next, so a row whose last page others name too gets one of its own:
+ * copy_keys[b] keys of page copy_src[b] are to be copied to copy_dst[b]
+ * (ffai_kv_copy_keys; 0 and -1: none).  If none but such rows name the page, the
+ * first of them keeps it.  Pages that the old table names and the new one does
+ * not are pushed on the stack first, in the order of their numbers; then the
+ * copies take theirs off it in row order.  A row that finds none there keeps
+ * its whole pages: lens_out[b] is rounded down to a multiple of 64.  Entries
+ * behind a row's pages are -1.  The table must name all that its pages are
+ * shared with: what another table holds is not seen.
+ *
+ * All arrays are DEVICE int32: src, keep, lens_out, copy_* (new_batch), lens
+ * (batch), block_table (batch, max_pages), table_out (new_batch, max_pages),
+ * free_pages (free_cap; written), free_count, free_count_out (1).  Outputs must
+ * not alias inputs.  Reported by ffai_attn_sync: src not below batch (the row
+ * is empty), lengths outside the table (none), page ids outside the pool (passed
+ * on as -1; on the stack: no page), a free_count outside 0 .. free_cap (the
+ * nearer end) and pushes past free_cap (lost).  Streams and captures: as
+ * ffai_attn_shared_prefix.  No reference counterpart on the device
+ * (TextDecoder::save/restore clone caches, text_decoder.rs:1363-1381). */
+int ffai_page_fork(ffai_attn_ctx* ctx, int32_t batch, int32_t new_batch, int32_t max_pages,
+                   int32_t num_pages, const int32_t* src, const int32_t* keep, const int32_t* lens,
+                   const int32_t* block_table, int32_t* free_pages, int32_t free_cap,
+                   const int32_t* free_count, int32_t* table_out, int32_t* lens_out,
+                   int32_t* copy_src, int32_t* copy_dst, int32_t* copy_keys,
+                   int32_t* free_count_out, void* stream);
+
+/* Compaction: of all pages that the table (its first ceil(lens / 64) entries a
+ * row) or the stack names, those in the table take the lowest numbers, so that
+ * what lies above them can be given back or the pool be shrunk.  Those that lie
+ * too high move, in order, to the free ones that lie low: page copy_src[i] is to
+ * be copied to copy_dst[i] (ffai_kv_copy_keys; -1 behind the last; copy_cap at
+ * least the smaller of batch * max_pages and free_cap).  table_out is the table
+ * with the new numbers (entries behind a row's pages as they are), free_out the
+ * stack with its lowest number on top (entries behind free_count as they are);
+ * free_count stays.  Shared pages move once.  A bad length, count or page id, and
+ * a page that is named by table and stack or twice on the stack, is reported by
+ * ffai_attn_sync; nothing moves then.  Arrays, aliasing, streams: as
+ * ffai_page_fork.  No reference counterpart. */
+int ffai_page_compact(ffai_attn_ctx* ctx, int32_t batch, int32_t max_pages, int32_t num_pages,
+                      const int32_t* lens, const int32_t* block_table, const int32_t* free_pages,
+                      int32_t free_cap, const int32_t* free_count, int32_t* table_out,
+                      int32_t* free_out, int32_t* copy_src, int32_t* copy_dst, int32_t copy_cap,
+                      void* stream);
+
+/* Copy the first keys[i] keys (DEVICE int32; null: all FFAI_PAGE_KEYS) of page
+ * src[i] to page dst[i] in both pools (num_pages, d->heads, FFAI_PAGE_KEYS, 64) of
+ * d->kv_dtype, n times; a negative src or dst is skipped.  No dst is another
+ * copy's src or dst.  Page ids past the pool and keys outside 0 .. 64 are not
+ * copied and reported by ffai_attn_sync. */
+int ffai_kv_copy_keys(ffai_attn_ctx* ctx, const ffai_attn_desc* d, void* k_pool, void* v_pool,
+                      int32_t num_pages, const int32_t* src, const int32_t* dst,
+                      const int32_t* keys, int32_t n, void* stream);
+
 /* ---- sampling ----------------------------------------------------------------
  * One token per row of logits (batch, vocab) of dtype, rows ld elements
  * apart, from the caller's uniform numbers u[b] in [0, 1).  A row's tokens
@@ -371,6 +461,37 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
                 int32_t vocab, const float* u, const float* temperature, const int32_t* top_k,
                 const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
                 void* stream);
+
+/* Verification of drafted tokens.  Request b has the packed rows [cu_rows[b],
+ * cu_rows[b + 1]): its last token and its drafts, tokens (rows) being what was
+ * fed there.  logits (rows, vocab) of dtype, rows ld elements apart, are the
+ * target's, draft_logits (the same type, draft_ld apart) those the drafts were
+ * drawn from, the token of row i + 1 from row i's; null when the drafts were
+ * given (looked up, or a greedy draft's).  With p and q the softmax of a row's
+ * logits over the temperatures (DEVICE (batch), null for 1; <= 0, or one whose
+ * reciprocal overflows: the first maximum has all), the draft x of row i stands
+ * if u[i] q(x) < p(x) (q(x) = 1 without draft_logits); at the first that does
+ * not, the token is taken by u_last[b] from max(0, p - q) over its sum, in the
+ * order of the vocabulary, or from the last row's p if all stand.  So the
+ * tokens are distributed as if the target alone had been sampled, one by one.
+ * Both are computed in whole weights as in ffai_sample (p and q below 2^-36 of a
+ * row's largest are 0): equal inputs give equal tokens.
+ *
+ * u (rows), u_last (batch): uniform numbers in [0, 1).  accepted (batch): drafts
+ * that stand, next (batch): the token behind them; tokens_out (rows): the
+ * request's accepted drafts, then next, at its first rows, -1 elsewhere; logprobs
+ * (optional, rows, f32): the emitted tokens' log-softmax of the logits as they
+ * are, 0 elsewhere.  A request without rows gives 0 and -1.  NaN logits count as
+ * -inf; a row with nothing above -inf accepts nothing and gives next -1; a draft
+ * outside the vocabulary does not stand.  A request whose cu_rows does not rise
+ * or leaves 0 .. rows counts as one without rows and is reported by
+ * ffai_attn_sync.  vocab at most 262144 (else FFAI_ATTN_DECLINED).  Streams and
+ * captures: as ffai_attn_shared_prefix.  No reference counterpart. */
+int ffai_verify(ffai_attn_ctx* ctx, const void* logits, int64_t ld, const void* draft_logits,
+                int64_t draft_ld, int32_t dtype, int32_t batch, int32_t rows, int32_t vocab,
+                const int32_t* cu_rows, const int32_t* tokens, const float* u, const float* u_last,
+                const float* temperature, const float* draft_temperature, int32_t* accepted,
+                int32_t* next, int32_t* tokens_out, float* logprobs, void* stream);
 
 /* ---- int8 GEMV ---------------------------------------------------------
  * The reference's block-scaled int8 GEMV (Int8Vocab, vocab_int8.rs), which
