@@ -1855,25 +1855,42 @@ int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t k
   p.err = ctx->d_err;
   DeviceGuard g(ctx->device);
   ProfScope ps(ctx, FFAI_OP_VARLEN, static_cast<cudaStream_t>(stream), "ffai_attn_chunk_paged");
-  if (units(16) * blocks > INT32_MAX / 2)
+  // With f32 queries and output nothing is rounded to 16 bits: a matter for the
+  // rows kernel.
+  p.precise = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32;
+  const double most = d->q_len > 0 ? std::min<double>(d->q_len, n_tokens)
+                                   : static_cast<double>(n_tokens) / d->batch;
+  const bool rows_way = p.precise || most * G <= kChRows;
+  const int unit_rows = rows_way ? kChRows : kPxRows;
+  const double steps = units(unit_rows) * blocks;
+  if (steps > INT32_MAX / 2)
     return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: too many rows and keys");
+  const int resident = rows_way ? (p.precise ? 2 : 3) : 1;
+  const int grid = static_cast<int>(std::min<double>(1.0 * resident * ctx->num_sms, steps));
+  p.min_share = rows_way ? 4 : 2;
   std::lock_guard<std::mutex> lock(ctx->space_mutex);
   StreamSpace* space = nullptr;
   int st = stream_space(ctx, stream, &space);
   if (st) return st;
-  const int resident = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32 ? 2 : 3;
-  const int grid = static_cast<int>(std::min<double>(1.0 * resident * ctx->num_sms, units(16) * blocks));
-  p.min_share = 4;
-  p.precise = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32;
-  st = grow(ctx, &space->tickets, static_cast<size_t>(grid) * 4, /*zero=*/true);
+  st = grow(ctx, &space->tickets, static_cast<size_t>(grid) * 8, /*zero=*/true);
   if (st) return st;
   p.tickets = static_cast<unsigned*>(space->tickets.ptr);
-  const size_t rows = static_cast<size_t>(grid) * kChunkRowsPerCta;
+  const size_t rows = static_cast<size_t>(grid) * 2 * unit_rows;
   st = grow(ctx, &space->chunk, rows * 66 * 4);
   if (st) return st;
   p.part_ml = static_cast<float*>(space->chunk.ptr);
   p.part_o = p.part_ml + rows * 2;
-  FFAI_CUDA(ctx, launch_chunk_rows(p, grid, static_cast<cudaStream_t>(stream)));
+  if (rows_way) {
+    FFAI_CUDA(ctx, launch_chunk_rows(p, grid, static_cast<cudaStream_t>(stream)));
+    return FFAI_ATTN_OK;
+  }
+  CUtensorMap tmk, tmv;
+  const long long heads = static_cast<long long>(num_pages) * kv_heads;
+  st = make_map(ctx, &tmk, k_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
+  if (st) return st;
+  st = make_map(ctx, &tmv, v_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
+  if (st) return st;
+  FFAI_CUDA(ctx, launch_chunk_tc(tmk, tmv, p, grid, static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }
 

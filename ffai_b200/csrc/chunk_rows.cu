@@ -27,135 +27,24 @@ namespace ffai {
 
 namespace {
 
-constexpr int kCrRows = 16;
-
-__device__ __forceinline__ int unit_steps(const ChunkParams& p, const ChunkSeq& s, int G, int m) {
-  const int last = min((m + 1) * kCrRows, s.n * G) - 1;
-  return chunk_blocks(chunk_limit(p, s, last / G));
-}
-__device__ __forceinline__ int head_steps(const ChunkParams& p, const ChunkSeq& s, int G) {
-  const int units = chunk_units<kCrRows>(s, G);
-  if (units == 0) return 0;
-  if (!p.causal) return units * chunk_blocks(s.len);
-  int n = 0;
-  for (int m = 0; m < units; ++m) n += unit_steps(p, s, G, m);
-  return n;
-}
-
-// A CTA's stretch of the line: where it starts, and how long it is.
-struct Stretch {
-  int b, h, m, step;  // sequence, KV head, unit, step within the unit
-  int left;           // steps
-  int share;          // of a CTA
-  int unit0;          // the unit's first step on the line
-};
-
-// All threads: every CTA scans the sequences.
-__device__ __forceinline__ void find_stretch(const ChunkParams& p, Stretch* out) {
-  __shared__ int s_warp[kSpWarps];
-  const int G = p.heads / p.kv_heads;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int per = (p.batch + kSpThreads - 1) / kSpThreads;
-  const int b0 = min(p.batch, static_cast<int>(threadIdx.x) * per), b1 = min(p.batch, b0 + per);
-  bool bad = false;
-  int sum = 0;
-#pragma unroll 4
-  for (int b = b0; b < b1; ++b) sum += p.kv_heads * head_steps(p, chunk_seq(p, b, bad), G);
-  if (bad && blockIdx.x == 0 && p.err) atomicOr(p.err, kErrBadArgs);
-  int at = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, at, o);
-    if (lane >= o) at += x;
-  }
-  if (lane == 31) s_warp[warp] = at;
-  __syncthreads();
-  int total = 0, base = 0;
-#pragma unroll
-  for (int w = 0; w < kSpWarps; ++w) {
-    if (w < warp) base += s_warp[w];
-    total += s_warp[w];
-  }
-  at += base - sum;
-  const int grid = static_cast<int>(gridDim.x);
-  const int share = max(p.min_share, (total + grid - 1) / grid);
-  const int first = static_cast<int>(blockIdx.x) * share;
-  const int left = min(total, first + share) - first;
-  if (threadIdx.x == 0) out->left = 0;
-  __syncthreads();
-  if (left > 0 && at <= first && first < at + sum) {  // one thread
-    int b = b0;
-    ChunkSeq s{};
-    int per_head = 0;
-    for (; b < b1; ++b) {
-      s = chunk_seq(p, b, bad);
-      per_head = head_steps(p, s, G);
-      if (first < at + p.kv_heads * per_head) break;
-      at += p.kv_heads * per_head;
-    }
-    Stretch w{};
-    if (b < b1) {  // (always, unless the lengths are written meanwhile)
-      w.b = b;
-      w.h = (first - at) / per_head;
-      at += w.h * per_head;
-      const int units = chunk_units<kCrRows>(s, G);
-      for (; w.m < units - 1; ++w.m) {
-        const int n = unit_steps(p, s, G, w.m);
-        if (first < at + n) break;
-        at += n;
-      }
-      w.unit0 = at;
-      w.step = first - at;
-      w.left = left;
-      w.share = share;
-    }
-    *out = w;
-  }
-  __syncthreads();
-}
-
-// One row's result, 8 head dims a thread.
-__device__ __forceinline__ void store_row(const ChunkParams& p, Merged& acc, int tok, int h, int part) {
-  const size_t at = (static_cast<size_t>(tok) * p.heads + h) * 64 + 8 * part;
-  const float inv = acc.l == 0.f ? 0.f : 1.f / acc.l;  // 0: the row saw no key
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc.o[e] *= inv;
-  if (p.out_dtype == 0) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-    o[0] = make_float4(acc.o[0], acc.o[1], acc.o[2], acc.o[3]);
-    o[1] = make_float4(acc.o[4], acc.o[5], acc.o[6], acc.o[7]);
-  } else {
-    uint4 x;
-    if (p.out_dtype == 1)
-      x = make_uint4(pack_bf16x2(acc.o[0], acc.o[1]), pack_bf16x2(acc.o[2], acc.o[3]),
-                     pack_bf16x2(acc.o[4], acc.o[5]), pack_bf16x2(acc.o[6], acc.o[7]));
-    else
-      x = make_uint4(pack_f16x2(acc.o[0], acc.o[1]), pack_f16x2(acc.o[2], acc.o[3]),
-                     pack_f16x2(acc.o[4], acc.o[5]), pack_f16x2(acc.o[6], acc.o[7]));
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = x;
-  }
-  if (p.lse && part == 0)
-    p.lse[static_cast<size_t>(h) * p.tokens + tok] =
-        acc.l == 0.f ? -INFINITY : (acc.m + log2f(acc.l)) * 0.69314718055994530942f;
-}
-
 template <int F16, int TERMS>
 __global__ void __launch_bounds__(kSpThreads, TERMS > 1 ? 2 : 3) chunk_rows_kernel(ChunkParams p) {
   extern __shared__ __align__(128) uint8_t sp_smem[];
   __shared__ Stretch s_start;
+  __shared__ int s_warp[kSpWarps];
   __shared__ int s_last;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2;
   const int G = p.heads / p.kv_heads;
   RowsMerge<kSpWarps>& sm = *reinterpret_cast<RowsMerge<kSpWarps>*>(sp_smem);
-  find_stretch(p, &s_start);
+  find_stretch<kChRows, kSpThreads>(p, &s_start, s_warp);
   Stretch w = s_start;
   bool bad = false;
   ChunkSeq s{};
   if (w.left > 0) s = chunk_seq(p, w.b, bad);
   while (w.left > 0) {
     // ---- the unit's rows, and the keys each sees
-    const int row0 = w.m * kCrRows, rows = min(kCrRows, s.n * G - row0);
-    const int steps = unit_steps(p, s, G, w.m), n = min(w.left, steps - w.step);
+    const int row0 = w.m * kChRows, rows = min(kChRows, s.n * G - row0);
+    const int steps = unit_steps<kChRows>(p, s, G, w.m), n = min(w.left, steps - w.step);
     const int k0 = w.step * kChKeys;
     int seq[2] = {0, 0}, tok[2], head[2], see[2];
 #pragma unroll
@@ -190,7 +79,7 @@ __global__ void __launch_bounds__(kSpThreads, TERMS > 1 ? 2 : 3) chunk_rows_kern
       const int c0 = w.unit0 / w.share;
       const int c1 = min((w.unit0 + steps - 1) / w.share, static_cast<int>(gridDim.x) - 1);
       const int cta = static_cast<int>(blockIdx.x);
-      const auto slot = [&](int c) { return (static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * kCrRows + row); };
+      const auto slot = [&](int c) { return (static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * kChRows + row); };
       float4* o = reinterpret_cast<float4*>(p.part_o + slot(cta) * 64 + 8 * part);
       __stcg(o, make_float4(acc.o[0], acc.o[1], acc.o[2], acc.o[3]));
       __stcg(o + 1, make_float4(acc.o[4], acc.o[5], acc.o[6], acc.o[7]));
@@ -223,7 +112,7 @@ __global__ void __launch_bounds__(kSpThreads, TERMS > 1 ? 2 : 3) chunk_rows_kern
     if (w.left > 0) {
       w.step = 0;
       w.unit0 += steps;
-      if (++w.m == chunk_units<kCrRows>(s, G)) {
+      if (++w.m == chunk_units<kChRows>(s, G)) {
         w.m = 0;
         if (++w.h == p.kv_heads) {
           w.h = 0;

@@ -391,15 +391,18 @@ struct ChunkParams {
   unsigned* err;
   // two partial results per CTA, of units that lie in several CTAs' stretches:
   // output sums (64 f32 a row), running maximum (log2 domain) and weight sum;
-  // and a ticket per CTA, zero between calls
+  // and two tickets per CTA, zero between calls
   float* part_o;
   float* part_ml;
   unsigned* tickets;
   int min_share;  // steps per CTA, at least
   int precise;    // f32 queries and weights are not rounded to 16 bits
 };
-constexpr int kChunkRowsPerCta = 2 * 16;  // rows of partial results
+constexpr int kChRows = 16;  // query rows per unit of the rows kernel (kPxRows of the other)
 cudaError_t launch_chunk_rows(const ChunkParams& p, int grid, cudaStream_t s);
+// tm*: as for launch_prefix_tc
+cudaError_t launch_chunk_tc(const CUtensorMap& tmK, const CUtensorMap& tmV, const ChunkParams& p,
+                            int grid, cudaStream_t s);
 
 // ---- page plans and slot writes (pages.cu) ----------------------------------
 
