@@ -86,7 +86,8 @@ struct StreamSpace {
   Grown pages;                     // words per page of forks and compactions
   Grown chunk;                     // partial results of a chunk's attention,
   Grown tickets;                   // and whose turn it is to merge them
-  Grown verify;                    // per-row state between the verifying kernels
+  Grown verify;                    // per-row state between the verifying kernels,
+  Grown fails;                     // the queue of rows, and the first of each request that fails
   StreamSpace* next = nullptr;
 };
 }  // namespace ffai
@@ -898,7 +899,8 @@ void ffai_attn_destroy(ffai_attn_ctx* ctx) {
   cudaFree(ctx->d_gemv_x);
   while (StreamSpace* w = ctx->spaces) {
     ctx->spaces = w->next;
-    for (Grown* b : {&w->prefix, &w->own, &w->queue, &w->sample, &w->pages, &w->chunk, &w->tickets, &w->verify})
+    for (Grown* b : {&w->prefix, &w->own, &w->queue, &w->sample, &w->pages, &w->chunk, &w->tickets, &w->verify,
+                     &w->fails})
       free_grown(b);
     if (w->mark) let_go(w->mark);
     delete w;
@@ -1968,9 +1970,12 @@ int ffai_verify(ffai_attn_ctx* ctx, const void* logits, int64_t ld, const void* 
   if (st) return st;
   st = grow(ctx, &space->verify, 2 * static_cast<size_t>(rows) * sizeof(VerifyRow));
   if (st) return st;
+  st = grow(ctx, &space->fails, 8 + static_cast<size_t>(batch) * 4, /*zero=*/true);
+  if (st) return st;
   VerifyParams p{logits, draft_logits, ld, draft_ld, batch, rows, vocab, dtype, cu_rows, tokens, u,
                  u_last, temperature, draft_temperature, accepted, next, tokens_out, logprobs,
-                 static_cast<VerifyRow*>(space->verify.ptr), ctx->d_err, 1, 1};
+                 static_cast<VerifyRow*>(space->verify.ptr), static_cast<int*>(space->fails.ptr) + 2,
+                 ctx->d_err, static_cast<unsigned long long*>(space->fails.ptr), 0, 1};
   FFAI_CUDA(ctx, launch_verify(p, ctx->num_sms, static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }

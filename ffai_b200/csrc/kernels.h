@@ -558,7 +558,7 @@ cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
 
 // What the first kernel leaves of a row for the second.
 struct VerifyRow {
-  unsigned long long mass, at;  // sum of the weights, and that of the token drafted there
+  unsigned long long mass;  // sum of the weights
   float xmax, log_z;
   int first;  // index of the first maximum
 };
@@ -578,8 +578,10 @@ struct VerifyParams {
   int* tokens_out;     // (rows)
   float* logprobs;     // (rows) or null
   VerifyRow* stats;    // (rows) of the target, then (rows) of the draft
+  int* fails;          // (batch), zero between calls: the first row that fails, counted down
   unsigned* err;
-  int row_ctas, pick_ctas;  // set by the launcher: CTAs per row, per request
+  unsigned long long* queue;  // of rows, zero between calls
+  int row_shift, pick_ctas;  // set by the launcher: CTAs per row (log2), per request
 };
 cudaError_t launch_verify(const VerifyParams& p, int sms, cudaStream_t s);
 
