@@ -1827,7 +1827,7 @@ int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t k
   if (static_cast<double>(n_tokens) * d->heads > (1 << 30) ||
       static_cast<double>(num_pages) * kv_heads > 2147483647.0)
     return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: too many rows");
-  // units of `rows` rows: one started per sequence, and as many as are full
+  // the most units of `rows` rows: one started per sequence, and as many as are full
   const auto units = [&](int rows) {
     return static_cast<double>(kv_heads) *
            (std::min<double>(d->batch, n_tokens) + static_cast<double>(n_tokens) * G / rows);
@@ -1860,39 +1860,54 @@ int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t k
   // With f32 queries and output nothing is rounded to 16 bits: a matter for the
   // rows kernel.
   p.precise = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32;
-  const double most = d->q_len > 0 ? std::min<double>(d->q_len, n_tokens)
-                                   : static_cast<double>(n_tokens) / d->batch;
-  const bool rows_way = p.precise || most * G <= kChRows;
-  const int unit_rows = rows_way ? kChRows : kPxRows;
-  const double steps = units(unit_rows) * blocks;
-  if (steps > INT32_MAX / 2)
+  // Rows of a sequence and KV head: the most, or the average if the host has no bound.
+  // Up to 128 the rows kernel serves them, beyond the tensor kernel.  Measured, rows
+  // and tensor kernel: 64 sequences of up to 8 tokens, 32 / 8 heads, 2000 keys 49 and
+  // 94 us, of up to 32 tokens 107 and 113; 4 of 2048 tokens, 20 heads, 267 and 127; 32
+  // single tokens beside four chunks of up to 700, 28 / 4 heads, 6000 keys, 400 and
+  // 160.  (Both kernels, each for its sequences: 152, but it costs long prompts 8 %.)
+  const double most = (d->q_len > 0 ? std::min<double>(d->q_len, n_tokens)
+                                    : static_cast<double>(n_tokens) / d->batch) * G;
+  const bool tensor = !p.precise && most > 128;
+  // Row groups of a unit: with many products, 64 rows share their keys (28 / 4 heads as
+  // above, f32: 390 us against 455).
+  const int r = p.precise && most > 32 ? 4 : 1;
+  const int unit_rows = tensor ? kPxRows : 16 * r;
+  // Warps that share a unit's keys: as many as leave every team about a unit.  Measured
+  // with 4, 2 and 1: 192 units of 30000 keys 134, 139 and 141 us; 400 of 1500 27, 20 and
+  // 24; 512 of 2000 47, 43 and 40; 1200 of 448 36, 37 and 21.
+  const double room = (tensor ? 1.0 : p.precise ? 2.0 : 3.0) * ctx->num_sms;  // CTAs
+  const double expected = kv_heads * std::max<double>(std::min<double>(d->batch, n_tokens), n_tokens * G / (16.0 * r));
+  const int w = r > 1 ? 1 : expected <= 0.6 * room ? 4 : expected <= room ? 2 : 1;
+  const double most_steps = units(unit_rows) * blocks * (tensor ? 1 : 4);
+  if (most_steps > INT32_MAX / 2)
     return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: too many rows and keys");
-  const int resident = rows_way ? (p.precise ? 2 : 3) : 1;
-  const int grid = static_cast<int>(std::min<double>(1.0 * resident * ctx->num_sms, steps));
-  p.min_share = rows_way ? 4 : 2;
+  const int grid = static_cast<int>(std::min<double>(room, most_steps));
+  const int teams = tensor ? grid : grid * 4 / (w * r);
+  p.min_share = tensor ? 2 : 16 / w;  // steps: 256 keys of 256 rows, 512 of 16
   std::lock_guard<std::mutex> lock(ctx->space_mutex);
   StreamSpace* space = nullptr;
   int st = stream_space(ctx, stream, &space);
   if (st) return st;
-  st = grow(ctx, &space->tickets, static_cast<size_t>(grid) * 8, /*zero=*/true);
+  st = grow(ctx, &space->tickets, static_cast<size_t>(teams) * 8, /*zero=*/true);
   if (st) return st;
   p.tickets = static_cast<unsigned*>(space->tickets.ptr);
-  const size_t rows = static_cast<size_t>(grid) * 2 * unit_rows;
+  const size_t rows = static_cast<size_t>(teams) * 2 * unit_rows;
   st = grow(ctx, &space->chunk, rows * 66 * 4);
   if (st) return st;
   p.part_ml = static_cast<float*>(space->chunk.ptr);
   p.part_o = p.part_ml + rows * 2;
-  if (rows_way) {
-    FFAI_CUDA(ctx, launch_chunk_rows(p, grid, static_cast<cudaStream_t>(stream)));
-    return FFAI_ATTN_OK;
-  }
   CUtensorMap tmk, tmv;
   const long long heads = static_cast<long long>(num_pages) * kv_heads;
-  st = make_map(ctx, &tmk, k_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
+  const int box = tensor ? kPageKeys : kPageKeys / 2;
+  st = make_map(ctx, &tmk, k_pool, false, 0, kPageKeys, heads, 0, box);
   if (st) return st;
-  st = make_map(ctx, &tmv, v_pool, false, 0, kPageKeys, heads, 0, kPageKeys);
+  st = make_map(ctx, &tmv, v_pool, false, 0, kPageKeys, heads, 0, box);
   if (st) return st;
-  FFAI_CUDA(ctx, launch_chunk_tc(tmk, tmv, p, grid, static_cast<cudaStream_t>(stream)));
+  if (tensor)
+    FFAI_CUDA(ctx, launch_chunk_tc(tmk, tmv, p, grid, static_cast<cudaStream_t>(stream)));
+  else
+    FFAI_CUDA(ctx, launch_chunk_rows(tmk, tmv, p, grid, w, r, static_cast<cudaStream_t>(stream)));
   return FFAI_ATTN_OK;
 }
 

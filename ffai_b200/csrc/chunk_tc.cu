@@ -64,7 +64,7 @@ __device__ __forceinline__ int walk_first(const Walk& w) { return walk_pair(w) ?
 __device__ __forceinline__ void walk_unit(Walk& w, const ChunkParams& p) {
   const int G = p.heads / p.kv_heads, end = min((w.m + 1) * kPxRows, w.s.n * G);
   w.rows = end - w.m * kPxRows;
-  w.nb = chunk_blocks(chunk_limit(p, w.s, (end - 1) / G));
+  w.nb = chunk_blocks<kChKeys>(chunk_limit(p, w.s, (end - 1) / G));
   w.steps = walk_pair(w) ? w.nb : (w.nb + 1) >> 1;
 }
 // To the next unit, if the stretch goes on.
@@ -335,13 +335,6 @@ __device__ __forceinline__ void load_q(const ChunkParams& p, const Walk& w, int 
     }
   }
   cp_async_wait_all();
-}
-
-// Which halves of a pair are infinite or NaN.
-template <int F16>
-__device__ __forceinline__ uint32_t odd_halves(uint32_t x) {
-  constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
-  return ((x & kExp) == kExp ? 0xffffu : 0u) | ((x >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
 }
 
 // The rest of a chain meets here (bounded, like every wait): its 256 threads.
@@ -655,11 +648,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
       const int share = bars->share;
       const int c0 = w.unit0 / share, c1 = min((w.unit0 + w.steps - 1) / share, static_cast<int>(gridDim.x) - 1);
       const int cta = static_cast<int>(blockIdx.x);
-      const int side = pair ? 128 * t : 0;
-      // row r of this tile in CTA x's partial of the unit
-      const auto partial = [&](int x, int r) {
-        return static_cast<size_t>(2 * x + (x == c0 ? 1 : 0)) * kPxRows + side + r;
-      };
+      const UnitParts u{c0, c1, kPxRows, pair ? 128 * t : 0, row0, rows, w.s.t0, w.h};
       if (active) {
         float inv[2];
         size_t at[2];
@@ -676,9 +665,9 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
               p.lse[static_cast<size_t>(h) * p.tokens + w.s.t0 + tok] =
                   l_run[v] == 0.f ? -INFINITY : (m_run[v] + log2f(l_run[v])) * 0.69314718055994530942f;
           } else {
-            at[v] = partial(cta, r) * 64 + 2 * t0;
+            at[v] = part_row(u, cta, r) * 64 + 2 * t0;
             if (t0 == 0 && r < rows)
-              __stcg(reinterpret_cast<float2*>(p.part_ml + 2 * partial(cta, r)),
+              __stcg(reinterpret_cast<float2*>(p.part_ml + 2 * part_row(u, cta, r)),
                      make_float2(m_run[v], l_run[v]));
           }
         }
@@ -733,12 +722,11 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
             Merged acc{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 2
             for (int x = c0; x <= c1; ++x) {
-              const size_t from = partial(x, r);
+              const size_t from = part_row(u, x, r);
               const float4* o = reinterpret_cast<const float4*>(p.part_o + from * 64 + 8 * part);
               acc.add(__ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * from)), __ldcg(o), __ldcg(o + 1));
             }
-            const int tok = (row0 + r) / G;
-            store_row(p, acc, w.s.t0 + tok, w.h * G + row0 + r - tok * G, part);
+            store_unit_row(p, u, acc, r, part);
           }
         }
       }
@@ -753,7 +741,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
 template <int F16>
 __global__ void __launch_bounds__(kCtThreads, 1)
     chunk_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const ChunkParams p) {
+                    const __grid_constant__ ChunkParams p) {
   if (smem_u32(ct_smem) % 1024 != 0) {  // the whole grid alike
     if (threadIdx.x == 0 && p.err) atomicOr(p.err, kErrBadArgs);
     return;
@@ -794,7 +782,7 @@ __global__ void __launch_bounds__(kCtThreads, 1)
   }
   // (the walks' place serves before they are)
   Stretch* start = reinterpret_cast<Stretch*>(ct_smem + kCtOffWalks);
-  find_stretch<kPxRows, kCtThreads>(p, start, reinterpret_cast<int*>(start + 1));
+  find_stretch<kPxRows, kChKeys, kCtThreads, 1>(p, start, reinterpret_cast<int2*>(start + 2));
   if (threadIdx.x == 0) {
     const Stretch x = *start;
     Walk w{};

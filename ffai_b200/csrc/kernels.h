@@ -389,17 +389,21 @@ struct ChunkParams {
   void* out;
   float* lse;  // (heads, tokens) or null
   unsigned* err;
-  // two partial results per CTA, of units that lie in several CTAs' stretches:
-  // output sums (64 f32 a row), running maximum (log2 domain) and weight sum;
-  // and two tickets per CTA, zero between calls
+  // two partial results per team of warps (the tensor kernel's CTAs are one each),
+  // of units that lie in several teams' stretches: output sums (64 f32 a row),
+  // running maximum (log2 domain) and weight sum; and two tickets per team, zero
+  // between calls
   float* part_o;
   float* part_ml;
   unsigned* tickets;
-  int min_share;  // steps per CTA, at least
+  int min_share;  // steps per team, at least
   int precise;    // f32 queries and weights are not rounded to 16 bits
 };
-constexpr int kChRows = 16;  // query rows per unit of the rows kernel (kPxRows of the other)
-cudaError_t launch_chunk_rows(const ChunkParams& p, int grid, cudaStream_t s);
+constexpr int kChRows = 16;  // query rows of a warp of the rows kernel (kPxRows per unit of the other)
+// r = 1 or 4 warps with 16 rows each to a group, w groups, which share the keys, to a
+// team: of a CTA's four warps w r.  tm*: as for launch_prefix_tc, boxes of half a page
+cudaError_t launch_chunk_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const ChunkParams& p,
+                              int grid, int w, int r, cudaStream_t s);
 // tm*: as for launch_prefix_tc
 cudaError_t launch_chunk_tc(const CUtensorMap& tmK, const CUtensorMap& tmV, const ChunkParams& p,
                             int grid, cudaStream_t s);

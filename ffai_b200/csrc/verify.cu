@@ -377,7 +377,7 @@ __device__ __noinline__ void finish_row(const VerifyParams& p, const RowParts& s
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads + 32, 2) verify_rows_kernel(VerifyParams p) {
+__global__ void __launch_bounds__(kVfThreads + 32, 2) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ RowParts s;
   griddep_launch_dependents();
   const int shift = p.row_shift, ctas = 1 << shift, cluster = blockIdx.x >> shift, rank = blockIdx.x & (ctas - 1);
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kVfThreads + 32, 2) verify_rows_kernel(VerifyP
 
 // The weights of a row's token: the target's, or what it has beyond the draft's.
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads, 2) verify_pick_kernel(VerifyParams p) {
+__global__ void __launch_bounds__(kVfThreads, 2) verify_pick_kernel(const __grid_constant__ VerifyParams p) {
   constexpr int kVec = 16 / sizeof(T);
   __shared__ unsigned long long s_part[2][kVfParts];
   const int ctas = p.pick_ctas, b = blockIdx.x / ctas, rank = blockIdx.x - b * ctas;
