@@ -188,8 +188,7 @@ struct RowPieces {
 };
 
 // The passes over a CTA's part [lo, hi) of a row's pieces, functions of their own
-// so that the loops have all registers (inlined they kept theirs in local memory:
-// 38 instructions a logit instead of WW).
+// so that the loops have all registers (inlined they kept theirs in local memory).
 template <typename T>
 __device__ __noinline__ float max_pass(const uint4* pieces, int lo, int hi) {
   constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
