@@ -33,6 +33,7 @@ namespace {
 constexpr int kMvThreads = 512;
 constexpr int kMvWarps = kMvThreads / 32;
 constexpr int kMvCluster = 8;
+constexpr int kMvAhead = 4;  // rows whose pages a warp has on their way
 
 __device__ __forceinline__ int pages_of(int keys) { return (keys + kPageKeys - 1) / kPageKeys; }
 
@@ -112,41 +113,64 @@ __global__ void __launch_bounds__(kMvThreads) page_fork_kernel(ForkParams p) {
   const int mp = p.max_pages;
   bool bad = false;
 
-  // ---- references of the new table, and the old table's pages
-  const int entries = p.new_batch * mp, old_entries = p.batch * mp;
-#pragma unroll 4
-  for (int e = t; e < entries; e += threads) {
-    const int b = e / mp, i = e - b * mp;
-    const NewRow r = new_row(p, b, bad);
-    int page = -1;
-    if (i < pages_of(r.n)) {
-      page = __ldg(p.block_table + static_cast<size_t>(r.src) * mp + i);
-      if (page < 0 || page >= p.num_pages) {
+  // ---- references of the new table, and the old table's pages: a warp looks at 32 rows'
+  // lengths at once and takes their entries 32 by 32
+  const int lane = threadIdx.x % 32, warps = threads / 32;
+  const int most = max(p.new_batch, p.batch);
+  const int per = min(32, (most + warps - 1) / warps);  // rows of a warp at a time
+  for (int b0 = t / 32 * per; b0 < most; b0 += warps * per) {
+    NewRow mine{-1, 0};
+    int old = 0;
+    if (lane < per && b0 + lane < p.new_batch) mine = new_row(p, b0 + lane, bad);
+    if (lane < per && b0 + lane < p.batch) {
+      old = __ldg(p.lens + b0 + lane);
+      if (old < 0 || old > mp * kPageKeys) {
         bad = true;
-        page = -1;
-      } else {
-        int* w = reinterpret_cast<int*>(p.words + page);
-        atomicAdd(w, 1);
-        if ((i + 1) * kPageKeys > r.n) {
-          atomicAdd(w + 1, 1);
-          atomicMax(w + 2, p.new_batch - b);
-        }
+        old = 0;
       }
     }
-    p.table_out[e] = page;
-  }
-#pragma unroll 4
-  for (int e = t; e < old_entries; e += threads) {
-    const int b = e / mp, i = e - b * mp;
-    const int len = __ldg(p.lens + b);
-    if (len < 0 || len > mp * kPageKeys) {
-      bad = true;
-    } else if (i < pages_of(len)) {
-      const int page = __ldg(p.block_table + e);
-      if (page < 0 || page >= p.num_pages)
-        bad = true;
-      else
-        __stcg(reinterpret_cast<int*>(p.words + page) + 3, 1);
+    const int rows = min(per, most - b0);
+    for (int i0 = 0; i0 < mp; i0 += 32) {
+      const int i = i0 + lane;
+      for (int k0 = 0; k0 < rows; k0 += kMvAhead) {
+        int page[kMvAhead], was[kMvAhead], n[kMvAhead], len[kMvAhead];
+#pragma unroll
+        for (int k = 0; k < kMvAhead; ++k) {  // (rows behind the last have no keys)
+          const int at = min(k0 + k, 31), b = b0 + at;
+          const int src = __shfl_sync(0xffffffffu, mine.src, at);
+          n[k] = k0 + k < rows ? __shfl_sync(0xffffffffu, mine.n, at) : 0;
+          len[k] = k0 + k < rows ? __shfl_sync(0xffffffffu, old, at) : 0;
+          page[k] = was[k] = 0;
+          if (i < pages_of(n[k])) page[k] = __ldg(p.block_table + static_cast<size_t>(src) * mp + i);
+          if (i < pages_of(len[k])) was[k] = __ldg(p.block_table + static_cast<size_t>(b) * mp + i);
+        }
+#pragma unroll
+        for (int k = 0; k < kMvAhead; ++k) {
+          const int b = b0 + k0 + k;
+          if (i < pages_of(len[k])) {
+            if (was[k] < 0 || was[k] >= p.num_pages)
+              bad = true;
+            else
+              __stcg(reinterpret_cast<int*>(p.words + was[k]) + 3, 1);
+          }
+          int g = -1;
+          if (i < pages_of(n[k])) {
+            g = page[k];
+            if (g < 0 || g >= p.num_pages) {
+              bad = true;
+              g = -1;
+            } else {
+              int* w = reinterpret_cast<int*>(p.words + g);
+              atomicAdd(w, 1);
+              if ((i + 1) * kPageKeys > n[k]) {
+                atomicAdd(w + 1, 1);
+                atomicMax(w + 2, p.new_batch - b);
+              }
+            }
+          }
+          if (i < mp && k0 + k < rows && b < p.new_batch) p.table_out[static_cast<size_t>(b) * mp + i] = g;
+        }
+      }
     }
   }
   cluster_sync();
@@ -161,9 +185,14 @@ __global__ void __launch_bounds__(kMvThreads) page_fork_kernel(ForkParams p) {
     const int4 w = __ldcg(p.words + g);
     sum.a += w.w != 0 && w.x == 0;
   }
-  for (int b = r0; b < r1; ++b) {
-    int page;
-    sum.b += copy_keys(p, b, new_row(p, b, bad), page) > 0;
+  for (int b = r0; b < r1; ++b) {  // (what this thread finds here it reads again below)
+    const NewRow r = new_row(p, b, bad);
+    int page = -1;
+    const int keys = copy_keys(p, b, r, page);
+    sum.b += keys > 0;
+    p.lens_out[b] = r.n;
+    p.copy_src[b] = keys > 0 ? page : -1;
+    p.copy_keys[b] = keys;
   }
   Pair total;
   Pair at = block_scan(sum, s_warp, &total);
@@ -192,6 +221,7 @@ __global__ void __launch_bounds__(kMvThreads) page_fork_kernel(ForkParams p) {
       if (at.a < p.free_cap - count) __stcg(p.free_pages + count + at.a, g);
       ++at.a;
     }
+    __stcg(p.words + g, make_int4(0, 0, 0, 0));  // for the next call
   }
   count = min(count + total.a, p.free_cap);
   if (ctas > 1)
@@ -201,8 +231,8 @@ __global__ void __launch_bounds__(kMvThreads) page_fork_kernel(ForkParams p) {
 
   // ---- rows: their copies, their last pages, their lengths
   for (int b = r0; b < r1; ++b) {
-    const NewRow r = new_row(p, b, bad);
-    int page = -1, fresh = -1, keys = copy_keys(p, b, r, page), n = r.n;
+    const int keys = p.copy_keys[b];
+    int fresh = -1;
     if (keys > 0) {
       if (at.b < count) {
         fresh = __ldcg(p.free_pages + (count - 1 - at.b));
@@ -212,25 +242,18 @@ __global__ void __launch_bounds__(kMvThreads) page_fork_kernel(ForkParams p) {
         }
       }
       ++at.b;
+      const int n = p.lens_out[b];
       p.table_out[static_cast<size_t>(b) * mp + n / kPageKeys] = fresh;
       if (fresh < 0) {  // no page: the whole pages stay
-        n -= keys;
-        keys = 0;
-        page = -1;
+        p.lens_out[b] = n - keys;
+        p.copy_src[b] = -1;
+        p.copy_keys[b] = 0;
       }
-    } else {
-      page = -1;
     }
-    p.lens_out[b] = n;
-    p.copy_src[b] = page;
     p.copy_dst[b] = fresh;
-    p.copy_keys[b] = keys;
   }
   if (t == 0) *p.free_count_out = count - min(total.b, count);
   if (__syncthreads_or(bad) && threadIdx.x == 0 && p.err) atomicOr(p.err, kErrBadArgs);
-  if (ctas > 1) cluster_sync();
-#pragma unroll 4
-  for (int g = p0; g < p1; ++g) __stcg(p.words + g, make_int4(0, 0, 0, 0));  // for the next call
 }
 
 __global__ void __launch_bounds__(kMvThreads) page_compact_kernel(CompactParams p) {
