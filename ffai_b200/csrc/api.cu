@@ -1884,7 +1884,10 @@ int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t k
     return set_error(ctx, FFAI_ATTN_DECLINED, "chunk: too many rows and keys");
   const int grid = static_cast<int>(std::min<double>(room, most_steps));
   const int teams = tensor ? grid : grid * 4 / (w * r);
-  p.min_share = tensor ? 2 : 16 / w;  // steps: 256 keys of 256 rows, 512 of 16
+  // the least steps of a team: 256 keys of 256 rows, 512 of 16 (none where so many units
+  // rounded up to it would pass 32 bits: a team has more than that anyway)
+  p.min_share = tensor ? 2 : 16 / w;
+  if (units(unit_rows) * p.min_share + most_steps > INT32_MAX) p.min_share = 1;
   std::lock_guard<std::mutex> lock(ctx->space_mutex);
   StreamSpace* space = nullptr;
   int st = stream_space(ctx, stream, &space);

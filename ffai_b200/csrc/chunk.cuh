@@ -80,6 +80,16 @@ struct Stretch {
   int unit0;          // the unit's first step on the line
 };
 
+// Where cu_q falls, sequences may name the same tokens many times, and the line
+// would be longer than the host allowed for: there is nothing to do then.
+__device__ __noinline__ bool repeats_rows(const ChunkParams& p) {
+  long long rows = 0;
+  bool bad = false;
+#pragma unroll 1
+  for (int b = 0; b < p.batch; ++b) rows += chunk_seq(p, b, bad).n;
+  return rows > p.tokens;
+}
+
 // All threads of a CTA: every CTA scans the sequences.  The line is dealt out
 // evenly, min_share steps a team at least.  Where so little is to be done that
 // every unit can begin with a team of its own at that share, it does: most units
@@ -90,10 +100,11 @@ __device__ __forceinline__ void find_stretch(const ChunkParams& p, Stretch* out,
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int per = (p.batch + THREADS - 1) / THREADS;
   const int b0 = min(p.batch, static_cast<int>(threadIdx.x) * per), b1 = min(p.batch, b0 + per);
-  bool bad = false;
+  bool bad = false, falls = false;
   HeadSteps sum{0, 0};
 #pragma unroll 4
   for (int b = b0; b < b1; ++b) {
+    falls |= __ldg(p.cu_q + b) > __ldg(p.cu_q + b + 1);
     const HeadSteps h = head_steps<RU, KEYS>(p, chunk_seq(p, b, bad), G);
     sum.n += p.kv_heads * h.n;
     sum.padded += p.kv_heads * h.padded;
@@ -110,7 +121,7 @@ __device__ __forceinline__ void find_stretch(const ChunkParams& p, Stretch* out,
   }
   if (lane == 31) s_warp[warp] = make_int2(at.n, at.padded);
   if (threadIdx.x < TEAMS) out[threadIdx.x].left = 0;
-  __syncthreads();
+  if (__syncthreads_or(falls) && repeats_rows(p)) return;  // (reported as bad above; all CTAs alike)
   HeadSteps total{0, 0};
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {

@@ -318,8 +318,9 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
  * d->q_len: the most tokens of a sequence, if the host knows it (0: n_tokens);
  * it chooses between kernels and binds nothing.  d->q_offset, kv_len and the
  * k/v layouts are ignored, flags must be 0.  A sequence whose cu_q does not
- * rise or leaves 0 .. n_tokens is skipped, a length outside the table cut, and
- * page ids outside the pool are not read: ffai_attn_sync then reports
+ * rise or leaves 0 .. n_tokens is skipped (all of them, if the others name more
+ * than n_tokens between them), a length outside the table cut, and page ids
+ * outside the pool are not read: ffai_attn_sync then reports
  * FFAI_ATTN_ERR_INVALID.  Streams and captures: as ffai_attn_shared_prefix.
  * No reference counterpart (prompts there run whole, text_decoder.rs:904-923). */
 int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t kv_heads,

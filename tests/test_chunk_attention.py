@@ -347,6 +347,25 @@ def test_bad_tables_are_reported_not_read(what, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 300])
+def test_tokens_named_many_times_are_refused(new):
+    """cu_q that rises and falls over the same tokens: nothing is written."""
+    from ffai_b200 import attention
+    c = build([new] * 9, [100] * 9, 4, 2, torch.bfloat16, seed=6)
+    good = run(c)
+    attention.sync(0)
+    c["cu_q"].copy_(torch.tensor([0, 9 * new] * 5, dtype=torch.int32))
+    out = torch.full_like(good, 7.0)
+    run(c, out=out)
+    with pytest.raises(attention.AttnError):
+        attention.sync(0)
+    assert (out == 7).all()
+    c["cu_q"].copy_(torch.tensor(c["cu"], dtype=torch.int32))
+    assert torch.equal(run(c), good)
+    attention.sync(0)
+
+
+@pytest.mark.gpu
 def test_streams_and_captures_do_not_share_partials():
     """Calls on two streams and two graphs captured on one stream, replayed together."""
     jobs = []
