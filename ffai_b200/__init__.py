@@ -18,6 +18,16 @@ A batched decode step on the device, from page tables to tokens:
                                              plan.free_count)
 
 group_decoder.GroupDecoder chains them around one attention layer.
+
+A step of prompts' chunks and drafted tokens, any mix of them:
+
+    o = chunk_attention.attend(q, k_pool, v_pool, cu_rows, table, plan.lens)
+    v = sampling.verify(logits, tokens, cu_rows, u, u_last, draft_logits=d)
+    f = kvcache.fork_pages(src, plan.lens, table, free_pages, free_count, keep=kept)
+    kvcache.copy_pages(k_pool, v_pool, f.copy_src, f.copy_dst, keys=f.copy_keys)
+    c = kvcache.compact_pages(f.lens, f.block_table, free_pages, f.free_count)
+
+draft_decoder.DraftDecoder chains these.
 """
 
 from . import _abi  # noqa: F401

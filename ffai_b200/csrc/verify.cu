@@ -23,6 +23,11 @@
 // first, and a row behind one that is known to have failed is left out: it
 // cannot matter.  (Which ones are left out depends on timing, the results do not.)
 // In the second launch a cluster per request walks the row of its token again.
+//
+// Bound by instructions, about 20 a logit for the exact weight's two halves, and for
+// few rows by the chain of a row's two passes and exchanges: 96 requests of four drafts
+// with the draft model's logits, 128000 f32: 142 us, the launches 97 and 56 apart (198 MB
+// at least, 30 us); 64 of seven looked-up drafts, 51865 bf16: 43 us; five, f32: 26 us.
 #include <algorithm>
 
 #include "common.cuh"
