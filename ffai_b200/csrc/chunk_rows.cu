@@ -33,8 +33,6 @@
 // merge and uneven ends where they are short (64 requests of up to 8 tokens, 32 / 8
 // heads, up to 2000 keys: 151 MB in 50 us = 3.0 TB/s; a short batch 10 us); by the
 // products with several terms (36 sequences, 28 / 4 heads, f32: 449 us, tensor pipe 45 %).
-#include <algorithm>
-
 #include "chunk.cuh"
 
 namespace ffai {
@@ -348,6 +346,7 @@ __global__ void __launch_bounds__(kCrThreads, TERMS > 1 ? 2 : 3)
   ChunkSeq s{};
   if (w.left > 0) s = chunk_seq(p, w.b, bad);
   uint32_t before = 0;  // steps of the group's ring before this unit
+  bool ok = true;       // no wait ran out; else nothing more is sent for or computed
   while (w.left > 0) {
     // ---- the unit's rows, and the team's n of its steps
     const int row0 = w.m * kRows, rows = min(kRows, s.n * G - row0), end = row0 + rows;
@@ -370,11 +369,11 @@ __global__ void __launch_bounds__(kCrThreads, TERMS > 1 ? 2 : 3)
     int ids = 0, issued = 0;  // lanes hold the pages of 32 steps
 #pragma unroll 1
     for (int i = -kAhead; i < count; ++i) {
-      if (i >= 0) {
+      if (i >= 0 && ok) {
         const uint32_t it = before + i;
         const int at = it % kDepth;
-        mbar_wait(&full[at], (it / kDepth) & 1, &bars.abort_flag, p.err, kErrTimeoutConsumer);
-        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[at], (it / kDepth) & 1, &bars.abort_flag, p.err,
+                                               kErrTimeoutConsumer));
         if (common >= kCrKeys)
           step32<F16, TERMS>(st, q, ring + at * kCrStage, see, false, kCrKeys, kCrKeys, p.scale_log2);
         else
@@ -383,7 +382,7 @@ __global__ void __launch_bounds__(kCrThreads, TERMS > 1 ? 2 : 3)
         __syncwarp();
         if (R > 1) mbar_arrive_w(&empty[at]);
       }
-      if (group == 0 && issued < count) {
+      if (group == 0 && issued < count && ok) {
         if (issued % 32 == 0) {
           ids = issued + lane < count ? __ldg(table + (k0 + (issued + lane) * kKeys) / kPageKeys) : 0;
           if (ids < 0 || ids >= p.num_pages) {  // reported; page 0 is read in its place
@@ -393,8 +392,11 @@ __global__ void __launch_bounds__(kCrThreads, TERMS > 1 ? 2 : 3)
         }
         const uint32_t it = before + issued;
         const int at = it % kDepth, page = __shfl_sync(0xffffffffu, ids, issued % 32);
-        if (R > 1 && it >= kDepth)
-          mbar_wait(&empty[at], ((it / kDepth) - 1) & 1, &bars.abort_flag, p.err, kErrTimeoutProducer);
+        if (R > 1 && it >= kDepth) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[at], ((it / kDepth) - 1) & 1, &bars.abort_flag,
+                                                 p.err, kErrTimeoutProducer));
+          if (!ok) continue;
+        }
         const int half = (k0 + issued * kKeys) % kPageKeys;
         __syncwarp();
         mbar_arrive_expect_tx_w(&full[at], kCrStage);
@@ -402,6 +404,11 @@ __global__ void __launch_bounds__(kCrThreads, TERMS > 1 ? 2 : 3)
         tma_load_3d_w(ring + at * kCrStage + kCrStage / 2, &tmV, &full[at], 0, half, page * p.kv_heads + w.h);
         ++issued;
       }
+    }
+    if (issued > 0 && !ok) {  // every copy lands before its place is used again
+      int none = 0;
+      for (uint32_t st0 = 0, it = before + issued; st0 < kDepth && st0 < it; ++st0)
+        mbar_wait(&full[st0], ((it - 1 - st0) / kDepth) & 1, &none, p.err, kErrTimeoutDrain);
     }
     before += count;
     team_sync<kWarps>(slot);  // the rings are done with: the warps' states take their place
