@@ -33,6 +33,8 @@
 // merge and uneven ends where they are short (64 requests of up to 8 tokens, 32 / 8
 // heads, up to 2000 keys: 151 MB in 50 us = 3.0 TB/s; a short batch 10 us); by the
 // products with several terms (36 sequences, 28 / 4 heads, f32: 449 us, tensor pipe 45 %).
+#include <atomic>
+
 #include "chunk.cuh"
 
 namespace ffai {
@@ -473,13 +475,21 @@ cudaError_t launch_w(const CUtensorMap& tmK, const CUtensorMap& tmV, const Chunk
                      int w, int r, cudaStream_t s) {
   // (64 rows share their keys where the products are many; else two tiles of 16 that
   // read the keys twice take less: 64 x 32 tokens, 32 / 8 heads, 2000 keys 107 and 116 us)
-  auto kern = (TERMS > 1 && r == 4) ? chunk_rows_kernel<F16, TERMS, 1, (TERMS > 1 ? 4 : 1)>
-              : w == 1 ? chunk_rows_kernel<F16, TERMS, 1, 1>
-              : w == 2 ? chunk_rows_kernel<F16, TERMS, 2, 1>
-                       : chunk_rows_kernel<F16, TERMS, 4, 1>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kCrSmem));
+  const int which = TERMS > 1 && r == 4 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 3;
+  auto kern = which == 0   ? chunk_rows_kernel<F16, TERMS, 1, (TERMS > 1 ? 4 : 1)>
+              : which == 1 ? chunk_rows_kernel<F16, TERMS, 1, 1>
+              : which == 2 ? chunk_rows_kernel<F16, TERMS, 2, 1>
+                           : chunk_rows_kernel<F16, TERMS, 4, 1>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  static std::atomic<bool> configured[4][64];
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[which][dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCrSmem));
+    if (e != cudaSuccess) return e;
+    configured[which][dev].store(true, std::memory_order_release);
+  }
   kern<<<grid, kCrThreads, kCrSmem, s>>>(tmK, tmV, p);
   return cudaGetLastError();
 }
