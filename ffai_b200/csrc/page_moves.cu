@@ -26,7 +26,8 @@
 // 60 rows of 7 pages takes 9 us, of 1000 rows of 32 pages in a pool of 13209 18 (22
 // before a warp had four rows' pages on their way); a compaction of 16 rows 9, of 300
 // rows of 32 pages in a pool of 13139 20.  The copies are bound by HBM: 3000 pages of
-// 8 heads, 784 MB read and written, 150 us = 5.2 TB/s; 1000 ends of pages 4.
+// 8 heads, 784 MB read and written, 128 us = 6.1 TB/s (150 before the copies at the
+// front of a list were dealt to all warps); 1000 ends of pages 4.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -386,14 +387,15 @@ __global__ void __launch_bounds__(kMvThreads) page_compact_kernel(CompactParams 
 }
 
 // One warp per (entry, KV head, pool): `keys` rows of a page, contiguous.  A warp
-// looks at `per` items at once, so that entries without a copy cost little.
+// looks at `per` items at once, so that entries without a copy cost little; they lie
+// a grid apart, since those with a copy lie together.
 __global__ void __launch_bounds__(256) kv_copy_keys_kernel(CopyParams p, long long items, int per) {
   const int lane = threadIdx.x % 32;
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x / 32);
   const long long w0 = blockIdx.x * static_cast<long long>(blockDim.x / 32) + threadIdx.x / 32;
-  for (long long base = w0 * per; base < items; base += warps * per) {
+  for (long long base = w0; base < items; base += warps * per) {
     int src = -1, dst = -1, keys = 0, part = 0;
-    const long long item = base + lane;
+    const long long item = base + lane * warps;
     if (lane < per && item < items) {
       part = static_cast<int>(item / p.n);
       const int e = static_cast<int>(item - static_cast<long long>(part) * p.n);
