@@ -11,7 +11,7 @@ without a host round trip:
   3. `kvcache.write_slots`: their keys and values into the page pools;
   4. `chunk_attention.attend`: each row over its request's keys up to its own;
   5. the out-projection with the residual in its epilogue;
-  6. the vocabulary projection of the rows that are judged;
+  6. the vocabulary projection of the rows that are to be verified;
   7. `sampling.verify`: the drafts that stand, and a token behind them;
   8. `kvcache.fork_pages`: the keys of the others are cut off, and pages that
      became empty go back.
@@ -97,7 +97,7 @@ class DraftDecoder:
                                    self.lens, scale=self.scale, max_q=max_rows)
         return linear(o.view(T, -1), self.w_out, residual=x), served
 
-    def judge(self, y, tokens, cu_rows, u, u_last, served, **settings) -> sampling.Verified:
+    def settle(self, y, tokens, cu_rows, u, u_last, served, **settings) -> sampling.Verified:
         """`sampling.verify` (its arguments and settings) on the layer's output
         rows y (R, D) of the last tokens and drafts that the last call of `hidden`
         took in, cu_rows[b] .. cu_rows[b + 1] request b's; the keys of the drafts
@@ -116,16 +116,17 @@ class DraftDecoder:
                                       self.free_count, keep=keep))
         i = torch.arange(tokens.numel(), device=y.device, dtype=torch.int32)
         b = torch.searchsorted(cu_rows[1:], i, right=True).clamp_(max=self.batch - 1)
+        logprobs = None if v.logprobs is None else torch.where(served[b], v.logprobs, 0.0)
         return v._replace(accepted=accepted, next=torch.where(served, v.next, -1),
-                          tokens=torch.where(served[b], v.tokens, -1))
+                          tokens=torch.where(served[b], v.tokens, -1), logprobs=logprobs)
 
     def step(self, x, tokens, cu_rows, u, u_last, *, max_rows: int | None = None,
              **settings) -> sampling.Verified:
         """A step in which every request brings its last token and its drafts
-        (tokens (T,) int32, x their hidden states): `hidden` and `judge` of all
+        (tokens (T,) int32, x their hidden states): `hidden` and `settle` of all
         rows."""
         y, served = self.hidden(x, cu_rows, max_rows=max_rows)
-        return self.judge(y, tokens, cu_rows, u, u_last, served, **settings)
+        return self.settle(y, tokens, cu_rows, u, u_last, served, **settings)
 
     def _take(self, f: kvcache.Fork) -> None:
         self.block_table.copy_(f.block_table)

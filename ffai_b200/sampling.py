@@ -92,7 +92,7 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, u:
            with_logprob: bool = False) -> Verified:
     """Request b has the rows cu_rows[b] .. cu_rows[b + 1] (B + 1, int32): its
     last token and its drafts, `tokens` (T,) int32 being what was fed at each.
-    The draft of row i + 1 is judged by row i's logits (T, V) with u[i] (T,) f32
+    The draft of row i + 1 is weighed by row i's logits (T, V) with u[i] (T,) f32
     in [0, 1): it stands if u q(x) < p(x).  q comes from row i of draft_logits
     (logits' shape and type; default: the drafts were given, q = 1).  Behind the
     last that stands, u_last[b] (B,) picks a token from what p leaves of q, or

@@ -84,13 +84,13 @@ def test_steps_match_a_dense_computation(drafted):
     for step in range(24):
         drafts = [[4, 0, 7, 1, 2, 3], [0, 0, 1, 12, 0, 2], [1] * 6][step % 3]
         if step == 0:  # the prompts, whole
-            ns, judged = prompts, [0] * 6
+            ns, settled = prompts, [0] * 6
         elif step in (5, 11):  # a chunk beside the others' drafts, one sits out
             ns = [d + 1 for d in drafts]
             ns[1], ns[4] = 70, 0
-            judged = [0 if b in (1, 4) else n for b, n in enumerate(ns)]
+            settled = [0 if b in (1, 4) else n for b, n in enumerate(ns)]
         else:
-            ns = judged = [d + 1 for d in drafts]
+            ns = settled = [d + 1 for d in drafts]
         cu, T = starts(ns), sum(ns)
         x = rand(T, D)
         y, served = dec.hidden(x, cu, max_rows=max(ns))
@@ -99,8 +99,8 @@ def test_steps_match_a_dense_computation(drafted):
         new = [(k[a:a + n], v[a:a + n]) for a, n in zip(cu.tolist(), ns)]
         grown = [tuple(torch.cat(p) for p in zip(own[b], new[b])) for b in range(B)]
         check_layer(dec, x, y, cu, grown)
-        rows = torch.cat([torch.arange(a, a + j) for a, j in zip(cu.tolist(), judged)]).to(DEV)
-        R, cj = rows.numel(), starts(judged)
+        rows = torch.cat([torch.arange(a, a + j) for a, j in zip(cu.tolist(), settled)]).to(DEV)
+        R, cj = rows.numel(), starts(settled)
         tokens = torch.randint(0, V, (R,), generator=g, device=DEV, dtype=torch.int32)
         u, u_last = (torch.rand(n, generator=g, device=DEV) for n in (R, B))
         settings = dict(temperature=0.8, draft_temperature=1.1)
@@ -108,14 +108,14 @@ def test_steps_match_a_dense_computation(drafted):
             settings["draft_logits"] = torch.randn(R, V, generator=g, device=DEV)
         else:
             u *= 2e-3  # (a given draft stands where u < p)
-        got = dec.judge(y[rows], tokens, cj, u, u_last, served, **settings)
+        got = dec.settle(y[rows], tokens, cj, u, u_last, served, **settings)
         if R:
             logits = gemm.linear(y[rows], dec.w_vocab, out_dtype=torch.float32)[:, :V]
             want = sampling.verify(logits, tokens, cj, u, u_last, **settings)
             for a, c in zip(got[:3], want[:3]):
                 assert torch.equal(a, torch.where(served, c, -1) if c is want.next else c)
         took += got.accepted.sum().item()
-        for b, (j, a) in enumerate(zip(judged, got.accepted.tolist())):
+        for b, (j, a) in enumerate(zip(settled, got.accepted.tolist())):
             n = grown[b][0].shape[0] - (j - 1 - a if j else 0)
             own[b] = tuple(t[:n] for t in grown[b])
         check_pages(dec, own)
@@ -144,12 +144,14 @@ def test_a_short_pool_refuses_requests_not_others():
     ns = [6, 3, 2, 0, 0, 2]  # the first takes the last page; two find none
     cu, T = starts(ns), sum(ns)
     tokens = torch.zeros(T, dtype=torch.int32, device=DEV)
-    v = dec.step(rand(T, D), tokens, cu, torch.ones(T, device=DEV) * 0.999, torch.zeros(B, device=DEV))
+    v = dec.step(rand(T, D), tokens, cu, torch.ones(T, device=DEV) * 0.999, torch.zeros(B, device=DEV),
+                 with_logprob=True)
     kept = [61, 64, 2, 0, 0, 0]
     assert dec.lens.tolist() == [k + a for k, a in zip(kept, v.accepted.tolist())]
     assert [t >= 0 for t in v.next.tolist()] == [True, False, True, False, False, False]
     rows = [(v.tokens[a:a + n] >= 0).any().item() for a, n in zip(cu.tolist(), ns)]
     assert rows == [True, False, True, False, False, False]
+    assert torch.equal(v.logprobs != 0, v.tokens >= 0)
     # a split needs a copy and finds no page: the whole pages stay
     dec.hidden(rand(66, D), starts([0, 0, 60, 0, 0, 6]))
     whole = dec.select(torch.tensor([2, 1, 2, -1, 1, 1], dtype=torch.int32, device=DEV))
