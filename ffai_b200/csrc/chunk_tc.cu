@@ -386,20 +386,22 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
       mbar_arrive(&bars->q_full[t]);
     }
     const bool active = 16 * c < rows;  // warp-uniform: some row of this warp is real
-    // Keys that this thread's two rows see (rows behind the last see what it does),
-    // counted from the chain's next block; and those that the whole tile sees.
-    const int stride = pair ? kChKeys : 2 * kChKeys;
-    int rel[2], common;
+    // Keys that the tile's first row sees, so the whole tile, counted from the chain's
+    // next block; and how many more this thread's two rows see (rows behind the last see
+    // what it does), in 16 bits each: registers are short.
+    int common;
+    uint32_t more = 0;
     {
-      const int G = p.heads / p.kv_heads, k0 = (walk_first(w) + (pair ? 0 : t)) * kChKeys;
+      const int G = p.heads / p.kv_heads, tok0 = row0 / G;
+      common = (p.causal ? w.s.len - (w.s.n - 1 - tok0) : w.s.len) - (walk_first(w) + (pair ? 0 : t)) * kChKeys;
+      if (p.causal)
 #pragma unroll
-      for (int v = 0; v < 2; ++v)
-        rel[v] = chunk_limit(p, w.s, (row0 + min(16 * c + t1 + 8 * v, rows - 1)) / G) - k0;
-      common = chunk_limit(p, w.s, row0 / G) - k0;
+        for (int v = 0; v < 2; ++v)
+          more |= static_cast<uint32_t>((row0 + min(16 * c + t1 + 8 * v, rows - 1)) / G - tok0) << 16 * v;
     }
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 #pragma unroll 1
-    for (int i = 0; i < cnt; ++i, ++n_s, rel[0] -= stride, rel[1] -= stride, common -= stride) {
+    for (int i = 0; i < cnt; ++i, ++n_s, common -= pair ? kChKeys : 2 * kChKeys) {
       if (!warp_wait(&bars->s_full[t], n_s & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return;
       tc_fence_after();
       if (common < kChKeys) {
@@ -447,7 +449,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
                 const uint32_t o = odd_halves<F16>(x);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                  if (key >= rel[r]) continue;
+                  if (key >= common + static_cast<int>(more >> 16 * r & 0xffffu)) continue;
                   if (o & 0xffffu)
                     o4[2 * r] = __float_as_uint(__uint_as_float(o4[2 * r]) + lo_half(x, F16));
                   if (o >> 16)
@@ -494,6 +496,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
       mbar_arrive(&bars->sc_done[t]);
       float* sf = reinterpret_cast<float*>(sr);
       if (common < kChKeys) {
+        const int rel[2] = {common + static_cast<int>(more & 0xffffu), common + static_cast<int>(more >> 16)};
 #pragma unroll
         for (int k = 0; k < 16; ++k)
 #pragma unroll
@@ -515,9 +518,10 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
       }
       // The reference value of a row moves only when the maximum outgrows it
       // by 2^8: weights stay below 2^8 and most blocks never rescale.
-      if (__any_sync(0xffffffffu, mx[0] * p.scale_log2 > m_run[0] + 8.0f ||
-                                      mx[1] * p.scale_log2 > m_run[1] + 8.0f)) {
-        float corr[2] = {1.f, 1.f};
+      float corr[2] = {1.f, 1.f};
+      const bool moves = __any_sync(0xffffffffu, mx[0] * p.scale_log2 > m_run[0] + 8.0f ||
+                                                     mx[1] * p.scale_log2 > m_run[1] + 8.0f);
+      if (moves) {
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           mx[v] = fmaxf(mx[v], __shfl_xor_sync(0xffffffffu, mx[v], 1));
@@ -529,22 +533,6 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
             m_run[v] = m_new;
             l_run[v] *= corr[v];
           }
-        }
-        if (i > 0) {  // the accumulator so far, once the last product is in it
-          if (!warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
-            return;
-          tc_fence_after();
-#pragma unroll 1
-          for (int h = 0; h < 8; ++h) {
-            uint32_t o4[4];
-            tmem_ld_16x256b_x1(tO + 8 * h, o4);
-            tmem_wait_ld_regs4(o4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              o4[e] = __float_as_uint(__uint_as_float(o4[e]) * corr[e >> 1]);
-            tmem_st_16x256b_x1(tO + 8 * h, o4);
-          }
-          tmem_wait_st();
         }
       }
       // weights in pairs; the sum takes them unrounded, the product in 16 bits
@@ -584,6 +572,21 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
           !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
         return;
       tc_fence_after();
+      // The accumulator so far, which that product was the last to add to: here, where
+      // the scores are no more, since with them the registers did not suffice (2.1 us a
+      // step of 256 rows and 128 keys instead of 1.6).
+      if (moves && i > 0) {
+#pragma unroll 1
+        for (int h = 0; h < 8; ++h) {
+          uint32_t o4[4];
+          tmem_ld_16x256b_x1(tO + 8 * h, o4);
+          tmem_wait_ld_regs4(o4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o4[e] = __float_as_uint(__uint_as_float(o4[e]) * corr[e >> 1]);
+          tmem_st_16x256b_x1(tO + 8 * h, o4);
+        }
+      }
       tmem_st_16x128b_x16(tP, pk);
       tmem_wait_st();
       tc_fence_before();
