@@ -1861,14 +1861,20 @@ int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t k
   // rows kernel.
   p.precise = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32;
   // Rows of a sequence and KV head: the most, or the average if the host has no bound.
-  // Up to 128 the rows kernel serves them, beyond the tensor kernel.  Measured, rows
-  // and tensor kernel: 64 sequences of up to 8 tokens, 32 / 8 heads, 2000 keys 49 and
-  // 94 us, of up to 32 tokens 107 and 113; 4 of 2048 tokens, 20 heads, 267 and 127; 32
-  // single tokens beside four chunks of up to 700, 28 / 4 heads, 6000 keys, 400 and
-  // 160.  (Both kernels, each for its sequences: 152, but it costs long prompts 8 %.)
-  const double most = (d->q_len > 0 ? std::min<double>(d->q_len, n_tokens)
-                                    : static_cast<double>(n_tokens) / d->batch) * G;
-  const bool tensor = !p.precise && most > 128;
+  // Beyond 128 the tensor kernel serves them, and with fewer on average too, unless there
+  // are many pairs of sequence and head: a unit's beginning and end cost it 15 us, the
+  // rows kernel every 16 rows their own pass over the keys.  Measured, rows and tensor
+  // kernel, 32 / 8 heads: 8 sequences of 16 tokens, 300 keys 23 and 25 us, 2000 keys 37
+  // and 31, 20000 keys 211 and 96, of 8 tokens 21 and 25, 31 and 31, 122 and 92; 18 of 16
+  // tokens, 2000 keys 52 and 34; 40 of them 108 and 80; 64 sequences of up to 8 tokens and
+  // 2000 keys 63 and 98, of up to 32 tokens 102 and 110, of up to 48 138 and 124; 4 of
+  // 2048, 20 heads, 439 and 156; 32 single tokens beside four chunks of up to 700, 28 / 4
+  // heads, 6000 keys, 483 and 192.
+  const double average = static_cast<double>(n_tokens) * G / d->batch;
+  const double most = d->q_len > 0 ? std::min<double>(d->q_len, n_tokens) * G : average;
+  const double pairs = static_cast<double>(kv_heads) * std::min(d->batch, n_tokens) / ctx->num_sms;
+  const double enough = 32 + 48 * std::min(std::max((pairs - 1) / 2.5, 0.0), 1.0);
+  const bool tensor = !p.precise && (most > 128 || average > enough);
   // Row groups of a unit: with many products, 64 rows share their keys (28 / 4 heads as
   // above, f32: 466 us against 577).
   const int r = p.precise && most > 32 ? 4 : 1;

@@ -24,9 +24,10 @@
 // it, and the product takes a copy of the block with zeros in its place.
 //
 // Bound by the exponentials, one a score on the 16-lane unit, and the moves between
-// tensor memory and registers around them: two chunks of 8192 tokens behind 24000 keys,
-// 32 / 8 heads, bf16: 1.94 ms, 780 TFLOP/s (the exponentials alone 1.3 ms, the products
-// 0.88).
+// tensor memory and registers around them: chunks of prompts, 32 / 8 heads,
+// bf16: one of 8192 behind 24000 keys 2.53 ms, 748 TFLOP/s, 1.66 us a step of
+// 256 rows and 128 keys (1.07 of it the exponentials, 0.8 the products); one of 8192 behind
+// 3000 and one of 2731 behind 24000 1.59 ms, 655 TFLOP/s.
 //
 // Every wait is bounded (common.cuh); on a timeout the CTA raises an error bit,
 // drains its copies and MMAs, frees tensor memory and exits.
