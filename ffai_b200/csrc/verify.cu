@@ -15,7 +15,8 @@
 //   x stands if  fl(fl(u v_x) W) < fl(w_x V)                        (f64 products)
 //   r_i = max(0, w_i - floor(fl(v_i fl(W / V)))),  R their sum
 //   the token is the first i with r_0 + .. + r_i > floor(fl(u' R)),
-// with w in r's place if R is 0.  T = 0 puts all weight on the first maximum.
+// with w in r's place if R is 0.  T = 0 puts all weight on the first maximum, an
+// infinite T the same on every finite logit.
 //
 // Two launches.  In the first a cluster of CTAs takes a row at a time, of target
 // and draft: the maximum, then the sum of the weights, the logits coming from L1 or
@@ -95,8 +96,10 @@ __device__ __forceinline__ Request request(const VerifyParams& p, int b, bool& b
 __device__ __forceinline__ float inverse(const float* temperature, int b) {
   const float t = temperature ? __ldg(temperature + b) : 1.0f;
   const float inv = t > 0.0f ? __fdiv_rn(1.0f, t) : INFINITY;
-  return isinf(inv) ? 0.0f : inv;  // 0: the first maximum alone
+  return isinf(inv) ? -1.0f : inv;  // (0 is an infinite T's)
 }
+// The first maximum has all weight.
+__device__ __forceinline__ bool greedy(float inv) { return inv < 0.0f; }
 
 // A weight's halves with the magic numbers' bits in them: fma and add towards zero
 // leave the whole part in the low mantissa bits.  e < 1 / 2^36 gives none.
@@ -141,16 +144,16 @@ __device__ __forceinline__ void add_halves(float e0, float e1, uint32_t& hi, uin
 // The distribution of a row: what its weights are relative to.
 struct Dist {
   float xmax, inv;
-  int first;  // index of the first maximum, for inv = 0
+  int first;  // index of the first maximum, if greedy(inv)
   // ordinary: weights are e^d; else all weight lies on some maxima, or there is none
-  __device__ __forceinline__ bool ordinary() const { return inv != 0.0f && !isinf(xmax); }
+  __device__ __forceinline__ bool ordinary() const { return !greedy(inv) && !isinf(xmax); }
   // e^d; what is not a number gives none
   __device__ __forceinline__ float power(float x) const {
     return expf(fmaxf(__fmul_rn(__fadd_rn(x, -xmax), inv), -100.0f));
   }
   __device__ __forceinline__ unsigned long long at(float x, int i) const {
     if (xmax == -INFINITY) return 0;
-    if (inv == 0.0f) return i == first ? 1ull << 36 : 0;
+    if (greedy(inv)) return i == first ? 1ull << 36 : 0;
     return weight(__fmul_rn(delta(clean(x), xmax), inv));
   }
 };
@@ -353,9 +356,9 @@ __device__ __noinline__ void finish_row(const VerifyParams& p, const RowParts& s
 #pragma unroll 1
   for (int which = 0; which < both; ++which) {
     const float inv = job.inv[which], t = top[which];
-    unsigned long long v = inv == 0.0f ? ~0ull : 0;
-    for (int i = lane; i < parts; i += 32) v = inv == 0.0f ? min(v, s.val[which][i]) : v + s.val[which][i];
-    v = inv == 0.0f ? __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(v)) : warp_sum(v);
+    unsigned long long v = greedy(inv) ? ~0ull : 0;
+    for (int i = lane; i < parts; i += 32) v = greedy(inv) ? min(v, s.val[which][i]) : v + s.val[which][i];
+    v = greedy(inv) ? __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(v)) : warp_sum(v);
     double z = 0.0;
     if (!which && p.logprobs) {
       for (int i = lane; i < parts; i += 32) z += __longlong_as_double(s.z[i]);
@@ -364,8 +367,8 @@ __device__ __noinline__ void finish_row(const VerifyParams& p, const RowParts& s
     }
     VerifyRow r;
     r.xmax = t;
-    r.first = inv == 0.0f ? static_cast<int>(v) : 0;
-    r.mass = t == -INFINITY ? 0 : inv == 0.0f ? 1ull << 36 : isinf(t) ? v << 36 : v;
+    r.first = greedy(inv) ? static_cast<int>(v) : 0;
+    r.mass = t == -INFINITY ? 0 : greedy(inv) ? 1ull << 36 : isinf(t) ? v << 36 : v;
     r.log_z = !which && p.logprobs ? static_cast<float>(log(z)) : 0.0f;
     w[which] = token >= 0 ? Dist{t, inv, r.first}.at(at[which], token) : 0;
     mass[which] = r.mass;
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(kVfThreads + 32, 2) verify_rows_kernel(const _
               }
               if (logs) z += x == x ? expf(delta(x, d.xmax)) : 0.0f;
             }
-            v = d.inv == 0.0f ? __reduce_min_sync(0xffffffffu, first) : __reduce_add_sync(0xffffffffu, n);
+            v = greedy(d.inv) ? __reduce_min_sync(0xffffffffu, first) : __reduce_add_sync(0xffffffffu, n);
           }
           tell_all(&s.val[which][part], v, ctas);
           if (logs) {

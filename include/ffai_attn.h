@@ -470,8 +470,8 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
  * drawn from, the token of row i + 1 from row i's; null when the drafts were
  * given (looked up, or a greedy draft's).  With p and q the softmax of a row's
  * logits over the temperatures (DEVICE (batch), null for 1; <= 0, or one whose
- * reciprocal overflows: the first maximum has all), the draft x of row i stands
- * if u[i] q(x) < p(x) (q(x) = 1 without draft_logits); at the first that does
+ * reciprocal overflows: the first maximum has all; infinite: the finite logits
+ * weigh alike), the draft x of row i stands if u[i] q(x) < p(x) (q(x) = 1 without draft_logits); at the first that does
  * not, the token is taken by u_last[b] from max(0, p - q) over its sum, in the
  * order of the vocabulary, or from the last row's p if all stand.  So the
  * tokens are distributed as if the target alone had been sampled, one by one.

@@ -299,3 +299,29 @@ def test_refusals():
     big = torch.zeros(1, 262145, device=DEV)
     with pytest.raises(attention.Declined):
         sampling.verify(big, tok[:1], torch.tensor([0, 1], device=DEV).int(), u[:1], last)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,B", [(31, 5), (1000, 40), (20011, 3)])
+def test_infinite_temperatures_weigh_finite_logits_alike(V, B, dtype):
+    """1 / T is 0 there: as for `sample`, every finite logit has the weight of the largest."""
+    from ffai_b200 import sampling
+    inf = float("inf")
+    for kind in ("normal", "masked"):
+        for with_draft in (True, False):
+            x, y, tokens, cu, u, u_last, _ = build(B, 3, V, 1, dtype, V + B, kind, with_draft)
+            hot = torch.full((B,), inf)
+            mixed = torch.tensor([inf, 1.0, 0.0])[torch.arange(B) % 3]
+            for t, dt in ((hot, hot), (hot, None), (mixed, mixed.flip(0).contiguous()), (torch.ones(B), hot)):
+                r = run(x, y, tokens, cu, u, u_last, t, dt, with_logprob=True)
+                want = reference(x, tokens.tolist(), cu, u, u_last, y, t.tolist(), None if dt is None else dt.tolist())
+                assert (r.accepted.tolist(), r.next.tolist(), r.tokens.tolist()) == want
+    # one row of each kind of logit, many uniform numbers: as often as `sample` takes them
+    row = torch.tensor([0.5, -inf, 9.0, float("nan"), -70.0, 9.0], device=DEV, dtype=dtype)
+    n = 600
+    x, u = row.expand(n, 6).contiguous(), (torch.arange(n) / n + 1e-4).to(DEV)
+    cu = torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    r = sampling.verify(x, torch.zeros(n, dtype=torch.int32, device=DEV), cu, u, u, temperature=inf)
+    got, want = (torch.bincount(v.long(), minlength=6).tolist() for v in (r.next, sampling.sample(x, u, temperature=inf)))
+    assert got == want == [150, 0, 150, 0, 150, 150]
