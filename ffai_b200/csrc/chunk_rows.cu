@@ -25,7 +25,7 @@
 //
 // f32 queries with an f32 output: q and the weights are sums of two f16 or three bf16
 // numbers, the products' terms smallest first, so that what is left of a rounding is
-// 2^-22 or 2^-24: at 28 / 4 heads and 6000 bf16 keys the error is 3.9e-7, that of a
+// 2^-22 or 2^-24 (of a weight in f16 2^-25 of the largest, where that is more): at 28 / 4 heads and 6000 bf16 keys the error is 3.9e-7, that of a
 // plain form in f32 1.3e-6 (two terms of the weights: 1.9e-6, 410 us instead of 449).
 //
 // Bound by HBM where the caches are long (192 units of one token behind up to 30000
@@ -71,13 +71,18 @@ struct RowState {
   float m[2], l[2];
   float o[8][4];
 };
-// The rows as A operands, in TERMS numbers of the cache's type that sum to them.
+// The rows as A operands, in TERMS numbers of the cache's type that sum to them, and
+// what their scores are to be multiplied by (scale log2 e).
 template <int TERMS>
 struct RowQ {
   uint32_t a[TERMS][4][4];
+  float scale_log2[2];
 };
 
-// Rows row0 .. end - 1 of the sequence and KV head (16 at most).
+// Rows row0 .. end - 1 of the sequence and KV head (16 at most).  Two f16 terms hold 22
+// bits of a number only while the second is no subnormal, and nothing above 65504: a row
+// is multiplied by the power of two that brings its largest element to 2^14 .. 2^15, so
+// that what is left of an element is 2^-22 of it, or 2^-39 of the largest.
 template <int TERMS>
 __device__ __forceinline__ void load_rows(RowQ<TERMS>& q, RowState& st, const ChunkParams& p,
                                           const ChunkSeq& s, int kvh, int row0, int end) {
@@ -87,24 +92,46 @@ __device__ __forceinline__ void load_rows(RowQ<TERMS>& q, RowState& st, const Ch
   for (int v = 0; v < 2; ++v) {
     const int row = row0 + g + 8 * v, i = row / G;
     const size_t off = static_cast<size_t>(s.t0 + i) * p.q_st + static_cast<size_t>(kvh * G + row - i * G) * p.q_sh;
+    const auto pair = [&](int k, int x) {  // two head dims of an f32 row
+      return row < end ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off + 16 * k + 8 * x + 2 * t))
+                       : make_float2(0.f, 0.f);
+    };
+    float up = 1.f, down = 1.f;
+    if constexpr (TERMS == 2) {
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float2 y = pair(k, x);
+          most = max3f(most, fabsf(y.x), fabsf(y.y));
+        }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      if (most > 0.f && most < INFINITY) {
+        // (2^100 at most: the scores' factor stays a normal number)
+        const int e = min(14 - (static_cast<int>(__float_as_uint(most) >> 23) - 127), 100);
+        up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      }
+    }
+    q.scale_log2[v] = p.scale_log2 * down;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int dim = 16 * k + 8 * x + 2 * t;
         uint32_t w[TERMS] = {};
-        if (row < end) {
-          if (p.q_dtype == 0) {  // f32 queries are rounded to the cache's type, and what that leaves again
-            float2 y = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + off + dim));
+        if (p.q_dtype == 0) {  // f32 queries are rounded to the cache's type, and what that leaves again
+          float2 y = pair(k, x);
+          y.x *= up, y.y *= up;
 #pragma unroll
-            for (int n = 0; n < TERMS; ++n) {
-              w[n] = f16 ? pack_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
-              y.x -= lo_half(w[n], f16);
-              y.y -= hi_half(w[n], f16);
-            }
-          } else {
-            w[0] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + off + dim));
+          for (int n = 0; n < TERMS; ++n) {
+            w[n] = f16 ? pack_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
+            y.x -= lo_half(w[n], f16);
+            y.y -= hi_half(w[n], f16);
           }
+        } else if (row < end) {
+          w[0] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + off + 16 * k + 8 * x + 2 * t));
         }
 #pragma unroll
         for (int n = 0; n < TERMS; ++n) q.a[n][k][2 * x + v] = w[n];
@@ -152,7 +179,7 @@ __device__ __forceinline__ bool guard_values(RowState& st, const uint8_t* v, con
 // the matrix instruction's sums are cut, not rounded.
 template <int F16, int TERMS>
 __device__ __forceinline__ void step32(RowState& st, const RowQ<TERMS>& q, const uint8_t* buf,
-                                       const int (&see)[2], bool tail, int lo, int hi, float scale_log2) {
+                                       const int (&see)[2], bool tail, int lo, int hi) {
   const int lane = threadIdx.x % 32, t = lane & 3;
   const uint32_t base = smem_u32(buf);
   // matrix m of a load: 8 rows of 16 bytes, lane 8 m + r gives row r's address
@@ -187,12 +214,12 @@ __device__ __forceinline__ void step32(RowState& st, const RowQ<TERMS>& q, const
     mx[r] = max3f(fmaxf(s[0][2 * r], s[0][2 * r + 1]), max3f(s[1][2 * r], s[1][2 * r + 1], s[2][2 * r]),
                   max3f(s[2][2 * r + 1], s[3][2 * r], s[3][2 * r + 1]));
   // The maximum moves at once, so that the largest weight is 1, which has no rounding.
-  if (__any_sync(0xffffffffu, mx[0] * scale_log2 > st.m[0] || mx[1] * scale_log2 > st.m[1])) {
+  if (__any_sync(0xffffffffu, mx[0] * q.scale_log2[0] > st.m[0] || mx[1] * q.scale_log2[1] > st.m[1])) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      const float m_new = mx[r] * scale_log2;
+      const float m_new = mx[r] * q.scale_log2[r];
       if (m_new > st.m[r]) {
         const float corr = ex2_approx(st.m[r] - m_new);
         st.m[r] = m_new;
@@ -212,8 +239,8 @@ __device__ __forceinline__ void step32(RowState& st, const RowQ<TERMS>& q, const
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float p0 = ex2_approx(fmaf(s[i][2 * r], scale_log2, neg));
-      const float p1 = ex2_approx(fmaf(s[i][2 * r + 1], scale_log2, neg));
+      const float p0 = ex2_approx(fmaf(s[i][2 * r], q.scale_log2[r], neg));
+      const float p1 = ex2_approx(fmaf(s[i][2 * r + 1], q.scale_log2[r], neg));
       sum += p0 + p1;
       // the weights enter the second product in the cache's 16-bit type (1 at
       // most, relative error 2^-9 or 2^-12); their sum stays unrounded f32
@@ -377,9 +404,9 @@ __global__ void __launch_bounds__(kCrThreads, TERMS > 1 ? 2 : 3)
         ok = __all_sync(0xffffffffu, mbar_wait(&full[at], (it / kDepth) & 1, &bars.abort_flag, p.err,
                                                kErrTimeoutConsumer));
         if (common >= kCrKeys)
-          step32<F16, TERMS>(st, q, ring + at * kCrStage, see, false, kCrKeys, kCrKeys, p.scale_log2);
+          step32<F16, TERMS>(st, q, ring + at * kCrStage, see, false, kCrKeys, kCrKeys);
         else
-          step32<F16, TERMS>(st, q, ring + at * kCrStage, see, true, max(common, 0), min(live, kCrKeys), p.scale_log2);
+          step32<F16, TERMS>(st, q, ring + at * kCrStage, see, true, max(common, 0), min(live, kCrKeys));
         see[0] -= kKeys, see[1] -= kKeys, common -= kKeys, live -= kKeys;
         __syncwarp();
         if (R > 1) mbar_arrive_w(&empty[at]);
@@ -498,7 +525,7 @@ cudaError_t launch_w(const CUtensorMap& tmK, const CUtensorMap& tmV, const Chunk
 
 cudaError_t launch_chunk_rows(const CUtensorMap& tmK, const CUtensorMap& tmV, const ChunkParams& p,
                               int grid, int w, int r, cudaStream_t s) {
-  // f16: two terms hold 22 of a query's 24 bits, bf16: three hold all
+  // f16: two terms hold 22 of 24 bits, bf16: three hold all
   if (p.kv_dtype == 2)
     return p.precise ? launch_w<1, 2>(tmK, tmV, p, grid, w, r, s) : launch_w<1, 1>(tmK, tmV, p, grid, w, r, s);
   return p.precise ? launch_w<0, 3>(tmK, tmV, p, grid, w, r, s) : launch_w<0, 1>(tmK, tmV, p, grid, w, r, s);

@@ -309,8 +309,10 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
  * q (n_tokens, heads, 64), token_stride as elsewhere, f32 or the cache's type;
  * o (n_tokens, heads, 64) dense, f32, bf16 or f16; layouts TOKEN_MAJOR.  With
  * both f32, queries and softmax weights enter the products as sums of two or
- * three numbers of the cache's type (22 bits of them at least), which costs two
- * to three times the products; else f32 queries are rounded to it.  Pools,
+ * three numbers of the cache's type, which costs two to three times the products:
+ * 24 bits of them in bf16; in f16 what is left of a number is 2^-22 of it, or 2^-39 of
+ * the query row's largest and 2^-25 of the largest weight.  Else f32 queries are
+ * rounded to it (in f16 what is above 65504 is infinite then).  Pools,
  * kv_heads, types, and otherwise the rounding of softmax weights, and values
  * that are not numbers: as ffai_attn_shared_prefix.  lse
  * (optional, f32): (heads, n_tokens).  A row that sees no key gives zeros and

@@ -426,3 +426,35 @@ def test_refusals():
         run(c, out=torch.empty(3, 4, 64, device=DEV)[:2])
     with pytest.raises(TypeError):
         run(c, out_dtype=torch.float64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1e-4, 1.0, 1e5, 1e20])
+@pytest.mark.parametrize("tokens,heads", [(1, 8), (9, 7), (40, 4), (300, 5)])
+def test_f32_queries_of_every_size_and_their_weights(tokens, heads, size, dtype):
+    """Two keys, 0 and e_0, with the values 0 and 1, and queries a e_0 (of another size
+    beside it, which no key meets): o = w / (1 + w), w = e^(scale a), |scale a| <= 2.
+    What a weight loses: its score is off by 2^-22 of it for the query's terms (two in
+    f16), 2 * 2^-23 for the matrix instruction's cut sums, 2^-23 for the scale, 2^-24 for
+    the last sum: 3 * 2^-22 * 2 at most; e^x by 2^-22, the weight's terms by 2^-22 (f16), the
+    sum, the quotient and its rounding by 2^-22 together; one more for what is of second
+    order: 10 * 2^-22.  (A weight in two bf16 terms is off by 2^-17 = 32 * 2^-22.)"""
+    from ffai_b200 import chunk_attention
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    pool = torch.full((2, 1, 64, 64), float("nan"), device=DEV, dtype=dtype)
+    kp, vp = pool.clone(), pool.clone()
+    kp[1, 0, :2], vp[1, 0, :2] = 0, 0
+    kp[1, 0, 1, 0] = 1
+    vp[1, 0, 1] = 1
+    q = torch.zeros(tokens, heads, 64, device=DEV)
+    scale = torch.tensor(0.25 / size).item()
+    q[:, :, 0] = -(torch.rand(tokens, heads, generator=g, device=DEV) * 8 * size)
+    q[:, ::2, 5] = torch.randn(tokens, (heads + 1) // 2, generator=g, device=DEV) * 1000 * size
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    a = q[:, :, 0].double() * torch.tensor(scale, dtype=torch.float32).double().item()
+    want = (torch.exp(a) / (1 + torch.exp(a))).unsqueeze(-1).expand(-1, -1, 64)
+    for max_q in (None, 1, tokens):
+        out = chunk_attention.attend(q, kp, vp, i32(0, tokens), i32(1).view(1, 1), i32(2), scale=scale,
+                                     causal=False, max_q=max_q)
+        assert ((out.double() - want).abs() <= 10 * 2.0 ** -22 * want).all()
