@@ -25,7 +25,7 @@
 //
 // f32 queries with an f32 output: q and the weights are sums of two f16 or three bf16
 // numbers, the products' terms smallest first, so that what is left of a rounding is
-// 2^-22 or 2^-24 (of a weight in f16 2^-25 of the largest, where that is more): at 28 / 4 heads and 6000 bf16 keys the error is 3.9e-7, that of a
+// 2^-22 or 2^-24 (of a weight in f16 2^-40 of the largest, where that is more): at 28 / 4 heads and 6000 bf16 keys the error is 3.9e-7, that of a
 // plain form in f32 1.3e-6 (two terms of the weights: 1.9e-6, 410 us instead of 449).
 //
 // Bound by HBM where the caches are long (192 units of one token behind up to 30000
@@ -213,13 +213,16 @@ __device__ __forceinline__ void step32(RowState& st, const RowQ<TERMS>& q, const
   for (int r = 0; r < 2; ++r)
     mx[r] = max3f(fmaxf(s[0][2 * r], s[0][2 * r + 1]), max3f(s[1][2 * r], s[1][2 * r + 1], s[2][2 * r]),
                   max3f(s[2][2 * r + 1], s[3][2 * r], s[3][2 * r + 1]));
-  // The maximum moves at once, so that the largest weight is 1, which has no rounding.
-  if (__any_sync(0xffffffffu, mx[0] * q.scale_log2[0] > st.m[0] || mx[1] * q.scale_log2[1] > st.m[1])) {
+  // The maximum moves at once, so that the largest weight is 1, which has no rounding; in
+  // f16 it is 2^15, so that none above 2^-29 of it is a subnormal number.
+  constexpr float kLift = F16 ? 15.f : 0.f;
+  if (__any_sync(0xffffffffu, fmaf(mx[0], q.scale_log2[0], -kLift) > st.m[0] ||
+                                  fmaf(mx[1], q.scale_log2[1], -kLift) > st.m[1])) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      const float m_new = mx[r] * q.scale_log2[r];
+      const float m_new = fmaf(mx[r], q.scale_log2[r], -kLift);
       if (m_new > st.m[r]) {
         const float corr = ex2_approx(st.m[r] - m_new);
         st.m[r] = m_new;
@@ -242,8 +245,9 @@ __device__ __forceinline__ void step32(RowState& st, const RowQ<TERMS>& q, const
       const float p0 = ex2_approx(fmaf(s[i][2 * r], q.scale_log2[r], neg));
       const float p1 = ex2_approx(fmaf(s[i][2 * r + 1], q.scale_log2[r], neg));
       sum += p0 + p1;
-      // the weights enter the second product in the cache's 16-bit type (1 at
-      // most, relative error 2^-9 or 2^-12); their sum stays unrounded f32
+      // the weights enter the second product in the cache's 16-bit type (off by
+      // 2^-8 or 2^-11 of them at most, in f16 by 2^-40 of the largest where that is
+      // more); their sum stays unrounded f32
       const uint32_t w = F16 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
       p[i >> 1][(i & 1) * 2 + r] = w;
       if constexpr (TERMS > 1) {

@@ -517,26 +517,29 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
         }
         mx[v] = fmaxf(a, b);
       }
-      // The reference value of a row moves only when the maximum outgrows it
-      // by 2^8: weights stay below 2^8 and most blocks never rescale.
+      // The reference value of a row moves only when the maximum outgrows it by 2^8, so
+      // that most blocks never rescale.  Weights stay below 2^8; in f16 below 2^15, and
+      // the largest is 2^6 at least, so that none above 2^-20 of it is a subnormal number.
+      constexpr float kLift = F16 ? 7.f : 0.f, kLag = 8.f + kLift;
       float corr[2] = {1.f, 1.f};
-      const bool moves = __any_sync(0xffffffffu, mx[0] * p.scale_log2 > m_run[0] + 8.0f ||
-                                                     mx[1] * p.scale_log2 > m_run[1] + 8.0f);
+      const bool moves = __any_sync(0xffffffffu, mx[0] * p.scale_log2 > m_run[0] + kLag ||
+                                                     mx[1] * p.scale_log2 > m_run[1] + kLag);
       if (moves) {
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           mx[v] = fmaxf(mx[v], __shfl_xor_sync(0xffffffffu, mx[v], 1));
           mx[v] = fmaxf(mx[v], __shfl_xor_sync(0xffffffffu, mx[v], 2));
           const float m_blk = mx[v] * p.scale_log2;
-          if (m_blk > m_run[v] + 8.0f) {
-            const float m_new = ceilf(m_blk);
+          if (m_blk > m_run[v] + kLag) {
+            const float m_new = ceilf(m_blk) - kLift;
             corr[v] = ex2_approx(m_run[v] - m_new);
             m_run[v] = m_new;
             l_run[v] *= corr[v];
           }
         }
       }
-      // weights in pairs; the sum takes them unrounded, the product in 16 bits
+      // weights in pairs; the sum takes them unrounded, the product in 16 bits (off by
+      // 2^-8 or 2^-11 of them, in f16 by 2^-31 of the largest where that is more)
       uint32_t pk[32];
       {
         const uint64_t c2 = f2_pack(p.scale_log2, p.scale_log2);

@@ -311,7 +311,7 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
  * both f32, queries and softmax weights enter the products as sums of two or
  * three numbers of the cache's type, which costs two to three times the products:
  * 24 bits of them in bf16; in f16 what is left of a number is 2^-22 of it, or 2^-39 of
- * the query row's largest and 2^-25 of the largest weight.  Else f32 queries are
+ * the query row's largest and 2^-40 of the largest weight.  Else f32 queries are
  * rounded to it (in f16 what is above 65504 is infinite then).  Pools,
  * kv_heads, types, and otherwise the rounding of softmax weights, and values
  * that are not numbers: as ffai_attn_shared_prefix.  lse

@@ -438,8 +438,9 @@ def test_f32_queries_of_every_size_and_their_weights(tokens, heads, size, dtype)
     What a weight loses: its score is off by 2^-22 of it for the query's terms (two in
     f16), 2 * 2^-23 for the matrix instruction's cut sums, 2^-23 for the scale, 2^-24 for
     the last sum: 3 * 2^-22 * 2 at most; e^x by 2^-22, the weight's terms by 2^-22 (f16), the
-    sum, the quotient and its rounding by 2^-22 together; one more for what is of second
-    order: 10 * 2^-22.  (A weight in two bf16 terms is off by 2^-17 = 32 * 2^-22.)"""
+    sum, the quotient and its rounding by 2^-22 together; its exponent, which is 15 more
+    than the score in f16, by 2^-21 ln 2; half a step for what is of second order:
+    11 * 2^-22.  (A weight in two bf16 terms is off by 2^-17 = 32 * 2^-22.)"""
     from ffai_b200 import chunk_attention
     g = torch.Generator(device=DEV).manual_seed(tokens)
     pool = torch.full((2, 1, 64, 64), float("nan"), device=DEV, dtype=dtype)
@@ -457,4 +458,35 @@ def test_f32_queries_of_every_size_and_their_weights(tokens, heads, size, dtype)
     for max_q in (None, 1, tokens):
         out = chunk_attention.attend(q, kp, vp, i32(0, tokens), i32(1).view(1, 1), i32(2), scale=scale,
                                      causal=False, max_q=max_q)
-        assert ((out.double() - want).abs() <= 10 * 2.0 ** -22 * want).all()
+        assert ((out.double() - want).abs() <= 11 * 2.0 ** -22 * want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("below", [12.0, 25.6])
+def test_many_small_weights_beside_a_large_one(below, dtype):
+    """One key of weight 1 and value 0 before 7999 of weight 2^-below and value 1, which
+    are rounded alike: o = n w / (1 + n w).  A weight is off by u of it (u = 2^-8, 2^-11; three
+    and two terms of f32 queries: 2^-22), in f16 by what half a subnormal step is of the
+    largest, 2^-25 / 2^15, or 2^-25 / 2^6 in the kernel for many rows; scores, sums and the
+    rest are f32, of 1e-5 together.  Many sequences, so that few are split."""
+    from ffai_b200 import chunk_attention
+    B, kv, n = 120, 8, 8000
+    kp = torch.zeros(125, kv, 64, 64, device=DEV, dtype=dtype)
+    vp = torch.ones_like(kp)
+    kp[:, :, :, 0], kp[0, :, 0], vp[0, :, 0] = 1, 0, 0
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    table, lens, cu = i32(torch.arange(125)).repeat(B, 1), i32([n] * B), i32(torch.arange(B + 1))
+    scale = torch.tensor(below * 0.6931471805599453 / 16).item()
+    w = torch.exp(torch.tensor(-16 * scale).double()).item()
+    want = (n - 1) * w / (1 + (n - 1) * w)
+    for q_dtype in (dtype, torch.float32):
+        q = torch.zeros(B, 2 * kv, 64, device=DEV, dtype=q_dtype)
+        q[:, :, 0] = -16
+        for max_q in (1, B):
+            out = chunk_attention.attend(q, kp, vp, cu, table, lens, scale=scale, max_q=max_q, out_dtype=torch.float32)
+            exact = q_dtype is torch.float32
+            u = 2.0 ** -22 if exact else U[dtype]
+            floor = 0 if dtype is torch.bfloat16 else 2.0 ** -31 if max_q > 1 and not exact else 2.0 ** -40
+            err = (out.double() - want).abs().max().item()
+            assert err <= (u + 1e-5) * want + n * floor, (q_dtype, max_q, err / want)
