@@ -30,7 +30,8 @@
 // 3000 and one of 2731 behind 24000 1.59 ms, 655 TFLOP/s.
 //
 // Every wait is bounded (common.cuh); on a timeout the CTA raises an error bit,
-// drains its copies and MMAs, frees tensor memory and exits.
+// drains its copies and MMAs, takes the tickets it has not come to, frees tensor
+// memory and exits.
 #include <atomic>
 
 #include "chunk.cuh"
@@ -95,6 +96,29 @@ __device__ __forceinline__ void walk_next(Walk& w, const ChunkParams& p) {
     }
   }
   walk_unit(w, p);
+}
+
+// The first and the last CTA that have a part of the unit; it is one's whole where they
+// are the same.  Else each takes a ticket for each of its tiles (one chain's, if there is
+// one tile), and the last to take it merges the parts.
+struct UnitTeams {
+  int c0, c1;
+};
+__device__ __forceinline__ UnitTeams walk_teams(const Walk& w, int share) {
+  return {w.unit0 / share, min((w.unit0 + w.steps - 1) / share, static_cast<int>(gridDim.x) - 1)};
+}
+__device__ __forceinline__ bool walk_whole(const Walk& w) { return walk_steps(w) == w.steps; }
+__device__ __forceinline__ bool take_ticket(const ChunkParams& p, const Walk& w, const UnitTeams& u, int t) {
+  const unsigned n = static_cast<unsigned>(u.c1 - u.c0);
+  return atomicInc(p.tickets + 2 * u.c0 + (walk_pair(w) ? t : 0), n) == n;
+}
+// A wait of chain t ran out: one of its threads takes the tickets that it has not come
+// to (not the current unit's, if `taken`), since those of the other CTAs would stay in
+// the words and mislead the calls behind this one.  (Whoever is the last now merges what
+// this CTA never wrote: the call is reported.)
+__device__ __noinline__ void take_the_rest(const ChunkParams& p, Walk& w, int share, int t, bool taken) {
+  for (; w.left > 0; walk_next(w, p), taken = false)
+    if (!taken && !walk_whole(w) && (walk_pair(w) || t == 0)) take_ticket(p, w, walk_teams(w, share), t);
 }
 
 struct __align__(8) CtBars {
@@ -349,8 +373,9 @@ __device__ __forceinline__ bool chain_sync(uint64_t* bar, uint32_t& n, volatile 
   return warp_wait(bar, n++ & 1, abort_flag, err, kErrTimeoutSoftmax);
 }
 
+// Where a wait runs out it returns at once: whether the current unit's ticket is taken.
 template <int F16>
-__device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) {
+__device__ __forceinline__ bool ct_softmax(const ChunkParams& p, uint32_t tmem) {
   CtBars* bars = CT_BARS;
   uint8_t* sQ = ct_smem;
   uint8_t* sV = ct_smem + kCtOffV;
@@ -403,7 +428,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 #pragma unroll 1
     for (int i = 0; i < cnt; ++i, ++n_s, common -= pair ? kChKeys : 2 * kChKeys) {
-      if (!warp_wait(&bars->s_full[t], n_s & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return;
+      if (!warp_wait(&bars->s_full[t], n_s & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return false;
       tc_fence_after();
       if (common < kChKeys) {
         // Some row of the tile does not see some key of this block.  Value rows
@@ -415,14 +440,14 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
         const int lo = max(0, min(common, live));
         if (!warp_wait(&bars->v_full[st], (it / kCtStages) & 1, abort_flag, p.err,
                        kErrTimeoutSoftmax))
-          return;
+          return false;
         uint4* v = reinterpret_cast<uint4*>(sV + st * kCtTile);
         for (int k = live * 8 + (threadIdx.x & 255); k < kChKeys * 8; k += 256)
           v[k] = make_uint4(0, 0, 0, 0);
         // the last product is done with the chain's copy, flags and accumulator
         if (n_s > 0 &&
             !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
-          return;
+          return false;
         bool odd = false;
         for (int k = lo * 8 + (threadIdx.x & 255); k < live * 8; k += 256) {
           const uint4 x = v[k];
@@ -430,7 +455,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
                         odd_halves<F16>(x.w));
         }
         if (odd) bars->odd[t] = static_cast<int>(n_s) + 1;
-        if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return;
+        if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return false;
         const bool fix = *static_cast<volatile int*>(&bars->odd[t]) == static_cast<int>(n_s) + 1;
         if (fix) {
           tc_fence_after();
@@ -461,7 +486,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
             }
             tmem_wait_st();
           }
-          if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return;
+          if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return false;
           // zeros in their places: in a copy if the other chain reads the block too
           uint4* to = pair ? reinterpret_cast<uint4*>(ct_smem + kCtOffCopy + t * kCtTile) : v;
           for (int k = threadIdx.x & 255; k < kChKeys * 8; k += 256) {
@@ -486,7 +511,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
         // the previous product must have left P before it is declared full again
         if (n_s > 0 &&
             !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
-          return;
+          return false;
         mbar_arrive(&bars->p_full[t]);
         continue;
       }
@@ -574,7 +599,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
       // P is free once the previous product has read it
       if (n_s > 0 &&
           !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
-        return;
+        return false;
       tc_fence_after();
       // The accumulator so far, which that product was the last to add to: here, where
       // the scores are no more, since with them the registers did not suffice (2.1 us a
@@ -599,7 +624,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
 
     // ---- end of the unit's stretch
     if (any && !warp_wait(&bars->o_done[t], (n_s - 1) & 1, abort_flag, p.err, kErrTimeoutSoftmax))
-      return;
+      return false;
     tc_fence_after();
     if (any && (threadIdx.x & 255) == 0) bars->copy[t] = bars->keep[t] = 0;  // (seen by the next unit's p_full)
     if (active) {
@@ -615,7 +640,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
     if (!pair && t == 1) {
       if (w.alt >= 1 && !warp_wait(&bars->mrg_empty[c], (w.alt - 1) & 1, abort_flag, p.err,
                                    kErrTimeoutSoftmax))
-        return;
+        return false;
       if (active) {
         if (any) {
 #pragma unroll 1
@@ -639,7 +664,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
     } else {
       float f0[2] = {1.f, 1.f}, f1[2] = {0.f, 0.f};
       if (!pair) {
-        if (!warp_wait(&bars->mrg_full[c], w.alt & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return;
+        if (!warp_wait(&bars->mrg_full[c], w.alt & 1, abort_flag, p.err, kErrTimeoutSoftmax)) return false;
         if (active) {
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
@@ -656,11 +681,10 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
         }
       }
       const int G = p.heads / p.kv_heads;
-      const bool whole = walk_steps(w) == w.steps;
-      const int share = bars->share;
-      const int c0 = w.unit0 / share, c1 = min((w.unit0 + w.steps - 1) / share, static_cast<int>(gridDim.x) - 1);
+      const bool whole = walk_whole(w);
+      const UnitTeams teams = walk_teams(w, bars->share);
       const int cta = static_cast<int>(blockIdx.x);
-      const UnitParts u{c0, c1, kPxRows, pair ? 128 * t : 0, row0, rows, w.s.t0, w.h};
+      const UnitParts u{teams.c0, teams.c1, kPxRows, pair ? 128 * t : 0, row0, rows, w.s.t0, w.h};
       if (active) {
         float inv[2];
         size_t at[2];
@@ -720,20 +744,19 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
       if (!whole) {
         // ---- the last of the unit's CTAs merges the parts of this tile, in their order
         __threadfence();
-        if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return;
+        if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return false;
         if ((threadIdx.x & 255) == 0) {
-          const unsigned n = static_cast<unsigned>(c1 - c0);
-          bars->last[t] = atomicInc(p.tickets + 2 * c0 + (pair ? t : 0), n) == n;
+          bars->last[t] = take_ticket(p, w, teams, t);
           __threadfence();
         }
-        if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return;
+        if (!chain_sync(&bars->sync[t], n_sync, abort_flag, p.err)) return true;
         if (*static_cast<volatile int*>(&bars->last[t])) {
           const int part = threadIdx.x & 7;
 #pragma unroll 1
           for (int r = (threadIdx.x & 255) >> 3; r < rows; r += 32) {
             Merged acc{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 2
-            for (int x = c0; x <= c1; ++x) {
+            for (int x = teams.c0; x <= teams.c1; ++x) {
               const size_t from = part_row(u, x, r);
               const float4* o = reinterpret_cast<const float4*>(p.part_o + from * 64 + 8 * part);
               acc.add(__ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * from)), __ldcg(o), __ldcg(o + 1));
@@ -748,6 +771,7 @@ __device__ __forceinline__ void ct_softmax(const ChunkParams& p, uint32_t tmem) 
     if (lane == 0) walk_next(w, p);
     __syncwarp();
   }
+  return false;
 }
 
 template <int F16>
@@ -823,7 +847,9 @@ __global__ void __launch_bounds__(kCtThreads, 1)
     mma_commit_w(&bars->drain);
     mbar_wait(&bars->drain, 0, &none, p.err, kErrTimeoutDrain);
   } else {
-    ct_softmax<F16>(p, tmem);
+    const bool taken = ct_softmax<F16>(p, tmem);
+    if ((threadIdx.x & 255) == 0)
+      take_the_rest(p, *(reinterpret_cast<Walk*>(ct_smem + kCtOffWalks) + warp), bars->share, warp / 8, taken);
   }
   __syncwarp();
   tc_fence_before();
