@@ -288,13 +288,13 @@ __device__ __forceinline__ void px_producer(const CUtensorMap* tmK, const CUtens
     }
     walk_next(w, p);
   }
-  if (!ok || *abort_flag) {  // every copy lands before the CTA exits
-    int none = 0;
-    for (uint32_t s = 0; s < static_cast<uint32_t>(kPxStages) && s < it; ++s) {
-      const uint32_t arms = (it - 1 - s) / kPxStages + 1;
-      mbar_wait(&bars->k_full[s], (arms - 1) & 1, &none, p.err, kErrTimeoutDrain);
-      mbar_wait(&bars->v_full[s], (arms - 1) & 1, &none, p.err, kErrTimeoutDrain);
-    }
+  // Every copy lands before the CTA exits, whether a wait has run out by now, will
+  // run out yet, or none does.
+  int none = 0;
+  for (uint32_t s = 0; s < static_cast<uint32_t>(kPxStages) && s < it; ++s) {
+    const uint32_t arms = (it - 1 - s) / kPxStages + 1;
+    mbar_wait(&bars->k_full[s], (arms - 1) & 1, &none, p.err, kErrTimeoutDrain);
+    mbar_wait(&bars->v_full[s], (arms - 1) & 1, &none, p.err, kErrTimeoutDrain);
   }
 }
 

@@ -174,6 +174,30 @@ int tickets(std::mt19937& g, bool rest) {
   return left;
 }
 
+// The producer of every CTA, where nothing has gone wrong yet when it has sent its last
+// copies: it has waited for the last one into each place all the same.
+int copies_in_flight(std::mt19937& g) {
+  int flying = 0;
+  for (int round = 0; round < 5; ++round) {
+    Problem a;
+    gridDim.x = 1 + g() % 20;
+    make(a, g, gridDim.x);
+    for (blockIdx.x = 0; blockIdx.x < gridDim.x; ++blockIdx.x) {
+      Stretch x{};
+      int2 s_warp[2];
+      fills.clear();
+      as_warp([&] {
+        find_stretch<kPxRows, kChKeys, 32, 1>(a.p, &x, s_warp);
+        if (threadIdx.x == 0) CT_BARS->start = start_of(a.p, x);
+        __syncthreads();
+        ct_producer(nullptr, nullptr, a.p);
+      });
+      for (const auto& [bar, f] : fills) flying += f.sent > 0 && f.awaited != (f.sent - 1) % 2;
+    }
+  }
+  return flying;
+}
+
 }  // namespace
 }  // namespace ffai
 
@@ -181,4 +205,5 @@ int main() {
   std::mt19937 g(1);
   if (const int n = ffai::tickets(g, true)) printf("%d words are above zero\n", n);
   if (!ffai::tickets(g, false)) printf("nothing is left in the words by CTAs that take no tickets on their way out\n");
+  if (const int n = ffai::copies_in_flight(g)) printf("%d copies may be in flight when their CTA exits\n", n);
 }
