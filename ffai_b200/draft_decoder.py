@@ -136,12 +136,15 @@ class DraftDecoder:
     def select(self, src):
         """Request b continues request src[b] (batch, int32; -1: it ends), sharing
         its pages.  Returns (batch,) bool: false where no page was left for the
-        copy of a last one, and the request was cut back to whole pages."""
-        old = self.lens[src.clamp(min=0)]
+        copy of a last one, and the request was cut back to whole pages, or where
+        src[b] is no request (b is empty then; `attention.sync` reports it)."""
+        if src.shape != self.rows.shape:
+            raise ValueError(f"draft decoder: src must be ({self.batch},)")
+        old = self.lens[src.clamp(0, self.batch - 1)]
         f = kvcache.fork_pages(src, self.lens, self.block_table, self.free_pages, self.free_count)
         kvcache.copy_pages(self.k_pool, self.v_pool, f.copy_src, f.copy_dst, keys=f.copy_keys)
         self._take(f)
-        return (src < 0) | (f.lens == old)
+        return (src < 0) | (src < self.batch) & (f.lens == old)
 
     def compact(self) -> None:
         """The pages in use move to the front of the pools, in order."""

@@ -209,3 +209,46 @@ def test_refusals():
               (dec.w_qkv, dec.w_out, dec.w_vocab[:, :64])):
         with pytest.raises(ValueError):
             DraftDecoder(*w, heads=H, kv_heads=HK, batch=B, max_len=64, num_pages=6)
+
+
+def on_the_host():
+    """A decoder whose tensors lie on the host; its operators are the caller's to replace."""
+    from ffai_b200.draft_decoder import DraftDecoder
+    w = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    return DraftDecoder(w((H + 2 * HK) * 64, D), w(D, H * 64), w(V, D), heads=H, kv_heads=HK, batch=B,
+                        max_len=128, num_pages=12)
+
+
+def test_a_selection_of_no_request_is_not_looked_up(monkeypatch):
+    """An index past the batch would end the process on a device."""
+    from ffai_b200 import kvcache
+    dec = on_the_host()
+    dec.lens.copy_(torch.arange(B, dtype=torch.int32) + 10)
+
+    def fork(src, lens, table, free_pages, free_count, keep=None):
+        real = (src >= 0) & (src < B)
+        return kvcache.Fork(table, torch.where(real, lens[src.clamp(0, B - 1)], 0), None, None, None, free_count)
+
+    monkeypatch.setattr(kvcache, "fork_pages", fork)
+    monkeypatch.setattr(kvcache, "copy_pages", lambda *a, **k: None)
+    for src in ([0, B, 2 ** 31 - 1, -5, 1, 1], [B] * B):
+        whole = dec.select(torch.tensor(src, dtype=torch.int32))
+        assert whole.tolist() == [s < B for s in src]
+    lens = dec.lens.clone()
+    for n in (B - 1, B + 1):
+        with pytest.raises(ValueError):
+            dec.select(torch.zeros(n, dtype=torch.int32))
+    assert torch.equal(dec.lens, lens)
+
+
+@pytest.mark.gpu
+def test_a_selection_of_no_request_is_reported():
+    from ffai_b200 import attention
+    dec, rand, _ = make()
+    dec.hidden(rand(110, D), starts([10, 70, 0, 30, 0, 0]))
+    whole = dec.select(torch.tensor([1, B, 2 ** 31 - 1, 3, -1, 0], dtype=torch.int32, device=DEV))
+    assert whole.tolist() == [True, False, False, True, True, True]
+    assert dec.lens.tolist() == [70, 0, 0, 30, 0, 10]
+    with pytest.raises(attention.AttnError):
+        attention.sync(0)
+    attention.sync(0)
