@@ -76,7 +76,7 @@ class DraftDecoder:
         (batch + 1, int32), whose keys and values are kept: (x + attention's
         output, served (batch,)), served[b] false for requests that brought
         nothing or found no page (nothing of them is kept).  Rows of those, and
-        behind the last request, hold nothing of use.  max_rows: the most rows of
+        before the first or behind the last request, hold nothing of use.  max_rows: the most rows of
         a request, if known."""
         T = x.shape[0]
         q, k, v = self._project(x)
@@ -88,7 +88,7 @@ class DraftDecoder:
         i = torch.arange(T, device=x.device, dtype=torch.int32)
         b = torch.searchsorted(cu_rows[1:], i, right=True).clamp_(max=self.batch - 1)
         at = plan.cu_new[b] + i - cu_rows[b]
-        here = served[b] & (i < cu_rows[-1])
+        here = served[b] & (i >= cu_rows[0]) & (i < cu_rows[-1])
         slots = torch.where(here, plan.slots[at.clamp_(0, max(T - 1, 0))], -1)
         self.lens.copy_(plan.lens)
         self.free_count.copy_(plan.free_count)

@@ -252,3 +252,36 @@ def test_a_selection_of_no_request_is_reported():
     with pytest.raises(attention.AttnError):
         attention.sync(0)
     attention.sync(0)
+
+
+def test_rows_outside_every_request_get_no_slot(monkeypatch):
+    """Rows before the first request and behind the last are nobody's: their keys go nowhere."""
+    from ffai_b200 import chunk_attention, draft_decoder, kvcache
+    dec, written = on_the_host(), []
+    monkeypatch.setattr(draft_decoder, "linear", lambda x, w, **k: torch.zeros(x.shape[0], w.shape[0], dtype=x.dtype))
+    monkeypatch.setattr(kvcache, "plan_pages", lambda lens, n, pages, count, table, slot_cap: kvcache.PagePlan(
+        lens=lens + n, cu_new=torch.cat([n.new_zeros(1), n.cumsum(0, dtype=torch.int32)]),
+        slots=torch.arange(100, 100 + slot_cap, dtype=torch.int32), positions=None, free_count=count))
+    monkeypatch.setattr(kvcache, "write_slots", lambda kp, vp, k, v, slots: written.append(slots.tolist()))
+    monkeypatch.setattr(chunk_attention, "attend", lambda q, *a, **k: torch.zeros(q.shape, dtype=q.dtype))
+    for first, last in ((0, 0), (3, 0), (0, 2), (5, 4)):
+        cu = torch.tensor([0, 2, 2, 3, 7, 8, 9], dtype=torch.int32) + first
+        T = first + 9 + last
+        _, served = dec.hidden(torch.zeros(T, D, dtype=torch.bfloat16), cu)
+        assert served.tolist() == [True, False, True, True, True, True]
+        assert written.pop() == [-1] * first + list(range(100, 109)) + [-1] * last
+
+
+@pytest.mark.gpu
+def test_rows_before_the_first_request_change_nothing():
+    from ffai_b200 import attention
+    dec, rand, _ = make(seed=1)
+    ns, first = [30, 70, 1, 0, 64, 5], 3
+    x, cu = rand(first + sum(ns) + 4, D), starts(ns) + first
+    y, served = dec.hidden(x, cu)
+    assert served.tolist() == [n > 0 for n in ns]
+    k, v = dec._project(x)[1:]
+    own = [(k[a:a + n], v[a:a + n]) for a, n in zip(cu.tolist(), ns)]
+    check_pages(dec, own)
+    check_layer(dec, x, y, cu, own)
+    attention.sync(0)
