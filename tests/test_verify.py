@@ -325,3 +325,25 @@ def test_infinite_temperatures_weigh_finite_logits_alike(V, B, dtype):
     r = sampling.verify(x, torch.zeros(n, dtype=torch.int32, device=DEV), cu, u, u, temperature=inf)
     got, want = (torch.bincount(v.long(), minlength=6).tolist() for v in (r.next, sampling.sample(x, u, temperature=inf)))
     assert got == want == [150, 0, 150, 0, 150, 150]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_one_long_request_among_many_without_drafts(with_draft):
+    """Far more places than rows: 3000 requests, most without a row, one with 60."""
+    g = torch.Generator().manual_seed(4)
+    rows = (torch.rand(3000, generator=g) < 0.1).int().tolist()
+    rows[1234], rows[7], rows[2999] = 60, 9, 5
+    cu = [0]
+    for n in rows:
+        cu.append(cu[-1] + n)
+    T, V = cu[-1], 40
+    x = torch.randn(T, V, generator=g).to(DEV)
+    y = x + 0.05 * torch.randn(T, V, generator=g).to(DEV) if with_draft else None
+    best = x.argmax(1).cpu()
+    tokens = torch.cat([best[:1], best[:-1]]).to(torch.int32)
+    u, u_last = torch.rand(T, generator=g) * (1 if with_draft else 0.1), torch.rand(3000, generator=g)
+    r = run(x, y, tokens, cu, u, u_last, None)
+    want = reference(x, tokens.tolist(), cu, u, u_last, y)
+    assert (r.accepted.tolist(), r.next.tolist(), r.tokens.tolist()) == want
+    assert max(want[0]) >= 5
