@@ -32,8 +32,8 @@ def attend(q, k_pool, v_pool, cu_q, block_table, seq_lens, *, scale: float = 1.0
            causal: bool = True, max_q: int | None = None, out_dtype=None, with_lse=False, out=None):
     """q (T, H, 64), possibly a view of a fused projection; cu_q (B + 1,),
     block_table (B, pages), seq_lens (B,) int32 on the device, seq_lens with the
-    new tokens.  max_q: the most tokens of a sequence, if known (it chooses the
-    kernel).  Returns out (T, H, 64) of out_dtype (default: q's) [, lse f32
+    new tokens.  max_q: the most tokens of a sequence, if known (it helps
+    to choose the kernel, one for all of them).  Returns out (T, H, 64) of out_dtype (default: q's) [, lse f32
     (H, T)]; rows outside every sequence are left as they are in `out`."""
     if not q.is_cuda:
         raise ValueError("operands must be CUDA tensors")

@@ -1861,7 +1861,7 @@ int ffai_attn_chunk_paged(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t k
   // rows kernel.
   p.precise = d->q_dtype == FFAI_DT_F32 && d->out_dtype == FFAI_DT_F32;
   // Rows of a sequence and KV head: the most, or the average if the host has no bound.
-  // Beyond 128 the tensor kernel serves them, and with fewer on average too, unless there
+  // Beyond 128 the tensor kernel serves them all, and with fewer on average too, unless there
   // are many pairs of sequence and head: a unit's beginning and end cost it 15 us, the
   // rows kernel every 16 rows their own pass over the keys.  Measured, rows and tensor
   // kernel, 32 / 8 heads: 8 sequences of 16 tokens, 300 keys 23 and 25 us, 2000 keys 37

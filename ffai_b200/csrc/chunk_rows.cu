@@ -25,14 +25,17 @@
 //
 // f32 queries with an f32 output: q and the weights are sums of two f16 or three bf16
 // numbers, the products' terms smallest first, so that what is left of a rounding is
-// 2^-22 or 2^-24 (of a weight in f16 2^-40 of the largest, where that is more): at 28 / 4 heads and 6000 bf16 keys the error is 3.9e-7, that of a
-// plain form in f32 1.3e-6 (two terms of the weights: 1.9e-6, 410 us instead of 449).
+// 2^-22 or 2^-24 (of a weight in f16 2^-40 of the largest, where that is more): at 28 / 4
+// heads and 6000 bf16 keys the error is 3.6e-7, that of a plain form in f32 1.1e-6 (two
+// terms of the weights: 1.9e-6 and a tenth less time).
 //
 // Bound by HBM where the caches are long (192 units of one token behind up to 30000
-// keys, f16: 831 MB in 134 us = 6.2 TB/s); by the latency of a team's first pages, its
-// merge and uneven ends where they are short (64 requests of up to 8 tokens, 32 / 8
-// heads, up to 2000 keys: 151 MB in 50 us = 3.0 TB/s; a short batch 10 us); by the
-// products with several terms (36 sequences, 28 / 4 heads, f32: 449 us, tensor pipe 45 %).
+// keys, f16: 831 MB in 136 us = 6.1 TB/s); by the latency of a team's first pages, its
+// merge and uneven ends, and by a second pass over the keys of a pair with more than
+// 16 rows, where they are short (64 requests of up to 8 tokens, 32 / 8 heads, up to 2000
+// keys: 151 MB in 51 us = 3.0 TB/s; a short batch 10.5 us); by the products with several
+// terms (36 sequences, 28 / 4 heads, f32: 466 us, tensor pipe 45 %, where the long chunks
+// meet the shorter caches; 640 on average).
 #include <atomic>
 
 #include "chunk.cuh"

@@ -25,10 +25,12 @@
 // cannot matter.  (Which ones are left out depends on timing, the results do not.)
 // In the second launch a cluster per request walks the row of its token again.
 //
-// Bound by instructions, about 20 a logit for the exact weight's two halves, and for
-// few rows by the chain of a row's two passes and exchanges: 96 requests of four drafts
-// with the draft model's logits, 128000 f32: 142 us, the launches 97 and 56 apart (198 MB
-// at least, 30 us); 64 of seven looked-up drafts, 51865 bf16: 43 us; five, f32: 26 us.
+// Bound by waiting: for the exchange behind each of a row's two passes, for loads that
+// start anew behind it (about 20 instructions a logit for the exact weight's two halves use
+// 14 to 35 % of the first launch's issue slots, up to 45 % of the second's), and for few
+// rows by the chain of all these: 96 requests of four drafts with the draft model's
+// logits, 128000 f32: 141 us, the launches 97 and 56 apart (198 MB at least, 30 us); 64 of
+// seven looked-up drafts, 51865 bf16: 43 us; five with a draft model's, f32: 26 us.
 #include <algorithm>
 
 #include "common.cuh"

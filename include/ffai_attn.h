@@ -310,17 +310,16 @@ int ffai_attn_shared_prefix(ffai_attn_ctx* ctx, const ffai_attn_desc* d, int32_t
  * o (n_tokens, heads, 64) dense, f32, bf16 or f16; layouts TOKEN_MAJOR.  With
  * both f32, queries and softmax weights enter the products as sums of two or
  * three numbers of the cache's type, which costs two to three times the products:
- * 24 bits of them in bf16; in f16 what is left of a number is 2^-22 of it, or 2^-39 of
- * the query row's largest and 2^-40 of the largest weight.  Else f32 queries are
- * rounded to it (in f16 what is above 65504 is infinite then).  Pools,
- * kv_heads, types, and otherwise the rounding of softmax weights, and values
- * that are not numbers: as ffai_attn_shared_prefix.  lse
- * (optional, f32): (heads, n_tokens).  A row that sees no key gives zeros and
+ * 24 bits of them in bf16; in f16 what is left of a number is 2^-22 of it, or 2^-39
+ * of the query row's largest and 2^-40 of the largest weight.  Else f32 queries are
+ * rounded to it (in f16 what is above 65504 is infinite then).  Pools, kv_heads,
+ * types, and otherwise the rounding of softmax weights, and values that are not
+ * numbers: as ffai_attn_shared_prefix.  lse (optional, f32): (heads, n_tokens).  A row that sees no key gives zeros and
  * -inf; rows of q outside every sequence's leave o and lse as they are.
- * d->q_len: the most tokens of a sequence, if the host knows it (0: n_tokens);
- * it chooses between kernels and binds nothing.  d->q_offset, kv_len and the
- * k/v layouts are ignored, flags must be 0.  A sequence whose cu_q does not
- * rise or leaves 0 .. n_tokens is skipped (all of them, if the others name more
+ * d->q_len: the most tokens of a sequence, if the host knows it (0: not known);
+ * it helps to choose a kernel, one for the call, and binds nothing.  d->q_offset,
+ * kv_len and the k/v layouts are ignored, flags must be 0.  A sequence whose cu_q
+ * does not rise or leaves 0 .. n_tokens is skipped (all of them, if the others name more
  * than n_tokens between them), a length outside the table cut, and page ids
  * outside the pool are not read: ffai_attn_sync then reports
  * FFAI_ATTN_ERR_INVALID.  Streams and captures: as ffai_attn_shared_prefix.
@@ -473,12 +472,12 @@ int ffai_sample(ffai_attn_ctx* ctx, const void* logits, int64_t ld, int32_t dtyp
  * given (looked up, or a greedy draft's).  With p and q the softmax of a row's
  * logits over the temperatures (DEVICE (batch), null for 1; <= 0, or one whose
  * reciprocal overflows: the first maximum has all; infinite: the finite logits
- * weigh alike), the draft x of row i stands if u[i] q(x) < p(x) (q(x) = 1 without draft_logits); at the first that does
- * not, the token is taken by u_last[b] from max(0, p - q) over its sum, in the
- * order of the vocabulary, or from the last row's p if all stand.  So the
- * tokens are distributed as if the target alone had been sampled, one by one.
- * Both are computed in whole weights as in ffai_sample (p and q below 2^-36 of a
- * row's largest are 0): equal inputs give equal tokens.
+ * weigh alike), the draft x of row i stands if u[i] q(x) < p(x) (q(x) = 1 without
+ * draft_logits); at the first that does not, the token is taken by u_last[b] from
+ * max(0, p - q) over its sum, in the order of the vocabulary, or from the last
+ * row's p if all stand.  So the tokens are distributed as if the target alone had
+ * been sampled, one by one.  Both are computed in whole weights as in ffai_sample
+ * (p and q below 2^-36 of a row's largest are 0): equal inputs give equal tokens.
  *
  * u (rows), u_last (batch): uniform numbers in [0, 1).  accepted (batch): drafts
  * that stand, next (batch): the token behind them; tokens_out (rows): the
