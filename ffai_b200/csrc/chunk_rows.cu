@@ -112,8 +112,8 @@ __device__ __forceinline__ void load_rows(RowQ<TERMS>& q, RowState& st, const Ch
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       if (most > 0.f && most < INFINITY) {
-        // (2^100 at most: the scores' factor stays a normal number)
-        const int e = min(14 - (static_cast<int>(__float_as_uint(most) >> 23) - 127), 100);
+        // (2^126 at most: both powers are normal numbers)
+        const int e = min(14 - (static_cast<int>(__float_as_uint(most) >> 23) - 127), 126);
         up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       }

@@ -430,7 +430,7 @@ def test_refusals():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("size", [1e-4, 1.0, 1e5, 1e20])
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 1.0, 1e5, 1e20])
 @pytest.mark.parametrize("tokens,heads", [(1, 8), (9, 7), (40, 4), (300, 5)])
 def test_f32_queries_of_every_size_and_their_weights(tokens, heads, size, dtype):
     """Two keys, 0 and e_0, with the values 0 and 1, and queries a e_0 (of another size
